@@ -16,6 +16,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libpaged_attn_b200.so"
 HEADER = PKG.parent / "include" / "paged_attention_b200.h"
+HEADER_KV8 = PKG.parent / "include" / "paged_kv8_b200.h"
 
 PA_OK = 0
 PA_ERR_INVALID_ARGUMENT = 1
@@ -36,6 +37,17 @@ PA_LAUNCH_PREFILL_TC = 8
 PA_LAUNCH_GENERIC = 16
 PA_LAUNCH_PREFILL_PAIR = 32
 PA_LAUNCH_PREFILL_PERSIST = 64
+
+PA_LAUNCH_KV8_ROWS = 128
+PA_LAUNCH_KV8_COMBINE = 256
+PA_LAUNCH_KV8_TILES = 512
+
+PA_KV8_ERR_BLOCK = 1
+PA_KV8_ERR_TIMEOUT = 4
+PA_KV8_ERR_STEP = 8
+PA_KV8_ERR_NO_BLOCKS = 16
+PA_KV8_MAX_ROWS = 4096
+PA_KV8_MAX_REQUESTS = 131072
 
 ABI_VERSION = 7
 
@@ -76,6 +88,12 @@ class StepPlan(ctypes.Structure):
         return {name: getattr(self, name) for name, _ in self._fields_}
 
 
+class Kv8Tiling(ctypes.Structure):
+    """Mirror of ``pa_kv8_tiling``."""
+
+    _fields_ = [("small_tokens", c_int32), ("small_max", c_int32), ("large_tokens", c_int32), ("row_groups", c_int32)]
+
+
 _SIGNATURES = {
     "pa_abi_version": (c_int32, []),
     "pa_prefill_tile_rows": (c_int32, [c_int32]),
@@ -114,6 +132,24 @@ _SIGNATURES = {
                                      c_void_p, c_void_p]),
     "pa_plan_decode_padded": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, POINTER(StepPlan)]),
+    "pa_kv8_choose_tiling": (c_int32, [c_int32, c_int32, POINTER(Kv8Tiling)]),
+    "pa_kv8_build_step": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
+                                    c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+                                    POINTER(Kv8Tiling), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
+                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "pa_kv8_commit": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p,
+                                c_void_p, c_void_p]),
+    "pa_kv8_release": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                                 c_int32, c_void_p, c_void_p]),
+    "pa_kv8_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
+                                c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p,
+                                c_void_p]),
+    "pa_kv8_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32]),
+    "pa_kv8_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
+                                   c_void_p, c_int64, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
+                                   c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
+                                   c_uint64, c_void_p]),
+    "pa_kv8_read_error": (c_int32, [c_int32, POINTER(c_int32), c_void_p]),
 }
 
 _lib = None
@@ -140,9 +176,9 @@ def lib():
     return _lib
 
 
-def declared_symbols() -> list[str]:
-    """Every function the public header declares."""
-    text = HEADER.read_text()
+def declared_symbols(header: Path = HEADER) -> list[str]:
+    """Every function a public header declares."""
+    text = header.read_text()
     return sorted(set(re.findall(r"^\s*(?:[\w\s\*]+?)\b(pa_\w+)\s*\(", text, flags=re.M)))
 
 
@@ -151,7 +187,8 @@ def last_launches() -> set[str]:
     mask = lib().pa_last_launches()
     names = {PA_LAUNCH_DECODE_MMA: "decode_mma", PA_LAUNCH_DECODE_SIMT: "decode_simt",
              PA_LAUNCH_COMBINE: "combine", PA_LAUNCH_PREFILL_TC: "prefill_tc", PA_LAUNCH_GENERIC: "generic",
-             PA_LAUNCH_PREFILL_PAIR: "prefill_pair", PA_LAUNCH_PREFILL_PERSIST: "prefill_persist"}
+             PA_LAUNCH_PREFILL_PAIR: "prefill_pair", PA_LAUNCH_PREFILL_PERSIST: "prefill_persist",
+             PA_LAUNCH_KV8_ROWS: "kv8_rows", PA_LAUNCH_KV8_COMBINE: "kv8_combine", PA_LAUNCH_KV8_TILES: "kv8_tiles"}
     return {n for bit, n in names.items() if mask & bit}
 
 

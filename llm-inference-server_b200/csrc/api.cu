@@ -148,6 +148,8 @@ static int32_t cuda_fail(cudaError_t e, const char* what) {
 }
 
 void reset_last_launches() { g_last_launches = 0; }
+void note_launches(int32_t bits) { g_last_launches |= bits; }
+void* tensor_map_encoder() { return reinterpret_cast<void*>(encode_fn()); }
 
 int32_t check_attention_args(int32_t num_tokens, int32_t num_heads, int32_t head_dim, int32_t block_size,
                              int32_t num_kv_heads, int32_t dtype, const pa_step_plan* plan) {

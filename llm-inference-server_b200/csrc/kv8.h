@@ -1,0 +1,69 @@
+// Parameters and launchers of the 8-bit paged KV cache's kernels (kv8_*.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "paged_kv8_b200.h"
+
+namespace pa {
+
+struct Kv8StepParams {
+  const int32_t *row_ids, *lens, *query_lens;
+  int32_t* tables;
+  int64_t table_stride;
+  const int32_t *held, *free_blocks, *num_free;
+  int32_t free_capacity, num_rows, num_slots, width, block_size, num_tokens, max_query_len;
+  int64_t pool_blocks;
+  pa_kv8_tiling tiling;
+  int32_t *out_tables, *context_lens, *query_out, *held_out, *cu_query, *seq_idx, *q_pos, *slots, *num_free_out;
+  int64_t* work;
+};
+
+struct Kv8AppendParams {
+  const void *key, *value;
+  int64_t k_st, k_sh, v_st, v_sh;
+  int32_t num_tokens, num_kv_heads, head_dim, block_size;
+  uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  int64_t num_slots;
+  const int32_t* slots;
+  bool vec16;  // every row starts on a 16-byte boundary
+};
+
+struct Kv8AttnParams {
+  const void* q;
+  int64_t q_st, q_sh;
+  void* out;
+  int64_t o_st, o_sh;
+  const uint8_t *k_pool, *v_pool, *k_scale, *v_scale;
+  const int32_t* tables;
+  int64_t table_stride;
+  const int32_t *ctx_lens, *cu_q;
+  const int64_t* work;  // this class's running sums [num_seqs + 1]
+  int32_t num_seqs, num_heads, num_kv_heads, group, block_shift, tile_tokens, slices;
+  int32_t pool_blocks;
+  float qscale;  // softmax scale * log2(e)
+  float* part_o;
+  float2* part_ml;
+};
+
+int* kv8_error_word();  // device address of the current device's error word
+
+cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+                              const int32_t* held_out, const int32_t* num_free_out, int32_t rows, int32_t slots,
+                              int32_t* lens, int32_t* held, int32_t* num_free, cudaStream_t stream);
+cudaError_t launch_kv8_release(const int32_t* ids, int32_t count, const int32_t* tables, int64_t table_stride,
+                               int32_t width, int32_t slots, int32_t* lens, int32_t* held, int32_t* free_blocks,
+                               int32_t free_capacity, int32_t* num_free, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t stream);
+
+// Slices of the work line for the kernel for few rows, and the rows a partial holds.
+int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
+cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
+                            const Kv8AttnParams& p, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
+                               cudaStream_t stream);
+
+}  // namespace pa

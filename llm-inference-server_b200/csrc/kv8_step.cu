@@ -1,0 +1,315 @@
+// A step's block tables, slot map and work sums built on the GPU from request lengths, and
+// the two small kernels that keep the request slots (commit, release).
+//
+//   context_i = lens[r_i] + q_i,   need_i = max(0, ceil(context_i / block_size) - held[r_i])
+//   new block k of row i = free[num_free - 1 - (need_0 + ... + need_{i-1}) - k]
+//   slot of token t of row i = table_i[p / block_size] * block_size + p % block_size,
+//                              p = context_i - q_i + t
+//
+// The prefix sums over rows are what every other output needs.  Rows are few (thousands at
+// most) and a grid-wide wait or a second launch costs more than the sums, so every CTA
+// computes them for itself in shared memory and then fills its share of the tables and of
+// the per-token arrays; no CTA reads what another writes (a new block's id comes from the
+// free list by arithmetic, not from the table that it is also written to).
+#include "kv8.h"
+#include "kv8_line.cuh"
+#include "pa_common.cuh"
+
+namespace pa {
+
+constexpr int kStepThreads = 512;
+
+// Sums over the block: v becomes the sum of the threads' v before this one; returns the
+// total.  `scratch` holds one value per warp.
+template <typename V>
+__device__ __forceinline__ V block_scan(V& v, V* scratch) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  V sum = v;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const V up = __shfl_up_sync(0xffffffffu, sum, d);
+    if (lane >= d) sum += up;
+  }
+  if (lane == 31) scratch[warp] = sum;
+  __syncthreads();
+  V before = 0, total = 0;
+  for (int w = 0; w < warps; ++w) {
+    if (w == warp) before = total;
+    total += scratch[w];
+  }
+  __syncthreads();
+  v = before + sum - v;
+  return total;
+}
+
+__global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepParams p, int* err) {
+  extern __shared__ int32_t sm[];
+  const int rows = p.num_rows;
+  int32_t* s_cu = sm;                 // [rows + 1] tokens before the row
+  int32_t* s_ctx = s_cu + rows + 1;   // [rows]
+  int32_t* s_new = s_ctx + rows;      // [rows] new blocks before the row
+  int32_t* s_held = s_new + rows;     // [rows]
+  int32_t* s_row = s_held + rows;     // [rows] request slot or -1
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_row + rows);  // a bit per slot, with row_ids only
+  __shared__ int32_t scan32[kStepThreads / 32];
+  __shared__ int64_t scan64[kStepThreads / 32];
+  const int tid = threadIdx.x;
+
+  if (p.row_ids)
+    for (int i = tid; i < (p.num_slots + 31) / 32; i += blockDim.x) s_seen[i] = 0u;
+  __syncthreads();
+
+  int bad = 0;
+  int64_t tokens = 0, blocks = 0, small = 0, large = 0;  // totals so far
+  for (int first = 0; first < rows; first += blockDim.x) {
+    const int i = first + tid;
+    int q = 0, ctx = 0, held = 0, need = 0, row = -1;
+    if (i < rows) {
+      row = p.row_ids ? p.row_ids[i] : i;
+      if (row >= p.num_slots || row < -1) {
+        bad |= PA_KV8_ERR_STEP;
+        row = -1;
+      }
+      if (row >= 0) {
+        if (p.row_ids && (atomicOr(&s_seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u)) bad |= PA_KV8_ERR_STEP;
+        q = p.query_lens[i];
+        const int64_t len = p.lens[row];
+        const int64_t c = p.held ? len + q : len;
+        held = p.held ? p.held[row] : 0;
+        const int64_t most = int64_t(p.width) * p.block_size;
+        if (q < 0 || q > p.max_query_len || len < 0 || c < q || c > most || held < 0 || held > p.width) {
+          bad |= PA_KV8_ERR_STEP;
+          q = held = 0;
+        } else {
+          ctx = int(c);
+          if (p.held) need = max(0, (ctx + p.block_size - 1) / p.block_size - held);
+        }
+      }
+      s_ctx[i] = ctx;
+      s_held[i] = held;
+      s_row[i] = row;
+    }
+    int at = q, nb = need;
+    const int step_tokens = block_scan(at, scan32);
+    const int step_blocks = block_scan(nb, scan32);
+    if (i < rows) {
+      s_cu[i] = int32_t(tokens + at);
+      s_new[i] = int32_t(blocks + nb);
+    }
+    tokens += step_tokens;
+    blocks += step_blocks;
+    if (tokens > p.num_tokens) bad |= PA_KV8_ERR_STEP;  // sums of one round stay below 2^31: see the host's checks
+    if (blockIdx.x == 0) {
+      const bool few = q <= p.tiling.small_max;
+      const int tt = few ? p.tiling.small_tokens : p.tiling.large_tokens;
+      const int64_t keys = q > 0 ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
+      int64_t ws = few ? keys : 0, wl = few ? 0 : keys;
+      const int64_t ts = block_scan(ws, scan64), tl = block_scan(wl, scan64);
+      if (i < rows) {
+        p.work[i] = small + ws;
+        p.work[rows + 1 + i] = large + wl;
+      }
+      small += ts;
+      large += tl;
+    }
+  }
+  int avail = 0;
+  if (p.held) {
+    avail = *p.num_free;
+    if (avail < 0 || avail > p.free_capacity)
+      bad |= PA_KV8_ERR_STEP;
+    else if (blocks > avail)
+      bad |= PA_KV8_ERR_NO_BLOCKS;
+  }
+  if (tid == 0) s_cu[rows] = int32_t(tokens);
+  const bool reject = __syncthreads_or(bad) != 0;
+  if (blockIdx.x == 0) {
+    if (bad) set_error(err, bad);
+    for (int i = tid; i <= rows; i += blockDim.x) {
+      p.cu_query[i] = reject ? 0 : s_cu[i];
+      if (reject) p.work[i] = p.work[rows + 1 + i] = 0;
+      if (i < rows) {
+        const int need = (i + 1 < rows ? s_new[i + 1] : int32_t(blocks)) - s_new[i];
+        p.context_lens[i] = reject ? 0 : s_ctx[i];
+        p.query_out[i] = reject ? 0 : s_cu[i + 1] - s_cu[i];
+        p.held_out[i] = reject ? 0 : s_held[i] + need;
+      }
+    }
+    if (tid == 0) {
+      if (!reject) {
+        p.work[rows] = small;
+        p.work[2 * rows + 1] = large;
+      }
+      *p.num_free_out = reject ? -1 : avail - int32_t(blocks);
+    }
+  }
+
+  // Block tables: what the row holds, then its new blocks, then zeros.
+  const int64_t stride = int64_t(gridDim.x) * blockDim.x, me = int64_t(blockIdx.x) * blockDim.x + tid;
+  auto block_of = [&](int i, int j) -> int {  // j below the row's blocks
+    const int k = j - s_held[i];
+    return k < 0 ? p.tables[int64_t(s_row[i]) * p.table_stride + j] : p.free_blocks[avail - 1 - s_new[i] - k];
+  };
+  if (p.held) {
+    const int64_t cells = int64_t(rows) * p.width;
+    for (int64_t c = me; c < cells; c += stride) {
+      const int i = int(c / p.width), j = int(c - int64_t(i) * p.width);
+      int id = 0;
+      if (!reject && s_row[i] >= 0) {
+        const int need = (i + 1 < rows ? s_new[i + 1] : int32_t(blocks)) - s_new[i];
+        if (j < s_held[i] + need) {
+          id = block_of(i, j);
+          if (id < 0 || id >= p.pool_blocks) set_error(err, PA_KV8_ERR_BLOCK);
+          if (j >= s_held[i]) p.tables[int64_t(s_row[i]) * p.table_stride + j] = id;
+        }
+      }
+      p.out_tables[c] = id;
+    }
+  }
+  // Per-token arrays.
+  for (int64_t t = me; t < p.num_tokens; t += stride) {
+    int seq = -1, pos = -1, slot = -1;
+    if (!reject && t < tokens) {
+      int lo = 0, hi = rows;  // s_cu[lo] <= t < s_cu[hi]
+      while (hi - lo > 1) {
+        const int m = (lo + hi) / 2;
+        if (s_cu[m] <= t)
+          lo = m;
+        else
+          hi = m;
+      }
+      seq = lo;
+      pos = s_ctx[lo] - s_cu[lo + 1] + int(t);
+      const int j = pos / p.block_size;
+      const int id = p.held ? block_of(lo, j) : p.tables[int64_t(s_row[lo]) * p.table_stride + j];
+      if (id < 0 || id >= p.pool_blocks)
+        set_error(err, PA_KV8_ERR_BLOCK);
+      else
+        slot = id * p.block_size + pos % p.block_size;
+    }
+    p.seq_idx[t] = seq;
+    p.q_pos[t] = pos;
+    p.slots[t] = slot;
+  }
+}
+
+__global__ void __launch_bounds__(256) kv8_commit_kernel(const int32_t* row_ids, const int32_t* query_lens,
+                                                         const int32_t* accepted, const int32_t* held_out,
+                                                         const int32_t* num_free_out, int rows, int slots,
+                                                         int32_t* lens, int32_t* held, int32_t* num_free) {
+  const int left = *num_free_out;
+  if (left < 0) return;  // the step was emptied
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+    const int row = row_ids ? row_ids[i] : i;
+    if (row < 0 || row >= slots) continue;
+    const int q = query_lens[i];
+    lens[row] += accepted ? max(0, min(accepted[i], q)) : q;
+    held[row] = held_out[i];
+  }
+  if (threadIdx.x == 0) *num_free = left;
+}
+
+// One CTA: a release is rare and short, and its places on the free list depend on one
+// another through the running sum.
+__global__ void __launch_bounds__(kStepThreads) kv8_release_kernel(const int32_t* ids, int count, const int32_t* tables,
+                                                                   int64_t table_stride, int width, int slots,
+                                                                   int32_t* lens, int32_t* held, int32_t* free_blocks,
+                                                                   int free_capacity, int32_t* num_free, int* err) {
+  extern __shared__ int32_t sm[];
+  int32_t* s_at = sm;            // [count + 1] blocks before the id
+  uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_at + count + 1);
+  __shared__ int32_t scan32[kStepThreads / 32];
+  const int tid = threadIdx.x;
+  for (int i = tid; i < (slots + 31) / 32; i += blockDim.x) s_seen[i] = 0u;
+  __syncthreads();
+  int bad = 0;
+  int64_t blocks = 0;
+  for (int first = 0; first < count; first += blockDim.x) {
+    const int i = first + tid;
+    int n = 0;
+    if (i < count) {
+      const int row = ids[i];
+      if (row >= slots || row < -1) {
+        bad = 1;
+      } else if (row >= 0) {
+        if (atomicOr(&s_seen[row >> 5], 1u << (row & 31)) >> (row & 31) & 1u) bad = 1;
+        n = held[row];
+        if (n < 0 || n > width) {
+          bad = 1;
+          n = 0;
+        }
+      }
+    }
+    int at = n;
+    const int sum = block_scan(at, scan32);
+    if (i < count) s_at[i] = int32_t(blocks + at);
+    blocks += sum;
+  }
+  const int have = *num_free;
+  if (have < 0 || have + blocks > free_capacity) bad = 1;
+  if (tid == 0) s_at[count] = int32_t(blocks);
+  if (__syncthreads_or(bad)) {
+    if (tid == 0) set_error(err, PA_KV8_ERR_STEP);
+    return;
+  }
+  for (int b = tid; b < int(blocks); b += blockDim.x) {
+    int lo = 0, hi = count;
+    while (hi - lo > 1) {
+      const int m = (lo + hi) / 2;
+      if (s_at[m] <= b)
+        lo = m;
+      else
+        hi = m;
+    }
+    free_blocks[have + b] = tables[int64_t(ids[lo]) * table_stride + (s_at[lo + 1] - 1 - b)];
+  }
+  for (int i = tid; i < count; i += blockDim.x)
+    if (ids[i] >= 0) lens[ids[i]] = held[ids[i]] = 0;
+  if (tid == 0) *num_free = have + int(blocks);
+}
+
+// ------------------------------------------------------------------ launch
+static __device__ int g_kv8_error;
+
+int* kv8_error_word() {
+  void* at = nullptr;
+  return cudaGetSymbolAddress(&at, g_kv8_error) == cudaSuccess ? static_cast<int*>(at) : nullptr;
+}
+
+static cudaError_t allow_smem(const void* kern, size_t bytes) {
+  return bytes <= 48 * 1024 ? cudaSuccess
+                            : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+}
+
+cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t stream) {
+  const size_t smem = sizeof(int32_t) * (5 * size_t(p.num_rows) + 1) +
+                      (p.row_ids ? sizeof(uint32_t) * ((size_t(p.num_slots) + 31) / 32) : 0);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_step_kernel), smem);
+  if (e != cudaSuccess) return e;
+  const int64_t cells = (p.held ? int64_t(p.num_rows) * p.width : 0) + p.num_tokens;
+  const int64_t want = (cells + kStepThreads - 1) / kStepThreads;
+  const int grid = int(want < 1 ? 1 : (want < 148 ? want : 148));
+  kv8_step_kernel<<<grid, kStepThreads, smem, stream>>>(p, err);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+                              const int32_t* held_out, const int32_t* num_free_out, int32_t rows, int32_t slots,
+                              int32_t* lens, int32_t* held, int32_t* num_free, cudaStream_t stream) {
+  kv8_commit_kernel<<<1, 256, 0, stream>>>(row_ids, query_lens, accepted, held_out, num_free_out, rows, slots, lens,
+                                           held, num_free);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_kv8_release(const int32_t* ids, int32_t count, const int32_t* tables, int64_t table_stride,
+                               int32_t width, int32_t slots, int32_t* lens, int32_t* held, int32_t* free_blocks,
+                               int32_t free_capacity, int32_t* num_free, int* err, cudaStream_t stream) {
+  const size_t smem = sizeof(int32_t) * (size_t(count) + 1) + sizeof(uint32_t) * ((size_t(slots) + 31) / 32);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_release_kernel), smem);
+  if (e != cudaSuccess) return e;
+  kv8_release_kernel<<<1, kStepThreads, smem, stream>>>(ids, count, tables, table_stride, width, slots, lens, held,
+                                                        free_blocks, free_capacity, num_free, err);
+  return cudaGetLastError();
+}
+
+}  // namespace pa

@@ -14,6 +14,11 @@ int32_t fail(int32_t code, const char* fmt, ...);
 
 // Clears the calling thread's record of the kernels its last attention call launched.
 void reset_last_launches();
+// Adds PA_LAUNCH_* bits to that record.
+void note_launches(int32_t bits);
+
+// The driver's cuTensorMapEncodeTiled (PFN_cuTensorMapEncodeTiled_v12000), or NULL.
+void* tensor_map_encoder();
 
 // The checks pa_paged_attention_fwd makes before it looks at any pointer or workspace:
 // dtype, head shape, and that `plan` was built for this token count and block size.

@@ -1,0 +1,560 @@
+"""The 8-bit paged KV cache, driven from the GPU.
+
+Half the bytes of a 16-bit pool per cached token, so about twice the decode rate where HBM
+bounds it and twice the tokens a pool holds.  Three operators that work together:
+
+* :class:`DeviceBlockTables` / :func:`device_step` — a step's block tables, slot map and
+  work sums built on the GPU from request lengths (blocks taken from a free list there), so
+  a decode loop needs no host plan;
+* :func:`reshape_and_cache_kv8` — the fused K+V append, quantising each row;
+* :func:`paged_attention_kv8` — causal attention of a chunk of new tokens (one and more)
+  over the 8-bit pools.
+
+Format: a row (one token of one KV head) is e4m3 payload ``[NB, BS, Hkv, D]`` and a scale
+byte ``[NB, Hkv, BS]`` that stands for ``2^(byte - 127)`` (``torch.float8_e8m0fnu``): the least
+exponent in [-14, 7] that brings the row's largest magnitude to 448.  Every cached value is
+exactly an fp16 number; magnitudes past 57,344 saturate; a row with a NaN reads as NaN.
+
+Lengths and ids that only the GPU sees are checked there: a bad step is emptied and leaves
+a bit in the device's error word, which :func:`read_kv8_error` returns.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .attention import _DTYPE_CODE
+from .kv_cache import HostBlocks, _error_word, copy_blocks, gather_blocks, scatter_blocks
+
+_PAYLOAD = torch.float8_e4m3fn
+
+
+def _stream(device: torch.device) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+class _On:
+    """Make ``device`` current for the library calls inside (they launch there)."""
+
+    __slots__ = ("index", "previous")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.previous = torch.cuda.current_device()
+        if self.index is not None and self.index != self.previous:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.index is not None and self.index != self.previous:
+            torch.cuda.set_device(self.previous)
+
+
+def _need_cuda(device: torch.device, what: str) -> None:
+    if device.type != "cuda":
+        raise NotImplementedError(f"ATTENTION=cuda: {what} needs a CUDA device, got {device}. There is no CPU fallback.")
+
+
+def _int32(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype != torch.int32:
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def read_kv8_error(device=None, clear: bool = True) -> int:
+    """The KV8 error word of ``device`` (0: nothing reported; else ``_lib.PA_KV8_ERR_*``
+    bits).  Synchronises the current stream."""
+    device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    word = ctypes.c_int32(0)
+    with _On(device):
+        _lib.check(_lib.lib().pa_kv8_read_error(int(clear), ctypes.byref(word), _stream(device)))
+    return int(word.value)
+
+
+# ---------------------------------------------------------------------------- steps
+_TILINGS: dict[tuple[int, int], _lib.Kv8Tiling] = {}
+
+
+def _tiling(group: int, max_query_len: int) -> _lib.Kv8Tiling:
+    t = _TILINGS.get((group, max_query_len))
+    if t is None:
+        t = _lib.Kv8Tiling()
+        _lib.check(_lib.lib().pa_kv8_choose_tiling(int(group), int(max_query_len), ctypes.byref(t)))
+        if len(_TILINGS) > 1024:
+            _TILINGS.clear()
+        _TILINGS[(group, max_query_len)] = t
+    return t
+
+
+class DeviceStep:
+    """One step's metadata on the GPU, shared by every layer: ``block_tables [B, W]``,
+    ``context_lens`` / ``query_lens [B]``, ``cu_query_lens [B + 1]``, per token ``seq_idx``,
+    ``q_pos`` and ``slot_mapping [T]`` (-1 past the step's last token), ``num_free [1]`` (the
+    free list's length once the step counts; -1: the step was emptied)."""
+
+    def __init__(self, num_rows: int, num_tokens: int, width: int, max_query_len: int, block_size: int,
+                 num_blocks: int, group: int, device: torch.device, own_tables: bool):
+        self.num_seqs, self.num_tokens, self.width = int(num_rows), int(num_tokens), int(width)
+        self.max_query_len, self.block_size, self.group = int(max_query_len), int(block_size), int(group)
+        self.num_blocks, self.device = int(num_blocks), device
+        b, t = self.num_seqs, self.num_tokens
+        # int64 sums first, then the int32 arrays, each on a 16-byte boundary.
+        sizes = [4 * (b + 1), b, b, b, b + 1, t, t, t, 1, b * self.width if own_tables else 0]
+        self._off = []
+        at = 0
+        for n in sizes:
+            self._off.append(at)
+            at += (n + 3) & ~3
+        self._sizes = sizes
+        self.buffer = torch.empty(at, dtype=torch.int32, device=device)
+        self._base = self.buffer.data_ptr()
+        self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
+        self._row_ids: torch.Tensor | None = None
+
+    def _ptr(self, i: int) -> int:
+        return self._base + 4 * self._off[i]
+
+    def _view(self, i: int) -> torch.Tensor:
+        return self.buffer[self._off[i]:self._off[i] + self._sizes[i]]
+
+    @property
+    def work(self) -> torch.Tensor:
+        return self._view(0).view(torch.int64).view(2, self.num_seqs + 1)
+
+    @property
+    def context_lens(self) -> torch.Tensor:
+        return self._view(1)
+
+    @property
+    def query_lens(self) -> torch.Tensor:
+        return self._view(2)
+
+    @property
+    def held(self) -> torch.Tensor:
+        return self._view(3)
+
+    @property
+    def cu_query_lens(self) -> torch.Tensor:
+        return self._view(4)
+
+    @property
+    def seq_idx(self) -> torch.Tensor:
+        return self._view(5)
+
+    @property
+    def q_pos(self) -> torch.Tensor:
+        return self._view(6)
+
+    @property
+    def slot_mapping(self) -> torch.Tensor:
+        return self._view(7)
+
+    @property
+    def num_free(self) -> torch.Tensor:
+        return self._view(8)
+
+    @property
+    def block_tables(self) -> torch.Tensor:
+        return self._tables if self._tables is not None else self._view(9).view(self.num_seqs, self.width)
+
+    def matches(self, num_tokens: int, block_size: int, num_blocks: int, group: int) -> bool:
+        """Whether this step can drive an attention call of these sizes."""
+        return (self.num_tokens == num_tokens and self.block_size == block_size and self.num_blocks == num_blocks
+                and self.group == group)
+
+
+def _check_step_sizes(num_tokens: int, max_query_len: int, block_size: int, num_blocks: int) -> None:
+    if num_tokens < 0 or max_query_len < 0:
+        raise ValueError("num_tokens and max_query_len must be non-negative")
+    if block_size <= 0 or num_blocks < 0:
+        raise ValueError("block_size must be positive and the pool's block count non-negative")
+
+
+def _reusable(out: DeviceStep | None, like: tuple, device) -> DeviceStep | None:
+    if out is None:
+        return None
+    have = (out.num_seqs, out.num_tokens, out.width, out.max_query_len, out.block_size, out.num_blocks, out.group)
+    if have != like or out.device != device:
+        raise ValueError(f"out was made for a step of other sizes: {have}, this one needs {like}")
+    return out
+
+
+def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_lens: torch.Tensor, *, num_tokens: int,
+                max_query_len: int, num_blocks: int, block_size: int, group: int = 1,
+                out: DeviceStep | None = None) -> DeviceStep:
+    """Prefix sums, per-token positions and the slot map of a step whose block tables are
+    already on the GPU (``block_tables [B, W]``, ``context_lens [B]`` with this step's tokens,
+    ``query_lens [B]``), in one launch and without the host reading a length.  ``num_tokens``
+    is the packed token count (tokens past ``sum(query_lens)`` get -1), ``max_query_len`` a
+    bound on the chunks, ``group`` the query heads per KV head of the attention that will use
+    the step.  ``out``: a step of the same sizes whose buffers are written again (for captured
+    graphs)."""
+    dev = block_tables.device
+    _need_cuda(dev, "device_step")
+    _check_step_sizes(num_tokens, max_query_len, block_size, num_blocks)
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [batch, max_blocks]")
+    b, w = block_tables.shape
+    if tuple(context_lens.shape) != (b,) or tuple(query_lens.shape) != (b,):
+        raise ValueError("context_lens and query_lens must be [batch] to match block_tables")
+    tables = block_tables
+    if tables.dtype != torch.int32 or (w and tables.stride(1) != 1) or (b > 1 and tables.stride(0) < w):
+        tables = _int32("block_tables", tables, dev)
+    ctx, ql = _int32("context_lens", context_lens, dev), _int32("query_lens", query_lens, dev)
+    tiling = _tiling(group, max_query_len)
+    step = _reusable(out, (b, num_tokens, w, max_query_len, block_size, num_blocks, group), dev)
+    if step is None:
+        step = DeviceStep(b, num_tokens, w, max_query_len, block_size, num_blocks, group, dev, own_tables=False)
+    elif step._sizes[9]:
+        raise ValueError("out was made by DeviceBlockTables.reserve")
+    step._tables, step._row_ids = tables, None
+    p = step._ptr
+    with _On(dev):
+        _lib.check(_lib.lib().pa_kv8_build_step(
+            None, ctx.data_ptr(), ql.data_ptr(), tables.data_ptr(), max(tables.stride(0), w), None, None, None, 0, b, b,
+            w, step.block_size, step.num_blocks, step.num_tokens, step.max_query_len, ctypes.byref(tiling), None, p(1),
+            p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(0), _stream(dev)))
+    return step
+
+
+class DeviceBlockTables:
+    """Block tables that live and grow on the GPU: per request slot a row of block ids, the
+    tokens cached and the blocks held, and one free list for the pool.
+
+    A step is ``reserve`` (blocks for the new tokens, the step's metadata), then the layers,
+    then ``commit`` — with the accepted counts, where a chunk of speculated tokens was only
+    partly accepted.  Until ``commit``, a step can be reserved again or dropped.  ``release``
+    returns a finished request's blocks.  Nothing here reads the GPU from the host, so the
+    whole loop can be captured in a CUDA graph.  Prefix sharing stays with the host allocator:
+    a block is held by one slot."""
+
+    def __init__(self, max_requests: int, width: int, num_blocks: int, block_size: int, device) -> None:
+        device = torch.device(device)
+        _need_cuda(device, "DeviceBlockTables")
+        if max_requests <= 0 or width <= 0 or num_blocks < 0 or block_size <= 0:
+            raise ValueError("max_requests, width and block_size must be positive, num_blocks non-negative")
+        zeros = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=device)  # noqa: E731
+        # Taken from the end of the list: block 0 first.
+        free = torch.arange(num_blocks - 1, -1, -1, dtype=torch.int32, device=device)
+        self._set(zeros(max_requests, width), zeros(max_requests), zeros(max_requests), free,
+                  torch.full((1,), num_blocks, dtype=torch.int32, device=device), num_blocks, block_size)
+
+    @classmethod
+    def adopt(cls, tables: torch.Tensor, lens: torch.Tensor, held: torch.Tensor, free: torch.Tensor,
+              num_free: torch.Tensor, *, num_blocks: int, block_size: int) -> "DeviceBlockTables":
+        """Over tensors the caller already keeps (all int32, contiguous, on one GPU): ``tables
+        [R, W]``, ``lens [R]``, ``held [R]``, ``free`` with its first ``num_free [1]`` entries
+        valid.  They are updated in place."""
+        dev = tables.device
+        _need_cuda(dev, "DeviceBlockTables")
+        if tables.dim() != 2 or tuple(lens.shape) != (tables.shape[0],) or tuple(held.shape) != (tables.shape[0],):
+            raise ValueError("tables must be [requests, width], lens and held [requests]")
+        if free.dim() != 1 or num_free.numel() != 1:
+            raise ValueError("free must be [capacity] and num_free [1]")
+        for name, t in (("tables", tables), ("lens", lens), ("held", held), ("free", free), ("num_free", num_free)):
+            if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous int32 on {dev}")
+        self = cls.__new__(cls)
+        self._set(tables, lens, held, free, num_free, num_blocks, block_size)
+        return self
+
+    def _set(self, tables, lens, held, free, num_free, num_blocks, block_size) -> None:
+        _check_step_sizes(0, 0, block_size, num_blocks)
+        self.tables, self.lens, self.held, self.free, self.num_free = tables, lens, held, free, num_free
+        self.num_blocks, self.block_size, self.device = int(num_blocks), int(block_size), tables.device
+        self.max_requests, self.width = (int(x) for x in tables.shape)
+
+    def reserve(self, request_ids: torch.Tensor, query_lens: torch.Tensor, *, num_tokens: int, max_query_len: int,
+                group: int = 1, out: DeviceStep | None = None) -> DeviceStep:
+        """The step that appends ``query_lens[i]`` tokens to request slot ``request_ids[i]``
+        (-1: a padding row; a slot at most once), in one launch.  A slot that needs more blocks
+        than it holds takes them from the free list, rows in order.  When the list is too short
+        or the arguments do not fit together, the step is emptied (``num_free`` -1, an error
+        bit) and no table changes."""
+        dev = self.device
+        _check_step_sizes(num_tokens, max_query_len, self.block_size, self.num_blocks)
+        if request_ids.dim() != 1 or query_lens.shape != request_ids.shape:
+            raise ValueError("request_ids and query_lens must both be [rows]")
+        ids, ql = _int32("request_ids", request_ids, dev), _int32("query_lens", query_lens, dev)
+        b = ids.shape[0]
+        tiling = _tiling(group, max_query_len)
+        step = _reusable(out, (b, num_tokens, self.width, max_query_len, self.block_size, self.num_blocks, group), dev)
+        if step is None:
+            step = DeviceStep(b, num_tokens, self.width, max_query_len, self.block_size, self.num_blocks, group, dev,
+                              own_tables=True)
+        elif step._tables is not None:
+            raise ValueError("out was made by device_step")
+        step._row_ids = ids
+        p = step._ptr
+        with _On(dev):
+            _lib.check(_lib.lib().pa_kv8_build_step(
+                ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(), self.tables.data_ptr(), self.width,
+                self.held.data_ptr(), self.free.data_ptr(), self.num_free.data_ptr(), self.free.numel(), b,
+                self.max_requests, self.width, self.block_size, self.num_blocks, step.num_tokens, step.max_query_len,
+                ctypes.byref(tiling), p(9), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(0), _stream(dev)))
+        return step
+
+    def commit(self, step: DeviceStep, accepted: torch.Tensor | None = None) -> None:
+        """Make a reserved step count: its tokens (or the ``accepted[i]`` first of row i) are
+        cached now and its blocks are held.  An emptied step changes nothing."""
+        if step._row_ids is None:
+            raise ValueError("commit needs a step made by reserve")
+        acc = None
+        if accepted is not None:
+            if tuple(accepted.shape) != (step.num_seqs,):
+                raise ValueError(f"accepted must be [{step.num_seqs}], got {tuple(accepted.shape)}")
+            acc = _int32("accepted", accepted, self.device)
+        with _On(self.device):
+            _lib.check(_lib.lib().pa_kv8_commit(
+                step._row_ids.data_ptr(), step._ptr(2), acc.data_ptr() if acc is not None else None, step._ptr(3),
+                step._ptr(8), step.num_seqs, self.max_requests, self.lens.data_ptr(), self.held.data_ptr(),
+                self.num_free.data_ptr(), _stream(self.device)))
+
+    def release(self, request_ids: torch.Tensor) -> None:
+        """Return the blocks of these request slots (-1 is passed over; a slot at most once) to
+        the free list and empty the slots."""
+        if request_ids.dim() != 1:
+            raise ValueError("request_ids must be [count]")
+        ids = _int32("request_ids", request_ids, self.device)
+        with _On(self.device):
+            _lib.check(_lib.lib().pa_kv8_release(
+                ids.data_ptr(), ids.shape[0], self.tables.data_ptr(), self.width, self.width, self.max_requests,
+                self.lens.data_ptr(), self.held.data_ptr(), self.free.data_ptr(), self.free.numel(),
+                self.num_free.data_ptr(), _stream(self.device)))
+
+
+# ---------------------------------------------------------------------------- the pools
+def _check_pools(k_pool, v_pool, k_scale, v_scale, device) -> tuple[int, int, int, int]:
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
+        raise ValueError("k_pool and v_pool must both be [blocks, block_size, kv_heads, dim]")
+    nb, bs, hkv, dim = k_pool.shape
+    for name, t, shape in (("k_pool", k_pool, k_pool.shape), ("v_pool", v_pool, k_pool.shape),
+                           ("k_scale", k_scale, (nb, hkv, bs)), ("v_scale", v_scale, (nb, hkv, bs))):
+        want = _PAYLOAD if name.endswith("pool") else torch.uint8
+        if t.dtype != want:
+            raise ValueError(f"{name} must be {want}, got {t.dtype}")
+        if t.device != device:
+            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous {tuple(shape)}, got {tuple(t.shape)}")
+    return nb, bs, hkv, dim
+
+
+def reshape_and_cache_kv8(key: torch.Tensor, value: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                          k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Quantise ``key``/``value`` ``[T, Hkv, D]`` (float32, float16 or bfloat16; D 64 or 128;
+    any token and head strides) and write them into the 8-bit pools at flat slots
+    ``slot_mapping [T]``; one launch for K and V.  Slots outside the pool (the -1 of padding
+    tokens) are passed over; a slot named twice must get the same row."""
+    dev = key.device
+    _need_cuda(dev, "the 8-bit KV append")
+    if key.dim() != 3 or value.shape != key.shape:
+        raise ValueError(f"key/value must both be [tokens, kv_heads, dim], got {tuple(key.shape)} and "
+                         f"{tuple(value.shape)}")
+    nb, bs, hkv, dim = _check_pools(k_pool, v_pool, k_scale, v_scale, dev)
+    if key.shape[1:] != (hkv, dim):
+        raise ValueError(f"key rows {tuple(key.shape[1:])} do not match the pool's {(hkv, dim)}")
+    if value.dtype != key.dtype or value.device != dev:
+        raise ValueError("key and value must share dtype and device")
+    if key.dtype not in _DTYPE_CODE:
+        raise NotImplementedError(f"ATTENTION=cuda: dtype {key.dtype} is not float32, float16 or bfloat16")
+    if key.stride(2) != 1 or value.stride(2) != 1:
+        key, value = key.contiguous(), value.contiguous()
+    if slot_mapping.shape != (key.shape[0],):
+        raise ValueError(f"slot_mapping must be [{key.shape[0]}], got {tuple(slot_mapping.shape)}")
+    slots = _int32("slot_mapping", slot_mapping, dev)
+    with _On(dev):
+        _lib.check(_lib.lib().pa_kv8_append(
+            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
+            key.shape[0], hkv, dim, _DTYPE_CODE[key.dtype], k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), nb, bs, slots.data_ptr(), _stream(dev)))
+
+
+def attach_step(block_tables: torch.Tensor, step: DeviceStep) -> torch.Tensor:
+    """Let a step ride on its block-table tensor (as ``metadata.attach`` does for host plans),
+    so that every layer's :func:`paged_attention_kv8` uses it instead of building its own."""
+    block_tables._kv8_step = step
+    return block_tables
+
+
+_SCRATCH_BYTES: dict[tuple[int, int, int, int], int] = {}
+
+
+def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
+                        v_scale: torch.Tensor, block_tables: torch.Tensor, context_lens: torch.Tensor,
+                        query_lens: torch.Tensor, scale: float, *, max_query_len: int | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal paged attention over the 8-bit pools: :func:`paged_attention_cuda`'s arguments
+    and rule with the pools' scales.  Lengths and tables are device tensors that the host never
+    reads; ``max_query_len`` bounds the chunks (default: the token count).  Builds the step
+    (one launch) unless ``block_tables`` carries one (:func:`attach_step`).
+
+    query ``[T, Hq, D]``, float16 or bfloat16, D 64 or 128, at most 16 query heads per KV
+    head; pools' block size a power of two times 16.  Rows past the last sequence's are left
+    as they were in ``out`` (undefined without ``out``)."""
+    if query.dim() != 3:
+        raise ValueError(f"query must be [num_tokens, heads, dim], got {tuple(query.shape)}")
+    dev = query.device
+    _need_cuda(dev, "attention over the 8-bit pools")
+    nb, bs, hkv, dim = _check_pools(k_pool, v_pool, k_scale, v_scale, dev)
+    tokens, heads, qdim = query.shape
+    if qdim != dim:
+        raise ValueError(f"query head_dim {qdim} != pool head_dim {dim}")
+    if heads == 0 or hkv == 0 or heads % hkv:
+        raise ValueError(f"{heads} query heads not divisible by {hkv} kv heads")
+    if query.dtype not in (torch.float16, torch.bfloat16):
+        raise NotImplementedError(f"ATTENTION=cuda: the 8-bit cache takes float16 and bfloat16 queries, not {query.dtype}")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError("out must be contiguous with the query's shape, dtype and device")
+    group = heads // hkv
+    step = getattr(block_tables, "_kv8_step", None)
+    if step is None or step.device != dev or not step.matches(tokens, bs, nb, group):
+        step = device_step(block_tables, context_lens, query_lens, num_tokens=tokens,
+                           max_query_len=tokens if max_query_len is None else min(int(max_query_len), tokens),
+                           num_blocks=nb, block_size=bs, group=group)
+    if tokens == 0:
+        return out
+    if query.stride(2) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.data_ptr() % 16:
+        query = query.contiguous()
+    lib = _lib.lib()
+    shape = (heads, hkv, dim, step.max_query_len)
+    nbytes = _SCRATCH_BYTES.get(shape)
+    if nbytes is None:
+        nbytes = int(lib.pa_kv8_workspace_bytes(*shape))
+        if len(_SCRATCH_BYTES) > 1024:
+            _SCRATCH_BYTES.clear()
+        _SCRATCH_BYTES[shape] = nbytes
+    # From the caching allocator, so that calls on two streams and captured graphs each have
+    # their own.
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    tables = step.block_tables
+    p = step._ptr
+    with _On(dev):
+        _lib.check(lib.pa_kv8_attention(
+            query.data_ptr(), query.stride(0), query.stride(1), tokens, heads, dim, k_pool.data_ptr(),
+            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, bs, hkv, _DTYPE_CODE[query.dtype],
+            float(scale), step.num_seqs, step.max_query_len, tables.data_ptr(), max(tables.stride(0), step.width), p(1),
+            p(4), p(0), out.data_ptr(), out.stride(0), out.stride(1), scratch.data_ptr(), nbytes, _stream(dev)))
+    return out
+
+
+class KV8Pool:
+    """Per-layer 8-bit K and V pools with :class:`KVPool`'s attributes and block moves: ``k`` /
+    ``v`` lists of e4m3 ``[num_blocks, block_size, Hkv, D]`` and ``k_scale`` / ``v_scale`` lists
+    of bytes ``[num_blocks, Hkv, block_size]``, all zero-initialised.  ``dtype`` is the
+    payload's."""
+
+    def __init__(self, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                 device) -> None:
+        if head_dim not in (64, 128):
+            raise NotImplementedError(f"ATTENTION=cuda: head_dim {head_dim}: the 8-bit cache supports 64 and 128")
+        if block_size < 16 or block_size & (block_size - 1) or block_size > 4096:
+            raise NotImplementedError(f"ATTENTION=cuda: block_size {block_size}: the 8-bit cache supports 16, 32, ... 4096")
+        self.num_blocks, self.block_size = num_blocks, block_size
+        self.num_kv_heads, self.head_dim, self.dtype = num_kv_heads, head_dim, _PAYLOAD
+        shape, sshape = (num_blocks, block_size, num_kv_heads, head_dim), (num_blocks, num_kv_heads, block_size)
+
+        def payload():
+            return torch.zeros(shape, dtype=torch.uint8, device=device).view(_PAYLOAD)
+
+        def scales():
+            return torch.zeros(sshape, dtype=torch.uint8, device=device)
+
+        layers = range(num_layers)
+        self.k, self.v = [payload() for _ in layers], [payload() for _ in layers]
+        self.k_scale, self.v_scale = [scales() for _ in layers], [scales() for _ in layers]
+
+    @classmethod
+    def from_model(cls, model, num_blocks: int, block_size: int = 16, device=None) -> "KV8Pool":
+        """Sizes off the model config as :meth:`KVPool.from_model` reads them."""
+        cfg = model.config
+        heads = getattr(cfg, "num_attention_heads", None) or cfg.n_head
+        hidden = getattr(cfg, "hidden_size", None) or cfg.n_embd
+        layers = getattr(cfg, "num_hidden_layers", None) or cfg.n_layer
+        kv_heads = getattr(cfg, "num_key_value_heads", None) or heads
+        head_dim = getattr(cfg, "head_dim", None) or hidden // heads
+        return cls(layers, num_blocks, block_size, kv_heads, head_dim, device or next(model.parameters()).device)
+
+    @property
+    def num_slots(self) -> int:
+        return self.num_blocks * self.block_size
+
+    @property
+    def nbytes(self) -> int:
+        return sum(t.numel() for t in self.k + self.v + self.k_scale + self.v_scale)
+
+    # ------------------------------------------------------------ block moves
+    def _bytes(self):
+        """The pools as byte tensors: payload lists, scale lists ``[blocks, 1, Hkv, BS]``."""
+        u8 = torch.uint8
+        return ([t.view(u8) for t in self.k], [t.view(u8) for t in self.v],
+                [t.unsqueeze(1) for t in self.k_scale], [t.unsqueeze(1) for t in self.v_scale])
+
+    def _err(self) -> torch.Tensor:
+        if getattr(self, "_err_word", None) is None:
+            self._err_word = _error_word(self.k[0].device)
+        return self._err_word
+
+    def read_error(self, clear: bool = True) -> int:
+        """Error bits block moves reported since the last clear (1 = a bad block id).
+        Synchronises the device."""
+        word = int(self._err().item())
+        if clear and word:
+            self._err().zero_()
+        return word
+
+    def copy_blocks(self, pairs) -> None:
+        """Copy-on-write moves ``pool[dst] = pool[src]`` for every layer, payload and scales."""
+        k, v, ks, vs = self._bytes()
+        pairs = list(pairs)
+        copy_blocks(k, v, pairs, self._err())
+        copy_blocks(ks, vs, pairs, self._err())
+
+    def _block_bytes(self) -> tuple[int, int]:
+        n = self.block_size * self.num_kv_heads
+        return n * self.head_dim, n
+
+    def swap_out(self, blocks) -> HostBlocks:
+        """Copy the named blocks of every layer to pinned host memory: ``k`` / ``v`` are byte
+        views per layer, ``flat`` holds [payload | scales], each [layer][K, V][n][block]."""
+        n, layers = len(blocks), len(self.k)
+        pb, sb = self._block_bytes()
+        split = layers * 2 * n * pb
+        flat = torch.empty(split + layers * 2 * n * sb, dtype=torch.uint8, pin_memory=True)
+        if n:
+            stage = torch.empty(flat.numel(), dtype=torch.uint8, device=self.k[0].device)
+            k, v, ks, vs = self._bytes()
+            gather_blocks(k, v, blocks, stage[:split], self._err())
+            gather_blocks(ks, vs, blocks, stage[split:], self._err())
+            flat.copy_(stage)
+            if self.read_error():
+                raise RuntimeError("swap_out: the gather kernel met a block id outside the pool")
+        view = flat[:split].view(layers, 2, n, self.block_size, self.num_kv_heads, self.head_dim)
+        return HostBlocks(k=[view[l, 0] for l in range(layers)], v=[view[l, 1] for l in range(layers)], flat=flat)
+
+    def swap_in(self, host: HostBlocks, blocks) -> None:
+        """Copy a host copy made by :meth:`swap_out` back into ``blocks``, which need not be the
+        ones it left."""
+        if len(blocks) != len(host):
+            raise ValueError(f"swap_in: {len(host)} host blocks into {len(blocks)} device blocks")
+        n, layers = len(blocks), len(self.k)
+        if n == 0:
+            return
+        pb, sb = self._block_bytes()
+        split = layers * 2 * n * pb
+        if host.flat is None or host.flat.dtype != torch.uint8 or host.flat.numel() != split + layers * 2 * n * sb:
+            raise ValueError("swap_in: the host copy was not made by a KV8Pool of this shape")
+        stage = host.flat.to(self.k[0].device, non_blocking=True)
+        k, v, ks, vs = self._bytes()
+        scatter_blocks(k, v, blocks, stage[:split], self._err())
+        scatter_blocks(ks, vs, blocks, stage[split:], self._err())
