@@ -127,17 +127,20 @@ int32_t pa_kv8_append(const void* key, int64_t k_stride_token, int64_t k_stride_
                       int32_t head_dim, int32_t dtype, void* k_pool, void* v_pool, void* k_scale, void* v_scale,
                       int64_t pool_num_blocks, int32_t block_size, const int32_t* slot_mapping, void* stream);
 
-/* Bytes of scratch that pa_kv8_attention needs for these shapes, whatever the lengths.
+/* Bytes of scratch that pa_kv8_attention needs for these sizes, whatever the lengths.
  * No reference counterpart. */
-uint64_t pa_kv8_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_query_len);
+uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t max_query_len);
 
 /*
  * Causal attention of each sequence's new tokens over the 8-bit pools: token t of sequence
  * i stands at p = context_lens[i] - query_lens[i] + t and attends to keys 0 .. p through
  * the block table (the rule of inference_server/core/attention.py:19-58).  Lengths and
  * tables stay on the device; the launches depend on the host's sizes only, so a captured
- * call can be replayed with other lengths.  context_lens, cu_query_lens and work come from
- * pa_kv8_build_step with the tiling of the same group and max_query_len.  Rows past the
+ * call can be replayed with other lengths.  cu_query_lens and work come from
+ * pa_kv8_build_step with the tiling of the same group and max_query_len; with both NULL
+ * the call sums query_lens and the work up in its workspace first (one more launch), with
+ * pa_kv8_build_step's checks.  table_width blocks of a table row are used.  Rows past the
  * last sequence's are left as they were.  head_dim 64 or 128, block_size a power of two
  * times 16, query fp16 or bf16 (strides in elements, multiples of 8; rows 16-byte aligned).
  */
@@ -145,9 +148,10 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
                          int32_t num_heads, int32_t head_dim, const void* k_pool, const void* v_pool,
                          const void* k_scale, const void* v_scale, int64_t pool_num_blocks, int32_t block_size,
                          int32_t num_kv_heads, int32_t dtype, float scale, int32_t num_seqs, int32_t max_query_len,
-                         const int32_t* block_tables, int64_t table_stride, const int32_t* context_lens,
-                         const int32_t* cu_query_lens, const int64_t* work, void* out, int64_t out_stride_token,
-                         int64_t out_stride_head, void* workspace, uint64_t workspace_bytes, void* stream);
+                         const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                         const int32_t* context_lens, const int32_t* query_lens, const int32_t* cu_query_lens,
+                         const int64_t* work, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                         void* workspace, uint64_t workspace_bytes, void* stream);
 
 /* Read (and, with `clear`, reset) the current device's KV8 error word.  Synchronises the
  * stream.  No reference counterpart. */

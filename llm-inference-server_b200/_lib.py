@@ -144,11 +144,11 @@ _SIGNATURES = {
     "pa_kv8_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
                                 c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p,
                                 c_void_p]),
-    "pa_kv8_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32]),
+    "pa_kv8_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
     "pa_kv8_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_int64, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
-                                   c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
-                                   c_uint64, c_void_p]),
+                                   c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                   c_int64, c_void_p, c_uint64, c_void_p]),
     "pa_kv8_read_error": (c_int32, [c_int32, POINTER(c_int32), c_void_p]),
 }
 

@@ -32,9 +32,11 @@ static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, in
 }
 
 static int sm_count() {
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
+  static int known[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!known[dev] && cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+  return known[dev];
 }
 
 static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -43,16 +45,37 @@ static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 1
 constexpr int kMaxSms = 160;
 
 struct Kv8Scratch {
-  uint64_t ml, o, bytes;
+  uint64_t work, cu, ml, o, bytes;
 };
-static Kv8Scratch rows_scratch(const pa_kv8_tiling& t, int32_t num_kv_heads, int32_t head_dim, int sms) {
+static Kv8Scratch attention_scratch(const pa_kv8_tiling& t, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim,
+                                    int sms) {
   const uint64_t rows =
       uint64_t(kv8_rows_slices(t.row_groups, num_kv_heads, sms)) * num_kv_heads * 2 * (8 * t.row_groups);
   Kv8Scratch s;
-  s.ml = 0;
-  s.o = (rows * sizeof(float2) + 255) / 256 * 256;
+  s.work = 0;
+  s.cu = (uint64_t(num_seqs) + 1) * 2 * sizeof(int64_t);
+  s.ml = (s.cu + (uint64_t(num_seqs) + 1) * sizeof(int32_t) + 255) / 256 * 256;
+  s.o = (s.ml + rows * sizeof(float2) + 255) / 256 * 256;
   s.bytes = s.o + rows * head_dim * sizeof(float);
   return s;
+}
+
+static int32_t check_step_sizes(const Kv8StepParams& p, int64_t table_stride) {
+  if (p.tiling.small_tokens < 1 || p.tiling.large_tokens < 1) return fail(PA_ERR_INVALID_ARGUMENT, "build_step: bad tiling");
+  if (p.num_rows < 0 || p.num_slots < 0 || p.width < 0 || p.block_size <= 0 || p.num_tokens < 0 ||
+      p.max_query_len < 0 || p.free_capacity < 0 || table_stride < p.width)
+    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: bad sizes");
+  if (p.num_rows > PA_KV8_MAX_ROWS)
+    return fail(PA_ERR_UNSUPPORTED, "build_step: %d rows, at most %d are supported", p.num_rows, PA_KV8_MAX_ROWS);
+  if (p.num_slots > PA_KV8_MAX_REQUESTS)
+    return fail(PA_ERR_UNSUPPORTED, "build_step: %d request slots, at most %d are supported", p.num_slots,
+                PA_KV8_MAX_REQUESTS);
+  if (p.max_query_len > (1 << 20) || p.width > (1 << 20) || int64_t(p.width) * p.block_size > (int64_t(1) << 30))
+    return fail(PA_ERR_UNSUPPORTED, "build_step: chunks up to 2^20 tokens and contexts up to 2^30 are supported");
+  if (p.pool_blocks < 0 || p.pool_blocks * int64_t(p.block_size) > (int64_t(1) << 31) - 1)
+    return fail(PA_ERR_UNSUPPORTED, "pool has more than 2^31 slots");
+  if (!p.row_ids && p.num_rows > p.num_slots) return fail(PA_ERR_INVALID_ARGUMENT, "build_step: more rows than slots");
+  return PA_OK;
 }
 
 }  // namespace pa
@@ -81,28 +104,7 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
                           int32_t* seq_idx, int32_t* q_pos, int32_t* slot_mapping, int32_t* num_free_out,
                           int64_t* work, void* stream_ptr) {
   using namespace pa;
-  if (!tiling || tiling->small_tokens < 1 || tiling->large_tokens < 1)
-    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: bad tiling");
-  if (num_rows < 0 || num_slots < 0 || width < 0 || block_size <= 0 || num_tokens < 0 || max_query_len < 0 ||
-      free_capacity < 0 || table_stride < width)
-    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: bad sizes");
-  if (num_rows > PA_KV8_MAX_ROWS)
-    return fail(PA_ERR_UNSUPPORTED, "build_step: %d rows, at most %d are supported", num_rows, PA_KV8_MAX_ROWS);
-  if (num_slots > PA_KV8_MAX_REQUESTS)
-    return fail(PA_ERR_UNSUPPORTED, "build_step: %d request slots, at most %d are supported", num_slots,
-                PA_KV8_MAX_REQUESTS);
-  if (max_query_len > (1 << 20) || width > (1 << 20) || int64_t(width) * block_size > (int64_t(1) << 30))
-    return fail(PA_ERR_UNSUPPORTED, "build_step: chunks up to 2^20 tokens and contexts up to 2^30 are supported");
-  if (pool_num_blocks < 0 || pool_num_blocks * int64_t(block_size) > (int64_t(1) << 31) - 1)
-    return fail(PA_ERR_UNSUPPORTED, "pool has more than 2^31 slots");
-  if (!row_ids && num_rows > num_slots) return fail(PA_ERR_INVALID_ARGUMENT, "build_step: more rows than slots");
-  if ((num_rows > 0 && (!lens || !query_lens || !context_lens || !query_lens_out || !held_out)) || !cu_query_lens ||
-      !num_free_out || !work || (num_tokens > 0 && (!seq_idx || !q_pos || !slot_mapping)) ||
-      (num_rows > 0 && width > 0 && !tables) ||
-      (held && (!num_free || (free_capacity > 0 && !free_blocks) || (num_rows > 0 && width > 0 && !out_tables))))
-    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: NULL device pointer");
-  int* err = kv8_error_word();
-  if (!err) return fail(PA_ERR_CUDA, "build_step: no CUDA device");
+  if (!tiling) return fail(PA_ERR_INVALID_ARGUMENT, "build_step: bad tiling");
   Kv8StepParams p{};
   p.row_ids = row_ids;
   p.lens = lens;
@@ -131,6 +133,15 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
   p.slots = slot_mapping;
   p.num_free_out = num_free_out;
   p.work = work;
+  const int32_t st = check_step_sizes(p, table_stride);
+  if (st != PA_OK) return st;
+  if ((num_rows > 0 && (!lens || !query_lens || !context_lens || !query_lens_out || !held_out)) || !cu_query_lens ||
+      !num_free_out || !work || (num_tokens > 0 && (!seq_idx || !q_pos || !slot_mapping)) ||
+      (num_rows > 0 && width > 0 && !tables) ||
+      (held && (!num_free || (free_capacity > 0 && !free_blocks) || (num_rows > 0 && width > 0 && !out_tables))))
+    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: NULL device pointer");
+  int* err = kv8_error_word();
+  if (!err) return fail(PA_ERR_CUDA, "build_step: no CUDA device");
   cudaError_t e = launch_kv8_step(p, err, static_cast<cudaStream_t>(stream_ptr));
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "build_step launch");
 }
@@ -180,8 +191,10 @@ int32_t pa_kv8_append(const void* key, int64_t k_stride_token, int64_t k_stride_
   if (num_tokens == 0) return PA_OK;
   if (!key || !value || !k_pool || !v_pool || !k_scale || !v_scale || !slot_mapping)
     return fail(PA_ERR_INVALID_ARGUMENT, "NULL device pointer");
-  if (reinterpret_cast<uintptr_t>(k_pool) % 8 || reinterpret_cast<uintptr_t>(v_pool) % 8)
-    return fail(PA_ERR_INVALID_ARGUMENT, "8-bit pools must be 8-byte aligned");
+  if (!aligned16(k_pool) || !aligned16(v_pool))
+    return fail(PA_ERR_INVALID_ARGUMENT, "8-bit pools must be 16-byte aligned");
+  if (int64_t(num_tokens) * num_kv_heads > (int64_t(1) << 31) - 1)
+    return fail(PA_ERR_UNSUPPORTED, "append of more than 2^31 rows");
   const int64_t es = dtype == PA_DTYPE_F32 ? 4 : 2;
   Kv8AppendParams p{};
   p.key = key;
@@ -206,22 +219,24 @@ int32_t pa_kv8_append(const void* key, int64_t k_stride_token, int64_t k_stride_
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "8-bit append launch");
 }
 
-uint64_t pa_kv8_workspace_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t max_query_len) {
+uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                int32_t max_query_len) {
   using namespace pa;
   pa_kv8_tiling t;
-  if (num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_heads % num_kv_heads ||
+  if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_heads % num_kv_heads ||
       pa_kv8_choose_tiling(num_heads / num_kv_heads, max_query_len, &t) != PA_OK)
     return 0;
-  return rows_scratch(t, num_kv_heads, head_dim, kMaxSms).bytes;
+  return attention_scratch(t, num_seqs, num_kv_heads, head_dim, kMaxSms).bytes;
 }
 
 int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t num_tokens,
                          int32_t num_heads, int32_t head_dim, const void* k_pool, const void* v_pool,
                          const void* k_scale, const void* v_scale, int64_t pool_num_blocks, int32_t block_size,
                          int32_t num_kv_heads, int32_t dtype, float scale, int32_t num_seqs, int32_t max_query_len,
-                         const int32_t* block_tables, int64_t table_stride, const int32_t* context_lens,
-                         const int32_t* cu_query_lens, const int64_t* work, void* out, int64_t out_stride_token,
-                         int64_t out_stride_head, void* workspace, uint64_t workspace_bytes, void* stream_ptr) {
+                         const int32_t* block_tables, int64_t table_stride, int32_t table_width,
+                         const int32_t* context_lens, const int32_t* query_lens, const int32_t* cu_query_lens,
+                         const int64_t* work, void* out, int64_t out_stride_token, int64_t out_stride_head,
+                         void* workspace, uint64_t workspace_bytes, void* stream_ptr) {
   using namespace pa;
   reset_last_launches();
   if (dtype != PA_DTYPE_F16 && dtype != PA_DTYPE_BF16)
@@ -240,11 +255,12 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     return fail(PA_ERR_UNSUPPORTED, "pool has more than 2^31 slots");
   pa_kv8_tiling t;
   const int group = num_heads / num_kv_heads;
-  const int32_t rc = pa_kv8_choose_tiling(group, max_query_len, &t);
-  if (rc != PA_OK) return rc;
+  int32_t st = pa_kv8_choose_tiling(group, max_query_len, &t);
+  if (st != PA_OK) return st;
   if (num_tokens == 0 || num_seqs == 0 || pool_num_blocks == 0) return PA_OK;
-  if (!query || !k_pool || !v_pool || !k_scale || !v_scale || !block_tables || !context_lens || !cu_query_lens ||
-      !work || !out || !workspace)
+  const bool build = !work && !cu_query_lens;
+  if (!query || !k_pool || !v_pool || !k_scale || !v_scale || !block_tables || !context_lens || !out || !workspace ||
+      (build ? !query_lens : (!cu_query_lens || !work)))
     return fail(PA_ERR_INVALID_ARGUMENT, "NULL device pointer");
   if (!aligned16(query) || q_stride_token % 8 || q_stride_head % 8 || !aligned16(out) || out_stride_token % 8 ||
       out_stride_head % 8)
@@ -252,7 +268,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_scale) || !aligned16(v_scale))
     return fail(PA_ERR_INVALID_ARGUMENT, "8-bit pools and their scales must be 16-byte aligned");
   const int sms = std::min(sm_count(), kMaxSms);
-  const Kv8Scratch s = rows_scratch(t, num_kv_heads, head_dim, sms);
+  const Kv8Scratch s = attention_scratch(t, num_seqs, num_kv_heads, head_dim, sms);
   if (workspace_bytes < s.bytes)
     return fail(PA_ERR_BUFFER_TOO_SMALL, "workspace holds %llu bytes, %llu needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
@@ -260,8 +276,30 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     return fail(PA_ERR_INVALID_ARGUMENT, "workspace must be 256-byte aligned");
   int* err = kv8_error_word();
   if (!err) return fail(PA_ERR_CUDA, "no CUDA device");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (build) {
+    Kv8StepParams b{};
+    b.lens = context_lens;
+    b.query_lens = query_lens;
+    b.num_rows = b.num_slots = num_seqs;
+    b.width = table_width;
+    b.block_size = block_size;
+    b.num_tokens = num_tokens;
+    b.max_query_len = max_query_len;
+    b.pool_blocks = pool_num_blocks;
+    b.tiling = t;
+    b.cu_query = reinterpret_cast<int32_t*>(ws + s.cu);
+    b.work = reinterpret_cast<int64_t*>(ws + s.work);
+    st = check_step_sizes(b, table_stride);
+    if (st != PA_OK) return st;
+    const cudaError_t eb = launch_kv8_step(b, err, stream);
+    if (eb != cudaSuccess) return kv8_cuda_fail(eb, "8-bit attention's step launch");
+    cu_query_lens = b.cu_query;
+    work = b.work;
+  }
   CUtensorMap tk, tv;
-  int32_t st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, 16, &tk);
+  st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, 16, &tk);
   if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, 16, &tv);
   if (st != PA_OK) return st;
   Kv8AttnParams p{};
@@ -289,9 +327,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.slices = kv8_rows_slices(t.row_groups, num_kv_heads, sms);
   p.pool_blocks = int32_t(pool_num_blocks);
   p.qscale = scale * kLog2e;
-  p.part_ml = reinterpret_cast<float2*>(static_cast<uint8_t*>(workspace) + s.ml);
-  p.part_o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + s.o);
-  cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  p.part_ml = reinterpret_cast<float2*>(ws + s.ml);
+  p.part_o = reinterpret_cast<float*>(ws + s.o);
   cudaError_t e = launch_kv8_rows(dtype, head_dim, t.row_groups, tk, tv, p, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
   note_launches(PA_LAUNCH_KV8_ROWS | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));

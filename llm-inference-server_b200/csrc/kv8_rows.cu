@@ -17,7 +17,9 @@
 // four consumer warps, which take blocks of 16 keys in turn, and a producer warp, which
 // walks the slice's pieces, reads the block table and keeps each consumer's ring full: the
 // rings run across pieces, so a new sequence costs no drain.  Per block: K and V tile by TMA
-// (a 16-row box), the 16 + 16 scale bytes by bulk copies.
+// (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round of 32
+// blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the tiles:
+// 177 us for 64 sequences of about 4,096 keys, 8 heads of 128).
 //
 // Widening costs one conversion per two elements and the transpose of V one byte permute per
 // four: with 16-byte chunks of head_dim dealt out to the MMA's k index as ldmatrix delivers
@@ -64,12 +66,6 @@ struct RowsPiece {      // part of a tile that a CTA works on
   int32_t pad;
 };
 
-__device__ __forceinline__ void bulk_copy16(void* dst, const void* src, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(smem_u32(bar))
-               : "memory");
-}
 __device__ __forceinline__ void rows_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
@@ -176,6 +172,27 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
     for (int w = 0; w < kRowsWarps; ++w) issued[w] = 0;
     int pieces = 0, hint = 0;
     bool ok = true;
+    struct BlockRef {
+      int slot;  // first slot of the 16 keys
+      uint4 ks, vs;
+    };
+    auto look_up = [&](const int32_t* row, int kb, int end) {
+      BlockRef r;
+      r.slot = 0;
+      if (kb < end) {
+        int id = row[kb >> p.block_shift];
+        if (id < 0 || id >= p.pool_blocks) {
+          set_error(err, PA_KV8_ERR_BLOCK);
+          id = 0;
+        }
+        const int sub = (kb & ((1 << p.block_shift) - 1)) * 16;
+        const int64_t at = ((int64_t(id) * p.num_kv_heads + kvh) << (p.block_shift + 4)) + sub;
+        r.slot = (id << (p.block_shift + 4)) + sub;
+        r.ks = __ldg(reinterpret_cast<const uint4*>(p.k_scale + at));
+        r.vs = __ldg(reinterpret_cast<const uint4*>(p.v_scale + at));
+      }
+      return r;
+    };
     while (ok) {
       LineTile t;
       t.seq = -1;
@@ -220,44 +237,35 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
       ++pieces;
       if (t.seq < 0) break;
       const int32_t* row = p.tables + int64_t(t.seq) * p.table_stride;
+      // Each lane looks up one of the next 32 blocks and reads its scales, one round ahead of
+      // the round whose tiles are being issued, and then issues its own block in turn.
+      BlockRef cur = look_up(row, kb0 + lane, kb1), nxt;
       for (int kb = kb0; kb < kb1 && ok; kb += 32) {
-        const int mine = kb + lane;
-        int id = 0;
-        if (mine < kb1) {
-          id = row[mine >> p.block_shift];
-          if (id < 0 || id >= p.pool_blocks) {
-            set_error(err, PA_KV8_ERR_BLOCK);
-            id = 0;
-          }
-        }
+        if (kb + 32 < kb1) nxt = look_up(row, kb + 32 + lane, kb1);
         const int n = min(32, kb1 - kb);
         for (int j = 0; j < n && ok; j += kRowsWarps) {
 #pragma unroll
           for (int w = 0; w < kRowsWarps; ++w) {
-            const int phys = __shfl_sync(0xffffffffu, id, (j + w) & 31);
-            if (j + w < n && ok) {
+            if (j + w < n) {
               const int st = issued[w] % C::STAGES;
-              uint64_t* bar = &full[w * C::STAGES + st];
               if (issued[w] >= C::STAGES)
-                ok = mbar_wait(&empty[w * C::STAGES + st], ((issued[w] / C::STAGES) - 1) & 1);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              if (lane == 0) {
-                const int sub = (kb + j + w) & ((1 << p.block_shift) - 1);
-                const int64_t at = ((int64_t(phys) * p.num_kv_heads + kvh) << (p.block_shift + 4)) + sub * 16;
-                const int coord = (phys << (p.block_shift + 4)) + sub * 16;
+                ok = mbar_wait(&empty[w * C::STAGES + st], ((issued[w] / C::STAGES) - 1) & 1) && ok;
+              if (ok && lane == j + w) {
+                uint64_t* bar = &full[w * C::STAGES + st];
                 uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE;
-                uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * 32;
-                mbar_arrive_expect_tx(bar, C::STAGE + 32);
-                tma_load_3d(stage, &tk, 0, kvh, coord, bar);
-                bulk_copy16(sc, p.k_scale + at, bar);
-                tma_load_3d(stage + C::TILE, &tv, 0, kvh, coord, bar);
-                bulk_copy16(sc + 16, p.v_scale + at, bar);
+                uint4* sc = reinterpret_cast<uint4*>(smem + C::OFF_SCALE + (w * C::STAGES + st) * 32);
+                sc[0] = cur.ks;
+                sc[1] = cur.vs;
+                mbar_arrive_expect_tx(bar, C::STAGE);  // releases the scales too
+                tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
+                tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
               }
-              ++issued[w];
+              if (ok) ++issued[w];
             }
           }
         }
+        ok = __all_sync(0xffffffffu, ok);
+        cur = nxt;
       }
     }
     if (!ok) {
@@ -306,15 +314,13 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
       limit[rr] = valid ? d.pos0 + tok : -1;
       const T* src = static_cast<const T*>(p.q) + int64_t(d.row0 + (valid ? tok : 0)) * p.q_st +
                      int64_t(kvh * p.group + head) * p.q_sh + 4 * tig;
-      float x[CH][4], big = 0.f;
+      // Two passes over the row (the second from L1) rather than a row in registers.
+      float big = 0.f;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
-        if (valid) VecLoad<T, 4>::run(src + 16 * c, x[c]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (!valid) x[c][e] = 0.f;
-          big = fmaxf(big, fabsf(x[c][e]));
-        }
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (valid) VecLoad<T, 4>::run(src + 16 * c, x);
+        big = fmaxf(fmaxf(fmaxf(big, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
@@ -323,8 +329,10 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         // fragment order {row g: k 2i..2i+1, (row g + 8: same), row g: k 2i+8.., (row g + 8)}
-        qa[c][0 * RG + rr] = pack2<__half>(x[c][0] * up, x[c][1] * up);
-        qa[c][1 * RG + rr] = pack2<__half>(x[c][2] * up, x[c][3] * up);
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        if (valid) VecLoad<T, 4>::run(src + 16 * c, x);
+        qa[c][0 * RG + rr] = pack2<__half>(x[0] * up, x[1] * up);
+        qa[c][1 * RG + rr] = pack2<__half>(x[2] * up, x[3] * up);
       }
     }
 
@@ -546,30 +554,49 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
   while (last + 1 < slices && line_cut(total, slices, last + 1) < end) ++last;
 
   // A slice's part of the tile is its slot 1 if it starts the tile, else slot 0; it is empty
-  // where both of its cuts move up to the same key.
-  auto part = [&](int i) { return ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r; };
-  auto some = [&](int i) {
-    return line_key(t, line_cut(total, slices, i + 1), key_step) > line_key(t, line_cut(total, slices, i), key_step);
-  };
-  float m = -INFINITY;
-  for (int i = s - 1 + lane; i <= last; i += 32)
-    if (some(i)) m = fmaxf(m, p.part_ml[part(i)].x);
-#pragma unroll
-  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-  if (m == -INFINITY) m = 0.f;
-  float acc[E], sum = 0.f;
+  // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time; the
+  // parts' accumulators are then read with nothing between the loads.
+  float acc[E], m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 8
-  for (int i = s - 1; i <= last; ++i) {
-    if (!some(i)) continue;
-    const float2 v = p.part_ml[part(i)];
-    const float f = ex2(v.x - m);
-    sum += v.y * f;
-    float o[E];
-    VecLoad<float, E>::run(p.part_o + part(i) * D + E * lane, o);
+  for (int i0 = s - 1; i0 <= last; i0 += 32) {
+    const int i = i0 + lane;
+    float2 v = make_float2(-INFINITY, 0.f);
+    int64_t at = 0;
+    if (i <= last &&
+        line_key(t, line_cut(total, slices, i + 1), key_step) > line_key(t, line_cut(total, slices, i), key_step)) {
+      at = ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r;
+      v = p.part_ml[at];
+    }
+    float mn = v.x;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] += o[e] * f;
+    for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+    mn = fmaxf(mn, m);
+    const float ref = mn == -INFINITY ? 0.f : mn, old = ex2(m - ref), f = ex2(v.x - ref);
+    m = mn;
+    float part = v.y * f;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+    sum = sum * old + part;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= old;
+    const int n = min(32, last + 1 - i0);
+    for (int k0 = 0; k0 < n; k0 += 8) {
+      float o[8][E], fk[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        fk[k] = __shfl_sync(0xffffffffu, f, k0 + k);
+        const int64_t ak = __shfl_sync(0xffffffffu, at, k0 + k);
+        const bool some = __shfl_sync(0xffffffffu, v.x, k0 + k) != -INFINITY;  // NaN counts
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[k][e] = 0.f;
+        if (some) VecLoad<float, E>::run(p.part_o + ak * D + E * lane, o[k]);
+      }
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += o[k][e] * fk[k];
+    }
   }
   T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
   const float inv = 1.f / sum;
@@ -584,10 +611,17 @@ static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const 
                             cudaStream_t stream) {
   using C = RowsCfg<D, RG>;
   auto kern = kv8_rows_kernel<T, D, RG>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  if (e != cudaSuccess) return e;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-  if (e != cudaSuccess) return e;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool configured[64] = {};
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
   kern<<<p.slices * p.num_kv_heads, kRowsThreads, C::SMEM, stream>>>(tk, tv, p, err);
   return cudaGetLastError();
 }

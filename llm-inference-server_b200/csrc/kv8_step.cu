@@ -19,27 +19,39 @@ namespace pa {
 
 constexpr int kStepThreads = 512;
 
-// Sums over the block: v becomes the sum of the threads' v before this one; returns the
-// total.  `scratch` holds one value per warp.
-template <typename V>
-__device__ __forceinline__ V block_scan(V& v, V* scratch) {
+// Sums over the block: each of v[N] becomes the sum of the threads' before this one; `total`
+// gets the sums over all.  `scratch` holds N values per warp; one pair of barriers for all N.
+template <int N>
+__device__ __forceinline__ void block_scan(int64_t (&v)[N], int64_t (&total)[N], int64_t (*scratch)[N]) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  V sum = v;
+  int64_t sum[N];
 #pragma unroll
-  for (int d = 1; d < 32; d <<= 1) {
-    const V up = __shfl_up_sync(0xffffffffu, sum, d);
-    if (lane >= d) sum += up;
-  }
-  if (lane == 31) scratch[warp] = sum;
+  for (int n = 0; n < N; ++n) sum[n] = v[n];
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1)
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, sum[n], d);
+      if (lane >= d) sum[n] += up;
+    }
+  if (lane == 31)
+#pragma unroll
+    for (int n = 0; n < N; ++n) scratch[warp][n] = sum[n];
   __syncthreads();
-  V before = 0, total = 0;
-  for (int w = 0; w < warps; ++w) {
-    if (w == warp) before = total;
-    total += scratch[w];
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    // One warp's worth of partial sums (at most 16 warps), added up by every warp.
+    int64_t w = lane < warps ? scratch[lane][n] : 0;
+#pragma unroll
+    for (int d = 1; d < 16; d <<= 1) {
+      const int64_t up = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += up;
+    }
+    total[n] = __shfl_sync(0xffffffffu, w, warps - 1);
+    const int64_t before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+    v[n] = (warp > 0 ? before : 0) + sum[n] - v[n];
   }
   __syncthreads();
-  v = before + sum - v;
-  return total;
 }
 
 __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepParams p, int* err) {
@@ -51,13 +63,14 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
   int32_t* s_held = s_new + rows;     // [rows]
   int32_t* s_row = s_held + rows;     // [rows] request slot or -1
   uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_row + rows);  // a bit per slot, with row_ids only
-  __shared__ int32_t scan32[kStepThreads / 32];
-  __shared__ int64_t scan64[kStepThreads / 32];
+  __shared__ int64_t scan[kStepThreads / 32][4];
   const int tid = threadIdx.x;
 
-  if (p.row_ids)
+  if (p.row_ids) {
     for (int i = tid; i < (p.num_slots + 31) / 32; i += blockDim.x) s_seen[i] = 0u;
-  __syncthreads();
+    __syncthreads();
+  }
+  const int avail = p.held ? *p.num_free : 0;
 
   int bad = 0;
   int64_t tokens = 0, blocks = 0, small = 0, large = 0;  // totals so far
@@ -89,33 +102,26 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
       s_held[i] = held;
       s_row[i] = row;
     }
-    int at = q, nb = need;
-    const int step_tokens = block_scan(at, scan32);
-    const int step_blocks = block_scan(nb, scan32);
+    const bool few = q <= p.tiling.small_max;
+    const int tt = few ? p.tiling.small_tokens : p.tiling.large_tokens;
+    const int64_t keys = q > 0 ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
+    int64_t v[4] = {q, need, few ? keys : 0, few ? 0 : keys}, total[4];
+    block_scan(v, total, scan);
     if (i < rows) {
-      s_cu[i] = int32_t(tokens + at);
-      s_new[i] = int32_t(blocks + nb);
-    }
-    tokens += step_tokens;
-    blocks += step_blocks;
-    if (tokens > p.num_tokens) bad |= PA_KV8_ERR_STEP;  // sums of one round stay below 2^31: see the host's checks
-    if (blockIdx.x == 0) {
-      const bool few = q <= p.tiling.small_max;
-      const int tt = few ? p.tiling.small_tokens : p.tiling.large_tokens;
-      const int64_t keys = q > 0 ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
-      int64_t ws = few ? keys : 0, wl = few ? 0 : keys;
-      const int64_t ts = block_scan(ws, scan64), tl = block_scan(wl, scan64);
-      if (i < rows) {
-        p.work[i] = small + ws;
-        p.work[rows + 1 + i] = large + wl;
+      s_cu[i] = int32_t(tokens + v[0]);
+      s_new[i] = int32_t(blocks + v[1]);
+      if (blockIdx.x == 0) {
+        p.work[i] = small + v[2];
+        p.work[rows + 1 + i] = large + v[3];
       }
-      small += ts;
-      large += tl;
     }
+    tokens += total[0];
+    blocks += total[1];
+    small += total[2];
+    large += total[3];
+    if (tokens > p.num_tokens) bad |= PA_KV8_ERR_STEP;
   }
-  int avail = 0;
   if (p.held) {
-    avail = *p.num_free;
     if (avail < 0 || avail > p.free_capacity)
       bad |= PA_KV8_ERR_STEP;
     else if (blocks > avail)
@@ -130,9 +136,11 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
       if (reject) p.work[i] = p.work[rows + 1 + i] = 0;
       if (i < rows) {
         const int need = (i + 1 < rows ? s_new[i + 1] : int32_t(blocks)) - s_new[i];
-        p.context_lens[i] = reject ? 0 : s_ctx[i];
-        p.query_out[i] = reject ? 0 : s_cu[i + 1] - s_cu[i];
-        p.held_out[i] = reject ? 0 : s_held[i] + need;
+        if (p.context_lens) {
+          p.context_lens[i] = reject ? 0 : s_ctx[i];
+          p.query_out[i] = reject ? 0 : s_cu[i + 1] - s_cu[i];
+          p.held_out[i] = reject ? 0 : s_held[i] + need;
+        }
       }
     }
     if (tid == 0) {
@@ -140,7 +148,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
         p.work[rows] = small;
         p.work[2 * rows + 1] = large;
       }
-      *p.num_free_out = reject ? -1 : avail - int32_t(blocks);
+      if (p.num_free_out) *p.num_free_out = reject ? -1 : avail - int32_t(blocks);
     }
   }
 
@@ -166,6 +174,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
       p.out_tables[c] = id;
     }
   }
+  if (!p.seq_idx) return;
   // Per-token arrays.
   for (int64_t t = me; t < p.num_tokens; t += stride) {
     int seq = -1, pos = -1, slot = -1;
@@ -218,7 +227,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_release_kernel(const int32_t
   extern __shared__ int32_t sm[];
   int32_t* s_at = sm;            // [count + 1] blocks before the id
   uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_at + count + 1);
-  __shared__ int32_t scan32[kStepThreads / 32];
+  __shared__ int64_t scan[kStepThreads / 32][1];
   const int tid = threadIdx.x;
   for (int i = tid; i < (slots + 31) / 32; i += blockDim.x) s_seen[i] = 0u;
   __syncthreads();
@@ -240,10 +249,10 @@ __global__ void __launch_bounds__(kStepThreads) kv8_release_kernel(const int32_t
         }
       }
     }
-    int at = n;
-    const int sum = block_scan(at, scan32);
-    if (i < count) s_at[i] = int32_t(blocks + at);
-    blocks += sum;
+    int64_t at[1] = {n}, sum[1];
+    block_scan(at, sum, scan);
+    if (i < count) s_at[i] = int32_t(blocks + at[0]);
+    blocks += sum[0];
   }
   const int have = *num_free;
   if (have < 0 || have + blocks > free_capacity) bad = 1;
@@ -272,8 +281,15 @@ __global__ void __launch_bounds__(kStepThreads) kv8_release_kernel(const int32_t
 static __device__ int g_kv8_error;
 
 int* kv8_error_word() {
-  void* at = nullptr;
-  return cudaGetSymbolAddress(&at, g_kv8_error) == cudaSuccess ? static_cast<int*>(at) : nullptr;
+  static int* known[64] = {};  // a device's word stays where it is
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+  if (!known[dev]) {
+    void* at = nullptr;
+    if (cudaGetSymbolAddress(&at, g_kv8_error) != cudaSuccess) return nullptr;
+    known[dev] = static_cast<int*>(at);
+  }
+  return known[dev];
 }
 
 static cudaError_t allow_smem(const void* kern, size_t bytes) {
@@ -286,10 +302,12 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
                       (p.row_ids ? sizeof(uint32_t) * ((size_t(p.num_slots) + 31) / 32) : 0);
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_step_kernel), smem);
   if (e != cudaSuccess) return e;
-  const int64_t cells = (p.held ? int64_t(p.num_rows) * p.width : 0) + p.num_tokens;
-  const int64_t want = (cells + kStepThreads - 1) / kStepThreads;
+  // As many threads as rows, within limits: a sum over fewer warps is quicker.
+  const int threads = p.num_rows <= 128 ? 128 : kStepThreads;
+  const int64_t cells = (p.held ? int64_t(p.num_rows) * p.width : 0) + (p.seq_idx ? p.num_tokens : 0);
+  const int64_t want = (cells + threads - 1) / threads;
   const int grid = int(want < 1 ? 1 : (want < 148 ? want : 148));
-  kv8_step_kernel<<<grid, kStepThreads, smem, stream>>>(p, err);
+  kv8_step_kernel<<<grid, threads, smem, stream>>>(p, err);
   return cudaGetLastError();
 }
 

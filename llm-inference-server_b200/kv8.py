@@ -32,26 +32,16 @@ from .kv_cache import HostBlocks, _error_word, copy_blocks, gather_blocks, scatt
 _PAYLOAD = torch.float8_e4m3fn
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-class _On:
-    """Make ``device`` current for the library calls inside (they launch there)."""
-
-    __slots__ = ("index", "previous")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self):
-        self.previous = torch.cuda.current_device()
-        if self.index is not None and self.index != self.previous:
-            torch.cuda.set_device(self.index)
-
-    def __exit__(self, *exc):
-        if self.index is not None and self.index != self.previous:
-            torch.cuda.set_device(self.previous)
+def _launch(device: torch.device, fn, *args) -> None:
+    """``fn(*args, stream)`` with ``device`` current and its current stream."""
+    index, current = device.index, torch._C._cuda_getDevice()
+    if index == current:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _lib.check(rc)
 
 
 def _need_cuda(device: torch.device, what: str) -> None:
@@ -60,6 +50,8 @@ def _need_cuda(device: torch.device, what: str) -> None:
 
 
 def _int32(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if t.dtype is torch.int32 and t.device == device and t.is_contiguous():
+        return t
     if t.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
     if t.device != device:
@@ -73,9 +65,11 @@ def read_kv8_error(device=None, clear: bool = True) -> int:
     """The KV8 error word of ``device`` (0: nothing reported; else ``_lib.PA_KV8_ERR_*``
     bits).  Synchronises the current stream."""
     device = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     word = ctypes.c_int32(0)
-    with _On(device):
-        _lib.check(_lib.lib().pa_kv8_read_error(int(clear), ctypes.byref(word), _stream(device)))
+    torch.cuda.init()
+    _launch(device, _lib.lib().pa_kv8_read_error, int(clear), ctypes.byref(word))
     return int(word.value)
 
 
@@ -94,76 +88,52 @@ def _tiling(group: int, max_query_len: int) -> _lib.Kv8Tiling:
     return t
 
 
+# The step's arrays in one int32 buffer: work (int64, so first), context_lens, query_lens,
+# held, cu_query_lens, seq_idx, q_pos, slot_mapping, num_free, block_tables.
+_CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _FREE, _TABLES = range(1, 10)
+
+
 class DeviceStep:
     """One step's metadata on the GPU, shared by every layer: ``block_tables [B, W]``,
     ``context_lens`` / ``query_lens [B]``, ``cu_query_lens [B + 1]``, per token ``seq_idx``,
-    ``q_pos`` and ``slot_mapping [T]`` (-1 past the step's last token), ``num_free [1]`` (the
-    free list's length once the step counts; -1: the step was emptied)."""
+    ``q_pos`` and ``slot_mapping [T]`` (-1 past the step's last token), ``held [B]`` (blocks of
+    each row's slot), ``num_free [1]`` (the free list's length once the step counts; -1: the
+    step was emptied)."""
 
     def __init__(self, num_rows: int, num_tokens: int, width: int, max_query_len: int, block_size: int,
                  num_blocks: int, group: int, device: torch.device, own_tables: bool):
-        self.num_seqs, self.num_tokens, self.width = int(num_rows), int(num_tokens), int(width)
-        self.max_query_len, self.block_size, self.group = int(max_query_len), int(block_size), int(group)
-        self.num_blocks, self.device = int(num_blocks), device
-        b, t = self.num_seqs, self.num_tokens
-        # int64 sums first, then the int32 arrays, each on a 16-byte boundary.
-        sizes = [4 * (b + 1), b, b, b, b + 1, t, t, t, 1, b * self.width if own_tables else 0]
-        self._off = []
-        at = 0
-        for n in sizes:
-            self._off.append(at)
-            at += (n + 3) & ~3
-        self._sizes = sizes
-        self.buffer = torch.empty(at, dtype=torch.int32, device=device)
-        self._base = self.buffer.data_ptr()
+        self.num_seqs, self.num_tokens, self.width, self.max_query_len = num_rows, num_tokens, width, max_query_len
+        self.block_size, self.num_blocks, self.group, self.device = block_size, num_blocks, group, device
+        b, t = num_rows, num_tokens
+        self._sizes = (4 * (b + 1), b, b, b, b + 1, t, t, t, 1, b * width if own_tables else 0)
+        self.buffer = torch.empty(sum(self._sizes), dtype=torch.int32, device=device)
+        at, ptrs = self.buffer.data_ptr(), []
+        for n in self._sizes:
+            ptrs.append(at)
+            at += 4 * n
+        self._ptr = ptrs
+        self._views: tuple[torch.Tensor, ...] | None = None
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
         self._row_ids: torch.Tensor | None = None
 
-    def _ptr(self, i: int) -> int:
-        return self._base + 4 * self._off[i]
-
     def _view(self, i: int) -> torch.Tensor:
-        return self.buffer[self._off[i]:self._off[i] + self._sizes[i]]
+        if self._views is None:
+            self._views = self.buffer.split(self._sizes)
+        return self._views[i]
 
-    @property
-    def work(self) -> torch.Tensor:
-        return self._view(0).view(torch.int64).view(2, self.num_seqs + 1)
-
-    @property
-    def context_lens(self) -> torch.Tensor:
-        return self._view(1)
-
-    @property
-    def query_lens(self) -> torch.Tensor:
-        return self._view(2)
-
-    @property
-    def held(self) -> torch.Tensor:
-        return self._view(3)
-
-    @property
-    def cu_query_lens(self) -> torch.Tensor:
-        return self._view(4)
-
-    @property
-    def seq_idx(self) -> torch.Tensor:
-        return self._view(5)
-
-    @property
-    def q_pos(self) -> torch.Tensor:
-        return self._view(6)
-
-    @property
-    def slot_mapping(self) -> torch.Tensor:
-        return self._view(7)
-
-    @property
-    def num_free(self) -> torch.Tensor:
-        return self._view(8)
+    work = property(lambda self: self._view(0).view(torch.int64).view(2, self.num_seqs + 1))
+    context_lens = property(lambda self: self._view(_CTX))
+    query_lens = property(lambda self: self._view(_QL))
+    held = property(lambda self: self._view(_HELD))
+    cu_query_lens = property(lambda self: self._view(_CU))
+    seq_idx = property(lambda self: self._view(_SEQ))
+    q_pos = property(lambda self: self._view(_POS))
+    slot_mapping = property(lambda self: self._view(_SLOT))
+    num_free = property(lambda self: self._view(_FREE))
 
     @property
     def block_tables(self) -> torch.Tensor:
-        return self._tables if self._tables is not None else self._view(9).view(self.num_seqs, self.width)
+        return self._tables if self._tables is not None else self._view(_TABLES).view(self.num_seqs, self.width)
 
     def matches(self, num_tokens: int, block_size: int, num_blocks: int, group: int) -> bool:
         """Whether this step can drive an attention call of these sizes."""
@@ -176,6 +146,16 @@ def _check_step_sizes(num_tokens: int, max_query_len: int, block_size: int, num_
         raise ValueError("num_tokens and max_query_len must be non-negative")
     if block_size <= 0 or num_blocks < 0:
         raise ValueError("block_size must be positive and the pool's block count non-negative")
+
+
+def _table_rows(tables: torch.Tensor, device: torch.device) -> torch.Tensor:
+    """Block tables as int32 rows of any stride (a slice of a wider table stays in place)."""
+    if tables.device != device:
+        raise ValueError(f"block_tables is on {tables.device}, expected {device}")
+    b, w = tables.shape
+    if tables.dtype is torch.int32 and (w < 2 or tables.stride(1) == 1) and (b < 2 or tables.stride(0) >= w):
+        return tables
+    return _int32("block_tables", tables, device)
 
 
 def _reusable(out: DeviceStep | None, like: tuple, device) -> DeviceStep | None:
@@ -205,23 +185,19 @@ def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_le
     b, w = block_tables.shape
     if tuple(context_lens.shape) != (b,) or tuple(query_lens.shape) != (b,):
         raise ValueError("context_lens and query_lens must be [batch] to match block_tables")
-    tables = block_tables
-    if tables.dtype != torch.int32 or (w and tables.stride(1) != 1) or (b > 1 and tables.stride(0) < w):
-        tables = _int32("block_tables", tables, dev)
+    tables = _table_rows(block_tables, dev)
     ctx, ql = _int32("context_lens", context_lens, dev), _int32("query_lens", query_lens, dev)
     tiling = _tiling(group, max_query_len)
     step = _reusable(out, (b, num_tokens, w, max_query_len, block_size, num_blocks, group), dev)
     if step is None:
         step = DeviceStep(b, num_tokens, w, max_query_len, block_size, num_blocks, group, dev, own_tables=False)
-    elif step._sizes[9]:
+    elif step._sizes[_TABLES]:
         raise ValueError("out was made by DeviceBlockTables.reserve")
     step._tables, step._row_ids = tables, None
     p = step._ptr
-    with _On(dev):
-        _lib.check(_lib.lib().pa_kv8_build_step(
-            None, ctx.data_ptr(), ql.data_ptr(), tables.data_ptr(), max(tables.stride(0), w), None, None, None, 0, b, b,
-            w, step.block_size, step.num_blocks, step.num_tokens, step.max_query_len, ctypes.byref(tiling), None, p(1),
-            p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(0), _stream(dev)))
+    _launch(dev, _lib.lib().pa_kv8_build_step, None, ctx.data_ptr(), ql.data_ptr(), tables.data_ptr(),
+            max(tables.stride(0), w), None, None, None, 0, b, b, w, block_size, num_blocks, num_tokens, max_query_len,
+            ctypes.byref(tiling), None, p[_CTX], p[_QL], p[_HELD], p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[0])
     return step
 
 
@@ -294,12 +270,11 @@ class DeviceBlockTables:
             raise ValueError("out was made by device_step")
         step._row_ids = ids
         p = step._ptr
-        with _On(dev):
-            _lib.check(_lib.lib().pa_kv8_build_step(
-                ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(), self.tables.data_ptr(), self.width,
-                self.held.data_ptr(), self.free.data_ptr(), self.num_free.data_ptr(), self.free.numel(), b,
-                self.max_requests, self.width, self.block_size, self.num_blocks, step.num_tokens, step.max_query_len,
-                ctypes.byref(tiling), p(9), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(0), _stream(dev)))
+        _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
+                self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
+                self.num_free.data_ptr(), self.free.shape[0], b, self.max_requests, self.width, self.block_size,
+                self.num_blocks, num_tokens, max_query_len, ctypes.byref(tiling), p[_TABLES], p[_CTX], p[_QL], p[_HELD],
+                p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[0])
         return step
 
     def commit(self, step: DeviceStep, accepted: torch.Tensor | None = None) -> None:
@@ -312,11 +287,10 @@ class DeviceBlockTables:
             if tuple(accepted.shape) != (step.num_seqs,):
                 raise ValueError(f"accepted must be [{step.num_seqs}], got {tuple(accepted.shape)}")
             acc = _int32("accepted", accepted, self.device)
-        with _On(self.device):
-            _lib.check(_lib.lib().pa_kv8_commit(
-                step._row_ids.data_ptr(), step._ptr(2), acc.data_ptr() if acc is not None else None, step._ptr(3),
-                step._ptr(8), step.num_seqs, self.max_requests, self.lens.data_ptr(), self.held.data_ptr(),
-                self.num_free.data_ptr(), _stream(self.device)))
+        p = step._ptr
+        _launch(self.device, _lib.lib().pa_kv8_commit, step._row_ids.data_ptr(), p[_QL],
+                acc.data_ptr() if acc is not None else None, p[_HELD], p[_FREE], step.num_seqs, self.max_requests,
+                self.lens.data_ptr(), self.held.data_ptr(), self.num_free.data_ptr())
 
     def release(self, request_ids: torch.Tensor) -> None:
         """Return the blocks of these request slots (-1 is passed over; a slot at most once) to
@@ -324,11 +298,9 @@ class DeviceBlockTables:
         if request_ids.dim() != 1:
             raise ValueError("request_ids must be [count]")
         ids = _int32("request_ids", request_ids, self.device)
-        with _On(self.device):
-            _lib.check(_lib.lib().pa_kv8_release(
-                ids.data_ptr(), ids.shape[0], self.tables.data_ptr(), self.width, self.width, self.max_requests,
-                self.lens.data_ptr(), self.held.data_ptr(), self.free.data_ptr(), self.free.numel(),
-                self.num_free.data_ptr(), _stream(self.device)))
+        _launch(self.device, _lib.lib().pa_kv8_release, ids.data_ptr(), ids.shape[0], self.tables.data_ptr(), self.width,
+                self.width, self.max_requests, self.lens.data_ptr(), self.held.data_ptr(), self.free.data_ptr(),
+                self.free.shape[0], self.num_free.data_ptr())
 
 
 # ---------------------------------------------------------------------------- the pools
@@ -336,6 +308,13 @@ def _check_pools(k_pool, v_pool, k_scale, v_scale, device) -> tuple[int, int, in
     if k_pool.dim() != 4 or k_pool.shape != v_pool.shape:
         raise ValueError("k_pool and v_pool must both be [blocks, block_size, kv_heads, dim]")
     nb, bs, hkv, dim = k_pool.shape
+    side = (nb, hkv, bs)
+    if (k_pool.dtype is _PAYLOAD and v_pool.dtype is _PAYLOAD and k_scale.dtype is torch.uint8
+            and v_scale.dtype is torch.uint8 and k_scale.shape == side and v_scale.shape == side
+            and k_pool.device == device and v_pool.device == device and k_scale.device == device
+            and v_scale.device == device and k_pool.is_contiguous() and v_pool.is_contiguous()
+            and k_scale.is_contiguous() and v_scale.is_contiguous()):
+        return nb, bs, hkv, dim
     for name, t, shape in (("k_pool", k_pool, k_pool.shape), ("v_pool", v_pool, k_pool.shape),
                            ("k_scale", k_scale, (nb, hkv, bs)), ("v_scale", v_scale, (nb, hkv, bs))):
         want = _PAYLOAD if name.endswith("pool") else torch.uint8
@@ -371,11 +350,10 @@ def reshape_and_cache_kv8(key: torch.Tensor, value: torch.Tensor, k_pool: torch.
     if slot_mapping.shape != (key.shape[0],):
         raise ValueError(f"slot_mapping must be [{key.shape[0]}], got {tuple(slot_mapping.shape)}")
     slots = _int32("slot_mapping", slot_mapping, dev)
-    with _On(dev):
-        _lib.check(_lib.lib().pa_kv8_append(
-            key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0), value.stride(1),
-            key.shape[0], hkv, dim, _DTYPE_CODE[key.dtype], k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
-            v_scale.data_ptr(), nb, bs, slots.data_ptr(), _stream(dev)))
+    ks, vs = key.stride(), value.stride()
+    _launch(dev, _lib.lib().pa_kv8_append, key.data_ptr(), ks[0], ks[1], value.data_ptr(), vs[0], vs[1], key.shape[0],
+            hkv, dim, _DTYPE_CODE[key.dtype], k_pool.data_ptr(), v_pool.data_ptr(), k_scale.data_ptr(),
+            v_scale.data_ptr(), nb, bs, slots.data_ptr())
 
 
 def attach_step(block_tables: torch.Tensor, step: DeviceStep) -> torch.Tensor:
@@ -385,7 +363,19 @@ def attach_step(block_tables: torch.Tensor, step: DeviceStep) -> torch.Tensor:
     return block_tables
 
 
-_SCRATCH_BYTES: dict[tuple[int, int, int, int], int] = {}
+_SCRATCH_BYTES: dict[tuple[int, ...], int] = {}
+
+
+def _scratch(device: torch.device, *sizes: int) -> torch.Tensor:
+    """Scratch of one call, from the caching allocator: calls on two streams and captured
+    graphs each have their own."""
+    n = _SCRATCH_BYTES.get(sizes)
+    if n is None:
+        n = int(_lib.lib().pa_kv8_workspace_bytes(*sizes))
+        if len(_SCRATCH_BYTES) > 1024:
+            _SCRATCH_BYTES.clear()
+        _SCRATCH_BYTES[sizes] = n
+    return torch.empty(max(n, 1), dtype=torch.uint8, device=device)
 
 
 def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, k_scale: torch.Tensor,
@@ -418,33 +408,37 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         raise ValueError("out must be contiguous with the query's shape, dtype and device")
     group = heads // hkv
     step = getattr(block_tables, "_kv8_step", None)
-    if step is None or step.device != dev or not step.matches(tokens, bs, nb, group):
-        step = device_step(block_tables, context_lens, query_lens, num_tokens=tokens,
-                           max_query_len=tokens if max_query_len is None else min(int(max_query_len), tokens),
-                           num_blocks=nb, block_size=bs, group=group)
+    if step is not None:
+        if step.device != dev or not step.matches(tokens, bs, nb, group):
+            raise ValueError(f"the attached step is for {step.num_tokens} tokens, {step.group} heads per KV head and "
+                             f"{step.num_blocks} blocks of {step.block_size} on {step.device}; the call has {tokens}, "
+                             f"{group}, {nb} of {bs} on {dev}")
+        tables, p = step.block_tables, step._ptr
+        b, w, most = step.num_seqs, step.width, step.max_query_len
+        ctx, lens, cu, work = p[_CTX], None, p[_CU], p[0]
+    else:
+        if block_tables.dim() != 2:
+            raise ValueError("block_tables must be [batch, max_blocks]")
+        b, w = block_tables.shape
+        if tuple(context_lens.shape) != (b,) or tuple(query_lens.shape) != (b,):
+            raise ValueError("context_lens and query_lens must be [batch] to match block_tables")
+        tables = _table_rows(block_tables, dev)
+        context_lens, query_lens = _int32("context_lens", context_lens, dev), _int32("query_lens", query_lens, dev)
+        most = tokens if max_query_len is None else min(int(max_query_len), tokens)
+        _check_step_sizes(tokens, most, bs, nb)
+        ctx, lens, cu, work = context_lens.data_ptr(), query_lens.data_ptr(), None, None
+    _tiling(group, most)                              # refuses what has no kernel, also for empty calls
     if tokens == 0:
         return out
-    if query.stride(2) != 1 or query.stride(0) % 8 or query.stride(1) % 8 or query.data_ptr() % 16:
+    qs = query.stride()
+    if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
         query = query.contiguous()
-    lib = _lib.lib()
-    shape = (heads, hkv, dim, step.max_query_len)
-    nbytes = _SCRATCH_BYTES.get(shape)
-    if nbytes is None:
-        nbytes = int(lib.pa_kv8_workspace_bytes(*shape))
-        if len(_SCRATCH_BYTES) > 1024:
-            _SCRATCH_BYTES.clear()
-        _SCRATCH_BYTES[shape] = nbytes
-    # From the caching allocator, so that calls on two streams and captured graphs each have
-    # their own.
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    tables = step.block_tables
-    p = step._ptr
-    with _On(dev):
-        _lib.check(lib.pa_kv8_attention(
-            query.data_ptr(), query.stride(0), query.stride(1), tokens, heads, dim, k_pool.data_ptr(),
-            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, bs, hkv, _DTYPE_CODE[query.dtype],
-            float(scale), step.num_seqs, step.max_query_len, tables.data_ptr(), max(tables.stride(0), step.width), p(1),
-            p(4), p(0), out.data_ptr(), out.stride(0), out.stride(1), scratch.data_ptr(), nbytes, _stream(dev)))
+        qs = query.stride()
+    scratch = _scratch(dev, b, heads, hkv, dim, most)
+    _launch(dev, _lib.lib().pa_kv8_attention, query.data_ptr(), qs[0], qs[1], tokens, heads, dim, k_pool.data_ptr(),
+            v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, bs, hkv, _DTYPE_CODE[query.dtype], scale, b,
+            most, tables.data_ptr(), max(tables.stride(0), w), w, ctx, lens, cu, work, out.data_ptr(), heads * dim, dim,
+            scratch.data_ptr(), scratch.shape[0])
     return out
 
 

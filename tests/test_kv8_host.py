@@ -147,7 +147,7 @@ def test_build_step_refusals(pkg, kw, exc, match):
 
 
 _ATTN = dict(q=4096, qst=512, qsh=64, tokens=1, heads=8, dim=64, k=4096, v=4096, ks=4096, vs=4096, blocks=8, bs=16,
-             hkv=8, dtype=1, scale=1.0, seqs=1, most=1, tables=16, stride=4, ctx=16, cu=16, work=16, out=4096, ost=512,
+             hkv=8, dtype=1, scale=1.0, seqs=1, most=1, tables=16, stride=4, width=4, ctx=16, ql=16, cu=16, work=16, out=4096, ost=512,
              osh=64, ws=4096, wsb=1 << 40, stream=None)
 
 
@@ -168,6 +168,9 @@ _ATTN = dict(q=4096, qst=512, qsh=64, tokens=1, heads=8, dim=64, k=4096, v=4096,
     (dict(k=4100), ValueError, "16-byte"),
     (dict(vs=4100), ValueError, "16-byte"),
     (dict(wsb=16), RuntimeError, "workspace holds"),
+    (dict(work=None), ValueError, "NULL"),
+    (dict(cu=None), ValueError, "NULL"),
+    (dict(work=None, cu=None, ql=None), ValueError, "NULL"),
     (dict(ws=4100), ValueError, "256-byte"),
 ])
 def test_attention_refusals(pkg, kw, exc, match):
@@ -181,7 +184,8 @@ def test_attention_refusals(pkg, kw, exc, match):
     (dict(dim=80), NotImplementedError, "head_dim 80"),
     (dict(hkv=0), ValueError, "append shape"),
     (dict(slots=None), ValueError, "NULL"),
-    (dict(kp=4100), ValueError, "8-byte"),
+    (dict(kp=4100), ValueError, "16-byte"),
+    (dict(tokens=1 << 30, hkv=4), NotImplementedError, "2\\^31"),
 ])
 def test_append_refusals(pkg, kw, exc, match):
     a = dict(key=16, kst=64, ksh=64, value=16, vst=64, vsh=64, tokens=1, hkv=1, dim=64, dtype=1, kp=4096, vp=4096,
