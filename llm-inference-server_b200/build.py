@@ -28,7 +28,7 @@ LIB = PKG / LIB_NAME
 CU_SOURCES = ["api.cu", "decode_splitk.cu", "decode_mma.cu", "prefill_tc.cu", "prefill_persist.cu", "prefill_pair.cu", "attention_generic.cu", "kv_append.cu",
               "attention_noalloc.cu",
               "block_copy.cu", "peer_allreduce.cu", "oproj_allreduce.cu",
-              "kv8_api.cu", "kv8_step.cu", "kv8_append.cu", "kv8_rows.cu"]
+              "kv8_api.cu", "kv8_step.cu", "kv8_append.cu", "kv8_rows.cu", "kv8_tiles.cu"]
 CXX_SOURCES = ["step_plan.cpp"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -45,10 +45,10 @@ static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 1
 constexpr int kMaxSms = 160;
 
 struct Kv8Scratch {
-  uint64_t work, cu, ml, o, bytes;
+  uint64_t work, cu, ml, o, tile_ml, tile_o, bytes;
 };
 static Kv8Scratch attention_scratch(const pa_kv8_tiling& t, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim,
-                                    int sms) {
+                                    int sms, bool tiles) {
   const uint64_t rows =
       uint64_t(kv8_rows_slices(t.row_groups, num_kv_heads, sms)) * num_kv_heads * 2 * (8 * t.row_groups);
   Kv8Scratch s;
@@ -56,7 +56,10 @@ static Kv8Scratch attention_scratch(const pa_kv8_tiling& t, int32_t num_seqs, in
   s.cu = (uint64_t(num_seqs) + 1) * 2 * sizeof(int64_t);
   s.ml = (s.cu + (uint64_t(num_seqs) + 1) * sizeof(int32_t) + 255) / 256 * 256;
   s.o = (s.ml + rows * sizeof(float2) + 255) / 256 * 256;
-  s.bytes = s.o + rows * head_dim * sizeof(float);
+  s.tile_ml = (s.o + rows * head_dim * sizeof(float) + 255) / 256 * 256;
+  const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * 128 : 0;
+  s.tile_o = (s.tile_ml + tile_rows * sizeof(float2) + 255) / 256 * 256;
+  s.bytes = s.tile_o + tile_rows * head_dim * sizeof(float);
   return s;
 }
 
@@ -87,10 +90,13 @@ int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, pa_kv8_tiling
   if (!tiling) return fail(PA_ERR_INVALID_ARGUMENT, "tiling must not be NULL");
   if (group < 1 || max_query_len < 0) return fail(PA_ERR_INVALID_ARGUMENT, "bad group or max_query_len");
   if (group > 16) return fail(PA_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16 are supported", group);
-  const int64_t rows = int64_t(group) * std::max(1, max_query_len);
-  tiling->row_groups = rows <= 8 ? 1 : 2;
+  // A sequence of up to 32 (token, head) rows goes to the kernel for few rows, one of more to
+  // the 128-row tiles.
+  const int few = std::max(1, 32 / group);
+  const int rows = group * std::max(1, std::min(max_query_len, few));
+  tiling->row_groups = (rows + 7) / 8;
   tiling->small_tokens = std::max(1, 8 * tiling->row_groups / group);
-  tiling->small_max = max_query_len;
+  tiling->small_max = std::min(max_query_len, few);
   tiling->large_tokens = 128 / group;
   return PA_OK;
 }
@@ -226,7 +232,7 @@ uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num
   if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_heads % num_kv_heads ||
       pa_kv8_choose_tiling(num_heads / num_kv_heads, max_query_len, &t) != PA_OK)
     return 0;
-  return attention_scratch(t, num_seqs, num_kv_heads, head_dim, kMaxSms).bytes;
+  return attention_scratch(t, num_seqs, num_kv_heads, head_dim, kMaxSms, max_query_len > t.small_max).bytes;
 }
 
 int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t num_tokens,
@@ -268,7 +274,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_scale) || !aligned16(v_scale))
     return fail(PA_ERR_INVALID_ARGUMENT, "8-bit pools and their scales must be 16-byte aligned");
   const int sms = std::min(sm_count(), kMaxSms);
-  const Kv8Scratch s = attention_scratch(t, num_seqs, num_kv_heads, head_dim, sms);
+  const Kv8Scratch s = attention_scratch(t, num_seqs, num_kv_heads, head_dim, sms, max_query_len > t.small_max);
   if (workspace_bytes < s.bytes)
     return fail(PA_ERR_BUFFER_TOO_SMALL, "workspace holds %llu bytes, %llu needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
@@ -332,6 +338,16 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   cudaError_t e = launch_kv8_rows(dtype, head_dim, t.row_groups, tk, tv, p, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
   note_launches(PA_LAUNCH_KV8_ROWS | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
+  if (max_query_len > t.small_max) {
+    p.work = work + num_seqs + 1;
+    p.tile_tokens = t.large_tokens;
+    p.slices = kv8_tiles_slices(num_kv_heads, sms);
+    p.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
+    p.part_o = reinterpret_cast<float*>(ws + s.tile_o);
+    e = launch_kv8_tiles(dtype, head_dim, p, err, stream);
+    if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
+    note_launches(PA_LAUNCH_KV8_TILES | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
+  }
   return PA_OK;
 }
 

@@ -14,20 +14,25 @@
 // HBM-bound: each K/V byte is read once per tile of rows.  The sequences' keys laid end to
 // end are cut into equal slices (kv8_line.cuh), a CTA per slice and KV head with the KV head
 // fastest, so that the CTAs of one slice read a pool block's heads side by side.  A CTA has
-// four consumer warps, which take blocks of 16 keys in turn, and a producer warp, which
+// four consumer warps, which take stages of 32 keys in turn, and a producer warp, which
 // walks the slice's pieces, reads the block table and keeps each consumer's ring full: the
-// rings run across pieces, so a new sequence costs no drain.  Per block: K and V tile by TMA
-// (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round of 32
-// blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the tiles:
-// 177 us for 64 sequences of about 4,096 keys, 8 heads of 128).
+// rings run across pieces, so a new sequence costs no drain.  Per 16 keys: K and V tile by
+// TMA (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round
+// of 32 blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the
+// tiles: 177 against 152 us for 64 sequences of about 4,096 keys, 8 heads of 128).
 //
-// Widening costs one conversion per two elements and the transpose of V one byte permute per
-// four: with 16-byte chunks of head_dim dealt out to the MMA's k index as ldmatrix delivers
-// bytes (lane 4g + i holds dims 4i .. 4i + 3), K needs no permute at all.
+// Both products are computed transposed, S^T = K Q^T and O^T = V^T W^T, because an MMA has
+// 16 rows and 8 columns and there are few query rows: 16 keys (or dims) fill the rows, 8
+// query rows the columns, so one group of 8 rows wastes nothing; the other way round half of
+// each MMA is zeros.  W moves from the accumulator's layout to the operand's by one
+// movmatrix per 8 x 8.  Widening costs one conversion per two elements; with 16-byte chunks
+// of head_dim dealt out to the MMA's k index as ldmatrix delivers bytes (lane 4g + i holds
+// dims 4i .. 4i + 3) K needs no permute, and V's transpose needs one byte permute per four.
 #include <cuda_fp16.h>
 
 #include "kv8.h"
 #include "kv8_line.cuh"
+#include "kv8_widen.cuh"
 #include "pa_common.cuh"
 #include "tc_softmax.cuh"
 
@@ -35,8 +40,9 @@ namespace pa {
 
 constexpr int kRowsWarps = 4;                       // consumers
 constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
-constexpr int kRowsKeys = 16;                       // keys a stage
-constexpr int kRowsDescs = 4;
+constexpr int kRowsStage = 32;                      // keys a stage: two 16-key blocks
+constexpr int kRowsKeys = 16;                       // keys a block; cuts fall on these
+constexpr int kRowsDescs = 2;
 // Fewest keys a slice gets: below this a CTA's set-up and its partial cost more than the
 // keys it takes over.
 constexpr int kRowsMinKeys = 128;
@@ -44,16 +50,24 @@ constexpr float kWeightShift = 256.f;               // 2^8, see above
 
 template <int D, int RG>
 struct RowsCfg {
-  static constexpr int STAGES = D == 128 ? 4 : 8;   // 16 KB in flight per warp
-  static constexpr int TILE = kRowsKeys * D;
-  static constexpr int STAGE = 2 * TILE;
-  static constexpr int NO = RG * (D / 8) * 2;       // accumulator registers
+  static constexpr int STAGES = D == 128 ? 2 : 4;   // 16 KB in flight per warp
+  static constexpr int TILE = kRowsKeys * D;        // K or V of a block
+  static constexpr int BLOCK = 2 * TILE;
+  static constexpr int STAGE = 2 * BLOCK;
+  static constexpr int CH = D / 16;                 // 16-byte chunks of a row = k steps of S
+  static constexpr int NO = CH * RG * 4;            // accumulator registers
   static constexpr int OFF_SCALE = kRowsWarps * STAGES * STAGE;
-  static constexpr int OFF_MERGE = OFF_SCALE + kRowsWarps * STAGES * 32;
+  static constexpr int OFF_Q = OFF_SCALE + kRowsWarps * STAGES * 2 * kRowsStage;
+  static constexpr int OFF_MERGE = OFF_Q + CH * RG * 32 * 8;
   static constexpr int OFF_ML = OFF_MERGE + 2 * NO * 32 * 4;
-  static constexpr int OFF_DESC = OFF_ML + kRowsWarps * RG * 8 * 8;
+  static constexpr int OFF_FACTOR = OFF_ML + kRowsWarps * RG * 8 * 8;
+  static constexpr int OFF_DESC = OFF_FACTOR + RG * 8 * 4;
   static constexpr int OFF_BAR = OFF_DESC + kRowsDescs * 32;
   static constexpr int SMEM = OFF_BAR + (2 * kRowsWarps * STAGES + 2 * kRowsDescs) * 8;
+  static constexpr bool Q_IN_REGS = RG <= 2;
+  // CTAs on an SM: 228 KB of shared memory, 1 KB of it taken per CTA.
+  static constexpr int CTAS = RG == 1 ? 3 : 2;
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory for the CTAs an SM is to hold");
 };
 
 struct RowsPiece {      // part of a tile that a CTA works on
@@ -81,30 +95,18 @@ __device__ __forceinline__ void ldm4t(uint32_t addr, uint32_t (&r)[4]) {
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(addr));
 }
-// Two e4m3 values (low or high half of a word) as two fp16 values, exactly.
-__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
-  uint32_t r;
-  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}\n" : "=r"(r) : "r"(w));
-  return r;
+// D += A B, m16n8k16, fp16 operands.
+__device__ __forceinline__ void mma16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                      uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+// The 8 x 8 tile of 16-bit elements, transposed across the warp.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   uint32_t r;
-  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}\n" : "=r"(r) : "r"(w));
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
-}
-// D += A B, m16n8k16, fp16 operands.  With one group of rows, rows 8..15 of A are zero.
-template <int RG>
-__device__ __forceinline__ void mma16(float* d, const uint32_t (&a)[2 * RG], uint32_t b0, uint32_t b1) {
-  if constexpr (RG == 1) {
-    float x, y;
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
-        : "+f"(d[0]), "+f"(d[1]), "=f"(x), "=f"(y)
-        : "r"(a[0]), "r"(0u), "r"(a[1]), "r"(b0), "r"(b1), "f"(0.f));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
 }
 
 // Byte offset of 16-byte chunk c of row r in a TMA tile whose rows are D bytes, with the
@@ -115,25 +117,17 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-// Four query elements as two fp16 pairs, times 2^shift; `factor` collects 2^-shift.
-template <typename T>
-__device__ __forceinline__ float row_scale(float big) {  // power of two that brings `big` to [2^14, 2^15)
-  const uint32_t e = (__float_as_uint(big) >> 23) & 0xffu;
-  if (sizeof(T) == 2 && DType<T>::code == PA_DTYPE_F16) return 1.f;
-  if (e == 0 || e == 255) return 1.f;
-  const int up = 14 - (int(e) - 127);
-  return __uint_as_float(uint32_t(127 + max(-126, min(127, up))) << 23);
-}
-
 template <typename T, int D, int RG>
-__global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
+__global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
     kv8_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const Kv8AttnParams p, int* err) {
   using C = RowsCfg<D, RG>;
-  constexpr int CH = D / 16;  // 16-byte chunks of a row = k steps of S
+  constexpr int CH = C::CH;
   extern __shared__ __align__(1024) uint8_t smem[];
+  uint2* sq = reinterpret_cast<uint2*>(smem + C::OFF_Q);
   float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
+  float* factors = reinterpret_cast<float*>(smem + C::OFF_FACTOR);
   RowsPiece* desc = reinterpret_cast<RowsPiece*>(smem + C::OFF_DESC);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + kRowsWarps * C::STAGES;
@@ -148,7 +142,7 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRowsWarps * C::STAGES; ++i) {
-      mbar_init(&full[i], 1);
+      mbar_init(&full[i], 2);  // one arrival per block
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kRowsDescs; ++i) {
@@ -238,27 +232,34 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
       if (t.seq < 0) break;
       const int32_t* row = p.tables + int64_t(t.seq) * p.table_stride;
       // Each lane looks up one of the next 32 blocks and reads its scales, one round ahead of
-      // the round whose tiles are being issued, and then issues its own block in turn.
-      BlockRef cur = look_up(row, kb0 + lane, kb1), nxt;
+      // the round whose tiles are being issued; lanes then issue their own blocks, two (a
+      // stage) at a time.
+      BlockRef cur = look_up(row, kb0 + lane, kb1), nxt = cur;
       for (int kb = kb0; kb < kb1 && ok; kb += 32) {
         if (kb + 32 < kb1) nxt = look_up(row, kb + 32 + lane, kb1);
         const int n = min(32, kb1 - kb);
-        for (int j = 0; j < n && ok; j += kRowsWarps) {
+        for (int j = 0; j < n && ok; j += 2 * kRowsWarps) {
 #pragma unroll
           for (int w = 0; w < kRowsWarps; ++w) {
-            if (j + w < n) {
+            const int b = j + 2 * w;
+            if (b < n) {
               const int st = issued[w] % C::STAGES;
               if (issued[w] >= C::STAGES)
                 ok = mbar_wait(&empty[w * C::STAGES + st], ((issued[w] / C::STAGES) - 1) & 1) && ok;
-              if (ok && lane == j + w) {
+              const int half = lane - b;
+              if (ok && (half == 0 || half == 1)) {
                 uint64_t* bar = &full[w * C::STAGES + st];
-                uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE;
-                uint4* sc = reinterpret_cast<uint4*>(smem + C::OFF_SCALE + (w * C::STAGES + st) * 32);
-                sc[0] = cur.ks;
-                sc[1] = cur.vs;
-                mbar_arrive_expect_tx(bar, C::STAGE);  // releases the scales too
-                tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
-                tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
+                if (lane < n) {
+                  uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE + half * C::BLOCK;
+                  uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * 2 * kRowsStage + 16 * half;
+                  *reinterpret_cast<uint4*>(sc) = cur.ks;
+                  *reinterpret_cast<uint4*>(sc + kRowsStage) = cur.vs;
+                  mbar_arrive_expect_tx(bar, C::BLOCK);  // releases the scales too
+                  tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
+                  tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
+                } else {
+                  rows_arrive(bar);  // the piece's last stage holds one block
+                }
               }
               if (ok) ++issued[w];
             }
@@ -303,151 +304,196 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
     if (lane == 0) rows_arrive(&d_empty[slot]);
     if (d.row0 < 0) break;
 
-    // Queries as A fragments: row r = 8 rr + g is (token r / group, head r % group).
-    uint32_t qa[CH][2 * RG];
-    float factor[RG];
-    int limit[RG];
+    // Queries as B fragments in shared memory: row r = (token r / group, head r % group),
+    // brought into fp16 by a power of two; a warp takes a row.
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) {
-      const int r = 8 * rr + g, tok = r / p.group, head = r - tok * p.group;
-      const bool valid = tok < d.tokens;
-      limit[rr] = valid ? d.pos0 + tok : -1;
-      const T* src = static_cast<const T*>(p.q) + int64_t(d.row0 + (valid ? tok : 0)) * p.q_st +
-                     int64_t(kvh * p.group + head) * p.q_sh + 4 * tig;
-      // Two passes over the row (the second from L1) rather than a row in registers.
+    for (int i = 0; i < 2 * RG; ++i) {
+      const int r = warp + kRowsWarps * i, tok = r / p.group, head = r - tok * p.group;
+      constexpr int E = D / 32;
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = 0.f;
+      if (tok < d.tokens)
+        VecLoad<T, E>::run(static_cast<const T*>(p.q) + int64_t(d.row0 + tok) * p.q_st +
+                               int64_t(kvh * p.group + head) * p.q_sh + E * lane,
+                           x);
       float big = 0.f;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (valid) VecLoad<T, 4>::run(src + 16 * c, x);
-        big = fmaxf(fmaxf(fmaxf(big, fabsf(x[0])), fmaxf(fabsf(x[1]), fabsf(x[2]))), fabsf(x[3]));
-      }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      const float up = row_scale<T>(big);
-      factor[rr] = p.qscale / up;  // exact: a power of two
+      for (int e = 0; e < E; ++e) big = fmaxf(big, fabsf(x[e]));
+      if (DType<T>::code == PA_DTYPE_BF16) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        // fragment order {row g: k 2i..2i+1, (row g + 8: same), row g: k 2i+8.., (row g + 8)}
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        if (valid) VecLoad<T, 4>::run(src + 16 * c, x);
-        qa[c][0 * RG + rr] = pack2<__half>(x[0] * up, x[1] * up);
-        qa[c][1 * RG + rr] = pack2<__half>(x[2] * up, x[3] * up);
+        for (int s = 16; s; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
+      }
+      const float up = query_power<T>(big);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(&sq[((E * lane / 16) * RG + (r >> 3)) * 32 + (r & 7) * 4 +
+                                                      (E * lane % 16) / 4]);
+      if constexpr (E == 4) {
+        dst[0] = pack2<__half>(x[0] * up, x[1] * up);
+        dst[1] = pack2<__half>(x[2] * up, x[3] * up);
+      } else {
+        dst[lane & 1] = pack2<__half>(x[0] * up, x[1] * up);
+      }
+      if (lane == 0) factors[r] = p.qscale / up;  // exact: a power of two
+    }
+    rows_sync();
+    float factor[RG][2];
+    int limit[RG][2];
+    uint2 qr[C::Q_IN_REGS ? CH : 1][RG];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * rg + 2 * tig + e, tok = r / p.group;
+        factor[rg][e] = factors[r];
+        limit[rg][e] = tok < d.tokens ? min(d.pos0 + tok, d.kb1 * kRowsKeys - 1) : -1;
+      }
+      if constexpr (C::Q_IN_REGS) {
+#pragma unroll
+        for (int c = 0; c < CH; ++c) qr[c][rg] = sq[(c * RG + rg) * 32 + lane];
       }
     }
 
-    float o[CH][2][2 * RG];  // chunk, even / odd dims, fragment
+    float o[CH][RG][4];  // dims 16 c + 2 g (+1: elements 2, 3), rows 8 rg + 2 tig + {0, 1}
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int e = 0; e < 2 * RG; ++e) o[c][0][e] = o[c][1][e] = 0.f;
-    float m[RG], l[RG];
+      for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) {
-      m[rr] = -INFINITY;
-      l[rr] = 0.f;
-    }
+        for (int e = 0; e < 4; ++e) o[c][rg][e] = 0.f;
+    float m[RG][2], l[RG][2];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        m[rg][e] = -INFINITY;
+        l[rg][e] = 0.f;
+      }
 
-    for (int kb = d.kb0 + warp; kb < d.kb1; kb += kRowsWarps, ++taken) {
+    for (int kb = d.kb0 + 2 * warp; kb < d.kb1; kb += 2 * kRowsWarps, ++taken) {
       const int st = taken % C::STAGES;
       if (ok) ok = mbar_wait(&full[warp * C::STAGES + st], (taken / C::STAGES) & 1);
-      const uint32_t kt = smem_u32(smem + (warp * C::STAGES + st) * C::STAGE), vt = kt + C::TILE;
-      const uint8_t* sc = smem + C::OFF_SCALE + (warp * C::STAGES + st) * 32;
-      // Scales of keys 2 tig, 2 tig + 1, 8 + 2 tig, 9 + 2 tig.
-      float ks[2][2], vs[2][2];
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        const uint32_t a = *reinterpret_cast<const uint16_t*>(sc + 8 * nt + 2 * tig);
-        const uint32_t b = *reinterpret_cast<const uint16_t*>(sc + 16 + 8 * nt + 2 * tig);
-        ks[nt][0] = __uint_as_float((a & 0xffu) << 23);
-        ks[nt][1] = __uint_as_float((a >> 8) << 23);
-        vs[nt][0] = __uint_as_float((b & 0xffu) << 23) * kWeightShift;
-        vs[nt][1] = __uint_as_float((b >> 8) << 23) * kWeightShift;
-      }
+      const uint32_t stage = smem_u32(smem + (warp * C::STAGES + st) * C::STAGE);
+      const uint8_t* sc = smem + C::OFF_SCALE + (warp * C::STAGES + st) * 2 * kRowsStage;
 
-      // ---- S over the payloads
-      float s[2][2 * RG];
+      // ---- S^T over the payloads: element 2 h + e is key 16 b + 8 h + g, row 8 rg + 2 tig + e
+      float s[2][RG][4];
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
+      for (int b = 0; b < 2; ++b) {
 #pragma unroll
-        for (int e = 0; e < 2 * RG; ++e) s[nt][e] = 0.f;
+        for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-        for (int c = 0; c < CH; c += 4) {
-          uint32_t w[4];
-          ldm4(kt + tile_at<D>(8 * nt + ri, c + mi), w);
+          for (int e = 0; e < 4; ++e) s[b][rg][e] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mma16<RG>(s[nt], qa[c + i], widen_lo(w[i]), widen_hi(w[i]));
+        for (int c = 0; c < CH; c += 2) {
+          uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
+          ldm4(stage + b * C::BLOCK + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t a0 = widen_lo(w[2 * i]), a1 = widen_lo(w[2 * i + 1]), a2 = widen_hi(w[2 * i]),
+                           a3 = widen_hi(w[2 * i + 1]);
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) {
+              uint2 q;
+              if constexpr (C::Q_IN_REGS)
+                q = qr[c + i][rg];
+              else
+                q = sq[((c + i) * RG + rg) * 32 + lane];
+              mma16(s[b][rg], a0, a1, a2, a3, q.x, q.y);
+            }
+          }
         }
       }
 
-      // ---- online softmax; fragment element 2 rr + e is row 8 rr + g, key 8 nt + 2 tig + e
-      const int key0 = kb * kRowsKeys + 2 * tig;
-      const bool masked = kb * kRowsKeys + kRowsKeys - 1 > d.pos0;  // spare rows compute, unmasked, and are not stored
-      uint32_t pa[2 * RG];
-      float alpha[RG];
+      // ---- online softmax
+      float ks[2][2], vs[2][2];  // scales of keys 16 b + 8 h + g
 #pragma unroll
-      for (int rr = 0; rr < RG; ++rr) {
-        float mx = -INFINITY;
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float& v = s[nt][2 * rr + e];
-            v *= ks[nt][e] * factor[rr];
-            if (masked && key0 + 8 * nt + e > limit[rr]) v = -INFINITY;
-            mx = fmaxf(mx, v);
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[rr], mx);
-        const float ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-        alpha[rr] = ex2(m[rr] - ref);
-        m[rr] = mn;
-        float sum = 0.f;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          float w[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float pr = ex2(s[nt][2 * rr + e] - ref);
-            sum += pr;
-            w[e] = pr * vs[nt][e];
-            if (masked && key0 + 8 * nt + e > limit[rr]) w[e] = 0.f;  // a hidden row may stand for NaN
-          }
-          pa[nt * RG + rr] = pack2<__half>(w[0], w[1]);
+        for (int h = 0; h < 2; ++h) {
+          ks[b][h] = __uint_as_float(uint32_t(sc[16 * b + 8 * h + g]) << 23);
+          vs[b][h] = __uint_as_float(uint32_t(sc[kRowsStage + 16 * b + 8 * h + g]) << 23) * kWeightShift;
         }
-        l[rr] = l[rr] * alpha[rr] + sum;
-      }
+      const int key0 = kb * kRowsKeys;
+      // Spare rows of the tile compute, unmasked, and are not stored.
+      const bool masked = key0 + kRowsStage - 1 > d.pos0 || kb + 2 > d.kb1;
+      uint32_t wt[2][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1) of block b, row 8 rg + g
       bool grown = false;
+      float alpha[RG][2];
 #pragma unroll
-      for (int rr = 0; rr < RG; ++rr) grown |= alpha[rr] != 1.f;
+      for (int rg = 0; rg < RG; ++rg) {
+        float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& v = s[b][rg][2 * h + e];
+              v *= ks[b][h] * factor[rg][e];
+              if (masked && key0 + 16 * b + 8 * h + g > limit[rg][e]) v = -INFINITY;
+              mx[e] = fmaxf(mx[e], v);
+            }
+        float ref[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+          const float mn = fmaxf(m[rg][e], mx[e]);
+          ref[e] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+          alpha[rg][e] = ex2(m[rg][e] - ref[e]);
+          grown |= alpha[rg][e] != 1.f;
+          m[rg][e] = mn;
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float w[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float pr = ex2(s[b][rg][2 * h + e] - ref[e]);
+              sum[e] += pr;
+              w[e] = pr * vs[b][h];
+              // A hidden key's row may stand for NaN.
+              if (masked && key0 + 16 * b + 8 * h + g > limit[rg][e]) w[e] = 0.f;
+            }
+            wt[b][rg][h] = transpose8(pack2<__half>(w[0], w[1]));
+          }
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[rg][e] = l[rg][e] * alpha[rg][e] + sum[e];
+      }
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int c = 0; c < CH; ++c)
 #pragma unroll
-          for (int e = 0; e < 2 * RG; ++e) {
-            o[c][0][e] *= alpha[e >> 1];
-            o[c][1][e] *= alpha[e >> 1];
-          }
+          for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[c][rg][e] *= alpha[rg][e & 1];
       }
 
-      // ---- O += W V
-      const int left = d.ctx - kb * kRowsKeys;  // keys of this block inside the context
-      uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
-      if (left < kRowsKeys) {
+      // ---- O^T += V^T W^T; bytes behind the context (or the stage's only block) read as zero
+      const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-          keep[hf] = (8 * hf + 2 * tig < left ? 0x0000ffffu : 0u) | (8 * hf + 2 * tig + 1 < left ? 0xffff0000u : 0u);
-      }
+      for (int b = 0; b < 2; ++b) {
+        uint32_t pick[2] = {0x3120u, 0x3120u};  // (t0 d0, t1 d0, t0 d1, t1 d1) of (t0 d0, t0 d1, t1 d0, t1 d1)
+        if (end < kRowsStage) {
 #pragma unroll
-      for (int c = 0; c < CH; c += 2) {
-        uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
-        ldm4t(vt + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+          for (int h = 0; h < 2; ++h) {
+            const int t0 = 16 * b + 8 * h + 2 * tig;
+            pick[h] = t0 + 1 < end ? 0x3120u : (t0 < end ? 0x4140u : 0x4444u);
+          }
+        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint32_t a = __byte_perm(w[2 * i] & keep[0], 0, 0x3120), b = __byte_perm(w[2 * i + 1] & keep[1], 0, 0x3120);
-          mma16<RG>(o[c + i][0], pa, widen_lo(a), widen_lo(b));
-          mma16<RG>(o[c + i][1], pa, widen_hi(a), widen_hi(b));
+        for (int c = 0; c < CH; c += 2) {
+          uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
+          ldm4t(stage + b * C::BLOCK + C::TILE + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint32_t x = __byte_perm(w[2 * i], 0, pick[0]), y = __byte_perm(w[2 * i + 1], 0, pick[1]);
+            const uint32_t a0 = widen_lo(x), a1 = widen_hi(x), a2 = widen_lo(y), a3 = widen_hi(y);
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[b][rg][0], wt[b][rg][1]);
+          }
         }
       }
       __syncwarp();
@@ -455,50 +501,50 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
     }
 
     // ---- join the four warps: common maximum, then a tree over the accumulators
-    float big[RG];
+    float big[RG][2];
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) {
-      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 1);
-      l[rr] += __shfl_xor_sync(0xffffffffu, l[rr], 2);
-      if (tig == 0) ml[warp * 8 * RG + 8 * rr + g] = make_float2(m[rr], l[rr]);
-    }
+    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) l[rg][e] += __shfl_xor_sync(0xffffffffu, l[rg][e], x);
+        if (g == 0) ml[warp * 8 * RG + 8 * rg + 2 * tig + e] = make_float2(m[rg][e], l[rg][e]);
+      }
     rows_sync();
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) {
-      float2 v[kRowsWarps];
-      big[rr] = -INFINITY;
+    for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) {
-        v[w] = ml[w * 8 * RG + 8 * rr + g];
-        big[rr] = fmaxf(big[rr], v[w].x);
-      }
-      const float ref = big[rr] == -INFINITY ? 0.f : big[rr];
-      float sum = 0.f;
+      for (int e = 0; e < 2; ++e) {
+        float2 v[kRowsWarps];
+        big[rg][e] = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w) sum += v[w].y * ex2(v[w].x - ref);
-      const float f = ex2(m[rr] - ref);
-      l[rr] = sum;
-#pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          o[c][0][2 * rr + e] *= f;
-          o[c][1][2 * rr + e] *= f;
+        for (int w = 0; w < kRowsWarps; ++w) {
+          v[w] = ml[w * 8 * RG + 8 * rg + 2 * tig + e];
+          big[rg][e] = fmaxf(big[rg][e], v[w].x);
         }
-    }
+        const float ref = big[rg][e] == -INFINITY ? 0.f : big[rg][e];
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < kRowsWarps; ++w) sum += v[w].y * ex2(v[w].x - ref);
+        const float f = ex2(m[rg][e] - ref);
+        l[rg][e] = sum;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          o[c][rg][e] *= f;
+          o[c][rg][2 + e] *= f;
+        }
+      }
     auto put = [&](int half) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int e = 0; e < 4 * RG; ++e)
-          merge[(half * C::NO + c * 4 * RG + e) * 32 + lane] = o[c][e / (2 * RG)][e % (2 * RG)];
+        for (int e = 0; e < 4 * RG; ++e) merge[(half * C::NO + c * 4 * RG + e) * 32 + lane] = o[c][e / 4][e % 4];
     };
     auto add = [&](int half) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int e = 0; e < 4 * RG; ++e)
-          o[c][e / (2 * RG)][e % (2 * RG)] += merge[(half * C::NO + c * 4 * RG + e) * 32 + lane];
+        for (int e = 0; e < 4 * RG; ++e) o[c][e / 4][e % 4] += merge[(half * C::NO + c * 4 * RG + e) * 32 + lane];
     };
     if (warp >= 2) put(warp - 2);
     rows_sync();
@@ -508,32 +554,32 @@ __global__ void __launch_bounds__(kRowsThreads, RG == 1 ? 3 : 2)
     if (warp != 0) continue;
     add(1);
 #pragma unroll
-    for (int rr = 0; rr < RG; ++rr) {
-      const int r = 8 * rr + g, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
-      if (tok >= d.tokens) continue;
-      const float f = (d.part < 0 ? 1.f / l[rr] : 1.f) * (1.f / kWeightShift);
-      if (d.part < 0) {
-        T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 4 * tig;
+    for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-          *reinterpret_cast<uint2*>(dst + 16 * c) =
-              make_uint2(pack2<T>(o[c][0][2 * rr] * f, o[c][1][2 * rr] * f),
-                         pack2<T>(o[c][0][2 * rr + 1] * f, o[c][1][2 * rr + 1] * f));
-      } else {
-        const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * rg + 2 * tig + e, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
+        if (tok >= d.tokens) continue;
+        const float f = (d.part < 0 ? 1.f / l[rg][e] : 1.f) * (1.f / kWeightShift);
+        if (d.part < 0) {
+          T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 2 * g;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-          *reinterpret_cast<float4*>(p.part_o + at * D + 16 * c + 4 * tig) = make_float4(
-              o[c][0][2 * rr] * f, o[c][1][2 * rr] * f, o[c][0][2 * rr + 1] * f, o[c][1][2 * rr + 1] * f);
-        if (tig == 0) p.part_ml[at] = make_float2(big[rr], l[rr]);
+          for (int c = 0; c < CH; ++c)
+            *reinterpret_cast<uint32_t*>(dst + 16 * c) = pack2<T>(o[c][rg][e] * f, o[c][rg][2 + e] * f);
+        } else {
+          const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            *reinterpret_cast<float2*>(p.part_o + at * D + 16 * c + 2 * g) =
+                make_float2(o[c][rg][e] * f, o[c][rg][2 + e] * f);
+          if (g == 0) p.part_ml[at] = make_float2(big[rg][e], l[rg][e]);
+        }
       }
-    }
   }
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
 }
 
 // Joins the partials of tiles that a cut fell into.  CTA (s, kvh): the tile that the end of
-// slice s falls into, if this is the first cut inside it.  A warp takes a row.
+// slice s falls into, if this is the first cut inside it.  A warp takes a row at a time.
 template <typename T, int D>
 __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys) {
   constexpr int E = D / 32;  // elements a lane
@@ -547,62 +593,63 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
   if (line_key(t, x, key_step) >= t.keys) return;  // the first slice did the whole tile
   const int first = p.cu_q[t.seq], q = p.cu_q[t.seq + 1] - first, t0 = t.index * p.tile_tokens;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r = blockIdx.z * 4 + warp, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
-  if (tok >= min(p.tile_tokens, q - t0)) return;
   const int64_t end = t.start + t.keys;
   int last = s;
   while (last + 1 < slices && line_cut(total, slices, last + 1) < end) ++last;
+  for (int r = blockIdx.z * 4 + warp; r < min(p.tile_tokens, q - t0) * p.group; r += 4 * gridDim.z) {
+    const int tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
 
-  // A slice's part of the tile is its slot 1 if it starts the tile, else slot 0; it is empty
-  // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time; the
-  // parts' accumulators are then read with nothing between the loads.
-  float acc[E], m = -INFINITY, sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  for (int i0 = s - 1; i0 <= last; i0 += 32) {
-    const int i = i0 + lane;
-    float2 v = make_float2(-INFINITY, 0.f);
-    int64_t at = 0;
-    if (i <= last &&
-        line_key(t, line_cut(total, slices, i + 1), key_step) > line_key(t, line_cut(total, slices, i), key_step)) {
-      at = ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r;
-      v = p.part_ml[at];
-    }
-    float mn = v.x;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
-    mn = fmaxf(mn, m);
-    const float ref = mn == -INFINITY ? 0.f : mn, old = ex2(m - ref), f = ex2(v.x - ref);
-    m = mn;
-    float part = v.y * f;
-#pragma unroll
-    for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-    sum = sum * old + part;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= old;
-    const int n = min(32, last + 1 - i0);
-    for (int k0 = 0; k0 < n; k0 += 8) {
-      float o[8][E], fk[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        fk[k] = __shfl_sync(0xffffffffu, f, k0 + k);
-        const int64_t ak = __shfl_sync(0xffffffffu, at, k0 + k);
-        const bool some = __shfl_sync(0xffffffffu, v.x, k0 + k) != -INFINITY;  // NaN counts
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[k][e] = 0.f;
-        if (some) VecLoad<float, E>::run(p.part_o + ak * D + E * lane, o[k]);
+    // A slice's part of the tile is its slot 1 if it starts the tile, else slot 0; it is empty
+    // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time; the
+    // parts' accumulators are then read with nothing between the loads.
+    float acc[E], m = -INFINITY, sum = 0.f;
+  #pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int i0 = s - 1; i0 <= last; i0 += 32) {
+      const int i = i0 + lane;
+      float2 v = make_float2(-INFINITY, 0.f);
+      int64_t at = 0;
+      if (i <= last &&
+          line_key(t, line_cut(total, slices, i + 1), key_step) > line_key(t, line_cut(total, slices, i), key_step)) {
+        at = ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r;
+        v = p.part_ml[at];
       }
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-#pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += o[k][e] * fk[k];
+      float mn = v.x;
+  #pragma unroll
+      for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+      mn = fmaxf(mn, m);
+      const float ref = mn == -INFINITY ? 0.f : mn, old = ex2(m - ref), f = ex2(v.x - ref);
+      m = mn;
+      float part = v.y * f;
+  #pragma unroll
+      for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+      sum = sum * old + part;
+  #pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= old;
+      const int n = min(32, last + 1 - i0);
+      for (int k0 = 0; k0 < n; k0 += 8) {
+        float o[8][E], fk[8];
+  #pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          fk[k] = __shfl_sync(0xffffffffu, f, k0 + k);
+          const int64_t ak = __shfl_sync(0xffffffffu, at, k0 + k);
+          const bool some = __shfl_sync(0xffffffffu, v.x, k0 + k) != -INFINITY;  // NaN counts
+  #pragma unroll
+          for (int e = 0; e < E; ++e) o[k][e] = 0.f;
+          if (some) VecLoad<float, E>::run(p.part_o + ak * D + E * lane, o[k]);
+        }
+  #pragma unroll
+        for (int k = 0; k < 8; ++k)
+  #pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] += o[k][e] * fk[k];
+      }
     }
+    T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
+    const float inv = 1.f / sum;
+  #pragma unroll
+    for (int e = 0; e < E; e += 2)
+      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
   }
-  T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
-  const float inv = 1.f / sum;
-#pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
 }
 
 // ------------------------------------------------------------------ dispatch
@@ -626,16 +673,27 @@ static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const 
   return cudaGetLastError();
 }
 
+template <typename T, int D>
+static cudaError_t rows_by_groups(int row_groups, const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p,
+                                  int* err, cudaStream_t s) {
+  switch (row_groups) {
+    case 1: return rows_one<T, D, 1>(tk, tv, p, err, s);
+    case 2: return rows_one<T, D, 2>(tk, tv, p, err, s);
+    case 3: return rows_one<T, D, 3>(tk, tv, p, err, s);
+    case 4: return rows_one<T, D, 4>(tk, tv, p, err, s);
+    default: return cudaErrorInvalidValue;
+  }
+}
+
 template <typename T>
 static cudaError_t rows_by_shape(int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const Kv8AttnParams& p, int* err, cudaStream_t s) {
-  if (head_dim == 64)
-    return row_groups == 1 ? rows_one<T, 64, 1>(tk, tv, p, err, s) : rows_one<T, 64, 2>(tk, tv, p, err, s);
-  return row_groups == 1 ? rows_one<T, 128, 1>(tk, tv, p, err, s) : rows_one<T, 128, 2>(tk, tv, p, err, s);
+  return head_dim == 64 ? rows_by_groups<T, 64>(row_groups, tk, tv, p, err, s)
+                        : rows_by_groups<T, 128>(row_groups, tk, tv, p, err, s);
 }
 
 int kv8_rows_slices(int row_groups, int num_kv_heads, int sms) {
-  // Resident CTAs per SM: three with one group of rows, two with two (registers).
+  // Resident CTAs per SM: three with one group of rows, else two (registers).
   const int n = sms * (row_groups == 1 ? 3 : 2) / num_kv_heads;
   return n < 1 ? 1 : n;
 }
@@ -651,7 +709,9 @@ cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUten
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
                                cudaStream_t stream) {
   if (p.slices < 2) return cudaSuccess;
-  const dim3 grid(p.slices - 1, p.num_kv_heads, (p.tile_tokens * p.group + 3) / 4);
+  // Four rows a CTA in small tiles, where the parts' latency counts; in tiles of 128 rows a
+  // CTA for every row quartet would mostly look for a cut and find none.
+  const dim3 grid(p.slices - 1, p.num_kv_heads, rows > 32 ? 8 : (p.tile_tokens * p.group + 3) / 4);
   if (dtype == PA_DTYPE_F16) {
     if (head_dim == 64)
       kv8_combine_kernel<__half, 64><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);

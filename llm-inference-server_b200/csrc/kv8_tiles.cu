@@ -1,0 +1,595 @@
+// Attention of longer chunks over the 8-bit paged cache on tcgen05: tiles of 128 (token, head)
+// rows, scores and output accumulated in tensor memory.
+//
+// The arithmetic is kv8_rows.cu's: K_j = k_j 2^a_j and V_j = v_j 2^b_j are exactly fp16 numbers
+// (the cache's exponents lie in [-14, 7]), so K and V tiles are widened to fp16 in shared
+// memory with their scales multiplied in, nothing is rounded, and both products run as
+// fp16 MMAs with float32 accumulators; queries come into fp16 by a power of two per row,
+// softmax weights are rounded to fp16.  An fp8 MMA would need Q and P split into several
+// 8-bit terms to keep their bits; widening costs 1.5 instructions per two elements and is
+// done once per 128 rows.
+//
+// Work: the tiles' keys laid end to end are cut into equal slices (kv8_line.cuh, steps of 64
+// keys), two CTAs per SM in all, so a chunk of few tiles over a long context is split along
+// the context and every CTA does the same number of keys; a tile that a cut falls into
+// leaves float32 partials that kv8_combine joins.
+//
+// Roles (384 threads, registers dealt out by setmaxnreg):
+//   warps 0-3   softmax, one thread per row (TMEM lane): loads its query row into shared
+//               memory, reads scores, keeps maximum and sum, writes P to TMEM, the epilogue
+//   warps 4-5   K: global e4m3 -> fp16 in the swizzled layout, one 64-key tile ahead in
+//               registers, 3-stage ring;  warps 6-7: the same for V, 2-stage ring
+//   warp 8      TMEM allocation, S = Q K^T issue;  warp 9: O += P V issue
+//   warp 10     finds the slice's pieces (a 2-slot ring)
+// TMEM columns: S [0, 64), O [64, 64 + D), two P buffers of 32.
+//
+// Widening in registers instead of staging e4m3 by TMA: the shared memory goes to three K
+// and two V tiles of fp16 beside Q at two CTAs per SM, and a warp's 16-byte loads of a row's
+// chunks (four 128-byte rows an instruction) come mostly from L2, where the other tiles of
+// the chunk have brought them.
+//
+// Every mbarrier wait is bounded; the TMEM allocation is released on every path.
+#include <cuda_fp16.h>
+
+#include "kv8.h"
+#include "kv8_line.cuh"
+#include "kv8_widen.cuh"
+#include "pa_common.cuh"
+#include "tc_common.cuh"
+#include "tc_softmax.cuh"
+
+namespace pa {
+
+constexpr int kTileRows = 128;
+constexpr int kTileKeys = 64;
+constexpr int kTileKStages = 3;
+constexpr int kTileVStages = 2;  // equal to the P buffer count: one "P.V retired" barrier frees both
+constexpr int kTileThreads = 384;
+constexpr int kTileQHalf = kTileRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
+constexpr int kTileHalf = kTileKeys * 128;   // 64 keys x 64 elements
+constexpr int kTileConsumers = 10;           // of a piece: 4 softmax, 4 widening warps, 2 issuers
+// Fewest keys a slice gets: below this its partial costs more than the keys it takes over.
+constexpr int kTileMinKeys = 512;
+// The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 and the
+// output accumulator is rarely rescaled.
+constexpr float kTileLazy = 8.f;
+
+template <int D>
+struct TileCfg {
+  static constexpr int NH = D / 64;
+  static constexpr int Q_BYTES = NH * kTileQHalf;
+  static constexpr int KV_BYTES = NH * kTileHalf;
+  static constexpr int OFF_K = Q_BYTES;
+  static constexpr int OFF_V = OFF_K + kTileKStages * KV_BYTES;
+  static constexpr int OFF_DESC = OFF_V + kTileVStages * KV_BYTES;
+  static constexpr int OFF_NAN = OFF_DESC + 64;
+  static constexpr int OFF_BAR = OFF_NAN + 16;
+  static constexpr int SMEM = OFF_BAR + 176;
+  static constexpr uint32_t TMEM_COLS = 256;
+  static constexpr uint32_t COL_O = kTileKeys, COL_P = kTileKeys + D;
+  static_assert(COL_P + 2 * (kTileKeys / 2) <= TMEM_COLS, "TMEM budget");
+  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
+};
+
+struct TilePiece {
+  int32_t row0;    // packed index of the tile's first token; -1: no more pieces
+  int32_t tokens;  // of the tile
+  int32_t pos0;    // position of the first token
+  int32_t ctx, seq;
+  int32_t j0, j1;  // tiles of 64 keys
+  int32_t part;    // -1: the whole tile, else the CTA's partial slot
+};
+
+struct TileBars {
+  // S of tile g retired: s_full[g % 3], waited on by the softmax (scores ready) and by the K
+  // warps (the stage is free).  P.V of tile g retired: p_free[g % 2], frees P buffer and V stage.
+  uint64_t k_full[kTileKStages], s_full[kTileKStages];
+  uint64_t v_full[kTileVStages], p_full[2], p_free[2];
+  uint64_t q_full, s_consumed;
+  uint64_t d_full[2], d_empty[2];
+  uint32_t tmem_base;
+};
+
+// A scale byte as two fp16 copies of 2^(b - 127); 255 is NaN.
+__device__ __forceinline__ uint32_t scale_h2(uint32_t b) {
+  const uint32_t h = b == 255u ? 0x7e00u : (max(113u, min(134u, b)) - 112u) << 10;
+  return h | (h << 16);
+}
+
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// One widening warp's half (32 keys) of a 64-key tile: loads into registers, later widened
+// into the swizzled tile.  Lanes take 16-byte chunks, D / 16 lanes a row.
+template <int D>
+struct WidenHalf {
+  static constexpr int LPR = D / 16;      // lanes a row
+  static constexpr int RPI = 32 / LPR;    // rows an instruction
+  static constexpr int N = 32 / RPI;      // instructions
+  uint4 x[N];
+  uint32_t scale;                         // of key `lane`
+  int live;                               // keys of this half inside the context
+
+  __device__ __forceinline__ void load(const uint8_t* pool, const uint8_t* scales, const int32_t* row, int key0,
+                                       int kvh, int lane, int ctx, const Kv8AttnParams& p, int* err) {
+    live = min(32, ctx - key0);
+    scale = 0;
+    const int shift = p.block_shift + 4;
+    // The 32 keys lie in two groups of 16, each inside one block.
+    int slot[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      slot[b] = 0;
+      const int k = key0 + 16 * b;
+      if (k < ctx) {
+        int id = __ldg(row + (k >> shift));
+        if (id < 0 || id >= p.pool_blocks) {
+          if (lane == 0) set_error(err, PA_KV8_ERR_BLOCK);
+          id = 0;
+        }
+        const int off = k & ((1 << shift) - 1);
+        slot[b] = (id << shift) + off;
+        if ((lane >> 4) == b && lane < live)
+          scale = __ldg(scales + ((int64_t(id) * p.num_kv_heads + kvh) << shift) + off + (lane & 15));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * RPI + lane / LPR;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if (r < live)
+        x[i] = __ldg(reinterpret_cast<const uint4*>(
+            pool + ((int64_t(slot[r >> 4]) + (r & 15)) * p.num_kv_heads + kvh) * D + 16 * (lane % LPR)));
+    }
+  }
+
+  // `nan_rows`: V's rows that stand for NaN are widened to zeros and reported as bits.
+  template <bool V>
+  __device__ __forceinline__ void store(uint8_t* tile, int row0, int lane, uint16_t* nan_rows) {
+    const bool bad = V && scale == 255u && lane < live;
+    const uint32_t nans = V ? __ballot_sync(0xffffffffu, bad) : 0u;
+    const uint32_t s2 = bad ? 0u : scale_h2(scale);
+    if (V && lane < 2) nan_rows[lane] = uint16_t(nans >> (16 * lane));
+    const int q = lane % LPR, half = D == 128 ? q >> 2 : 0, c0 = 2 * (q & 3);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int r = i * RPI + lane / LPR, row = row0 + r;
+      const uint32_t sc = __shfl_sync(0xffffffffu, s2, r);
+      const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+      uint4 o[2];
+      o[0] = make_uint4(mul_h2(widen_lo(w[0]), sc), mul_h2(widen_hi(w[0]), sc), mul_h2(widen_lo(w[1]), sc),
+                        mul_h2(widen_hi(w[1]), sc));
+      o[1] = make_uint4(mul_h2(widen_lo(w[2]), sc), mul_h2(widen_hi(w[2]), sc), mul_h2(widen_lo(w[3]), sc),
+                        mul_h2(widen_hi(w[3]), sc));
+      // The two 64-column halves of a row map to the same banks: the second goes odd chunk first.
+      uint8_t* dst = tile + half * kTileHalf;
+      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + half)) = half ? o[1] : o[0];
+      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + 1 - half)) = half ? o[0] : o[1];
+    }
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8AttnParams p, int* err) {
+  using C = TileCfg<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  uint8_t* sQ = smem;
+  uint8_t* sK = smem + C::OFF_K;
+  uint8_t* sV = smem + C::OFF_V;
+  TilePiece* desc = reinterpret_cast<TilePiece*>(smem + C::OFF_DESC);
+  uint16_t* nan_rows = reinterpret_cast<uint16_t*>(smem + C::OFF_NAN);  // [V stage][4]
+  TileBars* bars = reinterpret_cast<TileBars*>(smem + C::OFF_BAR);
+  static_assert(sizeof(TileBars) <= 176, "barrier area");
+  static_assert(2 * sizeof(TilePiece) <= 64, "descriptor area");
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
+  const int64_t total = p.work[p.num_seqs];
+  const int slices = line_slices(total, p.slices, kTileMinKeys);
+  if (total == 0 || slice >= slices) return;
+
+  if (warp == 8) {
+    tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int s = 0; s < kTileKStages; ++s) {
+      mbar_init(&bars->k_full[s], 2);
+      mbar_init(&bars->s_full[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bars->v_full[s], 2);
+      mbar_init(&bars->p_full[s], 128);
+      mbar_init(&bars->p_free[s], 1);
+      mbar_init(&bars->d_full[s], 1);
+      mbar_init(&bars->d_empty[s], kTileConsumers);
+    }
+    mbar_init(&bars->q_full, 128);
+    mbar_init(&bars->s_consumed, 128);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tbase = bars->tmem_base;
+  const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
+
+  // The next piece of the ring, for one consuming warp; false when a wait ran out.
+  auto next_piece = [&](int k, TilePiece& d) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->d_full[k & 1], (k >> 1) & 1));
+    if (ok) {
+      d = desc[k & 1];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bars->d_empty[k & 1]);
+    }
+    return ok;
+  };
+
+  bool ok = true;
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 10) {
+      // ---------------------------------------------------------- pieces
+      const int64_t x1 = line_cut(total, slices, slice + 1);
+      int64_t x = line_cut(total, slices, slice);
+      int hint = 0;
+      for (int k = 0;; ++k) {
+        LineTile t;
+        t.seq = -1;
+        int k0 = 0, k1 = 0;
+        while (x < x1) {
+          t = line_find(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens, x, hint);
+          if (t.seq < 0) break;
+          hint = t.seq;
+          k0 = line_key(t, x, kTileKeys);
+          k1 = line_key(t, x1, kTileKeys);
+          x = t.start + t.keys;
+          if (k1 > k0) break;
+          t.seq = -1;
+        }
+        if (k >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars->d_empty[k & 1], ((k >> 1) - 1) & 1));
+        if (!ok) break;
+        if (lane == 0) {
+          TilePiece d{};
+          d.row0 = -1;
+          if (t.seq >= 0) {
+            const int first = p.cu_q[t.seq], q = p.cu_q[t.seq + 1] - first, t0 = t.index * p.tile_tokens;
+            d.row0 = first + t0;
+            d.tokens = min(p.tile_tokens, q - t0);
+            d.ctx = p.ctx_lens[t.seq];
+            d.pos0 = d.ctx - q + t0;
+            d.seq = t.seq;
+            d.j0 = k0 / kTileKeys;
+            d.j1 = (k1 + kTileKeys - 1) / kTileKeys;
+            d.part = k0 > 0 ? 0 : (k1 < t.keys ? 1 : -1);
+          }
+          desc[k & 1] = d;
+          mbar_arrive(&bars->d_full[k & 1]);
+        }
+        if (t.seq < 0) break;
+      }
+    } else if (warp == 8) {
+      // ---------------------------------------------------------- S issue
+      int g = 0;
+      for (int k = 0; ok; ++k) {
+        TilePiece d;
+        ok = next_piece(k, d);
+        if (!ok || d.row0 < 0) break;
+        if (lane == 0) {
+          constexpr uint32_t idS = idesc_f16<__half>(kTileRows, kTileKeys, false);
+          const uint32_t q0 = smem_u32(sQ);
+          if (!mbar_wait(&bars->q_full, k & 1)) ok = false;
+          for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
+            const int s = g % kTileKStages;
+            if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1) ||
+                (g > 0 && !mbar_wait(&bars->s_consumed, (g - 1) & 1))) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t k0 = smem_u32(sK + s * C::KV_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < D / 16; ++kk) {
+              const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQHalf + (kk & 3) * 32, 16, 1024);
+              const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileHalf + (kk & 3) * 32, 16, 1024);
+              umma_f16(tS, ad, bd, idS, kk > 0 ? 1u : 0u);
+            }
+            umma_commit(&bars->s_full[s]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        g = __shfl_sync(0xffffffffu, g, 0);
+      }
+    } else if (warp == 9) {
+      // ---------------------------------------------------------- P.V issue
+      int g = 0;
+      for (int k = 0; ok; ++k) {
+        TilePiece d;
+        ok = next_piece(k, d);
+        if (!ok || d.row0 < 0) break;
+        if (lane == 0) {
+          constexpr uint32_t idO = idesc_f16<__half>(kTileRows, D, true);
+          for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
+            const int s = g & 1;
+            if (!mbar_wait(&bars->p_full[s], (g >> 1) & 1) || !mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint32_t v0 = smem_u32(sV + s * C::KV_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < kTileKeys / 16; ++kk) {
+              const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileHalf, 1024);
+              umma_f16_ts(tO, tP + s * (kTileKeys / 2) + 8 * kk, bd, idO, (j > d.j0 || kk > 0) ? 1u : 0u);
+            }
+            umma_commit(&bars->p_free[s]);
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+        g = __shfl_sync(0xffffffffu, g, 0);
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ widening
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    const bool is_v = warp >= 6;
+    const int row0 = 32 * (warp & 1);
+    const uint8_t* pool = is_v ? p.v_pool : p.k_pool;
+    const uint8_t* scales = is_v ? p.v_scale : p.k_scale;
+    const int stages = is_v ? kTileVStages : kTileKStages;
+    uint64_t* full = is_v ? bars->v_full : bars->k_full;
+    uint64_t* freed = is_v ? bars->p_free : bars->s_full;
+    uint8_t* ring = is_v ? sV : sK;
+    int s = 0, round = 0;
+    WidenHalf<D> half;
+    for (int k = 0; ok; ++k) {
+      TilePiece d;
+      ok = next_piece(k, d);
+      if (!ok || d.row0 < 0) break;
+      const int32_t* row = p.tables + int64_t(d.seq) * p.table_stride;
+      half.load(pool, scales, row, d.j0 * kTileKeys + row0, kvh, lane, d.ctx, p, err);
+      for (int j = d.j0; j < d.j1; ++j) {
+        if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&freed[s], (round - 1) & 1));
+        if (!ok) break;
+        if (is_v)
+          half.template store<true>(ring + s * C::KV_BYTES, row0, lane, nan_rows + 4 * s + 2 * (warp & 1));
+        else
+          half.template store<false>(ring + s * C::KV_BYTES, row0, lane, nullptr);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+        if (j + 1 < d.j1)
+          half.load(pool, scales, row, (j + 1) * kTileKeys + row0, kvh, lane, d.ctx, p, err);
+        if (++s == stages) {
+          s = 0;
+          ++round;
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ softmax (one row per thread)
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    const uint32_t lane_base = uint32_t(warp * 32) << 16;
+    const int r = tid, t_row = r / p.group, head = kvh * p.group + (r - t_row * p.group);
+    int g = 0;
+    for (int k = 0; ok; ++k) {
+      TilePiece d;
+      ok = next_piece(k, d);
+      if (!ok || d.row0 < 0) break;
+      const int t_eff = min(t_row, d.tokens - 1);  // spare rows repeat the last token and are not stored
+      const int qpos = d.pos0 + t_eff;
+
+      // The query row as fp16 into the swizzled tile.  The previous piece's last S has retired
+      // (its scores were read), so the tile is free.
+      float qs;
+      {
+        const T* src = static_cast<const T*>(p.q) + int64_t(d.row0 + t_eff) * p.q_st + int64_t(head) * p.q_sh;
+        float big = 0.f;
+        if (DType<T>::code == PA_DTYPE_BF16) {
+#pragma unroll 4
+          for (int c = 0; c < D / 8; ++c) {
+            const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * c);
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = unpack2(u[i], (T*)nullptr);
+              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+          }
+        }
+        // The scores' maximum is taken before the scale, so the scale's sign goes into the row.
+        const float up = query_power<T>(big);
+        qs = fmaxf(fabsf(p.qscale) / up, 1e-37f);
+        const float mul = p.qscale < 0.f ? -up : up;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+          const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * c);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          uint32_t o[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack2(u[i], (T*)nullptr);
+            o[i] = pack2<__half>(f.x * mul, f.y * mul);
+          }
+          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQHalf + sw_off(r, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(&bars->q_full);
+      }
+
+      float m_run = -INFINITY, l_run = 0.f;
+      for (int j = d.j0; j < d.j1; ++j, ++g) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[g % kTileKStages], (g / kTileKStages) & 1));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sr[kTileKeys];
+        tmem_ld32_at<0>(tS + lane_base + 0, sr);
+        tmem_ld32_at<32>(tS + lane_base + 32, sr);
+        tmem_wait_ld();
+        tc_fence_before();
+        mbar_arrive(&bars->s_consumed);
+
+        const int lim = qpos - j * kTileKeys;  // key column c is visible iff c <= lim
+        if (__any_sync(0xffffffffu, lim < kTileKeys - 1)) {
+#pragma unroll
+          for (int c = 0; c < kTileKeys; ++c) sr[c] = c <= lim ? sr[c] : __float_as_uint(-INFINITY);
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kTileKeys; c += 2)
+          mx4[(c >> 1) & 3] = fmax3(mx4[(c >> 1) & 3], __uint_as_float(sr[c]), __uint_as_float(sr[c + 1]));
+        const float mx_s = fmax3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * qs;
+        const bool grow = mx_s > m_run + kTileLazy;
+        const float m_new = grow ? mx_s : m_run;
+        const float alpha = grow ? ex2(m_run - m_new) : 1.f;
+        // A piece may start past a row's last key: nothing seen, all weights 0.
+        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const uint64_t sc2 = f2pack(qs, qs), mn2 = f2pack(-ref, -ref);
+        uint64_t rs2[2] = {0ull, 0ull};
+        uint32_t pk[kTileKeys / 2];
+#pragma unroll
+        for (int c = 0; c < kTileKeys; c += 2) {
+          float x0, x1;
+          f2unpack(fma2(f2pack(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), sc2, mn2), x0, x1);
+          const float e0 = ex2(x0), e1 = ex2(x1);
+          rs2[(c >> 1) & 1] = add2(rs2[(c >> 1) & 1], f2pack(e0, e1));
+          pk[c / 2] = pack2<__half>(e0, e1);
+        }
+        float r0, r1, r2, r3;
+        f2unpack(rs2[0], r0, r1);
+        f2unpack(rs2[1], r2, r3);
+        l_run = l_run * alpha + ((r0 + r1) + (r2 + r3));
+        m_run = m_new;
+
+        const int pb = g & 1;
+        if (g >= 2) {  // the P.V that read this buffer two tiles ago has retired
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[pb], ((g - 2) >> 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+        }
+        // V rows that stand for NaN: the weight of a key that is seen becomes NaN, others stay 0.
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[pb], (g >> 1) & 1));
+        if (!ok) break;
+        const uint2 nans = *reinterpret_cast<const uint2*>(nan_rows + 4 * pb);
+        if ((nans.x | nans.y) != 0u) {
+#pragma unroll
+          for (int c = 0; c < kTileKeys; ++c) {
+            const bool hit = (((c < 32 ? nans.x : nans.y) >> (c & 31)) & 1u) && c <= lim;
+            if (hit) pk[c / 2] |= (c & 1) ? 0x7e000000u : 0x00007e00u;
+          }
+        }
+        tmem_st32(tP + lane_base + pb * (kTileKeys / 2), *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+        if (j > d.j0 && __any_sync(0xffffffffu, grow)) {  // O *= alpha once the previous P.V retired
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[pb ^ 1], ((g - 1) >> 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            tmem_ld32(tO + lane_base + 32 * c, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32(tO + lane_base + 32 * c, o);
+          }
+        }
+        tmem_wait_st();
+        tc_fence_before();
+        mbar_arrive(&bars->p_full[pb]);
+      }
+      if (!ok) break;
+      // ---- epilogue, once the piece's last P.V retired
+      const int h = g - 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h & 1], (h >> 1) & 1));
+      if (!ok) break;
+      tc_fence_after();
+      const bool stored = t_row < d.tokens;
+      if (d.part < 0) {
+        const float inv = 1.f / l_run;
+        T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + t_eff) * p.o_st + int64_t(head) * p.o_sh;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + lane_base + 32 * c, o);
+          tmem_wait_ld();
+          if (stored) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint4 w;
+              w.x = pack2<T>(__uint_as_float(o[e + 0]) * inv, __uint_as_float(o[e + 1]) * inv);
+              w.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+              w.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+              w.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+              *reinterpret_cast<uint4*>(dst + 32 * c + e) = w;
+            }
+          }
+        }
+      } else {
+        const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * kTileRows + r;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld32(tO + lane_base + 32 * c, o);
+          tmem_wait_ld();
+          if (stored) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<uint4*>(p.part_o + at * D + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+        if (stored) p.part_ml[at] = make_float2(m_run, l_run);
+      }
+      // The next piece's first P.V overwrites O only after p_full, which these threads arrive
+      // on after the loads above completed (tcgen05.wait::ld).
+    }
+  }
+  if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tbase, C::TMEM_COLS);
+  }
+}
+
+// ------------------------------------------------------------------ dispatch
+template <typename T, int D>
+static cudaError_t tiles_one(const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+  using C = TileCfg<D>;
+  auto kern = kv8_tiles_kernel<T, D>;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  static bool configured[64] = {};
+  if (dev >= 64) return cudaErrorInvalidDevice;
+  if (!configured[dev]) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return e;
+    configured[dev] = true;
+  }
+  kern<<<p.slices * p.num_kv_heads, kTileThreads, C::SMEM, stream>>>(p, err);
+  return cudaGetLastError();
+}
+
+int kv8_tiles_slices(int num_kv_heads, int sms) {
+  const int n = 2 * sms / num_kv_heads;
+  return n < 1 ? 1 : n;
+}
+
+cudaError_t launch_kv8_tiles(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+  cudaError_t e;
+  if (dtype == PA_DTYPE_F16)
+    e = head_dim == 64 ? tiles_one<__half, 64>(p, err, stream) : tiles_one<__half, 128>(p, err, stream);
+  else
+    e = head_dim == 64 ? tiles_one<__nv_bfloat16, 64>(p, err, stream) : tiles_one<__nv_bfloat16, 128>(p, err, stream);
+  if (e != cudaSuccess) return e;
+  return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, stream);
+}
+
+}  // namespace pa

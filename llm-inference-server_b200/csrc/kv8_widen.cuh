@@ -1,0 +1,33 @@
+// e4m3 -> fp16 and queries -> fp16, shared by the KV8 attention kernels.
+#pragma once
+
+#include <stdint.h>
+
+#include "pa_common.cuh"
+
+namespace pa {
+
+// Two e4m3 values (low or high half of a word) as two fp16 values, exactly.
+__device__ __forceinline__ uint32_t widen_lo(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, l;\n}\n" : "=r"(r) : "r"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
+  uint32_t r;
+  asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}\n" : "=r"(r) : "r"(w));
+  return r;
+}
+
+// The power of two that brings a bf16 row with largest magnitude `big` to [2^14, 2^15), where
+// fp16 holds it exactly but for elements 2^-28 below `big`; fp16 rows stay as they are.
+template <typename T>
+__device__ __forceinline__ float query_power(float big) {
+  const uint32_t e = (__float_as_uint(big) >> 23) & 0xffu;
+  if (DType<T>::code == PA_DTYPE_F16) return 1.f;
+  if (e == 0 || e == 255) return 1.f;
+  const int up = 14 - (int(e) - 127);
+  return __uint_as_float(uint32_t(127 + max(-126, min(127, up))) << 23);
+}
+
+}  // namespace pa

@@ -439,6 +439,75 @@ def test_a_nan_row_reaches_only_the_tokens_that_see_it(pkg):
         assert torch.equal(got, clean2)
 
 
+TILES = {
+    "one tile": [(64, 64)],
+    "prompt": [(333, 333)],
+    "prompts": [(700, 700), (65, 65), (129, 129), (1, 1), (2, 2)],
+    "chunk over a prefix": [(3000, 100)],
+    "split along the context": [(9000, 40), (700, 90)],
+    "mixed with decodes": [(500, 1), (1200, 150), (64, 2), (900, 33), (0, 0), (77, 70)],
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d", [(32, 8, 128), (12, 12, 64), (14, 2, 128), (16, 1, 128), (6, 2, 64)])
+@pytest.mark.parametrize("which", list(TILES))
+def test_attention_of_long_chunks(pkg, dtype, hq, hkv, d, which):
+    lengths = TILES[which]
+    batch = _batch(lengths, hq, hkv, d, 16, dtype, seed=hq * d, extra_width=1)
+    _check_attention(pkg, *batch, d ** -0.5, most=max(q for _, q in lengths))
+    assert "kv8_tiles" in pkg._lib.last_launches()
+
+
+@pytest.mark.parametrize("bs", [32, 128])
+def test_long_chunks_other_block_sizes(pkg, bs):
+    batch = _batch([(517, 100), (70, 3), (1000, 64)], 8, 2, 128, bs, torch.bfloat16, seed=bs)
+    _check_attention(pkg, *batch, 0.1, most=100)
+
+
+def test_long_chunks_steep_scores_and_signs(pkg):
+    """Maxima that move past the headroom, a negative and a zero softmax scale, queries far
+    outside fp16."""
+    lengths = [(1500, 70), (400, 400)]
+    for dtype, q_factor, scale in ((torch.float16, 8.0, 0.3), (torch.bfloat16, 1.0, -0.2), (torch.bfloat16, 1.0, 0.0),
+                                   (torch.bfloat16, 2.0 ** -90, 0.1 * 2.0 ** 90), (torch.bfloat16, 2.0 ** 80, 2.0 ** -83)):
+        query, pools, tables, ctx, ql = _batch(lengths, 8, 2, 128, 16, dtype, seed=21, spread=2.0)
+        _check_attention(pkg, query * q_factor, pools, tables, ctx, ql, scale, most=400)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0])
+def test_few_rows_negative_and_zero_scale(pkg, scale):
+    query, pools, tables, ctx, ql = _batch([(700, 2), (33, 1)], 8, 2, 128, 16, torch.bfloat16, seed=22)
+    _check_attention(pkg, query, pools, tables, ctx, ql, scale, most=2)
+
+
+def test_long_chunks_ascending_scores(pkg):
+    """Scores that grow along the context: the running maximum rises in every tile."""
+    query, pools, tables, ctx, ql = _batch([(2000, 64)], 4, 1, 128, 16, torch.bfloat16, seed=23)
+    pools[2].fill_(120)
+    k = pools[0].view(torch.uint8)
+    pos = torch.arange(2000, device=DEV)
+    slots = tables[0].long()[pos // 16] * 16 + pos % 16
+    ramp = (pos.float() / 2000 * 400).to(ref.E4M3).view(torch.uint8)
+    k.view(-1, 1, 128)[slots] = ramp[:, None, None]
+    _check_attention(pkg, query.abs(), pools, tables, ctx, ql, 0.09, most=64)
+
+
+def test_a_nan_row_in_a_long_chunk_reaches_only_the_tokens_that_see_it(pkg):
+    query, pools, tables, ctx, ql = _batch([(300, 100), (90, 80)], 8, 2, 128, 16, torch.bfloat16, seed=24)
+    clean = pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.1, max_query_len=100)
+    for which in (0, 1):
+        p = [x.clone() for x in pools]
+        pos = 237                                     # token 37 of the first sequence
+        slot = int(tables[0, pos // 16]) * 16 + pos % 16
+        p[which].view(torch.uint8).view(-1, 2, 128)[slot] = 0
+        p[which + 2][slot // 16, 0, slot % 16] = 255
+        got = pkg.paged_attention_kv8(query, *p, tables, ctx, ql, 0.1, max_query_len=100)
+        assert got[37:100, :4].isnan().all() and not got[37:100, 4:].isnan().any()
+        got[37:100] = clean[37:100]                   # the other head's row there was zeroed with it
+        assert torch.equal(got, clean)
+
+
 def test_attention_is_deterministic_and_independent_of_neighbours(pkg):
     lengths = [(700, 2), (33, 1), (1500, 3)]
     query, pools, tables, ctx, ql = _batch(lengths, 8, 2, 128, 16, torch.bfloat16, seed=15)
