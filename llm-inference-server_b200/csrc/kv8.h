@@ -64,7 +64,9 @@ int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
 cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
                             const Kv8AttnParams& p, int* err, cudaStream_t stream);
 int kv8_tiles_slices(int num_kv_heads, int sms);
-cudaError_t launch_kv8_tiles(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const Kv8AttnParams& p, int* err, cudaStream_t stream);
+constexpr int kKv8TileRows = 256;  // (token, head) rows of its tiles
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
                                cudaStream_t stream);
 

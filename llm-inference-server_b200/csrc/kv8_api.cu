@@ -14,18 +14,19 @@ static int32_t kv8_cuda_fail(cudaError_t e, const char* what) {
   return fail(PA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-// A payload pool [NB, BS, Hkv, D] as the 3-D tensor (D, Hkv, NB * BS), box (D, 1, rows),
-// swizzled over the row's width.
-static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, int dim, int rows, CUtensorMap* out) {
+// A payload pool [NB, BS, Hkv, D] as the 3-D tensor (D, Hkv, NB * BS), box (D, 1, 16), dense
+// or swizzled over the row's width.
+static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, int dim, bool swizzle, CUtensorMap* out) {
   auto fn = tensor_map_encoder();
   if (!fn) return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   cuuint64_t gdim[3] = {cuuint64_t(dim), cuuint64_t(hkv), cuuint64_t(blocks) * cuuint64_t(bs)};
   cuuint64_t gstride[2] = {cuuint64_t(dim), cuuint64_t(hkv) * dim};
-  cuuint32_t box[3] = {cuuint32_t(dim), 1u, cuuint32_t(rows)};
+  cuuint32_t box[3] = {cuuint32_t(dim), 1u, 16u};
   cuuint32_t estride[3] = {1u, 1u, 1u};
   CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)(
       out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pool), gdim, gstride, box, estride,
-      CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+      CU_TENSOR_MAP_INTERLEAVE_NONE,
+      !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : (dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B),
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit pool) failed (CUresult %d)", int(r));
   return PA_OK;
@@ -57,7 +58,7 @@ static Kv8Scratch attention_scratch(const pa_kv8_tiling& t, int32_t num_seqs, in
   s.ml = (s.cu + (uint64_t(num_seqs) + 1) * sizeof(int32_t) + 255) / 256 * 256;
   s.o = (s.ml + rows * sizeof(float2) + 255) / 256 * 256;
   s.tile_ml = (s.o + rows * head_dim * sizeof(float) + 255) / 256 * 256;
-  const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * 128 : 0;
+  const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * kKv8TileRows : 0;
   s.tile_o = (s.tile_ml + tile_rows * sizeof(float2) + 255) / 256 * 256;
   s.bytes = s.tile_o + tile_rows * head_dim * sizeof(float);
   return s;
@@ -90,14 +91,14 @@ int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, pa_kv8_tiling
   if (!tiling) return fail(PA_ERR_INVALID_ARGUMENT, "tiling must not be NULL");
   if (group < 1 || max_query_len < 0) return fail(PA_ERR_INVALID_ARGUMENT, "bad group or max_query_len");
   if (group > 16) return fail(PA_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16 are supported", group);
-  // A sequence of up to 32 (token, head) rows goes to the kernel for few rows, one of more to
-  // the 128-row tiles.
-  const int few = std::max(1, 32 / group);
+  // A sequence of up to 16 (token, head) rows goes to the kernel for few rows, one of more to
+  // the 256-row tiles.
+  const int few = std::max(1, 16 / group);
   const int rows = group * std::max(1, std::min(max_query_len, few));
   tiling->row_groups = (rows + 7) / 8;
   tiling->small_tokens = std::max(1, 8 * tiling->row_groups / group);
   tiling->small_max = std::min(max_query_len, few);
-  tiling->large_tokens = 128 / group;
+  tiling->large_tokens = kKv8TileRows / group;
   return PA_OK;
 }
 
@@ -305,8 +306,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     work = b.work;
   }
   CUtensorMap tk, tv;
-  st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, 16, &tk);
-  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, 16, &tv);
+  st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, true, &tk);
+  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, true, &tv);
   if (st != PA_OK) return st;
   Kv8AttnParams p{};
   p.q = query;
@@ -344,7 +345,10 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     p.slices = kv8_tiles_slices(num_kv_heads, sms);
     p.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
     p.part_o = reinterpret_cast<float*>(ws + s.tile_o);
-    e = launch_kv8_tiles(dtype, head_dim, p, err, stream);
+    st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tk);
+    if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tv);
+    if (st != PA_OK) return st;
+    e = launch_kv8_tiles(dtype, head_dim, tk, tv, p, err, stream);
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
     note_launches(PA_LAUNCH_KV8_TILES | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
   }

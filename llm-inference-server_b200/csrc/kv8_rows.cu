@@ -579,10 +579,13 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
 }
 
 // Joins the partials of tiles that a cut fell into.  CTA (s, kvh): the tile that the end of
-// slice s falls into, if this is the first cut inside it.  A warp takes a row at a time.
-template <typename T, int D>
+// slice s falls into, if this is the first cut inside it.  A warp takes NR rows at a time, a
+// lane D / 32 elements of each.  What bounds it is latency (places, then (m, l), then
+// accumulators), so NR x P accumulator loads are in flight: one row and eight parts for the
+// few rows of a long context, four rows and two parts for 256-row tiles.
+template <typename T, int D, int NR, int P>
 __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys) {
-  constexpr int E = D / 32;  // elements a lane
+  constexpr int E = D / 32;
   const int64_t total = p.work[p.num_seqs];
   const int slices = line_slices(total, p.slices, min_keys);
   const int s = blockIdx.x + 1, kvh = blockIdx.y;
@@ -596,59 +599,78 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
   const int64_t end = t.start + t.keys;
   int last = s;
   while (last + 1 < slices && line_cut(total, slices, last + 1) < end) ++last;
-  for (int r = blockIdx.z * 4 + warp; r < min(p.tile_tokens, q - t0) * p.group; r += 4 * gridDim.z) {
-    const int tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
-
+  const int live = min(p.tile_tokens, q - t0) * p.group;  // rows of the tile
+  for (int r0 = (blockIdx.z * 4 + warp) * NR; r0 < live; r0 += 4 * NR * gridDim.z) {
     // A slice's part of the tile is its slot 1 if it starts the tile, else slot 0; it is empty
-    // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time; the
-    // parts' accumulators are then read with nothing between the loads.
-    float acc[E], m = -INFINITY, sum = 0.f;
-  #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time.
+    float acc[NR][E], m[NR], sum[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      m[n] = -INFINITY;
+      sum[n] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
+    }
     for (int i0 = s - 1; i0 <= last; i0 += 32) {
       const int i = i0 + lane;
-      float2 v = make_float2(-INFINITY, 0.f);
-      int64_t at = 0;
-      if (i <= last &&
-          line_key(t, line_cut(total, slices, i + 1), key_step) > line_key(t, line_cut(total, slices, i), key_step)) {
-        at = ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r;
-        v = p.part_ml[at];
+      const bool mine = i <= last && line_key(t, line_cut(total, slices, i + 1), key_step) >
+                                         line_key(t, line_cut(total, slices, i), key_step);
+      const int64_t at = mine ? ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r0 : -1;
+      float2 v[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n)
+        v[n] = mine && r0 + n < live ? p.part_ml[at + n] : make_float2(-INFINITY, 0.f);
+      float f[NR];
+#pragma unroll
+      for (int n = 0; n < NR; ++n) {
+        float mn = v[n].x;
+#pragma unroll
+        for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
+        mn = fmaxf(mn, m[n]);
+        const float ref = mn == -INFINITY ? 0.f : mn, old = ex2(m[n] - ref);
+        f[n] = ex2(v[n].x - ref);
+        m[n] = mn;
+        float part = v[n].y * f[n];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
+        sum[n] = sum[n] * old + part;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[n][e] *= old;
       }
-      float mn = v.x;
-  #pragma unroll
-      for (int d = 16; d; d >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, d));
-      mn = fmaxf(mn, m);
-      const float ref = mn == -INFINITY ? 0.f : mn, old = ex2(m - ref), f = ex2(v.x - ref);
-      m = mn;
-      float part = v.y * f;
-  #pragma unroll
-      for (int d = 16; d; d >>= 1) part += __shfl_xor_sync(0xffffffffu, part, d);
-      sum = sum * old + part;
-  #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] *= old;
-      const int n = min(32, last + 1 - i0);
-      for (int k0 = 0; k0 < n; k0 += 8) {
-        float o[8][E], fk[8];
-  #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          fk[k] = __shfl_sync(0xffffffffu, f, k0 + k);
-          const int64_t ak = __shfl_sync(0xffffffffu, at, k0 + k);
-          const bool some = __shfl_sync(0xffffffffu, v.x, k0 + k) != -INFINITY;  // NaN counts
-  #pragma unroll
-          for (int e = 0; e < E; ++e) o[k][e] = 0.f;
-          if (some) VecLoad<float, E>::run(p.part_o + ak * D + E * lane, o[k]);
+      const int parts = min(32, last + 1 - i0);
+      for (int k0 = 0; k0 < parts; k0 += P) {
+        float o[P][NR][E], fk[P][NR];
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+          const int64_t ak = __shfl_sync(0xffffffffu, at, (k0 + k) & 31);
+#pragma unroll
+          for (int n = 0; n < NR; ++n) {
+            fk[k][n] = __shfl_sync(0xffffffffu, f[n], (k0 + k) & 31);
+#pragma unroll
+            for (int e = 0; e < E; ++e) o[k][n][e] = 0.f;
+            if (k0 + k < parts && ak >= 0 && r0 + n < live)
+              VecLoad<float, E>::run(p.part_o + (ak + n) * D + E * lane, o[k][n]);
+          }
         }
-  #pragma unroll
-        for (int k = 0; k < 8; ++k)
-  #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] += o[k][e] * fk[k];
+#pragma unroll
+        for (int k = 0; k < P; ++k)
+#pragma unroll
+          for (int n = 0; n < NR; ++n)
+            if (k0 + k < parts)
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc[n][e] += o[k][n][e] * fk[k][n];
       }
     }
-    T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
-    const float inv = 1.f / sum;
-  #pragma unroll
-    for (int e = 0; e < E; e += 2)
-      *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[e] * inv, acc[e + 1] * inv);
+#pragma unroll
+    for (int n = 0; n < NR; ++n) {
+      const int r = r0 + n, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
+      if (r >= live) break;
+      T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
+      const float inv = 1.f / sum[n];
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        *reinterpret_cast<uint32_t*>(dst + e) = pack2<T>(acc[n][e] * inv, acc[n][e + 1] * inv);
+    }
   }
 }
 
@@ -706,23 +728,27 @@ cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUten
   return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, kRowsMinKeys, p, stream);
 }
 
+template <typename T, int D>
+static void combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, cudaStream_t stream) {
+  const int live = p.tile_tokens * p.group;
+  if (rows <= 32) {
+    const dim3 grid(p.slices - 1, p.num_kv_heads, (live + 3) / 4);
+    kv8_combine_kernel<T, D, 1, 8><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
+  } else {
+    const dim3 grid(p.slices - 1, p.num_kv_heads, (live + 15) / 16);
+    kv8_combine_kernel<T, D, 4, 2><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
+  }
+}
+
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
                                cudaStream_t stream) {
   if (p.slices < 2) return cudaSuccess;
-  // Four rows a CTA in small tiles, where the parts' latency counts; in tiles of 128 rows a
-  // CTA for every row quartet would mostly look for a cut and find none.
-  const dim3 grid(p.slices - 1, p.num_kv_heads, rows > 32 ? 8 : (p.tile_tokens * p.group + 3) / 4);
-  if (dtype == PA_DTYPE_F16) {
-    if (head_dim == 64)
-      kv8_combine_kernel<__half, 64><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-    else
-      kv8_combine_kernel<__half, 128><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-  } else {
-    if (head_dim == 64)
-      kv8_combine_kernel<__nv_bfloat16, 64><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-    else
-      kv8_combine_kernel<__nv_bfloat16, 128><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-  }
+  if (dtype == PA_DTYPE_F16)
+    head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, stream)
+                   : combine_one<__half, 128>(rows, key_step, min_keys, p, stream);
+  else
+    head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, stream)
+                   : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, stream);
   return cudaGetLastError();
 }
 

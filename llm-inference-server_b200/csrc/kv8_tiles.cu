@@ -1,5 +1,6 @@
-// Attention of longer chunks over the 8-bit paged cache on tcgen05: tiles of 128 (token, head)
-// rows, scores and output accumulated in tensor memory.
+// Attention of longer chunks over the 8-bit paged cache on tcgen05: tiles of 256 (token, head)
+// rows, two halves of 128 that share every K and V tile, scores and output accumulated in
+// tensor memory.
 //
 // The arithmetic is kv8_rows.cu's: K_j = k_j 2^a_j and V_j = v_j 2^b_j are exactly fp16 numbers
 // (the cache's exponents lie in [-14, 7]), so K and V tiles are widened to fp16 in shared
@@ -7,26 +8,29 @@
 // fp16 MMAs with float32 accumulators; queries come into fp16 by a power of two per row,
 // softmax weights are rounded to fp16.  An fp8 MMA would need Q and P split into several
 // 8-bit terms to keep their bits; widening costs 1.5 instructions per two elements and is
-// done once per 128 rows.
+// done once per 256 rows.
 //
 // Work: the tiles' keys laid end to end are cut into equal slices (kv8_line.cuh, steps of 64
-// keys), two CTAs per SM in all, so a chunk of few tiles over a long context is split along
+// keys), one CTA per SM in all, so a chunk of few tiles over a long context is split along
 // the context and every CTA does the same number of keys; a tile that a cut falls into
 // leaves float32 partials that kv8_combine joins.
 //
-// Roles (384 threads, registers dealt out by setmaxnreg):
-//   warps 0-3   softmax, one thread per row (TMEM lane): loads its query row into shared
-//               memory, reads scores, keeps maximum and sum, writes P to TMEM, the epilogue
-//   warps 4-5   K: global e4m3 -> fp16 in the swizzled layout, one 64-key tile ahead in
-//               registers, 3-stage ring;  warps 6-7: the same for V, 2-stage ring
-//   warp 8      TMEM allocation, S = Q K^T issue;  warp 9: O += P V issue
-//   warp 10     finds the slice's pieces (a 2-slot ring)
-// TMEM columns: S [0, 64), O [64, 64 + D), two P buffers of 32.
+// Roles (640 threads, registers dealt out by setmaxnreg):
+//   warps 0-3, 4-7  softmax of rows 0-127 / 128-255, one thread per row (TMEM lane): loads its
+//                   query row into shared memory, reads scores, keeps maximum and sum, writes
+//                   P to TMEM, the epilogue
+//   warps 8-9       K: staged e4m3 -> fp16 in the swizzled layout (3 stages); 10-11: V (2)
+//   warps 12, 13    S = Q K^T issue of either half (12 also allocates TMEM)
+//   warps 14, 15    O += P V issue of either half
+//   warps 16, 17    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
+//                   staging rings of 4 tiles
+//   warp 18         finds the slice's pieces (a 2-slot ring)
+// TMEM columns of a half: S [0, 64), O [64, 64 + D), two P buffers of 32.
 //
-// Widening in registers instead of staging e4m3 by TMA: the shared memory goes to three K
-// and two V tiles of fp16 beside Q at two CTAs per SM, and a warp's 16-byte loads of a row's
-// chunks (four 128-byte rows an instruction) come mostly from L2, where the other tiles of
-// the chunk have brought them.
+// The staging rings are what the widening needs: with a tile's loads in registers, one tile
+// ahead, 128-row tiles and two CTAs per SM the loads' latency (over 1 us per tile) was
+// exposed and 1,000 tokens over 16,384 keys took 546 us; without any loads the same kernel
+// took 291, without widening 254.
 //
 // Every mbarrier wait is bounded; the TMEM allocation is released on every path.
 #include <cuda_fp16.h>
@@ -40,36 +44,21 @@
 
 namespace pa {
 
-constexpr int kTileRows = 128;
+constexpr int kTileRows = kKv8TileRows;
+constexpr int kHalfRows = 128;
 constexpr int kTileKeys = 64;
 constexpr int kTileKStages = 3;
 constexpr int kTileVStages = 2;  // equal to the P buffer count: one "P.V retired" barrier frees both
-constexpr int kTileThreads = 384;
-constexpr int kTileQHalf = kTileRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
-constexpr int kTileHalf = kTileKeys * 128;   // 64 keys x 64 elements
-constexpr int kTileConsumers = 10;           // of a piece: 4 softmax, 4 widening warps, 2 issuers
+constexpr int kTileRing = 4;     // staged e4m3 tiles, K and V each
+constexpr int kTileThreads = 640;
+constexpr int kTileQBox = kHalfRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
+constexpr int kTileBox = kTileKeys * 128;   // 64 keys x 64 elements
+constexpr int kTileConsumers = 18;          // warps that read a piece: 8 softmax, 4 widening, 4 issuers, 2 producers
 // Fewest keys a slice gets: below this its partial costs more than the keys it takes over.
 constexpr int kTileMinKeys = 512;
 // The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 and the
 // output accumulator is rarely rescaled.
 constexpr float kTileLazy = 8.f;
-
-template <int D>
-struct TileCfg {
-  static constexpr int NH = D / 64;
-  static constexpr int Q_BYTES = NH * kTileQHalf;
-  static constexpr int KV_BYTES = NH * kTileHalf;
-  static constexpr int OFF_K = Q_BYTES;
-  static constexpr int OFF_V = OFF_K + kTileKStages * KV_BYTES;
-  static constexpr int OFF_DESC = OFF_V + kTileVStages * KV_BYTES;
-  static constexpr int OFF_NAN = OFF_DESC + 64;
-  static constexpr int OFF_BAR = OFF_NAN + 16;
-  static constexpr int SMEM = OFF_BAR + 176;
-  static constexpr uint32_t TMEM_COLS = 256;
-  static constexpr uint32_t COL_O = kTileKeys, COL_P = kTileKeys + D;
-  static_assert(COL_P + 2 * (kTileKeys / 2) <= TMEM_COLS, "TMEM budget");
-  static_assert(2 * (SMEM + 1024) <= 228 * 1024, "two CTAs per SM");
-};
 
 struct TilePiece {
   int32_t row0;    // packed index of the tile's first token; -1: no more pieces
@@ -81,13 +70,35 @@ struct TilePiece {
 };
 
 struct TileBars {
-  // S of tile g retired: s_full[g % 3], waited on by the softmax (scores ready) and by the K
-  // warps (the stage is free).  P.V of tile g retired: p_free[g % 2], frees P buffer and V stage.
-  uint64_t k_full[kTileKStages], s_full[kTileKStages];
-  uint64_t v_full[kTileVStages], p_full[2], p_free[2];
-  uint64_t q_full, s_consumed;
+  // Staging: tile s of a ring has landed (an arrival per 16 keys) / was read by both warps.
+  uint64_t st_full[2][kTileRing], st_empty[2][kTileRing];
+  // S of tile g retired (per half): s_full[h][g % 3]; both halves' free K stage g % 3.
+  // P.V of tile g retired: p_free[h][g % 2], frees the half's P buffer and, both, V stage g % 2.
+  uint64_t k_full[kTileKStages], s_full[2][kTileKStages];
+  uint64_t v_full[kTileVStages], p_full[2][2], p_free[2][2];
+  uint64_t q_full[2], s_consumed[2];
   uint64_t d_full[2], d_empty[2];
   uint32_t tmem_base;
+};
+
+template <int D>
+struct TileCfg {
+  static constexpr int NH = D / 64;
+  static constexpr int Q_BYTES = 2 * NH * kTileQBox;
+  static constexpr int KV_BYTES = NH * kTileBox;
+  static constexpr int ST_BYTES = kTileKeys * D;
+  static constexpr int OFF_K = Q_BYTES;
+  static constexpr int OFF_V = OFF_K + kTileKStages * KV_BYTES;
+  static constexpr int OFF_ST = OFF_V + kTileVStages * KV_BYTES;          // [K, V][ring]
+  static constexpr int OFF_SCALE = OFF_ST + 2 * kTileRing * ST_BYTES;     // [K, V][ring][64]
+  static constexpr int OFF_DESC = OFF_SCALE + 2 * kTileRing * kTileKeys;
+  static constexpr int OFF_NAN = OFF_DESC + 2 * int(sizeof(TilePiece));   // [V stage][4 x 16 keys]
+  static constexpr int OFF_BAR = OFF_NAN + 16;
+  static constexpr int SMEM = OFF_BAR + int(sizeof(TileBars));
+  static constexpr uint32_t TMEM_COLS = 512, COL_HALF = 256;
+  static constexpr uint32_t COL_O = kTileKeys, COL_P = kTileKeys + D;
+  static_assert(COL_P + 2 * (kTileKeys / 2) <= COL_HALF, "TMEM budget");
+  static_assert(SMEM <= 227 * 1024 && OFF_DESC % 16 == 0 && OFF_BAR % 8 == 0, "shared memory");
 };
 
 // A scale byte as two fp16 copies of 2^(b - 127); 255 is NaN.
@@ -102,7 +113,7 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// One widening warp's half (32 keys) of a 64-key tile: loads into registers, later widened
+// A widening warp's half (32 keys) of a staged 64-key tile: read into registers, then widened
 // into the swizzled tile.  Lanes take 16-byte chunks, D / 16 lanes a row.
 template <int D>
 struct WidenHalf {
@@ -111,49 +122,25 @@ struct WidenHalf {
   static constexpr int N = 32 / RPI;      // instructions
   uint4 x[N];
   uint32_t scale;                         // of key `lane`
-  int live;                               // keys of this half inside the context
 
-  __device__ __forceinline__ void load(const uint8_t* pool, const uint8_t* scales, const int32_t* row, int key0,
-                                       int kvh, int lane, int ctx, const Kv8AttnParams& p, int* err) {
-    live = min(32, ctx - key0);
-    scale = 0;
-    const int shift = p.block_shift + 4;
-    // The 32 keys lie in two groups of 16, each inside one block.
-    int slot[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      slot[b] = 0;
-      const int k = key0 + 16 * b;
-      if (k < ctx) {
-        int id = __ldg(row + (k >> shift));
-        if (id < 0 || id >= p.pool_blocks) {
-          if (lane == 0) set_error(err, PA_KV8_ERR_BLOCK);
-          id = 0;
-        }
-        const int off = k & ((1 << shift) - 1);
-        slot[b] = (id << shift) + off;
-        if ((lane >> 4) == b && lane < live)
-          scale = __ldg(scales + ((int64_t(id) * p.num_kv_heads + kvh) << shift) + off + (lane & 15));
-      }
-    }
+  // Rows at and past `live` (behind the context) read as zeros.
+  __device__ __forceinline__ void read(const uint8_t* staged, const uint8_t* scales, int lane, int live) {
+    scale = lane < live ? scales[lane] : 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = i * RPI + lane / LPR;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if (r < live)
-        x[i] = __ldg(reinterpret_cast<const uint4*>(
-            pool + ((int64_t(slot[r >> 4]) + (r & 15)) * p.num_kv_heads + kvh) * D + 16 * (lane % LPR)));
+      x[i] = *reinterpret_cast<const uint4*>(staged + 16 * (32 * i + lane));
+      if (i * RPI + lane / LPR >= live) x[i] = make_uint4(0, 0, 0, 0);
     }
   }
 
   // `nan_rows`: V's rows that stand for NaN are widened to zeros and reported as bits.
   template <bool V>
   __device__ __forceinline__ void store(uint8_t* tile, int row0, int lane, uint16_t* nan_rows) {
-    const bool bad = V && scale == 255u && lane < live;
+    const bool bad = V && scale == 255u;
     const uint32_t nans = V ? __ballot_sync(0xffffffffu, bad) : 0u;
     const uint32_t s2 = bad ? 0u : scale_h2(scale);
     if (V && lane < 2) nan_rows[lane] = uint16_t(nans >> (16 * lane));
-    const int q = lane % LPR, half = D == 128 ? q >> 2 : 0, c0 = 2 * (q & 3);
+    const int q = lane % LPR, box = D == 128 ? q >> 2 : 0, c0 = 2 * (q & 3);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int r = i * RPI + lane / LPR, row = row0 + r;
@@ -164,26 +151,25 @@ struct WidenHalf {
                         mul_h2(widen_hi(w[1]), sc));
       o[1] = make_uint4(mul_h2(widen_lo(w[2]), sc), mul_h2(widen_hi(w[2]), sc), mul_h2(widen_lo(w[3]), sc),
                         mul_h2(widen_hi(w[3]), sc));
-      // The two 64-column halves of a row map to the same banks: the second goes odd chunk first.
-      uint8_t* dst = tile + half * kTileHalf;
-      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + half)) = half ? o[1] : o[0];
-      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + 1 - half)) = half ? o[0] : o[1];
+      // The two 64-column boxes of a row map to the same banks: the second goes odd chunk first.
+      uint8_t* dst = tile + box * kTileBox;
+      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + box)) = box ? o[1] : o[0];
+      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + 1 - box)) = box ? o[0] : o[1];
     }
   }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8AttnParams p, int* err) {
+__global__ void __launch_bounds__(kTileThreads, 1)
+    kv8_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const Kv8AttnParams p, int* err) {
   using C = TileCfg<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
-  uint8_t* sQ = smem;
   uint8_t* sK = smem + C::OFF_K;
   uint8_t* sV = smem + C::OFF_V;
   TilePiece* desc = reinterpret_cast<TilePiece*>(smem + C::OFF_DESC);
-  uint16_t* nan_rows = reinterpret_cast<uint16_t*>(smem + C::OFF_NAN);  // [V stage][4]
+  uint16_t* nan_rows = reinterpret_cast<uint16_t*>(smem + C::OFF_NAN);
   TileBars* bars = reinterpret_cast<TileBars*>(smem + C::OFF_BAR);
-  static_assert(sizeof(TileBars) <= 176, "barrier area");
-  static_assert(2 * sizeof(TilePiece) <= 64, "descriptor area");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
@@ -191,31 +177,36 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
   const int slices = line_slices(total, p.slices, kTileMinKeys);
   if (total == 0 || slice >= slices) return;
 
-  if (warp == 8) {
+  if (warp == 12) {
     tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
     tmem_relinquish();
   }
   if (tid == 0) {
+    for (int i = 0; i < 2; ++i)
+      for (int s = 0; s < kTileRing; ++s) {
+        mbar_init(&bars->st_full[i][s], kTileKeys / 16);
+        mbar_init(&bars->st_empty[i][s], 2);
+      }
     for (int s = 0; s < kTileKStages; ++s) {
       mbar_init(&bars->k_full[s], 2);
-      mbar_init(&bars->s_full[s], 1);
+      for (int h = 0; h < 2; ++h) mbar_init(&bars->s_full[h][s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->v_full[s], 2);
-      mbar_init(&bars->p_full[s], 128);
-      mbar_init(&bars->p_free[s], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars->p_full[h][s], 128);
+        mbar_init(&bars->p_free[h][s], 1);
+      }
+      mbar_init(&bars->q_full[s], 128);
+      mbar_init(&bars->s_consumed[s], 128);
       mbar_init(&bars->d_full[s], 1);
       mbar_init(&bars->d_empty[s], kTileConsumers);
     }
-    mbar_init(&bars->q_full, 128);
-    mbar_init(&bars->s_consumed, 128);
     fence_mbar_init();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tbase = bars->tmem_base;
-  const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
 
   // The next piece of the ring, for one consuming warp; false when a wait ran out.
   auto next_piece = [&](int k, TilePiece& d) {
@@ -227,11 +218,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
     }
     return ok;
   };
+  // A piece of at most 128 rows leaves the second half without work.  Its warps go through the
+  // barriers all the same: a parity wait tells only neighbouring phases apart, so a ring may
+  // not run ahead of anyone who waits on it.
+  auto halves = [&](const TilePiece& d) { return d.tokens * p.group > kHalfRows ? 2 : 1; };
 
   bool ok = true;
-  if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    if (warp == 10) {
+  if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 18) {
       // ---------------------------------------------------------- pieces
       const int64_t x1 = line_cut(total, slices, slice + 1);
       int64_t x = line_cut(total, slices, slice);
@@ -271,98 +266,175 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
         }
         if (t.seq < 0) break;
       }
-    } else if (warp == 8) {
-      // ---------------------------------------------------------- S issue
+    } else if (warp < 18) {
+      // ---------------------------------------------------------- producers: warp 16 K, 17 V
+      const int v = warp - 16;
+      const CUtensorMap* map = v ? &tv : &tk;
+      const uint8_t* scales = v ? p.v_scale : p.k_scale;
+      uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES;
+      uint8_t* scale_ring = smem + C::OFF_SCALE + v * kTileRing * kTileKeys;
+      if (lane == 0) prefetch_tmap(map);
+      const int shift = p.block_shift;
+      // Each lane looks after one of 32 groups of 16 keys (8 tiles): its slot and scales are
+      // read one round ahead; the lane issues its own box.
+      auto look_up = [&](const int32_t* row, int group, int ctx, int& slot, uint4& sc) {
+        slot = -1;
+        if (16 * group < ctx) {
+          int id = __ldg(row + (group >> shift));
+          if (id < 0 || id >= p.pool_blocks) {
+            set_error(err, PA_KV8_ERR_BLOCK);
+            id = 0;
+          }
+          const int off = (group & ((1 << shift) - 1)) * 16;
+          slot = (id << (shift + 4)) + off;
+          sc = __ldg(reinterpret_cast<const uint4*>(
+              scales + ((int64_t(id) * p.num_kv_heads + kvh) << (shift + 4)) + off));
+        }
+      };
+      int n = 0;  // tiles issued
+      for (int k = 0; ok; ++k) {
+        TilePiece d;
+        ok = next_piece(k, d);
+        if (!ok || d.row0 < 0) break;
+        const int32_t* row = p.tables + int64_t(d.seq) * p.table_stride;
+        int slot, slot_next = -1;
+        uint4 sc = make_uint4(0, 0, 0, 0), sc_next = sc;
+        look_up(row, 4 * d.j0 + lane, d.ctx, slot, sc);
+        for (int j0 = d.j0; j0 < d.j1 && ok; j0 += 8) {
+          if (j0 + 8 < d.j1) look_up(row, 4 * (j0 + 8) + lane, d.ctx, slot_next, sc_next);
+          for (int j = j0; j < min(j0 + 8, d.j1); ++j, ++n) {
+            const int s = n % kTileRing;
+            if (n >= kTileRing)
+              ok = __all_sync(0xffffffffu, mbar_wait(&bars->st_empty[v][s], ((n / kTileRing) - 1) & 1));
+            if (!ok) break;
+            const int part = lane - 4 * (j - j0);
+            if (part >= 0 && part < 4) {
+              uint64_t* bar = &bars->st_full[v][s];
+              if (slot >= 0) {
+                *reinterpret_cast<uint4*>(scale_ring + s * kTileKeys + 16 * part) = sc;
+                mbar_arrive_expect_tx(bar, 16 * D);  // releases the scales too
+                tma_load_3d(ring + s * C::ST_BYTES + part * 16 * D, map, 0, kvh, slot, bar);
+              } else {
+                mbar_arrive(bar);  // behind the context: the widening warps put zeros
+              }
+            }
+            __syncwarp();
+          }
+          slot = slot_next;
+          sc = sc_next;
+        }
+      }
+      if (!ok)  // leave with no copy into this CTA's shared memory in flight
+        for (int i = max(0, n - kTileRing); i < n; ++i) mbar_wait(&bars->st_full[v][i % kTileRing], (i / kTileRing) & 1);
+    }
+  } else if (warp >= 12) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    const int h = warp & 1;
+    const uint32_t tbase = bars->tmem_base + h * C::COL_HALF;
+    const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
+    if (warp < 14) {
+      // ---------------------------------------------------------- S issue of half h
       int g = 0;
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
         if (!ok || d.row0 < 0) break;
+        const bool active = h < halves(d);
         if (lane == 0) {
-          constexpr uint32_t idS = idesc_f16<__half>(kTileRows, kTileKeys, false);
-          const uint32_t q0 = smem_u32(sQ);
-          if (!mbar_wait(&bars->q_full, k & 1)) ok = false;
+          constexpr uint32_t idS = idesc_f16<__half>(kHalfRows, kTileKeys, false);
+          const uint32_t q0 = smem_u32(smem + h * (C::Q_BYTES / 2));
+          if (!mbar_wait(&bars->q_full[h], k & 1)) ok = false;
           for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
             const int s = g % kTileKStages;
             if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1) ||
-                (g > 0 && !mbar_wait(&bars->s_consumed, (g - 1) & 1))) {
+                (g > 0 && !mbar_wait(&bars->s_consumed[h], (g - 1) & 1))) {
               ok = false;
               break;
+            }
+            if (!active) {
+              mbar_arrive(&bars->s_full[h][s]);
+              continue;
             }
             tc_fence_after();
             const uint32_t k0 = smem_u32(sK + s * C::KV_BYTES);
 #pragma unroll
             for (int kk = 0; kk < D / 16; ++kk) {
-              const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQHalf + (kk & 3) * 32, 16, 1024);
-              const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileHalf + (kk & 3) * 32, 16, 1024);
+              const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQBox + (kk & 3) * 32, 16, 1024);
+              const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileBox + (kk & 3) * 32, 16, 1024);
               umma_f16(tS, ad, bd, idS, kk > 0 ? 1u : 0u);
             }
-            umma_commit(&bars->s_full[s]);
+            umma_commit(&bars->s_full[h][s]);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        g = __shfl_sync(0xffffffffu, g, 0);
       }
-    } else if (warp == 9) {
-      // ---------------------------------------------------------- P.V issue
+    } else {
+      // ---------------------------------------------------------- P.V issue of half h
       int g = 0;
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
         if (!ok || d.row0 < 0) break;
+        const bool active = h < halves(d);
         if (lane == 0) {
-          constexpr uint32_t idO = idesc_f16<__half>(kTileRows, D, true);
+          constexpr uint32_t idO = idesc_f16<__half>(kHalfRows, D, true);
           for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
             const int s = g & 1;
-            if (!mbar_wait(&bars->p_full[s], (g >> 1) & 1) || !mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
+            if (!mbar_wait(&bars->p_full[h][s], (g >> 1) & 1) || !mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
               ok = false;
               break;
+            }
+            if (!active) {
+              mbar_arrive(&bars->p_free[h][s]);
+              continue;
             }
             tc_fence_after();
             const uint32_t v0 = smem_u32(sV + s * C::KV_BYTES);
 #pragma unroll
             for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-              const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileHalf, 1024);
+              const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileBox, 1024);
               umma_f16_ts(tO, tP + s * (kTileKeys / 2) + 8 * kk, bd, idO, (j > d.j0 || kk > 0) ? 1u : 0u);
             }
-            umma_commit(&bars->p_free[s]);
+            umma_commit(&bars->p_free[h][s]);
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
-        g = __shfl_sync(0xffffffffu, g, 0);
       }
     }
-  } else if (warp >= 4) {
-    // ------------------------------------------------------------ widening
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    const bool is_v = warp >= 6;
-    const int row0 = 32 * (warp & 1);
-    const uint8_t* pool = is_v ? p.v_pool : p.k_pool;
-    const uint8_t* scales = is_v ? p.v_scale : p.k_scale;
-    const int stages = is_v ? kTileVStages : kTileKStages;
-    uint64_t* full = is_v ? bars->v_full : bars->k_full;
-    uint64_t* freed = is_v ? bars->p_free : bars->s_full;
-    uint8_t* ring = is_v ? sV : sK;
-    int s = 0, round = 0;
+  } else if (warp >= 8) {
+    // ------------------------------------------------------------ widening: warps 8-9 K, 10-11 V
+    const int v = warp >= 10 ? 1 : 0, row0 = 32 * (warp & 1);
+    const int stages = v ? kTileVStages : kTileKStages;
+    uint64_t* full = v ? bars->v_full : bars->k_full;
+    const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES + row0 * D;
+    const uint8_t* scale_ring = smem + C::OFF_SCALE + v * kTileRing * kTileKeys + row0;
+    uint8_t* out = v ? sV : sK;
+    int n = 0, s = 0, round = 0;
     WidenHalf<D> half;
     for (int k = 0; ok; ++k) {
       TilePiece d;
       ok = next_piece(k, d);
       if (!ok || d.row0 < 0) break;
-      const int32_t* row = p.tables + int64_t(d.seq) * p.table_stride;
-      half.load(pool, scales, row, d.j0 * kTileKeys + row0, kvh, lane, d.ctx, p, err);
-      for (int j = d.j0; j < d.j1; ++j) {
-        if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&freed[s], (round - 1) & 1));
+      for (int j = d.j0; j < d.j1; ++j, ++n) {
+        const int st = n % kTileRing;
+        ok = mbar_wait(&bars->st_full[v][st], (n / kTileRing) & 1);
+        // Both halves are done with the tile that was in this stage.
+        if (ok && round > 0)
+          for (int h = 0; h < 2 && ok; ++h)
+            ok = mbar_wait(v ? &bars->p_free[h][s] : &bars->s_full[h][s], (round - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        if (is_v)
-          half.template store<true>(ring + s * C::KV_BYTES, row0, lane, nan_rows + 4 * s + 2 * (warp & 1));
+        half.read(ring + st * C::ST_BYTES, scale_ring + st * kTileKeys, lane, d.ctx - j * kTileKeys - row0);
+        if (v)
+          half.template store<true>(out + s * C::KV_BYTES, row0, lane, nan_rows + 4 * s + 2 * (warp & 1));
         else
-          half.template store<false>(ring + s * C::KV_BYTES, row0, lane, nullptr);
+          half.template store<false>(out + s * C::KV_BYTES, row0, lane, nullptr);
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
-        if (j + 1 < d.j1)
-          half.load(pool, scales, row, (j + 1) * kTileKeys + row0, kvh, lane, d.ctx, p, err);
+        if (lane == 0) {
+          mbar_arrive(&bars->st_empty[v][st]);
+          mbar_arrive(&full[s]);
+        }
         if (++s == stages) {
           s = 0;
           ++round;
@@ -371,14 +443,30 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
     }
   } else {
     // ------------------------------------------------------------ softmax (one row per thread)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
-    const uint32_t lane_base = uint32_t(warp * 32) << 16;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    const int h = warp >> 2;
+    const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
+    const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
     const int r = tid, t_row = r / p.group, head = kvh * p.group + (r - t_row * p.group);
+    uint8_t* sQ = smem + h * (C::Q_BYTES / 2);
     int g = 0;
     for (int k = 0; ok; ++k) {
       TilePiece d;
       ok = next_piece(k, d);
       if (!ok || d.row0 < 0) break;
+      if (h >= halves(d)) {
+        mbar_arrive(&bars->q_full[h]);
+        for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][g % kTileKStages], (g / kTileKStages) & 1));
+          if (!ok) break;
+          mbar_arrive(&bars->s_consumed[h]);
+          if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][g & 1], ((g - 2) >> 1) & 1));
+          if (!ok) break;
+          mbar_arrive(&bars->p_full[h][g & 1]);
+        }
+        continue;
+      }
       const int t_eff = min(t_row, d.tokens - 1);  // spare rows repeat the last token and are not stored
       const int qpos = d.pos0 + t_eff;
 
@@ -414,23 +502,23 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
             const float2 f = unpack2(u[i], (T*)nullptr);
             o[i] = pack2<__half>(f.x * mul, f.y * mul);
           }
-          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQHalf + sw_off(r, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQBox + sw_off(r & 127, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
-        mbar_arrive(&bars->q_full);
+        mbar_arrive(&bars->q_full[h]);
       }
 
       float m_run = -INFINITY, l_run = 0.f;
       for (int j = d.j0; j < d.j1; ++j, ++g) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[g % kTileKStages], (g / kTileKStages) & 1));
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][g % kTileKStages], (g / kTileKStages) & 1));
         if (!ok) break;
         tc_fence_after();
         uint32_t sr[kTileKeys];
-        tmem_ld32_at<0>(tS + lane_base + 0, sr);
-        tmem_ld32_at<32>(tS + lane_base + 32, sr);
+        tmem_ld32_at<0>(tS + 0, sr);
+        tmem_ld32_at<32>(tS + 32, sr);
         tmem_wait_ld();
         tc_fence_before();
-        mbar_arrive(&bars->s_consumed);
+        mbar_arrive(&bars->s_consumed[h]);
 
         const int lim = qpos - j * kTileKeys;  // key column c is visible iff c <= lim
         if (__any_sync(0xffffffffu, lim < kTileKeys - 1)) {
@@ -466,7 +554,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
 
         const int pb = g & 1;
         if (g >= 2) {  // the P.V that read this buffer two tiles ago has retired
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[pb], ((g - 2) >> 1) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][pb], ((g - 2) >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
         }
@@ -481,29 +569,28 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
             if (hit) pk[c / 2] |= (c & 1) ? 0x7e000000u : 0x00007e00u;
           }
         }
-        tmem_st32(tP + lane_base + pb * (kTileKeys / 2), *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+        tmem_st32(tP + pb * (kTileKeys / 2), *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
         if (j > d.j0 && __any_sync(0xffffffffu, grow)) {  // O *= alpha once the previous P.V retired
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[pb ^ 1], ((g - 1) >> 1) & 1));
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][pb ^ 1], ((g - 1) >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
-            tmem_ld32(tO + lane_base + 32 * c, o);
+            tmem_ld32(tO + 32 * c, o);
             tmem_wait_ld();
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32(tO + lane_base + 32 * c, o);
+            tmem_st32(tO + 32 * c, o);
           }
         }
         tmem_wait_st();
         tc_fence_before();
-        mbar_arrive(&bars->p_full[pb]);
+        mbar_arrive(&bars->p_full[h][pb]);
       }
       if (!ok) break;
       // ---- epilogue, once the piece's last P.V retired
-      const int h = g - 1;
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h & 1], (h >> 1) & 1));
+      ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][(g - 1) & 1], ((g - 1) >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
       const bool stored = t_row < d.tokens;
@@ -513,7 +600,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + lane_base + 32 * c, o);
+          tmem_ld32(tO + 32 * c, o);
           tmem_wait_ld();
           if (stored) {
 #pragma unroll
@@ -532,7 +619,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + lane_base + 32 * c, o);
+          tmem_ld32(tO + 32 * c, o);
           tmem_wait_ld();
           if (stored) {
 #pragma unroll
@@ -550,16 +637,17 @@ __global__ void __launch_bounds__(kTileThreads, 2) kv8_tiles_kernel(const Kv8Att
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 12) {
     __syncwarp();
     tc_fence_after();
-    tmem_dealloc(tbase, C::TMEM_COLS);
+    tmem_dealloc(bars->tmem_base, C::TMEM_COLS);
   }
 }
 
 // ------------------------------------------------------------------ dispatch
 template <typename T, int D>
-static cudaError_t tiles_one(const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+static cudaError_t tiles_one(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int* err,
+                             cudaStream_t stream) {
   using C = TileCfg<D>;
   auto kern = kv8_tiles_kernel<T, D>;
   int dev = 0;
@@ -573,21 +661,25 @@ static cudaError_t tiles_one(const Kv8AttnParams& p, int* err, cudaStream_t stre
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  kern<<<p.slices * p.num_kv_heads, kTileThreads, C::SMEM, stream>>>(p, err);
+  kern<<<p.slices * p.num_kv_heads, kTileThreads, C::SMEM, stream>>>(tk, tv, p, err);
   return cudaGetLastError();
 }
 
 int kv8_tiles_slices(int num_kv_heads, int sms) {
-  const int n = 2 * sms / num_kv_heads;
+  const int n = sms / num_kv_heads;
   return n < 1 ? 1 : n;
 }
 
-cudaError_t launch_kv8_tiles(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
-  cudaError_t e;
-  if (dtype == PA_DTYPE_F16)
-    e = head_dim == 64 ? tiles_one<__half, 64>(p, err, stream) : tiles_one<__half, 128>(p, err, stream);
-  else
-    e = head_dim == 64 ? tiles_one<__nv_bfloat16, 64>(p, err, stream) : tiles_one<__nv_bfloat16, 128>(p, err, stream);
+template <typename T>
+static cudaError_t tiles_by_dim(int head_dim, const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p,
+                                int* err, cudaStream_t s) {
+  return head_dim == 64 ? tiles_one<T, 64>(tk, tv, p, err, s) : tiles_one<T, 128>(tk, tv, p, err, s);
+}
+
+cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
+                             const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+  const cudaError_t e = dtype == PA_DTYPE_F16 ? tiles_by_dim<__half>(head_dim, tk, tv, p, err, stream)
+                                              : tiles_by_dim<__nv_bfloat16>(head_dim, tk, tv, p, err, stream);
   if (e != cudaSuccess) return e;
   return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, stream);
 }

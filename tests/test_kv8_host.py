@@ -44,7 +44,7 @@ def test_tiling_fits_its_kernels(pkg, group):
         assert t.row_groups in (1, 2, 3, 4)
         assert t.small_tokens >= 1
         assert t.small_tokens * group <= 8 * t.row_groups
-        assert 1 <= t.large_tokens * group <= 128
+        assert 1 <= t.large_tokens * group <= 256
         assert t.small_max >= 0
 
 
