@@ -61,8 +61,10 @@ cudaError_t launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t 
 
 // Slices of the work line for the kernel for few rows, and the rows a partial holds.
 int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
-cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const Kv8AttnParams& p, int* err, cudaStream_t stream);
+// `pair`: p.num_kv_heads counts pairs of KV heads of 64 dims, p.group the query heads of a pair.
+cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
+                            const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream);
+constexpr int kKv8RowGroups = 3;  // most groups of 8 rows
 int kv8_tiles_slices(int num_kv_heads, int sms);
 cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
                              const Kv8AttnParams& p, int* err, cudaStream_t stream);

@@ -45,13 +45,26 @@ static bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 1
 // Slices for which the workspace holds partials, for the SMs of any sm_100 part.
 constexpr int kMaxSms = 160;
 
+// How the kernel for few rows runs a call: KV heads of 64 dims in pairs where that fits.
+struct Kv8Rows {
+  bool pair;
+  int row_groups, num_kv_heads, group;
+};
+static Kv8Rows rows_form(const pa_kv8_tiling& t, int num_kv_heads, int group, int head_dim, int max_query_len) {
+  const int tokens = std::max(1, std::min(t.small_tokens, max_query_len));  // of a tile, at most
+  const int paired = (2 * group * tokens + 7) / 8;
+  if (head_dim == 64 && num_kv_heads % 2 == 0 && paired <= kKv8RowGroups)
+    return {true, paired, num_kv_heads / 2, 2 * group};
+  return {false, t.row_groups, num_kv_heads, group};
+}
+
 struct Kv8Scratch {
   uint64_t work, cu, ml, o, tile_ml, tile_o, bytes;
 };
-static Kv8Scratch attention_scratch(const pa_kv8_tiling& t, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim,
-                                    int sms, bool tiles) {
+static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int sms,
+                                    bool tiles) {
   const uint64_t rows =
-      uint64_t(kv8_rows_slices(t.row_groups, num_kv_heads, sms)) * num_kv_heads * 2 * (8 * t.row_groups);
+      uint64_t(kv8_rows_slices(f.row_groups, f.num_kv_heads, sms)) * f.num_kv_heads * 2 * (8 * f.row_groups);
   Kv8Scratch s;
   s.work = 0;
   s.cu = (uint64_t(num_seqs) + 1) * 2 * sizeof(int64_t);
@@ -91,9 +104,9 @@ int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, pa_kv8_tiling
   if (!tiling) return fail(PA_ERR_INVALID_ARGUMENT, "tiling must not be NULL");
   if (group < 1 || max_query_len < 0) return fail(PA_ERR_INVALID_ARGUMENT, "bad group or max_query_len");
   if (group > 16) return fail(PA_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16 are supported", group);
-  // A sequence of up to 16 (token, head) rows goes to the kernel for few rows, one of more to
+  // A sequence of up to 24 (token, head) rows goes to the kernel for few rows, one of more to
   // the 256-row tiles.
-  const int few = std::max(1, 16 / group);
+  const int few = std::max(1, 8 * kKv8RowGroups / group);
   const int rows = group * std::max(1, std::min(max_query_len, few));
   tiling->row_groups = (rows + 7) / 8;
   tiling->small_tokens = std::max(1, 8 * tiling->row_groups / group);
@@ -233,7 +246,8 @@ uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num
   if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_heads % num_kv_heads ||
       pa_kv8_choose_tiling(num_heads / num_kv_heads, max_query_len, &t) != PA_OK)
     return 0;
-  return attention_scratch(t, num_seqs, num_kv_heads, head_dim, kMaxSms, max_query_len > t.small_max).bytes;
+  const Kv8Rows f = rows_form(t, num_kv_heads, num_heads / num_kv_heads, head_dim, max_query_len);
+  return attention_scratch(f, num_seqs, num_kv_heads, head_dim, kMaxSms, max_query_len > t.small_max).bytes;
 }
 
 int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_stride_head, int32_t num_tokens,
@@ -275,7 +289,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_scale) || !aligned16(v_scale))
     return fail(PA_ERR_INVALID_ARGUMENT, "8-bit pools and their scales must be 16-byte aligned");
   const int sms = std::min(sm_count(), kMaxSms);
-  const Kv8Scratch s = attention_scratch(t, num_seqs, num_kv_heads, head_dim, sms, max_query_len > t.small_max);
+  const Kv8Rows f = rows_form(t, num_kv_heads, group, head_dim, max_query_len);
+  const Kv8Scratch s = attention_scratch(f, num_seqs, num_kv_heads, head_dim, sms, max_query_len > t.small_max);
   if (workspace_bytes < s.bytes)
     return fail(PA_ERR_BUFFER_TOO_SMALL, "workspace holds %llu bytes, %llu needed",
                 (unsigned long long)workspace_bytes, (unsigned long long)s.bytes);
@@ -306,8 +321,9 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     work = b.work;
   }
   CUtensorMap tk, tv;
-  st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, true, &tk);
-  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, true, &tv);
+  const int row_dim = f.pair ? 2 * head_dim : head_dim;
+  st = payload_map(k_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, true, &tk);
+  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, true, &tv);
   if (st != PA_OK) return st;
   Kv8AttnParams p{};
   p.q = query;
@@ -327,20 +343,22 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.work = work;
   p.num_seqs = num_seqs;
   p.num_heads = num_heads;
-  p.num_kv_heads = num_kv_heads;
-  p.group = group;
+  p.num_kv_heads = f.num_kv_heads;
+  p.group = f.group;
   p.block_shift = shift;
   p.tile_tokens = t.small_tokens;
-  p.slices = kv8_rows_slices(t.row_groups, num_kv_heads, sms);
+  p.slices = kv8_rows_slices(f.row_groups, f.num_kv_heads, sms);
   p.pool_blocks = int32_t(pool_num_blocks);
   p.qscale = scale * kLog2e;
   p.part_ml = reinterpret_cast<float2*>(ws + s.ml);
   p.part_o = reinterpret_cast<float*>(ws + s.o);
-  cudaError_t e = launch_kv8_rows(dtype, head_dim, t.row_groups, tk, tv, p, err, stream);
+  cudaError_t e = launch_kv8_rows(dtype, head_dim, f.pair, f.row_groups, tk, tv, p, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
   note_launches(PA_LAUNCH_KV8_ROWS | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
   if (max_query_len > t.small_max) {
     p.work = work + num_seqs + 1;
+    p.num_kv_heads = num_kv_heads;
+    p.group = group;
     p.tile_tokens = t.large_tokens;
     p.slices = kv8_tiles_slices(num_kv_heads, sms);
     p.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);

@@ -28,6 +28,11 @@
 // movmatrix per 8 x 8.  Widening costs one conversion per two elements; with 16-byte chunks
 // of head_dim dealt out to the MMA's k index as ldmatrix delivers bytes (lane 4g + i holds
 // dims 4i .. 4i + 3) K needs no permute, and V's transpose needs one byte permute per four.
+//
+// head_dim 64 with an even number of KV heads runs two KV heads as one of 128 dims (PAIR): a
+// pool row of 64 bytes costs the copy engine as much as one of 128.  A query row then has
+// zeros in the other head's dims, its scores take its own head's scales, and of O^T its own
+// head's dims are kept; the columns that this costs were zeros before.
 #include <cuda_fp16.h>
 
 #include "kv8.h"
@@ -48,8 +53,16 @@ constexpr int kRowsDescs = 2;
 constexpr int kRowsMinKeys = 128;
 constexpr float kWeightShift = 256.f;               // 2^8, see above
 
-template <int D, int RG>
+// D: dims of the payload rows (two heads' with PAIR), RG: groups of 8 query rows.
+template <int D, int RG, bool PAIR>
 struct RowsCfg {
+  static_assert(!PAIR || D == 128, "pairs of heads of 64");
+  static constexpr int DO = PAIR ? 64 : D;          // dims of a query and an output row
+  static constexpr int SUBS = PAIR ? 2 : 1;         // KV heads of a payload row
+  // Blocks a softmax step takes: with three groups of rows one block's scores at a time fit
+  // the registers.
+  static constexpr int NB = RG <= 2 ? 2 : 1;
+  static constexpr int SCALES = 2 * SUBS * kRowsStage;  // bytes a stage: K then V
   static constexpr int STAGES = D == 128 ? 2 : 4;   // 16 KB in flight per warp
   static constexpr int TILE = kRowsKeys * D;        // K or V of a block
   static constexpr int BLOCK = 2 * TILE;
@@ -57,11 +70,13 @@ struct RowsCfg {
   static constexpr int CH = D / 16;                 // 16-byte chunks of a row = k steps of S
   static constexpr int NO = CH * RG * 4;            // accumulator registers
   static constexpr int OFF_SCALE = kRowsWarps * STAGES * STAGE;
-  static constexpr int OFF_Q = OFF_SCALE + kRowsWarps * STAGES * 2 * kRowsStage;
-  static constexpr int OFF_MERGE = OFF_Q + CH * RG * 32 * 8;
+  static constexpr int OFF_Q = OFF_SCALE + kRowsWarps * STAGES * SCALES;
+  static constexpr int OFF_MERGE = OFF_Q;           // the queries are no longer read by then
   static constexpr int OFF_ML = OFF_MERGE + 2 * NO * 32 * 4;
+  static_assert(2 * NO * 32 * 4 >= CH * RG * 32 * 8, "merge area holds the queries");
   static constexpr int OFF_FACTOR = OFF_ML + kRowsWarps * RG * 8 * 8;
-  static constexpr int OFF_DESC = OFF_FACTOR + RG * 8 * 4;
+  static constexpr int OFF_LIMIT = OFF_FACTOR + RG * 8 * 4;
+  static constexpr int OFF_DESC = OFF_LIMIT + RG * 8 * 4;
   static constexpr int OFF_BAR = OFF_DESC + kRowsDescs * 32;
   static constexpr int SMEM = OFF_BAR + (2 * kRowsWarps * STAGES + 2 * kRowsDescs) * 8;
   static constexpr bool Q_IN_REGS = RG <= 2;
@@ -117,17 +132,18 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c) {
   return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
-template <typename T, int D, int RG>
-__global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
+template <typename T, int D, int RG, bool PAIR>
+__global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
     kv8_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const Kv8AttnParams p, int* err) {
-  using C = RowsCfg<D, RG>;
-  constexpr int CH = C::CH;
+  using C = RowsCfg<D, RG, PAIR>;
+  constexpr int CH = C::CH, DO = C::DO;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint2* sq = reinterpret_cast<uint2*>(smem + C::OFF_Q);
   float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
   float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);
   float* factors = reinterpret_cast<float*>(smem + C::OFF_FACTOR);
+  int* limits = reinterpret_cast<int*>(smem + C::OFF_LIMIT);
   RowsPiece* desc = reinterpret_cast<RowsPiece*>(smem + C::OFF_DESC);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
   uint64_t* empty = full + kRowsWarps * C::STAGES;
@@ -168,7 +184,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
     bool ok = true;
     struct BlockRef {
       int slot;  // first slot of the 16 keys
-      uint4 ks, vs;
+      uint4 ks[C::SUBS], vs[C::SUBS];
     };
     auto look_up = [&](const int32_t* row, int kb, int end) {
       BlockRef r;
@@ -180,10 +196,14 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
           id = 0;
         }
         const int sub = (kb & ((1 << p.block_shift) - 1)) * 16;
-        const int64_t at = ((int64_t(id) * p.num_kv_heads + kvh) << (p.block_shift + 4)) + sub;
         r.slot = (id << (p.block_shift + 4)) + sub;
-        r.ks = __ldg(reinterpret_cast<const uint4*>(p.k_scale + at));
-        r.vs = __ldg(reinterpret_cast<const uint4*>(p.v_scale + at));
+#pragma unroll
+        for (int u = 0; u < C::SUBS; ++u) {
+          const int64_t at =
+              (((int64_t(id) * p.num_kv_heads + kvh) * C::SUBS + u) << (p.block_shift + 4)) + sub;
+          r.ks[u] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + at));
+          r.vs[u] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + at));
+        }
       }
       return r;
     };
@@ -251,9 +271,12 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
                 uint64_t* bar = &full[w * C::STAGES + st];
                 if (lane < n) {
                   uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE + half * C::BLOCK;
-                  uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * 2 * kRowsStage + 16 * half;
-                  *reinterpret_cast<uint4*>(sc) = cur.ks;
-                  *reinterpret_cast<uint4*>(sc + kRowsStage) = cur.vs;
+                  uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * C::SCALES + 16 * half;
+#pragma unroll
+                  for (int u = 0; u < C::SUBS; ++u) {
+                    *reinterpret_cast<uint4*>(sc + u * kRowsStage) = cur.ks[u];
+                    *reinterpret_cast<uint4*>(sc + (C::SUBS + u) * kRowsStage) = cur.vs[u];
+                  }
                   mbar_arrive_expect_tx(bar, C::BLOCK);  // releases the scales too
                   tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
                   tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
@@ -309,7 +332,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
 #pragma unroll
     for (int i = 0; i < 2 * RG; ++i) {
       const int r = warp + kRowsWarps * i, tok = r / p.group, head = r - tok * p.group;
-      constexpr int E = D / 32;
+      constexpr int E = DO / 32;
       float x[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) x[e] = 0.f;
@@ -325,33 +348,42 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
         for (int s = 16; s; s >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, s));
       }
       const float up = query_power<T>(big);
-      uint32_t* dst = reinterpret_cast<uint32_t*>(&sq[((E * lane / 16) * RG + (r >> 3)) * 32 + (r & 7) * 4 +
-                                                      (E * lane % 16) / 4]);
+      // Fragment words of row r: chunk c, (r & 7, dims 4 t .. 4 t + 3) at lane 4 (r & 7) + t.
+      auto word = [&](int c, int t, int half) -> uint32_t& {
+        return reinterpret_cast<uint32_t*>(&sq[(c * RG + (r >> 3)) * 32 + (r & 7) * 4 + t])[half];
+      };
       if constexpr (E == 4) {
-        dst[0] = pack2<__half>(x[0] * up, x[1] * up);
-        dst[1] = pack2<__half>(x[2] * up, x[3] * up);
+        word(lane / 4, lane % 4, 0) = pack2<__half>(x[0] * up, x[1] * up);
+        word(lane / 4, lane % 4, 1) = pack2<__half>(x[2] * up, x[3] * up);
       } else {
-        dst[lane & 1] = pack2<__half>(x[0] * up, x[1] * up);
+        const int own = PAIR && 2 * head >= p.group ? 4 : 0;  // first chunk of the row's head
+        word(own + lane / 8, lane % 8 / 2, lane & 1) = pack2<__half>(x[0] * up, x[1] * up);
+        if (PAIR) word((own ^ 4) + lane / 8, lane % 8 / 2, lane & 1) = 0u;
       }
-      if (lane == 0) factors[r] = p.qscale / up;  // exact: a power of two
+      if (lane == 0) {
+        factors[r] = p.qscale / up;  // exact: a power of two
+        limits[r] = tok < d.tokens ? min(d.pos0 + tok, d.kb1 * kRowsKeys - 1) : -1;
+      }
     }
     rows_sync();
-    float factor[RG][2];
-    int limit[RG][2];
     uint2 qr[C::Q_IN_REGS ? CH : 1][RG];
+    if constexpr (C::Q_IN_REGS) {
 #pragma unroll
-    for (int rg = 0; rg < RG; ++rg) {
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int r = 8 * rg + 2 * tig + e, tok = r / p.group;
-        factor[rg][e] = factors[r];
-        limit[rg][e] = tok < d.tokens ? min(d.pos0 + tok, d.kb1 * kRowsKeys - 1) : -1;
-      }
-      if constexpr (C::Q_IN_REGS) {
+      for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
         for (int c = 0; c < CH; ++c) qr[c][rg] = sq[(c * RG + rg) * 32 + lane];
-      }
     }
+    // Rows 8 rg + 2 tig + {0, 1} of this lane; with PAIR, where their head's scales lie.
+    const float2* my_factors = reinterpret_cast<const float2*>(factors) + tig;
+    const int2* my_limits = reinterpret_cast<const int2*>(limits) + tig;
+    int own[RG][2];
+#pragma unroll
+    for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int r = 8 * rg + 2 * tig + e;
+        own[rg][e] = PAIR && 2 * (r % p.group) >= p.group ? kRowsStage : 0;
+      }
 
     float o[CH][RG][4];  // dims 16 c + 2 g (+1: elements 2, 3), rows 8 rg + 2 tig + {0, 1}
 #pragma unroll
@@ -373,126 +405,138 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
       const int st = taken % C::STAGES;
       if (ok) ok = mbar_wait(&full[warp * C::STAGES + st], (taken / C::STAGES) & 1);
       const uint32_t stage = smem_u32(smem + (warp * C::STAGES + st) * C::STAGE);
-      const uint8_t* sc = smem + C::OFF_SCALE + (warp * C::STAGES + st) * 2 * kRowsStage;
-
-      // ---- S^T over the payloads: element 2 h + e is key 16 b + 8 h + g, row 8 rg + 2 tig + e
-      float s[2][RG][4];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-#pragma unroll
-        for (int rg = 0; rg < RG; ++rg)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[b][rg][e] = 0.f;
-#pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-          uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
-          ldm4(stage + b * C::BLOCK + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t a0 = widen_lo(w[2 * i]), a1 = widen_lo(w[2 * i + 1]), a2 = widen_hi(w[2 * i]),
-                           a3 = widen_hi(w[2 * i + 1]);
-#pragma unroll
-            for (int rg = 0; rg < RG; ++rg) {
-              uint2 q;
-              if constexpr (C::Q_IN_REGS)
-                q = qr[c + i][rg];
-              else
-                q = sq[((c + i) * RG + rg) * 32 + lane];
-              mma16(s[b][rg], a0, a1, a2, a3, q.x, q.y);
-            }
-          }
-        }
-      }
-
-      // ---- online softmax
-      float ks[2][2], vs[2][2];  // scales of keys 16 b + 8 h + g
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          ks[b][h] = __uint_as_float(uint32_t(sc[16 * b + 8 * h + g]) << 23);
-          vs[b][h] = __uint_as_float(uint32_t(sc[kRowsStage + 16 * b + 8 * h + g]) << 23) * kWeightShift;
-        }
+      const uint8_t* sc = smem + C::OFF_SCALE + (warp * C::STAGES + st) * C::SCALES;
       const int key0 = kb * kRowsKeys;
       // Spare rows of the tile compute, unmasked, and are not stored.
       const bool masked = key0 + kRowsStage - 1 > d.pos0 || kb + 2 > d.kb1;
-      uint32_t wt[2][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1) of block b, row 8 rg + g
-      bool grown = false;
-      float alpha[RG][2];
+      const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;  // keys of the stage that are there
 #pragma unroll
-      for (int rg = 0; rg < RG; ++rg) {
-        float mx[2] = {-INFINITY, -INFINITY};
+      for (int b0 = 0; b0 < 2; b0 += C::NB) {
+        // ---- S^T over the payloads: element 2 h + e is key 16 b + 8 h + g, row 8 rg + 2 tig + e
+        float s[C::NB][RG][4];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& v = s[b][rg][2 * h + e];
-              v *= ks[b][h] * factor[rg][e];
-              if (masked && key0 + 16 * b + 8 * h + g > limit[rg][e]) v = -INFINITY;
-              mx[e] = fmaxf(mx[e], v);
-            }
-        float ref[2], sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-          const float mn = fmaxf(m[rg][e], mx[e]);
-          ref[e] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
-          alpha[rg][e] = ex2(m[rg][e] - ref[e]);
-          grown |= alpha[rg][e] != 1.f;
-          m[rg][e] = mn;
-        }
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float w[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float pr = ex2(s[b][rg][2 * h + e] - ref[e]);
-              sum[e] += pr;
-              w[e] = pr * vs[b][h];
-              // A hidden key's row may stand for NaN.
-              if (masked && key0 + 16 * b + 8 * h + g > limit[rg][e]) w[e] = 0.f;
-            }
-            wt[b][rg][h] = transpose8(pack2<__half>(w[0], w[1]));
-          }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) l[rg][e] = l[rg][e] * alpha[rg][e] + sum[e];
-      }
-      if (__any_sync(0xffffffffu, grown)) {
-#pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int n = 0; n < C::NB; ++n) {
 #pragma unroll
           for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[c][rg][e] *= alpha[rg][e & 1];
-      }
-
-      // ---- O^T += V^T W^T; bytes behind the context (or the stage's only block) read as zero
-      const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;
+            for (int e = 0; e < 4; ++e) s[n][rg][e] = 0.f;
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t pick[2] = {0x3120u, 0x3120u};  // (t0 d0, t1 d0, t0 d1, t1 d1) of (t0 d0, t0 d1, t1 d0, t1 d1)
-        if (end < kRowsStage) {
+          for (int c = 0; c < CH; c += 2) {
+            uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
+            ldm4(stage + (b0 + n) * C::BLOCK + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int t0 = 16 * b + 8 * h + 2 * tig;
-            pick[h] = t0 + 1 < end ? 0x3120u : (t0 < end ? 0x4140u : 0x4444u);
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t a0 = widen_lo(w[2 * i]), a1 = widen_lo(w[2 * i + 1]), a2 = widen_hi(w[2 * i]),
+                             a3 = widen_hi(w[2 * i + 1]);
+#pragma unroll
+              for (int rg = 0; rg < RG; ++rg) {
+                uint2 q;
+                if constexpr (C::Q_IN_REGS)
+                  q = qr[c + i][rg];
+                else
+                  q = sq[((c + i) * RG + rg) * 32 + lane];
+                mma16(s[n][rg], a0, a1, a2, a3, q.x, q.y);
+              }
+            }
           }
         }
+
+        // ---- online softmax
+        float ks[C::NB][2], vs[C::NB][2];  // scales of keys 16 b + 8 h + g
+        if constexpr (!PAIR) {
 #pragma unroll
-        for (int c = 0; c < CH; c += 2) {
-          uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
-          ldm4t(stage + b * C::BLOCK + C::TILE + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+          for (int n = 0; n < C::NB; ++n)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint32_t x = __byte_perm(w[2 * i], 0, pick[0]), y = __byte_perm(w[2 * i + 1], 0, pick[1]);
-            const uint32_t a0 = widen_lo(x), a1 = widen_hi(x), a2 = widen_lo(y), a3 = widen_hi(y);
+            for (int h = 0; h < 2; ++h) {
+              const int key = 16 * (b0 + n) + 8 * h + g;
+              ks[n][h] = __uint_as_float(uint32_t(sc[key]) << 23);
+              vs[n][h] = __uint_as_float(uint32_t(sc[kRowsStage + key]) << 23) * kWeightShift;
+            }
+        }
+        uint32_t wt[C::NB][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
+        bool grown = false;
+        float alpha[RG][2];
 #pragma unroll
-            for (int rg = 0; rg < RG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[b][rg][0], wt[b][rg][1]);
+        for (int rg = 0; rg < RG; ++rg) {
+          const float2 factor = my_factors[4 * rg];
+          int2 limit = make_int2(0, 0);
+          if (masked) limit = my_limits[4 * rg];
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+          for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const int key = 16 * (b0 + n) + 8 * h + g;
+                float& v = s[n][rg][2 * h + e];
+                const float k = PAIR ? __uint_as_float(uint32_t(sc[own[rg][e] + key]) << 23) : ks[n][h];
+                v *= k * (e ? factor.y : factor.x);
+                if (masked && key0 + key > (e ? limit.y : limit.x)) v = -INFINITY;
+                mx[e] = fmaxf(mx[e], v);
+              }
+          float ref[2], sum[2] = {0.f, 0.f};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
+            const float mn = fmaxf(m[rg][e], mx[e]);
+            ref[e] = mn == -INFINITY ? 0.f : mn;  // nothing seen yet
+            alpha[rg][e] = ex2(m[rg][e] - ref[e]);
+            grown |= alpha[rg][e] != 1.f;
+            m[rg][e] = mn;
+          }
+#pragma unroll
+          for (int n = 0; n < C::NB; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = 16 * (b0 + n) + 8 * h + g;
+              float w[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float pr = ex2(s[n][rg][2 * h + e] - ref[e]);
+                sum[e] += pr;
+                w[e] = pr * (PAIR ? __uint_as_float(uint32_t(sc[2 * kRowsStage + own[rg][e] + key]) << 23) * kWeightShift
+                                  : vs[n][h]);
+                // A hidden key's row may stand for NaN.
+                if (masked && key0 + key > (e ? limit.y : limit.x)) w[e] = 0.f;
+              }
+              wt[n][rg][h] = transpose8(pack2<__half>(w[0], w[1]));
+            }
+#pragma unroll
+          for (int e = 0; e < 2; ++e) l[rg][e] = l[rg][e] * alpha[rg][e] + sum[e];
+        }
+        if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+#pragma unroll
+            for (int rg = 0; rg < RG; ++rg)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) o[c][rg][e] *= alpha[rg][e & 1];
+        }
+
+        // ---- O^T += V^T W^T; bytes behind the context (or the stage's only block) read as zero
+#pragma unroll
+        for (int n = 0; n < C::NB; ++n) {
+          uint32_t pick[2] = {0x3120u, 0x3120u};  // (t0 d0, t1 d0, t0 d1, t1 d1) of (t0 d0, t0 d1, t1 d0, t1 d1)
+          if (end < kRowsStage) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int t0 = 16 * (b0 + n) + 8 * h + 2 * tig;
+              pick[h] = t0 + 1 < end ? 0x3120u : (t0 < end ? 0x4140u : 0x4444u);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < CH; c += 2) {
+            uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
+            ldm4t(stage + (b0 + n) * C::BLOCK + C::TILE + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const uint32_t x = __byte_perm(w[2 * i], 0, pick[0]), y = __byte_perm(w[2 * i + 1], 0, pick[1]);
+              const uint32_t a0 = widen_lo(x), a1 = widen_hi(x), a2 = widen_lo(y), a3 = widen_hi(y);
+#pragma unroll
+              for (int rg = 0; rg < RG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[n][rg][0], wt[n][rg][1]);
+            }
           }
         }
       }
@@ -560,19 +604,22 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG>::CTAS)
         const int r = 8 * rg + 2 * tig + e, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
         if (tok >= d.tokens) continue;
         const float f = (d.part < 0 ? 1.f / l[rg][e] : 1.f) * (1.f / kWeightShift);
-        if (d.part < 0) {
-          T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 2 * g;
+        const bool second = PAIR && own[rg][e] != 0;  // its head's dims are the second 64
+        const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
+        T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 2 * g;
 #pragma unroll
-          for (int c = 0; c < CH; ++c)
-            *reinterpret_cast<uint32_t*>(dst + 16 * c) = pack2<T>(o[c][rg][e] * f, o[c][rg][2 + e] * f);
-        } else {
-          const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
-#pragma unroll
-          for (int c = 0; c < CH; ++c)
-            *reinterpret_cast<float2*>(p.part_o + at * D + 16 * c + 2 * g) =
-                make_float2(o[c][rg][e] * f, o[c][rg][2 + e] * f);
-          if (g == 0) p.part_ml[at] = make_float2(big[rg][e], l[rg][e]);
+        for (int c = 0; c < DO / 16; ++c) {
+          float x = o[c][rg][e], y = o[c][rg][2 + e];
+          if (PAIR && second) {
+            x = o[(c + 4) % CH][rg][e];
+            y = o[(c + 4) % CH][rg][2 + e];
+          }
+          if (d.part < 0)
+            *reinterpret_cast<uint32_t*>(dst + 16 * c) = pack2<T>(x * f, y * f);
+          else
+            *reinterpret_cast<float2*>(p.part_o + at * DO + 16 * c + 2 * g) = make_float2(x * f, y * f);
         }
+        if (d.part >= 0 && g == 0) p.part_ml[at] = make_float2(big[rg][e], l[rg][e]);
       }
   }
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
@@ -675,11 +722,11 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
 }
 
 // ------------------------------------------------------------------ dispatch
-template <typename T, int D, int RG>
+template <typename T, int D, int RG, bool PAIR>
 static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p, int* err,
                             cudaStream_t stream) {
-  using C = RowsCfg<D, RG>;
-  auto kern = kv8_rows_kernel<T, D, RG>;
+  using C = RowsCfg<D, RG, PAIR>;
+  auto kern = kv8_rows_kernel<T, D, RG, PAIR>;
   int dev = 0;
   cudaGetDevice(&dev);
   static bool configured[64] = {};
@@ -695,23 +742,23 @@ static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const 
   return cudaGetLastError();
 }
 
-template <typename T, int D>
+template <typename T, int D, bool PAIR>
 static cudaError_t rows_by_groups(int row_groups, const CUtensorMap& tk, const CUtensorMap& tv, const Kv8AttnParams& p,
                                   int* err, cudaStream_t s) {
   switch (row_groups) {
-    case 1: return rows_one<T, D, 1>(tk, tv, p, err, s);
-    case 2: return rows_one<T, D, 2>(tk, tv, p, err, s);
-    case 3: return rows_one<T, D, 3>(tk, tv, p, err, s);
-    case 4: return rows_one<T, D, 4>(tk, tv, p, err, s);
+    case 1: return rows_one<T, D, 1, PAIR>(tk, tv, p, err, s);
+    case 2: return rows_one<T, D, 2, PAIR>(tk, tv, p, err, s);
+    case 3: return rows_one<T, D, 3, PAIR>(tk, tv, p, err, s);
     default: return cudaErrorInvalidValue;
   }
 }
 
 template <typename T>
-static cudaError_t rows_by_shape(int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
+static cudaError_t rows_by_shape(int head_dim, bool pair, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
                                  const Kv8AttnParams& p, int* err, cudaStream_t s) {
-  return head_dim == 64 ? rows_by_groups<T, 64>(row_groups, tk, tv, p, err, s)
-                        : rows_by_groups<T, 128>(row_groups, tk, tv, p, err, s);
+  if (pair) return rows_by_groups<T, 128, true>(row_groups, tk, tv, p, err, s);
+  return head_dim == 64 ? rows_by_groups<T, 64, false>(row_groups, tk, tv, p, err, s)
+                        : rows_by_groups<T, 128, false>(row_groups, tk, tv, p, err, s);
 }
 
 int kv8_rows_slices(int row_groups, int num_kv_heads, int sms) {
@@ -720,10 +767,11 @@ int kv8_rows_slices(int row_groups, int num_kv_heads, int sms) {
   return n < 1 ? 1 : n;
 }
 
-cudaError_t launch_kv8_rows(int dtype, int head_dim, int row_groups, const CUtensorMap& tk, const CUtensorMap& tv,
-                            const Kv8AttnParams& p, int* err, cudaStream_t stream) {
-  cudaError_t e = dtype == PA_DTYPE_F16 ? rows_by_shape<__half>(head_dim, row_groups, tk, tv, p, err, stream)
-                                        : rows_by_shape<__nv_bfloat16>(head_dim, row_groups, tk, tv, p, err, stream);
+cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
+                            const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+  cudaError_t e = dtype == PA_DTYPE_F16
+                      ? rows_by_shape<__half>(head_dim, pair, row_groups, tk, tv, p, err, stream)
+                      : rows_by_shape<__nv_bfloat16>(head_dim, pair, row_groups, tk, tv, p, err, stream);
   if (e != cudaSuccess) return e;
   return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, kRowsMinKeys, p, stream);
 }

@@ -25,7 +25,10 @@
 //   warps 16, 17    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
 //                   staging rings of 4 tiles
 //   warp 18         finds the slice's pieces (a 2-slot ring)
-// TMEM columns of a half: S [0, 64), O [64, 64 + D), two P buffers of 32.
+// TMEM columns of a half: two score buffers of 64, O [128, 128 + D).  A row's weights go over
+// the first 32 columns of the scores they came from (each thread has read its own by then),
+// so S of the next tile is issued a tile ahead and its latency lies behind a softmax: with one
+// score buffer and P beside it a tile of keys took 1.6 us, of which the softmax is 0.7.
 //
 // The staging rings are what the widening needs: with a tile's loads in registers, one tile
 // ahead, 128-row tiles and two CTAs per SM the loads' latency (over 1 us per tile) was
@@ -73,10 +76,10 @@ struct TileBars {
   // Staging: tile s of a ring has landed (an arrival per 16 keys) / was read by both warps.
   uint64_t st_full[2][kTileRing], st_empty[2][kTileRing];
   // S of tile g retired (per half): s_full[h][g % 3]; both halves' free K stage g % 3.
-  // P.V of tile g retired: p_free[h][g % 2], frees the half's P buffer and, both, V stage g % 2.
+  // P.V of tile g retired: p_free[h][g % 2], frees the half's score buffer and, both, V stage g % 2.
   uint64_t k_full[kTileKStages], s_full[2][kTileKStages];
   uint64_t v_full[kTileVStages], p_full[2][2], p_free[2][2];
-  uint64_t q_full[2], s_consumed[2];
+  uint64_t q_full[2];
   uint64_t d_full[2], d_empty[2];
   uint32_t tmem_base;
 };
@@ -96,8 +99,8 @@ struct TileCfg {
   static constexpr int OFF_BAR = OFF_NAN + 16;
   static constexpr int SMEM = OFF_BAR + int(sizeof(TileBars));
   static constexpr uint32_t TMEM_COLS = 512, COL_HALF = 256;
-  static constexpr uint32_t COL_O = kTileKeys, COL_P = kTileKeys + D;
-  static_assert(COL_P + 2 * (kTileKeys / 2) <= COL_HALF, "TMEM budget");
+  static constexpr uint32_t COL_O = 2 * kTileKeys;
+  static_assert(COL_O + D <= COL_HALF, "TMEM budget");
   static_assert(SMEM <= 227 * 1024 && OFF_DESC % 16 == 0 && OFF_BAR % 8 == 0, "shared memory");
 };
 
@@ -198,7 +201,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mbar_init(&bars->p_free[h][s], 1);
       }
       mbar_init(&bars->q_full[s], 128);
-      mbar_init(&bars->s_consumed[s], 128);
       mbar_init(&bars->d_full[s], 1);
       mbar_init(&bars->d_empty[s], kTileConsumers);
     }
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     const int h = warp & 1;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF;
-    const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
+    const uint32_t tS = tbase, tO = tbase + C::COL_O;
     if (warp < 14) {
       // ---------------------------------------------------------- S issue of half h
       int g = 0;
@@ -347,7 +349,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
             const int s = g % kTileKStages;
             if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1) ||
-                (g > 0 && !mbar_wait(&bars->s_consumed[h], (g - 1) & 1))) {
+                (g >= 2 && !mbar_wait(&bars->p_free[h][g & 1], ((g - 2) >> 1) & 1))) {
               ok = false;
               break;
             }
@@ -361,7 +363,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQBox + (kk & 3) * 32, 16, 1024);
               const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileBox + (kk & 3) * 32, 16, 1024);
-              umma_f16(tS, ad, bd, idS, kk > 0 ? 1u : 0u);
+              umma_f16(tS + (g & 1) * kTileKeys, ad, bd, idS, kk > 0 ? 1u : 0u);
             }
             umma_commit(&bars->s_full[h][s]);
           }
@@ -393,7 +395,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
             for (int kk = 0; kk < kTileKeys / 16; ++kk) {
               const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileBox, 1024);
-              umma_f16_ts(tO, tP + s * (kTileKeys / 2) + 8 * kk, bd, idO, (j > d.j0 || kk > 0) ? 1u : 0u);
+              umma_f16_ts(tO, tS + s * kTileKeys + 8 * kk, bd, idO, (j > d.j0 || kk > 0) ? 1u : 0u);
             }
             umma_commit(&bars->p_free[h][s]);
           }
@@ -447,7 +449,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int h = warp >> 2;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
-    const uint32_t tS = tbase, tO = tbase + C::COL_O, tP = tbase + C::COL_P;
+    const uint32_t tS = tbase, tO = tbase + C::COL_O;
     const int r = tid, t_row = r / p.group, head = kvh * p.group + (r - t_row * p.group);
     uint8_t* sQ = smem + h * (C::Q_BYTES / 2);
     int g = 0;
@@ -459,9 +461,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         mbar_arrive(&bars->q_full[h]);
         for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
           ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][g % kTileKStages], (g / kTileKStages) & 1));
-          if (!ok) break;
-          mbar_arrive(&bars->s_consumed[h]);
-          if (g >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][g & 1], ((g - 2) >> 1) & 1));
           if (!ok) break;
           mbar_arrive(&bars->p_full[h][g & 1]);
         }
@@ -514,11 +513,10 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok) break;
         tc_fence_after();
         uint32_t sr[kTileKeys];
-        tmem_ld32_at<0>(tS + 0, sr);
-        tmem_ld32_at<32>(tS + 32, sr);
+        const int pb = g & 1;
+        tmem_ld32_at<0>(tS + pb * kTileKeys, sr);
+        tmem_ld32_at<32>(tS + pb * kTileKeys + 32, sr);
         tmem_wait_ld();
-        tc_fence_before();
-        mbar_arrive(&bars->s_consumed[h]);
 
         const int lim = qpos - j * kTileKeys;  // key column c is visible iff c <= lim
         if (__any_sync(0xffffffffu, lim < kTileKeys - 1)) {
@@ -552,12 +550,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         l_run = l_run * alpha + ((r0 + r1) + (r2 + r3));
         m_run = m_new;
 
-        const int pb = g & 1;
-        if (g >= 2) {  // the P.V that read this buffer two tiles ago has retired
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][pb], ((g - 2) >> 1) & 1));
-          if (!ok) break;
-          tc_fence_after();
-        }
         // V rows that stand for NaN: the weight of a key that is seen becomes NaN, others stay 0.
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[pb], (g >> 1) & 1));
         if (!ok) break;
@@ -569,7 +561,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (hit) pk[c / 2] |= (c & 1) ? 0x7e000000u : 0x00007e00u;
           }
         }
-        tmem_st32(tP + pb * (kTileKeys / 2), *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
+        tmem_st32(tS + pb * kTileKeys, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
         if (j > d.j0 && __any_sync(0xffffffffu, grow)) {  // O *= alpha once the previous P.V retired
           ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][pb ^ 1], ((g - 1) >> 1) & 1));
           if (!ok) break;
