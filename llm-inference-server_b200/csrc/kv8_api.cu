@@ -59,7 +59,7 @@ static Kv8Rows rows_form(const pa_kv8_tiling& t, int num_kv_heads, int group, in
 }
 
 struct Kv8Scratch {
-  uint64_t work, cu, ml, o, tile_ml, tile_o, bytes;
+  uint64_t work, cu, ml, o, tile_ml, tile_o, twin_o, bytes;
 };
 static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int sms,
                                     bool tiles) {
@@ -73,7 +73,8 @@ static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t 
   s.tile_ml = (s.o + rows * head_dim * sizeof(float) + 255) / 256 * 256;
   const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * kKv8TileRows : 0;
   s.tile_o = (s.tile_ml + tile_rows * sizeof(float2) + 255) / 256 * 256;
-  s.bytes = s.tile_o + tile_rows * head_dim * sizeof(float);
+  s.twin_o = s.tile_o + tile_rows * head_dim * sizeof(float);
+  s.bytes = s.twin_o + tile_rows / 4 * head_dim * sizeof(float);  // 128 rows per CTA
   return s;
 }
 
@@ -363,6 +364,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     p.slices = kv8_tiles_slices(num_kv_heads, sms);
     p.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
     p.part_o = reinterpret_cast<float*>(ws + s.tile_o);
+    p.twin_o = reinterpret_cast<float*>(ws + s.twin_o);
     st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tk);
     if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tv);
     if (st != PA_OK) return st;

@@ -23,12 +23,19 @@
 //   warps 12, 13    S = Q K^T issue of either half (12 also allocates TMEM)
 //   warps 14, 15    O += P V issue of either half
 //   warps 16, 17    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
-//                   staging rings of 4 tiles
+//                   staging rings of 4 tiles (K's with V's scale bytes beside, for the rows
+//                   that stand for NaN: the softmax learns of them with the scores)
 //   warp 18         finds the slice's pieces (a 2-slot ring)
 // TMEM columns of a half: two score buffers of 64, O [128, 128 + D).  A row's weights go over
 // the first 32 columns of the scores they came from (each thread has read its own by then),
 // so S of the next tile is issued a tile ahead and its latency lies behind a softmax: with one
 // score buffer and P beside it a tile of keys took 1.6 us, of which the softmax is 0.7.
+//
+// A piece of at most 128 rows runs as twins: both halves hold the same rows and take every
+// other key tile, each with its own maximum, sum and accumulator, and the second half's are
+// joined to the first's through scratch memory at the end.  What bounds a half is the chain
+// scores -> softmax -> P V -> buffer free of one tile (about 2 us over two buffers), not
+// arithmetic, so two chains do almost twice the keys.
 //
 // The staging rings are what the widening needs: with a tile's loads in registers, one tile
 // ahead, 128-row tiles and two CTAs per SM the loads' latency (over 1 us per tile) was
@@ -72,17 +79,21 @@ struct TilePiece {
   int32_t part;    // -1: the whole tile, else the CTA's partial slot
 };
 
+// g counts the CTA's key tiles, n those that a half works on (all of them, or as a twin every
+// other).  A parity wait tells only neighbouring phases apart, so whoever waits on a ring also
+// holds it back: a half passes the K and V stages of the other's tiles on itself.
 struct TileBars {
-  // Staging: tile s of a ring has landed (an arrival per 16 keys) / was read by both warps.
-  uint64_t st_full[2][kTileRing], st_empty[2][kTileRing];
-  // S of tile g retired (per half): s_full[h][g % 3]; both halves' free K stage g % 3.
-  // P.V of tile g retired: p_free[h][g % 2], frees the half's score buffer and, both, V stage g % 2.
-  uint64_t k_full[kTileKStages], s_full[2][kTileKStages];
-  uint64_t v_full[kTileVStages], p_full[2][2], p_free[2][2];
+  uint64_t st_full[2][kTileRing], st_empty[2][kTileRing];  // staging of K, V: landed / read
+  uint64_t k_full[kTileKStages], k_free[2][kTileKStages];  // fp16 tiles, by g; freed by each half
+  uint64_t v_full[kTileVStages], v_free[2][kTileVStages];
+  uint64_t s_full[2][2], s_free[2][2], p_full[2][2];       // score buffers of a half, by n
   uint64_t q_full[2];
+  uint64_t x_full, x_free;                                 // the twin's result
   uint64_t d_full[2], d_empty[2];
   uint32_t tmem_base;
 };
+
+constexpr int kTileNanRing = 16;  // tiles whose NaN rows are kept: K runs at most 8 ahead of a softmax
 
 template <int D>
 struct TileCfg {
@@ -93,10 +104,11 @@ struct TileCfg {
   static constexpr int OFF_K = Q_BYTES;
   static constexpr int OFF_V = OFF_K + kTileKStages * KV_BYTES;
   static constexpr int OFF_ST = OFF_V + kTileVStages * KV_BYTES;          // [K, V][ring]
-  static constexpr int OFF_SCALE = OFF_ST + 2 * kTileRing * ST_BYTES;     // [K, V][ring][64]
-  static constexpr int OFF_DESC = OFF_SCALE + 2 * kTileRing * kTileKeys;
-  static constexpr int OFF_NAN = OFF_DESC + 2 * int(sizeof(TilePiece));   // [V stage][4 x 16 keys]
-  static constexpr int OFF_BAR = OFF_NAN + 16;
+  static constexpr int OFF_SCALE = OFF_ST + 2 * kTileRing * ST_BYTES;
+  static constexpr int OFF_DESC = OFF_SCALE + 3 * kTileRing * kTileKeys;  // [ring][K 64, V 64], [ring][V 64]
+  static constexpr int OFF_NAN = OFF_DESC + 2 * int(sizeof(TilePiece));   // [tile][4 x 16 keys]
+  static constexpr int OFF_TWIN = OFF_NAN + kTileNanRing * 8;             // (m, l) of the twin's rows
+  static constexpr int OFF_BAR = OFF_TWIN + kHalfRows * 8;
   static constexpr int SMEM = OFF_BAR + int(sizeof(TileBars));
   static constexpr uint32_t TMEM_COLS = 512, COL_HALF = 256;
   static constexpr uint32_t COL_O = 2 * kTileKeys;
@@ -136,13 +148,9 @@ struct WidenHalf {
     }
   }
 
-  // `nan_rows`: V's rows that stand for NaN are widened to zeros and reported as bits.
-  template <bool V>
-  __device__ __forceinline__ void store(uint8_t* tile, int row0, int lane, uint16_t* nan_rows) {
-    const bool bad = V && scale == 255u;
-    const uint32_t nans = V ? __ballot_sync(0xffffffffu, bad) : 0u;
-    const uint32_t s2 = bad ? 0u : scale_h2(scale);
-    if (V && lane < 2) nan_rows[lane] = uint16_t(nans >> (16 * lane));
+  // V's rows that stand for NaN are widened to zeros (the softmax puts the NaN in the weight).
+  __device__ __forceinline__ void store(uint8_t* tile, int row0, int lane, bool is_v) {
+    const uint32_t s2 = is_v && scale == 255u ? 0u : scale_h2(scale);
     const int q = lane % LPR, box = D == 128 ? q >> 2 : 0, c0 = 2 * (q & 3);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -172,6 +180,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   uint8_t* sV = smem + C::OFF_V;
   TilePiece* desc = reinterpret_cast<TilePiece*>(smem + C::OFF_DESC);
   uint16_t* nan_rows = reinterpret_cast<uint16_t*>(smem + C::OFF_NAN);
+  float2* twin_ml = reinterpret_cast<float2*>(smem + C::OFF_TWIN);
   TileBars* bars = reinterpret_cast<TileBars*>(smem + C::OFF_BAR);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -192,18 +201,22 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     for (int s = 0; s < kTileKStages; ++s) {
       mbar_init(&bars->k_full[s], 2);
-      for (int h = 0; h < 2; ++h) mbar_init(&bars->s_full[h][s], 1);
+      for (int h = 0; h < 2; ++h) mbar_init(&bars->k_free[h][s], 1);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->v_full[s], 2);
       for (int h = 0; h < 2; ++h) {
+        mbar_init(&bars->v_free[h][s], 1);
+        mbar_init(&bars->s_full[h][s], 1);
+        mbar_init(&bars->s_free[h][s], 1);
         mbar_init(&bars->p_full[h][s], 128);
-        mbar_init(&bars->p_free[h][s], 1);
       }
       mbar_init(&bars->q_full[s], 128);
       mbar_init(&bars->d_full[s], 1);
       mbar_init(&bars->d_empty[s], kTileConsumers);
     }
+    mbar_init(&bars->x_full, kHalfRows);
+    mbar_init(&bars->x_free, kHalfRows);
     fence_mbar_init();
   }
   tc_fence_before();
@@ -220,10 +233,11 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
     return ok;
   };
-  // A piece of at most 128 rows leaves the second half without work.  Its warps go through the
-  // barriers all the same: a parity wait tells only neighbouring phases apart, so a ring may
-  // not run ahead of anyone who waits on it.
-  auto halves = [&](const TilePiece& d) { return d.tokens * p.group > kHalfRows ? 2 : 1; };
+  auto is_twin = [&](const TilePiece& d) { return d.tokens * p.group <= kHalfRows; };
+  // Whether half h works on key tile j of a piece.
+  auto works = [](bool twin, int h, const TilePiece& d, int j) { return !twin || ((j - d.j0) & 1) == h; };
+  // The second twin of a piece with one key tile: its query rows are not loaded and not waited for.
+  auto is_idle = [](bool twin, int h, const TilePiece& d) { return twin && h == 1 && d.j1 - d.j0 < 2; };
 
   bool ok = true;
   if (warp >= 16) {
@@ -272,14 +286,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // ---------------------------------------------------------- producers: warp 16 K, 17 V
       const int v = warp - 16;
       const CUtensorMap* map = v ? &tv : &tk;
-      const uint8_t* scales = v ? p.v_scale : p.k_scale;
       uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES;
-      uint8_t* scale_ring = smem + C::OFF_SCALE + v * kTileRing * kTileKeys;
+      uint8_t* scale_ring = smem + C::OFF_SCALE + (v ? 2 * kTileRing * kTileKeys : 0);
+      const int scale_step = v ? kTileKeys : 2 * kTileKeys;
       if (lane == 0) prefetch_tmap(map);
       const int shift = p.block_shift;
       // Each lane looks after one of 32 groups of 16 keys (8 tiles): its slot and scales are
       // read one round ahead; the lane issues its own box.
-      auto look_up = [&](const int32_t* row, int group, int ctx, int& slot, uint4& sc) {
+      auto look_up = [&](const int32_t* row, int group, int ctx, int& slot, uint4 (&sc)[2]) {
         slot = -1;
         if (16 * group < ctx) {
           int id = __ldg(row + (group >> shift));
@@ -289,8 +303,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           const int off = (group & ((1 << shift) - 1)) * 16;
           slot = (id << (shift + 4)) + off;
-          sc = __ldg(reinterpret_cast<const uint4*>(
-              scales + ((int64_t(id) * p.num_kv_heads + kvh) << (shift + 4)) + off));
+          const int64_t at = ((int64_t(id) * p.num_kv_heads + kvh) << (shift + 4)) + off;
+          sc[1] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + at));
+          if (!v) sc[0] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + at));
         }
       };
       int n = 0;  // tiles issued
@@ -300,7 +315,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok || d.row0 < 0) break;
         const int32_t* row = p.tables + int64_t(d.seq) * p.table_stride;
         int slot, slot_next = -1;
-        uint4 sc = make_uint4(0, 0, 0, 0), sc_next = sc;
+        uint4 sc[2] = {}, sc_next[2] = {};
         look_up(row, 4 * d.j0 + lane, d.ctx, slot, sc);
         for (int j0 = d.j0; j0 < d.j1 && ok; j0 += 8) {
           if (j0 + 8 < d.j1) look_up(row, 4 * (j0 + 8) + lane, d.ctx, slot_next, sc_next);
@@ -313,7 +328,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             if (part >= 0 && part < 4) {
               uint64_t* bar = &bars->st_full[v][s];
               if (slot >= 0) {
-                *reinterpret_cast<uint4*>(scale_ring + s * kTileKeys + 16 * part) = sc;
+                uint8_t* dst = scale_ring + s * scale_step + 16 * part;
+                if (!v) {
+                  *reinterpret_cast<uint4*>(dst) = sc[0];
+                  dst += kTileKeys;
+                }
+                *reinterpret_cast<uint4*>(dst) = sc[1];
                 mbar_arrive_expect_tx(bar, 16 * D);  // releases the scales too
                 tma_load_3d(ring + s * C::ST_BYTES + part * 16 * D, map, 0, kvh, slot, bar);
               } else {
@@ -323,7 +343,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             __syncwarp();
           }
           slot = slot_next;
-          sc = sc_next;
+          sc[0] = sc_next[0];
+          sc[1] = sc_next[1];
         }
       }
       if (!ok)  // leave with no copy into this CTA's shared memory in flight
@@ -336,26 +357,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t tS = tbase, tO = tbase + C::COL_O;
     if (warp < 14) {
       // ---------------------------------------------------------- S issue of half h
-      int g = 0;
+      int g = 0, n = 0, queries = 0;
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
         if (!ok || d.row0 < 0) break;
-        const bool active = h < halves(d);
+        const bool twin = is_twin(d);
         if (lane == 0) {
           constexpr uint32_t idS = idesc_f16<__half>(kHalfRows, kTileKeys, false);
           const uint32_t q0 = smem_u32(smem + h * (C::Q_BYTES / 2));
-          if (!mbar_wait(&bars->q_full[h], k & 1)) ok = false;
+          if (!is_idle(twin, h, d) && !mbar_wait(&bars->q_full[h], queries++ & 1)) ok = false;
           for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
             const int s = g % kTileKStages;
-            if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1) ||
-                (g >= 2 && !mbar_wait(&bars->p_free[h][g & 1], ((g - 2) >> 1) & 1))) {
+            if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1)) {
               ok = false;
               break;
             }
-            if (!active) {
-              mbar_arrive(&bars->s_full[h][s]);
+            if (!works(twin, h, d, j)) {
+              mbar_arrive(&bars->k_free[h][s]);
               continue;
+            }
+            if (n >= 2 && !mbar_wait(&bars->s_free[h][n & 1], ((n >> 1) - 1) & 1)) {
+              ok = false;
+              break;
             }
             tc_fence_after();
             const uint32_t k0 = smem_u32(sK + s * C::KV_BYTES);
@@ -363,41 +387,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             for (int kk = 0; kk < D / 16; ++kk) {
               const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQBox + (kk & 3) * 32, 16, 1024);
               const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileBox + (kk & 3) * 32, 16, 1024);
-              umma_f16(tS + (g & 1) * kTileKeys, ad, bd, idS, kk > 0 ? 1u : 0u);
+              umma_f16(tS + (n & 1) * kTileKeys, ad, bd, idS, kk > 0 ? 1u : 0u);
             }
-            umma_commit(&bars->s_full[h][s]);
+            umma_commit(&bars->s_full[h][n & 1]);
+            umma_commit(&bars->k_free[h][s]);
+            ++n;
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
     } else {
       // ---------------------------------------------------------- P.V issue of half h
-      int g = 0;
+      int g = 0, n = 0;
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
         if (!ok || d.row0 < 0) break;
-        const bool active = h < halves(d);
+        const bool twin = is_twin(d);
         if (lane == 0) {
           constexpr uint32_t idO = idesc_f16<__half>(kHalfRows, D, true);
+          bool first = true;
           for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
-            const int s = g & 1;
-            if (!mbar_wait(&bars->p_full[h][s], (g >> 1) & 1) || !mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
+            const int s = g & 1, b = n & 1;
+            if (!mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
               ok = false;
               break;
             }
-            if (!active) {
-              mbar_arrive(&bars->p_free[h][s]);
+            if (!works(twin, h, d, j)) {
+              mbar_arrive(&bars->v_free[h][s]);
               continue;
+            }
+            if (!mbar_wait(&bars->p_full[h][b], (n >> 1) & 1)) {
+              ok = false;
+              break;
             }
             tc_fence_after();
             const uint32_t v0 = smem_u32(sV + s * C::KV_BYTES);
 #pragma unroll
             for (int kk = 0; kk < kTileKeys / 16; ++kk) {
               const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileBox, 1024);
-              umma_f16_ts(tO, tS + s * kTileKeys + 8 * kk, bd, idO, (j > d.j0 || kk > 0) ? 1u : 0u);
+              umma_f16_ts(tO, tS + b * kTileKeys + 8 * kk, bd, idO, (!first || kk > 0) ? 1u : 0u);
             }
-            umma_commit(&bars->p_free[h][s]);
+            umma_commit(&bars->s_free[h][b]);
+            umma_commit(&bars->v_free[h][s]);
+            first = false;
+            ++n;
           }
         }
         ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
@@ -409,7 +443,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int stages = v ? kTileVStages : kTileKStages;
     uint64_t* full = v ? bars->v_full : bars->k_full;
     const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES + row0 * D;
-    const uint8_t* scale_ring = smem + C::OFF_SCALE + v * kTileRing * kTileKeys + row0;
+    const uint8_t* scale_ring = smem + C::OFF_SCALE + (v ? 2 * kTileRing * kTileKeys : 0) + row0;
+    const int scale_step = v ? kTileKeys : 2 * kTileKeys;
     uint8_t* out = v ? sV : sK;
     int n = 0, s = 0, round = 0;
     WidenHalf<D> half;
@@ -423,14 +458,17 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         // Both halves are done with the tile that was in this stage.
         if (ok && round > 0)
           for (int h = 0; h < 2 && ok; ++h)
-            ok = mbar_wait(v ? &bars->p_free[h][s] : &bars->s_full[h][s], (round - 1) & 1);
+            ok = mbar_wait(v ? &bars->v_free[h][s] : &bars->k_free[h][s], (round - 1) & 1);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
-        half.read(ring + st * C::ST_BYTES, scale_ring + st * kTileKeys, lane, d.ctx - j * kTileKeys - row0);
-        if (v)
-          half.template store<true>(out + s * C::KV_BYTES, row0, lane, nan_rows + 4 * s + 2 * (warp & 1));
-        else
-          half.template store<false>(out + s * C::KV_BYTES, row0, lane, nullptr);
+        const int live = d.ctx - j * kTileKeys - row0;
+        const uint8_t* sc = scale_ring + st * scale_step;
+        half.read(ring + st * C::ST_BYTES, sc, lane, live);
+        if (!v) {
+          const uint32_t nans = __ballot_sync(0xffffffffu, lane < live && sc[kTileKeys + lane] == 255);
+          if (lane < 2) nan_rows[4 * (n % kTileNanRing) + 2 * (warp & 1) + lane] = uint16_t(nans >> (16 * lane));
+        }
+        half.store(out + s * C::KV_BYTES, row0, lane, v != 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -450,29 +488,23 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
     const uint32_t tS = tbase, tO = tbase + C::COL_O;
-    const int r = tid, t_row = r / p.group, head = kvh * p.group + (r - t_row * p.group);
     uint8_t* sQ = smem + h * (C::Q_BYTES / 2);
-    int g = 0;
+    const int lane_row = tid & (kHalfRows - 1);
+    float* twin_o = p.twin_o + int64_t(blockIdx.x) * kHalfRows * D + lane_row;  // [D][rows]
+    int g0 = 0, n = 0, twins = 0;  // tiles of the CTA before this piece, tiles of this half, twin pieces
     for (int k = 0; ok; ++k) {
       TilePiece d;
       ok = next_piece(k, d);
       if (!ok || d.row0 < 0) break;
-      if (h >= halves(d)) {
-        mbar_arrive(&bars->q_full[h]);
-        for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][g % kTileKStages], (g / kTileKStages) & 1));
-          if (!ok) break;
-          mbar_arrive(&bars->p_full[h][g & 1]);
-        }
-        continue;
-      }
+      const bool twin = is_twin(d);
+      const int r = twin ? lane_row : tid, t_row = r / p.group, head = kvh * p.group + (r - t_row * p.group);
       const int t_eff = min(t_row, d.tokens - 1);  // spare rows repeat the last token and are not stored
       const int qpos = d.pos0 + t_eff;
 
       // The query row as fp16 into the swizzled tile.  The previous piece's last S has retired
       // (its scores were read), so the tile is free.
-      float qs;
-      {
+      float qs = 0.f;
+      if (!is_idle(twin, h, d)) {
         const T* src = static_cast<const T*>(p.q) + int64_t(d.row0 + t_eff) * p.q_st + int64_t(head) * p.q_sh;
         float big = 0.f;
         if (DType<T>::code == PA_DTYPE_BF16) {
@@ -501,19 +533,20 @@ __global__ void __launch_bounds__(kTileThreads, 1)
             const float2 f = unpack2(u[i], (T*)nullptr);
             o[i] = pack2<__half>(f.x * mul, f.y * mul);
           }
-          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQBox + sw_off(r & 127, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQBox + sw_off(lane_row, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
         }
         fence_proxy_async_smem();
         mbar_arrive(&bars->q_full[h]);
       }
 
       float m_run = -INFINITY, l_run = 0.f;
-      for (int j = d.j0; j < d.j1; ++j, ++g) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][g % kTileKStages], (g / kTileKStages) & 1));
+      bool first = true;
+      for (int j = d.j0 + (twin ? h : 0); j < d.j1; j += twin ? 2 : 1, ++n) {
+        const int pb = n & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full[h][pb], (n >> 1) & 1));
         if (!ok) break;
         tc_fence_after();
         uint32_t sr[kTileKeys];
-        const int pb = g & 1;
         tmem_ld32_at<0>(tS + pb * kTileKeys, sr);
         tmem_ld32_at<32>(tS + pb * kTileKeys + 32, sr);
         tmem_wait_ld();
@@ -551,9 +584,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         m_run = m_new;
 
         // V rows that stand for NaN: the weight of a key that is seen becomes NaN, others stay 0.
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[pb], (g >> 1) & 1));
-        if (!ok) break;
-        const uint2 nans = *reinterpret_cast<const uint2*>(nan_rows + 4 * pb);
+        const uint2 nans = *reinterpret_cast<const uint2*>(nan_rows + 4 * ((g0 + j - d.j0) % kTileNanRing));
         if ((nans.x | nans.y) != 0u) {
 #pragma unroll
           for (int c = 0; c < kTileKeys; ++c) {
@@ -562,8 +593,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
         }
         tmem_st32(tS + pb * kTileKeys, *reinterpret_cast<const uint32_t(*)[32]>(&pk[0]));
-        if (j > d.j0 && __any_sync(0xffffffffu, grow)) {  // O *= alpha once the previous P.V retired
-          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][pb ^ 1], ((g - 1) >> 1) & 1));
+        if (!first && __any_sync(0xffffffffu, grow)) {  // O *= alpha once the previous P.V retired
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_free[h][pb ^ 1], ((n - 1) >> 1) & 1));
           if (!ok) break;
           tc_fence_after();
 #pragma unroll
@@ -579,12 +610,55 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         tmem_wait_st();
         tc_fence_before();
         mbar_arrive(&bars->p_full[h][pb]);
+        first = false;
       }
       if (!ok) break;
-      // ---- epilogue, once the piece's last P.V retired
-      ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_free[h][(g - 1) & 1], ((g - 1) >> 1) & 1));
+      g0 += d.j1 - d.j0;
+      // ---- epilogue, once the half's last P.V of the piece retired (a twin may have had none)
+      if (!first) ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_free[h][(n - 1) & 1], ((n - 1) >> 1) & 1));
       if (!ok) break;
       tc_fence_after();
+      float mine = 1.f, other = 0.f;  // weights of the two halves' accumulators
+      if (twin) {
+        if (h == 1) {
+          if (twins > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_free, (twins - 1) & 1));
+          if (!ok) break;
+          ++twins;
+          twin_ml[lane_row] = make_float2(m_run, l_run);
+          if (!first) {
+#pragma unroll
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              tmem_ld32(tO + 32 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 32; ++e) twin_o[(32 * c + e) * kHalfRows] = __uint_as_float(o[e]);
+            }
+          }
+          mbar_arrive(&bars->x_full);
+          continue;
+        }
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_full, twins & 1));
+        if (!ok) break;
+        ++twins;
+        const float2 v = twin_ml[lane_row];
+        const float m = fmaxf(m_run, v.x), ref = m == -INFINITY ? 0.f : m;
+        mine = ex2(m_run - ref);
+        other = ex2(v.x - ref);
+        l_run = l_run * mine + v.y * other;
+        m_run = m;
+      }
+      // A twin without a tile left nothing in its scratch.
+      const bool joined = twin && d.j1 - d.j0 > 1;
+      auto result = [&](int c, uint32_t (&o)[32]) {
+        tmem_ld32(tO + 32 * c, o);
+        tmem_wait_ld();
+        if (joined) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * mine + twin_o[(32 * c + e) * kHalfRows] * other);
+        }
+      };
       const bool stored = t_row < d.tokens;
       if (d.part < 0) {
         const float inv = 1.f / l_run;
@@ -592,8 +666,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + 32 * c, o);
-          tmem_wait_ld();
+          result(c, o);
           if (stored) {
 #pragma unroll
             for (int e = 0; e < 32; e += 8) {
@@ -611,8 +684,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
-          tmem_ld32(tO + 32 * c, o);
-          tmem_wait_ld();
+          result(c, o);
           if (stored) {
 #pragma unroll
             for (int e = 0; e < 32; e += 4)
@@ -621,6 +693,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (stored) p.part_ml[at] = make_float2(m_run, l_run);
       }
+      if (twin) mbar_arrive(&bars->x_free);
       // The next piece's first P.V overwrites O only after p_full, which these threads arrive
       // on after the loads above completed (tcgen05.wait::ld).
     }
