@@ -59,9 +59,10 @@ struct RowsCfg {
   static_assert(!PAIR || D == 128, "pairs of heads of 64");
   static constexpr int DO = PAIR ? 64 : D;          // dims of a query and an output row
   static constexpr int SUBS = PAIR ? 2 : 1;         // KV heads of a payload row
-  // Blocks a softmax step takes: with three groups of rows one block's scores at a time fit
-  // the registers.
-  static constexpr int NB = RG <= 2 ? 2 : 1;
+  // Blocks a softmax step takes.  With three groups of rows both blocks' scores do not quite
+  // fit the registers, but a block at a time is slower all the same (24 chunks of 5 tokens over
+  // 6,000 keys: 176 against 118 us): the steps are chains of dependent instructions.
+  static constexpr int NB = 2;
   static constexpr int SCALES = 2 * SUBS * kRowsStage;  // bytes a stage: K then V
   static constexpr int STAGES = D == 128 ? 2 : 4;   // 16 KB in flight per warp
   static constexpr int TILE = kRowsKeys * D;        // K or V of a block

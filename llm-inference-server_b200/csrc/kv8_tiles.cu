@@ -15,17 +15,19 @@
 // the context and every CTA does the same number of keys; a tile that a cut falls into
 // leaves float32 partials that kv8_combine joins.
 //
-// Roles (640 threads, registers dealt out by setmaxnreg):
+// Roles (768 threads, registers dealt out by setmaxnreg):
 //   warps 0-3, 4-7  softmax of rows 0-127 / 128-255, one thread per row (TMEM lane): loads its
 //                   query row into shared memory, reads scores, keeps maximum and sum, writes
 //                   P to TMEM, the epilogue
-//   warps 8-9       K: staged e4m3 -> fp16 in the swizzled layout (3 stages); 10-11: V (2)
-//   warps 12, 13    S = Q K^T issue of either half (12 also allocates TMEM)
-//   warps 14, 15    O += P V issue of either half
-//   warps 16, 17    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
+//   warps 8-11      K: staged e4m3 -> fp16 in the swizzled layout (3 stages), 16 keys a warp;
+//                   12-15: V (2 stages).  Two warps each took 1 us per tile of 64 keys, more
+//                   than anything else
+//   warps 16, 17    S = Q K^T issue of either half (16 also allocates TMEM)
+//   warps 18, 19    O += P V issue of either half
+//   warps 20, 21    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
 //                   staging rings of 4 tiles (K's with V's scale bytes beside, for the rows
 //                   that stand for NaN: the softmax learns of them with the scores)
-//   warp 18         finds the slice's pieces (a 2-slot ring)
+//   warp 22         finds the slice's pieces (a 2-slot ring)
 // TMEM columns of a half: two score buffers of 64, O [128, 128 + D).  A row's weights go over
 // the first 32 columns of the scores they came from (each thread has read its own by then),
 // so S of the next tile is issued a tile ahead and its latency lies behind a softmax: with one
@@ -60,10 +62,10 @@ constexpr int kTileKeys = 64;
 constexpr int kTileKStages = 3;
 constexpr int kTileVStages = 2;  // equal to the P buffer count: one "P.V retired" barrier frees both
 constexpr int kTileRing = 4;     // staged e4m3 tiles, K and V each
-constexpr int kTileThreads = 640;
+constexpr int kTileThreads = 768;
 constexpr int kTileQBox = kHalfRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kTileBox = kTileKeys * 128;   // 64 keys x 64 elements
-constexpr int kTileConsumers = 18;          // warps that read a piece: 8 softmax, 4 widening, 4 issuers, 2 producers
+constexpr int kTileConsumers = 22;          // warps that read a piece: 8 softmax, 8 widening, 4 issuers, 2 producers
 // Fewest keys a slice gets: below this its partial costs more than the keys it takes over.
 constexpr int kTileMinKeys = 512;
 // The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 and the
@@ -128,19 +130,19 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// A widening warp's half (32 keys) of a staged 64-key tile: read into registers, then widened
-// into the swizzled tile.  Lanes take 16-byte chunks, D / 16 lanes a row.
+// A widening warp's 16 keys of a staged 64-key tile: read into registers, then widened into the
+// swizzled tile.  Lanes take 16-byte chunks, D / 16 lanes a row.
 template <int D>
-struct WidenHalf {
+struct WidenPart {
   static constexpr int LPR = D / 16;      // lanes a row
   static constexpr int RPI = 32 / LPR;    // rows an instruction
-  static constexpr int N = 32 / RPI;      // instructions
+  static constexpr int N = 16 / RPI;      // instructions
   uint4 x[N];
-  uint32_t scale;                         // of key `lane`
+  uint32_t scale;                         // of key `lane`, lanes 0-15
 
   // Rows at and past `live` (behind the context) read as zeros.
   __device__ __forceinline__ void read(const uint8_t* staged, const uint8_t* scales, int lane, int live) {
-    scale = lane < live ? scales[lane] : 0u;
+    scale = lane < min(16, live) ? scales[lane] : 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       x[i] = *reinterpret_cast<const uint4*>(staged + 16 * (32 * i + lane));
@@ -189,7 +191,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   const int slices = line_slices(total, p.slices, kTileMinKeys);
   if (total == 0 || slice >= slices) return;
 
-  if (warp == 12) {
+  if (warp == 16) {
     tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
     tmem_relinquish();
   }
@@ -197,14 +199,14 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     for (int i = 0; i < 2; ++i)
       for (int s = 0; s < kTileRing; ++s) {
         mbar_init(&bars->st_full[i][s], kTileKeys / 16);
-        mbar_init(&bars->st_empty[i][s], 2);
+        mbar_init(&bars->st_empty[i][s], 4);
       }
     for (int s = 0; s < kTileKStages; ++s) {
-      mbar_init(&bars->k_full[s], 2);
+      mbar_init(&bars->k_full[s], 4);
       for (int h = 0; h < 2; ++h) mbar_init(&bars->k_free[h][s], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars->v_full[s], 2);
+      mbar_init(&bars->v_full[s], 4);
       for (int h = 0; h < 2; ++h) {
         mbar_init(&bars->v_free[h][s], 1);
         mbar_init(&bars->s_full[h][s], 1);
@@ -240,9 +242,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   auto is_idle = [](bool twin, int h, const TilePiece& d) { return twin && h == 1 && d.j1 - d.j0 < 2; };
 
   bool ok = true;
-  if (warp >= 16) {
+  if (warp >= 20) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-    if (warp == 18) {
+    if (warp == 22) {
       // ---------------------------------------------------------- pieces
       const int64_t x1 = line_cut(total, slices, slice + 1);
       int64_t x = line_cut(total, slices, slice);
@@ -282,9 +284,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         }
         if (t.seq < 0) break;
       }
-    } else if (warp < 18) {
-      // ---------------------------------------------------------- producers: warp 16 K, 17 V
-      const int v = warp - 16;
+    } else if (warp < 22) {
+      // ---------------------------------------------------------- producers: warp 20 K, 21 V
+      const int v = warp - 20;
       const CUtensorMap* map = v ? &tv : &tk;
       uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES;
       uint8_t* scale_ring = smem + C::OFF_SCALE + (v ? 2 * kTileRing * kTileKeys : 0);
@@ -350,12 +352,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       if (!ok)  // leave with no copy into this CTA's shared memory in flight
         for (int i = max(0, n - kTileRing); i < n; ++i) mbar_wait(&bars->st_full[v][i % kTileRing], (i / kTileRing) & 1);
     }
-  } else if (warp >= 12) {
+  } else if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     const int h = warp & 1;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF;
     const uint32_t tS = tbase, tO = tbase + C::COL_O;
-    if (warp < 14) {
+    if (warp < 18) {
       // ---------------------------------------------------------- S issue of half h
       int g = 0, n = 0, queries = 0;
       for (int k = 0; ok; ++k) {
@@ -438,8 +440,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     }
   } else if (warp >= 8) {
-    // ------------------------------------------------------------ widening: warps 8-9 K, 10-11 V
-    const int v = warp >= 10 ? 1 : 0, row0 = 32 * (warp & 1);
+    // ------------------------------------------------------------ widening: warps 8-11 K, 12-15 V
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    const int v = warp >= 12 ? 1 : 0, row0 = 16 * (warp & 3);
     const int stages = v ? kTileVStages : kTileKStages;
     uint64_t* full = v ? bars->v_full : bars->k_full;
     const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES + row0 * D;
@@ -447,7 +450,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int scale_step = v ? kTileKeys : 2 * kTileKeys;
     uint8_t* out = v ? sV : sK;
     int n = 0, s = 0, round = 0;
-    WidenHalf<D> half;
+    WidenPart<D> part;
     for (int k = 0; ok; ++k) {
       TilePiece d;
       ok = next_piece(k, d);
@@ -463,12 +466,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         if (!ok) break;
         const int live = d.ctx - j * kTileKeys - row0;
         const uint8_t* sc = scale_ring + st * scale_step;
-        half.read(ring + st * C::ST_BYTES, sc, lane, live);
+        part.read(ring + st * C::ST_BYTES, sc, lane, live);
         if (!v) {
-          const uint32_t nans = __ballot_sync(0xffffffffu, lane < live && sc[kTileKeys + lane] == 255);
-          if (lane < 2) nan_rows[4 * (n % kTileNanRing) + 2 * (warp & 1) + lane] = uint16_t(nans >> (16 * lane));
+          const uint32_t nans = __ballot_sync(0xffffffffu, lane < min(16, live) && sc[kTileKeys + lane] == 255);
+          if (lane == 0) nan_rows[4 * (n % kTileNanRing) + (warp & 3)] = uint16_t(nans);
         }
-        half.store(out + s * C::KV_BYTES, row0, lane, v != 0);
+        part.store(out + s * C::KV_BYTES, row0, lane, v != 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -483,7 +486,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax (one row per thread)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
     const int h = warp >> 2;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
@@ -702,7 +705,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 16) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(bars->tmem_base, C::TMEM_COLS);
