@@ -63,12 +63,17 @@ cudaError_t launch_kv8_append(int dtype, const Kv8AppendParams& p, cudaStream_t 
 // Slices of the work line for the kernel for few rows, and the rows a partial holds.
 int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
 // `pair`: p.num_kv_heads counts pairs of KV heads of 64 dims, p.group the query heads of a pair.
+// The kernels of a call, in this order: rows, tiles, then the joins.  The tiles kernel starts
+// while the one for few rows runs, so it must directly follow it.
 cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
                             const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream);
 constexpr int kKv8RowGroups = 3;  // most groups of 8 rows
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
+                                    cudaStream_t stream);
 int kv8_tiles_slices(int num_kv_heads, int sms);
 cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
                              const Kv8AttnParams& p, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream);
 constexpr int kKv8TileRows = 256;  // (token, head) rows of its tiles
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
                                cudaStream_t stream);

@@ -355,23 +355,30 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.part_o = reinterpret_cast<float*>(ws + s.o);
   cudaError_t e = launch_kv8_rows(dtype, head_dim, f.pair, f.row_groups, tk, tv, p, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
-  note_launches(PA_LAUNCH_KV8_ROWS | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
-  if (max_query_len > t.small_max) {
-    p.work = work + num_seqs + 1;
-    p.num_kv_heads = num_kv_heads;
-    p.group = group;
-    p.tile_tokens = t.large_tokens;
-    p.slices = kv8_tiles_slices(num_kv_heads, sms);
-    p.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
-    p.part_o = reinterpret_cast<float*>(ws + s.tile_o);
-    p.twin_o = reinterpret_cast<float*>(ws + s.twin_o);
+  int32_t launched = PA_LAUNCH_KV8_ROWS;
+  Kv8AttnParams q = p;  // of the tiles kernel
+  const bool tiles = max_query_len > t.small_max;
+  if (tiles) {
+    q.work = work + num_seqs + 1;
+    q.num_kv_heads = num_kv_heads;
+    q.group = group;
+    q.tile_tokens = t.large_tokens;
+    q.slices = kv8_tiles_slices(num_kv_heads, sms);
+    q.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
+    q.part_o = reinterpret_cast<float*>(ws + s.tile_o);
+    q.twin_o = reinterpret_cast<float*>(ws + s.twin_o);
     st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tk);
     if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tv);
     if (st != PA_OK) return st;
-    e = launch_kv8_tiles(dtype, head_dim, tk, tv, p, err, stream);
+    e = launch_kv8_tiles(dtype, head_dim, tk, tv, q, err, stream);
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
-    note_launches(PA_LAUNCH_KV8_TILES | (p.slices > 1 ? PA_LAUNCH_KV8_COMBINE : 0));
+    launched |= PA_LAUNCH_KV8_TILES;
   }
+  e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, stream);
+  if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, stream);
+  if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention join launch");
+  if (p.slices > 1 || (tiles && q.slices > 1)) launched |= PA_LAUNCH_KV8_COMBINE;
+  note_launches(launched);
   return PA_OK;
 }
 

@@ -29,6 +29,7 @@ struct LineTile {
   int index;        // tile of the sequence
   int64_t start;    // place of its first key on the line
   int keys;
+  int first, q, ctx;  // of the sequence: packed index of its first token, new tokens, context
 };
 
 // End of slice s - 1 / start of slice s out of n over a line of `total` keys.
@@ -48,48 +49,86 @@ __device__ __forceinline__ int line_key(const LineTile& t, int64_t x, int step) 
   return k < t.keys ? int(k) : t.keys;
 }
 
-// The tile that holds place x.  Called by a whole warp; `work` is the class's running sum.
-__device__ __forceinline__ LineTile line_find(const int64_t* work, int num_seqs, const int32_t* ctx_lens,
-                                              const int32_t* cu_q, int tt, int64_t x, int hint) {
-  const int lane = threadIdx.x & 31;
-  LineTile t;
-  t.seq = -1;
-  if (x >= work[num_seqs]) return t;
-  // Largest i with work[i] <= x; the next 32 sequences first, then a 32-way search.
-  int lo = 0, hi = num_seqs;  // work[lo] <= x < work[hi]
-  {
-    const int i = min(hint + 1 + lane, num_seqs);
-    const unsigned above = __ballot_sync(0xffffffffu, work[i] > x);
-    if (above) {
-      hi = min(hint + __ffs(above), num_seqs);
-      lo = hi - 1;
-    } else {
-      lo = min(hint + 32, num_seqs - 1);
+// Looks tiles up by place; a whole warp's.  Finding one is a chain of dependent loads, which is
+// most of what a short call costs, so lane i keeps what belongs to sequence hint + i: loaded
+// in one go, before the first place is even known, and enough for any batch of up to 32
+// sequences and for walking from a sequence to the next.
+struct LineFinder {
+  const int64_t* work;
+  const int32_t *ctx_lens, *cu_q;
+  int num_seqs, tt, hint;
+  int64_t begin, end;  // of the lane's sequence on the line
+  int first, next, ctx;
+
+  __device__ __forceinline__ void load(int from) {
+    hint = from;
+    const int i = min(from + int(threadIdx.x & 31), num_seqs - 1);
+    begin = work[i];
+    end = work[i + 1];
+    first = cu_q[i];
+    next = cu_q[i + 1];
+    ctx = ctx_lens[i];
+  }
+
+  __device__ __forceinline__ LineFinder(const int64_t* work_, int num_seqs_, const int32_t* ctx_lens_,
+                                        const int32_t* cu_q_, int tile_tokens)
+      : work(work_), ctx_lens(ctx_lens_), cu_q(cu_q_), num_seqs(num_seqs_), tt(tile_tokens) {
+    load(0);
+  }
+
+  // The tile that holds place x, with work[hint] <= x < total.
+  __device__ __forceinline__ LineTile find(int64_t x) {
+    const int lane = threadIdx.x & 31;
+    unsigned above = __ballot_sync(0xffffffffu, end > x);
+    if (!above) {
+      // Largest i with work[i] <= x: a 32-way search, then the sequences from there.
+      int lo = min(hint + 32, num_seqs - 1), hi = num_seqs;  // work[lo] <= x < work[hi]
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const unsigned up = __ballot_sync(0xffffffffu, work[min(lo + step * (lane + 1), hi)] > x);
+        const int f = __ffs(up) - 1;  // lane 31 probes hi
+        hi = min(lo + step * (f + 1), hi);
+        lo = lo + step * f;
+      }
+      load(lo);
+      above = 1u;
     }
+    const int f = __ffs(above) - 1;
+    LineTile t;
+    t.seq = hint + f;
+    t.first = __shfl_sync(0xffffffffu, first, f);
+    t.q = __shfl_sync(0xffffffffu, next, f) - t.first;
+    t.ctx = __shfl_sync(0xffffffffu, ctx, f);
+    const int64_t at = __shfl_sync(0xffffffffu, begin, f), base = t.ctx - t.q, rest = x - at;
+    int a = 0, b = (t.q + tt - 1) / tt;  // keys_before(a) <= rest < keys_before(b)
+    while (b - a > 1) {
+      const int m = (a + b) / 2;
+      if (line_keys_before(base, t.q, tt, m) <= rest)
+        a = m;
+      else
+        b = m;
+    }
+    t.index = a;
+    t.start = at + line_keys_before(base, t.q, tt, a);
+    t.keys = int(line_tile_keys(base, t.q, tt, a));
+    return t;
   }
-  while (hi - lo > 1) {
-    const int step = (hi - lo + 31) / 32;
-    const int i = min(lo + step * (lane + 1), hi);
-    const unsigned above = __ballot_sync(0xffffffffu, work[i] > x);
-    const int f = __ffs(above) - 1;  // lane 31 probes hi
-    hi = min(lo + step * (f + 1), hi);
-    lo = lo + step * f;
+};
+
+// The pieces of a slice [x, end), in order: the parts of its tiles, cut at multiples of `step`.
+struct LinePiece {
+  LineTile t;
+  int k0, k1;  // keys
+};
+__device__ __forceinline__ bool line_next_piece(LineFinder& f, int64_t& x, int64_t end, int step, LinePiece& d) {
+  while (x < end) {
+    d.t = f.find(x);
+    d.k0 = line_key(d.t, x, step);
+    d.k1 = line_key(d.t, end, step);
+    x = d.t.start + d.t.keys;
+    if (d.k1 > d.k0) return true;
   }
-  const int q = cu_q[lo + 1] - cu_q[lo], ctx = ctx_lens[lo];
-  const int64_t base = ctx - q, rest = x - work[lo];
-  int a = 0, b = (q + tt - 1) / tt;  // keys_before(a) <= rest < keys_before(b)
-  while (b - a > 1) {
-    const int m = (a + b) / 2;
-    if (line_keys_before(base, q, tt, m) <= rest)
-      a = m;
-    else
-      b = m;
-  }
-  t.seq = lo;
-  t.index = a;
-  t.start = work[lo] + line_keys_before(base, q, tt, a);
-  t.keys = int(line_tile_keys(base, q, tt, a));
-  return t;
+  return false;
 }
 
 }  // namespace pa

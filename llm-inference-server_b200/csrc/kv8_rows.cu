@@ -36,6 +36,7 @@
 #include <cuda_fp16.h>
 
 #include "kv8.h"
+#include "kv8_launch.cuh"
 #include "kv8_line.cuh"
 #include "kv8_widen.cuh"
 #include "pa_common.cuh"
@@ -153,13 +154,9 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
-  const int64_t total = p.work[p.num_seqs];
-  const int slices = line_slices(total, p.slices, kRowsMinKeys);
-  if (total == 0 || slice >= slices) return;
-
   if (threadIdx.x == 0) {
     for (int i = 0; i < kRowsWarps * C::STAGES; ++i) {
-      mbar_init(&full[i], 2);  // one arrival per block
+      mbar_init(&full[i], 4);  // per block: its tiles are on their way, its scales are there
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kRowsDescs; ++i) {
@@ -167,21 +164,25 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
       mbar_init(&d_empty[i], kRowsWarps);
     }
     fence_mbar_init();
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
   }
   __syncthreads();
+  pdl_wait();
+  pdl_release();
+  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
+  const int64_t total = p.work[p.num_seqs];
+  const int slices = line_slices(total, p.slices, kRowsMinKeys);
+  if (total == 0 || slice >= slices) return;
 
   if (warp == kRowsWarps) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
-      prefetch_tmap(&tk);
-      prefetch_tmap(&tv);
-    }
-    const int64_t x0 = line_cut(total, slices, slice), x1 = line_cut(total, slices, slice + 1);
-    int64_t x = x0;
+    const int64_t x1 = line_cut(total, slices, slice + 1);
+    int64_t x = line_cut(total, slices, slice);
     int issued[kRowsWarps];
 #pragma unroll
     for (int w = 0; w < kRowsWarps; ++w) issued[w] = 0;
-    int pieces = 0, hint = 0;
+    int pieces = 0;
     bool ok = true;
     struct BlockRef {
       int slot;  // first slot of the 16 keys
@@ -209,48 +210,33 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
       return r;
     };
     while (ok) {
-      LineTile t;
-      t.seq = -1;
-      int k0 = 0, k1 = 0;
-      while (x < x1) {
-        t = line_find(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens, x, hint);
-        if (t.seq < 0) break;
-        hint = t.seq;
-        k0 = line_key(t, x, kRowsKeys);
-        k1 = line_key(t, x1, kRowsKeys);
-        x = t.start + t.keys;
-        if (k1 > k0) break;
-        t.seq = -1;
-      }
+      LinePiece at;
+      const bool more = line_next_piece(finder, x, x1, kRowsKeys, at);
       const int slot = pieces % kRowsDescs;
       if (pieces >= kRowsDescs) ok = mbar_wait(&d_empty[slot], ((pieces / kRowsDescs) - 1) & 1);
       ok = __all_sync(0xffffffffu, ok);
       if (!ok) break;
-      int ctx = 0, kb0 = 0, kb1 = 0;
-      if (t.seq >= 0) {
-        ctx = p.ctx_lens[t.seq];
-        kb0 = k0 / kRowsKeys;
-        kb1 = (k1 + kRowsKeys - 1) / kRowsKeys;
-      }
+      const LineTile& t = at.t;
+      const int kb0 = at.k0 / kRowsKeys, kb1 = (at.k1 + kRowsKeys - 1) / kRowsKeys;
       if (lane == 0) {
         RowsPiece d;
         d.row0 = -1;
         d.pad = 0;
-        if (t.seq >= 0) {
-          const int first = p.cu_q[t.seq], q = p.cu_q[t.seq + 1] - first, t0 = t.index * p.tile_tokens;
-          d.row0 = first + t0;
-          d.tokens = min(p.tile_tokens, q - t0);
-          d.pos0 = ctx - q + t0;
-          d.ctx = ctx;
+        if (more) {
+          const int t0 = t.index * p.tile_tokens;
+          d.row0 = t.first + t0;
+          d.tokens = min(p.tile_tokens, t.q - t0);
+          d.pos0 = t.ctx - t.q + t0;
+          d.ctx = t.ctx;
           d.kb0 = kb0;
           d.kb1 = kb1;
-          d.part = k0 > 0 ? 0 : (k1 < t.keys ? 1 : -1);
+          d.part = at.k0 > 0 ? 0 : (at.k1 < t.keys ? 1 : -1);
         }
         desc[slot] = d;
         rows_arrive(&d_full[slot]);
       }
       ++pieces;
-      if (t.seq < 0) break;
+      if (!more) break;
       const int32_t* row = p.tables + int64_t(t.seq) * p.table_stride;
       // Each lane looks up one of the next 32 blocks and reads its scales, one round ahead of
       // the round whose tiles are being issued; lanes then issue their own blocks, two (a
@@ -272,17 +258,19 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
                 uint64_t* bar = &full[w * C::STAGES + st];
                 if (lane < n) {
                   uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE + half * C::BLOCK;
+                  mbar_arrive_expect_tx(bar, C::BLOCK);
+                  tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
+                  tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
                   uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * C::SCALES + 16 * half;
 #pragma unroll
                   for (int u = 0; u < C::SUBS; ++u) {
                     *reinterpret_cast<uint4*>(sc + u * kRowsStage) = cur.ks[u];
                     *reinterpret_cast<uint4*>(sc + (C::SUBS + u) * kRowsStage) = cur.vs[u];
                   }
-                  mbar_arrive_expect_tx(bar, C::BLOCK);  // releases the scales too
-                  tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
-                  tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
+                  rows_arrive(bar);
                 } else {
                   rows_arrive(bar);  // the piece's last stage holds one block
+                  rows_arrive(bar);
                 }
               }
               if (ok) ++issued[w];
@@ -626,29 +614,42 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
 }
 
-// Joins the partials of tiles that a cut fell into.  CTA (s, kvh): the tile that the end of
-// slice s falls into, if this is the first cut inside it.  A warp takes NR rows at a time, a
-// lane D / 32 elements of each.  What bounds it is latency (places, then (m, l), then
-// accumulators), so NR x P accumulator loads are in flight: one row and eight parts for the
-// few rows of a long context, four rows and two parts for 256-row tiles.
-template <typename T, int D, int NR, int P>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys) {
-  constexpr int E = D / 32;
+// Joins the partials of tiles that a cut fell into.  CTA (s, kvh, z): the tile that the end of
+// slice s falls into, if this is the first cut inside it, and some of its rows; a lane takes
+// D / 32 elements of a row.  What bounds it is latency (places, then (m, l), then
+// accumulators), so loads are kept in flight side by side: in small tiles, which a long
+// context leaves in many parts, the CTA's warps share out the parts of NR rows (BY_PARTS); in
+// 256-row tiles, of two or three parts, every warp has rows of its own, NR at a time.
+constexpr int kCombineWarps = 8;
+
+template <typename T, int D, int NR, bool BY_PARTS>
+__global__ void __launch_bounds__(32 * kCombineWarps)
+    kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys) {
+  constexpr int E = D / 32, P = 2;
+  __shared__ float s_acc[BY_PARTS ? kCombineWarps : 1][NR][D];
+  __shared__ float2 s_ml[BY_PARTS ? kCombineWarps : 1][NR];
+  pdl_wait();
+  pdl_release();
+  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
   const int64_t total = p.work[p.num_seqs];
   const int slices = line_slices(total, p.slices, min_keys);
   const int s = blockIdx.x + 1, kvh = blockIdx.y;
   if (total == 0 || s >= slices) return;
   const int64_t x = line_cut(total, slices, s);
-  const LineTile t = line_find(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens, x, 0);
-  if (t.seq < 0 || x <= t.start || line_cut(total, slices, s - 1) > t.start) return;
+  const LineTile t = finder.find(x);
+  if (x <= t.start || line_cut(total, slices, s - 1) > t.start) return;
   if (line_key(t, x, key_step) >= t.keys) return;  // the first slice did the whole tile
-  const int first = p.cu_q[t.seq], q = p.cu_q[t.seq + 1] - first, t0 = t.index * p.tile_tokens;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t end = t.start + t.keys;
-  int last = s;
-  while (last + 1 < slices && line_cut(total, slices, last + 1) < end) ++last;
-  const int live = min(p.tile_tokens, q - t0) * p.group;  // rows of the tile
-  for (int r0 = (blockIdx.z * 4 + warp) * NR; r0 < live; r0 += 4 * NR * gridDim.z) {
+  // The last slice with a part of the tile: the largest i with cut(i) < end.
+  int last = int((end * slices - 1) / total);
+  last = min(last, slices - 1);
+  const int t0 = t.index * p.tile_tokens;
+  const int live = min(p.tile_tokens, t.q - t0) * p.group;  // rows of the tile
+  constexpr int ROWS = BY_PARTS ? NR : kCombineWarps * NR;  // of the CTA at a time
+  const int first_part = BY_PARTS ? warp : 0, part_step = BY_PARTS ? kCombineWarps : 1;
+  for (int z0 = blockIdx.z * ROWS; z0 < live; z0 += ROWS * gridDim.z) {
+    const int r0 = z0 + (BY_PARTS ? 0 : warp * NR);
     // A slice's part of the tile is its slot 1 if it starts the tile, else slot 0; it is empty
     // where both of its cuts move up to the same key.  Lanes look after 32 parts at a time.
     float acc[NR][E], m[NR], sum[NR];
@@ -659,8 +660,8 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[n][e] = 0.f;
     }
-    for (int i0 = s - 1; i0 <= last; i0 += 32) {
-      const int i = i0 + lane;
+    for (int i0 = s - 1 + first_part; i0 <= last; i0 += 32 * part_step) {
+      const int i = i0 + lane * part_step;
       const bool mine = i <= last && line_key(t, line_cut(total, slices, i + 1), key_step) >
                                          line_key(t, line_cut(total, slices, i), key_step);
       const int64_t at = mine ? ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r0 : -1;
@@ -685,7 +686,7 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[n][e] *= old;
       }
-      const int parts = min(32, last + 1 - i0);
+      const int parts = min(32, (last - i0) / part_step + 1);
       for (int k0 = 0; k0 < parts; k0 += P) {
         float o[P][NR][E], fk[P][NR];
 #pragma unroll
@@ -709,11 +710,38 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const Kv8AttnParams p,
               for (int e = 0; e < E; ++e) acc[n][e] += o[k][n][e] * fk[k][n];
       }
     }
+    if constexpr (BY_PARTS) {  // join the warps; warp n finishes row n
 #pragma unroll
-    for (int n = 0; n < NR; ++n) {
-      const int r = r0 + n, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
-      if (r >= live) break;
-      T* dst = static_cast<T*>(p.out) + int64_t(first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
+      for (int n = 0; n < NR; ++n) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) s_acc[warp][n][E * lane + e] = acc[n][e];
+        if (lane == 0) s_ml[warp][n] = make_float2(m[n], sum[n]);
+      }
+      __syncthreads();
+      if (warp < NR) {
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kCombineWarps; ++w) mm = fmaxf(mm, s_ml[w][warp].x);
+        const float ref = mm == -INFINITY ? 0.f : mm;
+        sum[0] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[0][e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kCombineWarps; ++w) {
+          const float2 v = s_ml[w][warp];
+          const float f = ex2(v.x - ref);
+          sum[0] += v.y * f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[0][e] += s_acc[w][warp][E * lane + e] * f;
+        }
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int n = 0; n < (BY_PARTS ? 1 : NR); ++n) {
+      const int r = BY_PARTS ? r0 + warp : r0 + n, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
+      if (r >= live || (BY_PARTS && warp >= NR)) break;
+      T* dst = static_cast<T*>(p.out) + int64_t(t.first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
       const float inv = 1.f / sum[n];
 #pragma unroll
       for (int e = 0; e < E; e += 2)
@@ -739,8 +767,7 @@ static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const 
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  kern<<<p.slices * p.num_kv_heads, kRowsThreads, C::SMEM, stream>>>(tk, tv, p, err);
-  return cudaGetLastError();
+  return launch_pdl(kern, dim3(p.slices * p.num_kv_heads), dim3(kRowsThreads), C::SMEM, stream, tk, tv, p, err);
 }
 
 template <typename T, int D, bool PAIR>
@@ -770,35 +797,34 @@ int kv8_rows_slices(int row_groups, int num_kv_heads, int sms) {
 
 cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
                             const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
-  cudaError_t e = dtype == PA_DTYPE_F16
-                      ? rows_by_shape<__half>(head_dim, pair, row_groups, tk, tv, p, err, stream)
-                      : rows_by_shape<__nv_bfloat16>(head_dim, pair, row_groups, tk, tv, p, err, stream);
-  if (e != cudaSuccess) return e;
-  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, kRowsMinKeys, p, stream);
+  return dtype == PA_DTYPE_F16 ? rows_by_shape<__half>(head_dim, pair, row_groups, tk, tv, p, err, stream)
+                               : rows_by_shape<__nv_bfloat16>(head_dim, pair, row_groups, tk, tv, p, err, stream);
 }
 
 template <typename T, int D>
-static void combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, cudaStream_t stream) {
+static cudaError_t combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, cudaStream_t stream) {
   const int live = p.tile_tokens * p.group;
-  if (rows <= 32) {
-    const dim3 grid(p.slices - 1, p.num_kv_heads, (live + 3) / 4);
-    kv8_combine_kernel<T, D, 1, 8><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-  } else {
-    const dim3 grid(p.slices - 1, p.num_kv_heads, (live + 15) / 16);
-    kv8_combine_kernel<T, D, 4, 2><<<grid, 128, 0, stream>>>(p, rows, key_step, min_keys);
-  }
+  const dim3 block(32 * kCombineWarps);
+  if (rows <= 8 * kKv8RowGroups)
+    return launch_pdl(kv8_combine_kernel<T, D, 4, true>, dim3(p.slices - 1, p.num_kv_heads, (live + 3) / 4), block, 0,
+                      stream, p, rows, key_step, min_keys);
+  return launch_pdl(kv8_combine_kernel<T, D, 4, false>, dim3(p.slices - 1, p.num_kv_heads, (live + 63) / 64), block, 0,
+                    stream, p, rows, key_step, min_keys);
 }
 
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
                                cudaStream_t stream) {
   if (p.slices < 2) return cudaSuccess;
   if (dtype == PA_DTYPE_F16)
-    head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, stream)
-                   : combine_one<__half, 128>(rows, key_step, min_keys, p, stream);
-  else
-    head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, stream)
-                   : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, stream);
-  return cudaGetLastError();
+    return head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, stream)
+                          : combine_one<__half, 128>(rows, key_step, min_keys, p, stream);
+  return head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, stream)
+                        : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, stream);
+}
+
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
+                                    cudaStream_t stream) {
+  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, kRowsMinKeys, p, stream);
 }
 
 }  // namespace pa

@@ -12,6 +12,7 @@
 // the per-token arrays; no CTA reads what another writes (a new block's id comes from the
 // free list by arithmetic, not from the table that it is also written to).
 #include "kv8.h"
+#include "kv8_launch.cuh"
 #include "kv8_line.cuh"
 #include "pa_common.cuh"
 
@@ -65,6 +66,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
   uint32_t* s_seen = reinterpret_cast<uint32_t*>(s_row + rows);  // a bit per slot, with row_ids only
   __shared__ int64_t scan[kStepThreads / 32][4];
   const int tid = threadIdx.x;
+  pdl_release();
 
   if (p.row_ids) {
     for (int i = tid; i < (p.num_slots + 31) / 32; i += blockDim.x) s_seen[i] = 0u;

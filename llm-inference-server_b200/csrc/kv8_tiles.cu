@@ -48,6 +48,7 @@
 #include <cuda_fp16.h>
 
 #include "kv8.h"
+#include "kv8_launch.cuh"
 #include "kv8_line.cuh"
 #include "kv8_widen.cuh"
 #include "pa_common.cuh"
@@ -187,9 +188,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
+  // What this reads was complete before the kernel for few rows let it start; the wait before
+  // every end makes its completion imply that kernel's.
+  pdl_release();
+  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
   const int64_t total = p.work[p.num_seqs];
   const int slices = line_slices(total, p.slices, kTileMinKeys);
-  if (total == 0 || slice >= slices) return;
+  if (total == 0 || slice >= slices) {
+    pdl_wait();
+    return;
+  }
 
   if (warp == 16) {
     tmem_alloc(&bars->tmem_base, C::TMEM_COLS);
@@ -248,41 +256,30 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // ---------------------------------------------------------- pieces
       const int64_t x1 = line_cut(total, slices, slice + 1);
       int64_t x = line_cut(total, slices, slice);
-      int hint = 0;
       for (int k = 0;; ++k) {
-        LineTile t;
-        t.seq = -1;
-        int k0 = 0, k1 = 0;
-        while (x < x1) {
-          t = line_find(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens, x, hint);
-          if (t.seq < 0) break;
-          hint = t.seq;
-          k0 = line_key(t, x, kTileKeys);
-          k1 = line_key(t, x1, kTileKeys);
-          x = t.start + t.keys;
-          if (k1 > k0) break;
-          t.seq = -1;
-        }
+        LinePiece at;
+        const bool more = line_next_piece(finder, x, x1, kTileKeys, at);
         if (k >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars->d_empty[k & 1], ((k >> 1) - 1) & 1));
         if (!ok) break;
         if (lane == 0) {
           TilePiece d{};
           d.row0 = -1;
-          if (t.seq >= 0) {
-            const int first = p.cu_q[t.seq], q = p.cu_q[t.seq + 1] - first, t0 = t.index * p.tile_tokens;
-            d.row0 = first + t0;
-            d.tokens = min(p.tile_tokens, q - t0);
-            d.ctx = p.ctx_lens[t.seq];
-            d.pos0 = d.ctx - q + t0;
+          if (more) {
+            const LineTile& t = at.t;
+            const int t0 = t.index * p.tile_tokens;
+            d.row0 = t.first + t0;
+            d.tokens = min(p.tile_tokens, t.q - t0);
+            d.ctx = t.ctx;
+            d.pos0 = t.ctx - t.q + t0;
             d.seq = t.seq;
-            d.j0 = k0 / kTileKeys;
-            d.j1 = (k1 + kTileKeys - 1) / kTileKeys;
-            d.part = k0 > 0 ? 0 : (k1 < t.keys ? 1 : -1);
+            d.j0 = at.k0 / kTileKeys;
+            d.j1 = (at.k1 + kTileKeys - 1) / kTileKeys;
+            d.part = at.k0 > 0 ? 0 : (at.k1 < t.keys ? 1 : -1);
           }
           desc[k & 1] = d;
           mbar_arrive(&bars->d_full[k & 1]);
         }
-        if (t.seq < 0) break;
+        if (!more) break;
       }
     } else if (warp < 22) {
       // ---------------------------------------------------------- producers: warp 20 K, 21 V
@@ -703,6 +700,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   }
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
 
+  pdl_wait();
   tc_fence_before();
   __syncthreads();
   if (warp == 16) {
@@ -729,8 +727,7 @@ static cudaError_t tiles_one(const CUtensorMap& tk, const CUtensorMap& tv, const
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  kern<<<p.slices * p.num_kv_heads, kTileThreads, C::SMEM, stream>>>(tk, tv, p, err);
-  return cudaGetLastError();
+  return launch_pdl(kern, dim3(p.slices * p.num_kv_heads), dim3(kTileThreads), C::SMEM, stream, tk, tv, p, err);
 }
 
 int kv8_tiles_slices(int num_kv_heads, int sms) {
@@ -746,9 +743,11 @@ static cudaError_t tiles_by_dim(int head_dim, const CUtensorMap& tk, const CUten
 
 cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
                              const Kv8AttnParams& p, int* err, cudaStream_t stream) {
-  const cudaError_t e = dtype == PA_DTYPE_F16 ? tiles_by_dim<__half>(head_dim, tk, tv, p, err, stream)
-                                              : tiles_by_dim<__nv_bfloat16>(head_dim, tk, tv, p, err, stream);
-  if (e != cudaSuccess) return e;
+  return dtype == PA_DTYPE_F16 ? tiles_by_dim<__half>(head_dim, tk, tv, p, err, stream)
+                               : tiles_by_dim<__nv_bfloat16>(head_dim, tk, tv, p, err, stream);
+}
+
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream) {
   return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, stream);
 }
 
