@@ -93,6 +93,21 @@ def _tiling(group: int, max_query_len: int) -> _lib.Kv8Tiling:
 _CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _FREE, _TABLES = range(1, 10)
 
 
+_LAYOUTS: dict[tuple[int, int, int], tuple[tuple[int, ...], tuple[int, ...], int]] = {}
+
+
+def _layout(b: int, t: int, cells: int) -> tuple[tuple[int, ...], tuple[int, ...], int]:
+    """(words of each array, their byte offsets, words in all)."""
+    got = _LAYOUTS.get((b, t, cells))
+    if got is None:
+        sizes = (4 * (b + 1), b, b, b, b + 1, t, t, t, 1, cells)
+        got = (sizes, tuple(4 * sum(sizes[:i]) for i in range(len(sizes))), sum(sizes))
+        if len(_LAYOUTS) > 1024:
+            _LAYOUTS.clear()
+        _LAYOUTS[(b, t, cells)] = got
+    return got
+
+
 class DeviceStep:
     """One step's metadata on the GPU, shared by every layer: ``block_tables [B, W]``,
     ``context_lens`` / ``query_lens [B]``, ``cu_query_lens [B + 1]``, per token ``seq_idx``,
@@ -104,36 +119,33 @@ class DeviceStep:
                  num_blocks: int, group: int, device: torch.device, own_tables: bool):
         self.num_seqs, self.num_tokens, self.width, self.max_query_len = num_rows, num_tokens, width, max_query_len
         self.block_size, self.num_blocks, self.group, self.device = block_size, num_blocks, group, device
-        b, t = num_rows, num_tokens
-        self._sizes = (4 * (b + 1), b, b, b, b + 1, t, t, t, 1, b * width if own_tables else 0)
-        self.buffer = torch.empty(sum(self._sizes), dtype=torch.int32, device=device)
-        at, ptrs = self.buffer.data_ptr(), []
-        for n in self._sizes:
-            ptrs.append(at)
-            at += 4 * n
-        self._ptr = ptrs
+        self._sizes, offsets, words = _layout(num_rows, num_tokens, num_rows * width if own_tables else 0)
+        self.buffer = torch.empty(words, dtype=torch.int32, device=device)
+        at = self.buffer.data_ptr()
+        self._ptr = [at + o for o in offsets]
         self._views: tuple[torch.Tensor, ...] | None = None
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
         self._row_ids: torch.Tensor | None = None
 
-    def _view(self, i: int) -> torch.Tensor:
+    @property
+    def _arrays(self) -> tuple[torch.Tensor, ...]:
         if self._views is None:
-            self._views = self.buffer.split(self._sizes)
-        return self._views[i]
+            self._views = torch.split_with_sizes(self.buffer, self._sizes)
+        return self._views
 
-    work = property(lambda self: self._view(0).view(torch.int64).view(2, self.num_seqs + 1))
-    context_lens = property(lambda self: self._view(_CTX))
-    query_lens = property(lambda self: self._view(_QL))
-    held = property(lambda self: self._view(_HELD))
-    cu_query_lens = property(lambda self: self._view(_CU))
-    seq_idx = property(lambda self: self._view(_SEQ))
-    q_pos = property(lambda self: self._view(_POS))
-    slot_mapping = property(lambda self: self._view(_SLOT))
-    num_free = property(lambda self: self._view(_FREE))
+    work = property(lambda self: self._arrays[0].view(torch.int64).view(2, self.num_seqs + 1))
+    context_lens = property(lambda self: self._arrays[_CTX])
+    query_lens = property(lambda self: self._arrays[_QL])
+    held = property(lambda self: self._arrays[_HELD])
+    cu_query_lens = property(lambda self: self._arrays[_CU])
+    seq_idx = property(lambda self: self._arrays[_SEQ])
+    q_pos = property(lambda self: self._arrays[_POS])
+    slot_mapping = property(lambda self: self._arrays[_SLOT])
+    num_free = property(lambda self: self._arrays[_FREE])
 
     @property
     def block_tables(self) -> torch.Tensor:
-        return self._tables if self._tables is not None else self._view(_TABLES).view(self.num_seqs, self.width)
+        return self._tables if self._tables is not None else self._arrays[_TABLES].view(self.num_seqs, self.width)
 
     def matches(self, num_tokens: int, block_size: int, num_blocks: int, group: int) -> bool:
         """Whether this step can drive an attention call of these sizes."""
@@ -229,15 +241,21 @@ class DeviceBlockTables:
         """Over tensors the caller already keeps (all int32, contiguous, on one GPU): ``tables
         [R, W]``, ``lens [R]``, ``held [R]``, ``free`` with its first ``num_free [1]`` entries
         valid.  They are updated in place."""
-        dev = tables.device
-        _need_cuda(dev, "DeviceBlockTables")
-        if tables.dim() != 2 or tuple(lens.shape) != (tables.shape[0],) or tuple(held.shape) != (tables.shape[0],):
+        dev, i32 = tables.device, torch.int32
+        if not (tables.dtype is i32 and lens.dtype is i32 and held.dtype is i32 and free.dtype is i32
+                and num_free.dtype is i32 and dev == lens.device and dev == held.device and dev == free.device
+                and dev == num_free.device and tables.is_contiguous() and lens.is_contiguous()
+                and held.is_contiguous() and free.is_contiguous()):
+            _need_cuda(dev, "DeviceBlockTables")
+            for name, t in (("tables", tables), ("lens", lens), ("held", held), ("free", free), ("num_free", num_free)):
+                if t.dtype != i32 or t.device != dev or not t.is_contiguous():
+                    raise ValueError(f"{name} must be contiguous int32 on {dev}")
+        shape = tables.shape
+        if len(shape) != 2 or lens.shape != shape[:1] or held.shape != shape[:1]:
             raise ValueError("tables must be [requests, width], lens and held [requests]")
         if free.dim() != 1 or num_free.numel() != 1:
             raise ValueError("free must be [capacity] and num_free [1]")
-        for name, t in (("tables", tables), ("lens", lens), ("held", held), ("free", free), ("num_free", num_free)):
-            if t.dtype != torch.int32 or t.device != dev or not t.is_contiguous():
-                raise ValueError(f"{name} must be contiguous int32 on {dev}")
+        _need_cuda(dev, "DeviceBlockTables")
         self = cls.__new__(cls)
         self._set(tables, lens, held, free, num_free, num_blocks, block_size)
         return self
@@ -246,7 +264,7 @@ class DeviceBlockTables:
         _check_step_sizes(0, 0, block_size, num_blocks)
         self.tables, self.lens, self.held, self.free, self.num_free = tables, lens, held, free, num_free
         self.num_blocks, self.block_size, self.device = int(num_blocks), int(block_size), tables.device
-        self.max_requests, self.width = (int(x) for x in tables.shape)
+        self.max_requests, self.width = tables.shape
 
     def reserve(self, request_ids: torch.Tensor, query_lens: torch.Tensor, *, num_tokens: int, max_query_len: int,
                 group: int = 1, out: DeviceStep | None = None) -> DeviceStep:
