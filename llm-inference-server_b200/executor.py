@@ -22,6 +22,10 @@ Sequences and pools are duck-typed exactly as the reference uses them: a sequenc
 ``blocks``, ``block_size``, ``capacity`` and ``ensure_private(logical, copy)``
 (inference_server/core/sequence.py, core/block_table.py); a pool has per-layer ``k`` /
 ``v`` lists of ``[num_blocks, block_size, Hkv, D]`` tensors (core/kv_pool.py:106-125).
+
+With a :class:`~.kv8.KV8Pool` (16-bit models) the same passes run over the 8-bit cache: the
+append quantises, attention reads e4m3, and the step's sums for it are made on the GPU from
+the uploaded metadata.
 """
 
 from __future__ import annotations
@@ -33,6 +37,7 @@ import torch
 from transformers import AttentionInterface, Cache
 
 from .attention import paged_attention_cuda
+from .kv8 import KV8Pool, attach_step, paged_attention_kv8, reshape_and_cache_kv8, step_of_metadata
 from .kv_cache import copy_blocks, reshape_and_cache
 from .metadata import StepMetadata, attach, prefill_tile_tokens
 
@@ -65,6 +70,10 @@ class PagedCache(Cache):
         k = key_states[0].transpose(0, 1)
         v = value_states[0].transpose(0, 1)
         pool = self.ctx.pool
+        if isinstance(pool, KV8Pool):
+            reshape_and_cache_kv8(k, v, pool.k[layer_idx], pool.v[layer_idx], pool.k_scale[layer_idx],
+                                  pool.v_scale[layer_idx], self.ctx.meta.slot_mapping())
+            return key_states, value_states
         reshape_and_cache(k, v, pool.k[layer_idx], pool.v[layer_idx], self.ctx.meta.slot_mapping())
         return key_states, value_states
 
@@ -83,6 +92,11 @@ def paged_attention_forward(module, query, key, value, attention_mask, scaling=N
     if scaling is None:
         scaling = query.shape[-1] ** -0.5
     q = query[0].transpose(0, 1)                                  # [T, H, D], strided
+    if isinstance(ctx.pool, KV8Pool):
+        layer, pool = module.layer_idx, ctx.pool
+        out = paged_attention_kv8(q, pool.k[layer], pool.v[layer], pool.k_scale[layer], pool.v_scale[layer],
+                                  ctx.block_tables, ctx.context_lens, ctx.query_lens, scaling)
+        return out.unsqueeze(0), None
     out = paged_attention_cuda(q, ctx.pool.k[module.layer_idx], ctx.pool.v[module.layer_idx], ctx.block_tables,
                                ctx.context_lens, ctx.query_lens, scaling)
     return out.unsqueeze(0), None
@@ -113,6 +127,9 @@ class CudaPagedExecutor:
         self.num_blocks, self.block_size, self.num_kv_heads, head_dim = pool.k[0].shape
         cfg = model.config
         heads = getattr(cfg, "num_attention_heads", None) or cfg.n_head
+        self.group = heads // self.num_kv_heads
+        if isinstance(pool, KV8Pool) and next(model.parameters()).dtype == torch.float32:
+            raise NotImplementedError("ATTENTION=cuda: the 8-bit cache takes float16 and bfloat16 models, not float32")
         self.tile_tokens = prefill_tile_tokens(heads, self.num_kv_heads, head_dim)
 
     @torch.inference_mode()
@@ -207,6 +224,8 @@ class CudaPagedExecutor:
         buf = meta.device_buffer
         ctx_lens = buf[meta.plan.off_context_lens:meta.plan.off_context_lens + len(seqs)]
         query_lens = buf[meta.plan.off_query_lens:meta.plan.off_query_lens + len(seqs)]
+        if isinstance(self.pool, KV8Pool):
+            attach_step(block_tables, step_of_metadata(meta, self.group))
         ctx = StepContext(meta=meta, block_tables=block_tables, context_lens=ctx_lens, query_lens=query_lens,
                           pool=self.pool)
         input_ids = torch.tensor([ids], dtype=torch.long).pin_memory().to(dev, non_blocking=True)
@@ -215,8 +234,12 @@ class CudaPagedExecutor:
 
     def _copy_block(self, src: int, dst: int) -> None:
         """Move one block's K/V, every layer, for ``BlockTable.ensure_private``
-        (paged_executor.py:265-270): one block-copy launch for all layers."""
-        copy_blocks(self.pool.k, self.pool.v, [(src, dst)])
+        (paged_executor.py:265-270): one block-copy launch for all layers (a second one for
+        an 8-bit pool's scales)."""
+        if isinstance(self.pool, KV8Pool):
+            self.pool.copy_blocks([(src, dst)])
+        else:
+            copy_blocks(self.pool.k, self.pool.v, [(src, dst)])
 
     # ------------------------------------------------------------------ forward
     def _forward(self, input_ids, position_ids, ctx: StepContext):

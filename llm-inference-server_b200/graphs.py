@@ -25,6 +25,7 @@ import torch
 
 from . import _lib
 from .attention import _DTYPE_CODE
+from .kv8 import KV8Pool, attach_step, step_of_metadata
 from .metadata import StepMetadata, attach, sm_count
 
 BucketOverflow = _lib.BucketOverflow
@@ -200,8 +201,10 @@ class ModelDecodeGraph:
         from .executor import StepContext   # the executor module imports this one
 
         buf, plan = self.meta.device_buffer, self.meta.plan
-        ctx = StepContext(meta=self.meta, block_tables=attach(torch.empty(0, dtype=torch.long, device=buf.device),
-                                                              self.meta),
+        tables = attach(torch.empty(0, dtype=torch.long, device=buf.device), self.meta)
+        if isinstance(self.ex.pool, KV8Pool):   # its sums are made inside the graph, from this step's metadata
+            attach_step(tables, step_of_metadata(self.meta, self.ex.group))
+        ctx = StepContext(meta=self.meta, block_tables=tables,
                           context_lens=buf[plan.off_context_lens:plan.off_context_lens + self.B],
                           query_lens=buf[plan.off_query_lens:plan.off_query_lens + self.B], pool=self.ex.pool)
         logits = self.ex._forward(self.ids, self.meta.q_pos().unsqueeze(0), ctx)

@@ -213,6 +213,17 @@ def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_le
     return step
 
 
+def step_of_metadata(meta, group: int) -> DeviceStep:
+    """The step of host-planned metadata (:class:`~.metadata.StepMetadata`, uploaded): its
+    tables and lengths are read where they lie."""
+    plan, buf = meta.plan, meta.device_buffer
+    n = plan.num_seqs
+    return device_step(meta.block_tables(), buf[plan.off_context_lens:plan.off_context_lens + n],
+                       buf[plan.off_query_lens:plan.off_query_lens + n], num_tokens=plan.num_tokens,
+                       max_query_len=max(1, plan.max_query_len), num_blocks=meta.pool_num_blocks,
+                       block_size=plan.block_size, group=group)
+
+
 class DeviceBlockTables:
     """Block tables that live and grow on the GPU: per request slot a row of block ids, the
     tokens cached and the blocks held, and one free list for the pool.

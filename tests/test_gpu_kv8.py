@@ -648,6 +648,56 @@ def test_a_decode_loop_on_the_gpu(pkg):
     assert torch.equal(outs, third)
 
 
+@pytest.fixture(scope="module")
+def small_llama():
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig(hidden_size=512, intermediate_size=512, num_attention_heads=8, num_key_value_heads=2,
+                      head_dim=64, num_hidden_layers=2, vocab_size=1024, max_position_embeddings=2048)
+    return LlamaForCausalLM(cfg).to(DEV, torch.bfloat16).eval()
+
+
+def test_the_executor_over_an_8_bit_pool(pkg, small_llama):
+    """The executor's passes (mixed prefill and decode, then decode) over the 8-bit cache: layer
+    0's K/V depend on the embeddings only, so its cache is the quantised form of what the
+    16-bit pool holds; captured decode passes give the eager ones' tokens and cache."""
+    import importlib
+
+    from _engine import generate
+
+    mod = importlib.import_module(f"{pkg.__name__}.executor")
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, 1024, size=n).tolist() for n in (40, 7, 130, 16)]
+    nb, steps, join = 64, 12, {3: [3]}
+    wide = pkg.KVPool.from_model(small_llama, num_blocks=nb)
+    generate(mod.CudaPagedExecutor(small_llama, None, wide), prompts, 1, nb)
+    pools = [pkg.KV8Pool.from_model(small_llama, num_blocks=nb) for _ in range(2)]
+    generate(mod.CudaPagedExecutor(small_llama, None, pools[0]), prompts, 1, nb)
+    for x, payload, scale in ((wide.k[0], pools[0].k[0], pools[0].k_scale[0]),
+                              (wide.v[0], pools[0].v[0], pools[0].v_scale[0])):
+        codes, byte = ref.quantise(x.double().cpu().numpy())
+        written = byte[..., 0] != 113                      # the smallest scale: a row of zeros, never written
+        assert written.sum() == sum(len(p) for p in prompts)
+        np.testing.assert_array_equal(payload.view(torch.uint8).cpu().numpy(), codes)
+        np.testing.assert_array_equal(scale.transpose(1, 2).cpu().numpy()[written], byte[written])
+    pools = [pkg.KV8Pool.from_model(small_llama, num_blocks=nb) for _ in range(2)]
+    eager = generate(mod.CudaPagedExecutor(small_llama, None, pools[0]), prompts, steps, nb, join_at=join)
+    graph = generate(mod.CudaPagedExecutor(small_llama, None, pools[1], decode_graphs=True), prompts, steps, nb,
+                     join_at=join)
+    assert [len(t) for t in eager] == [len(t) for t in graph] and eager == graph
+    assert "kv8_rows" in pkg._lib.last_launches()
+
+
+def test_the_executor_refuses_a_float32_model(pkg, small_llama):
+    import copy
+    import importlib
+
+    mod = importlib.import_module(f"{pkg.__name__}.executor")
+    with pytest.raises(NotImplementedError, match="float32"):
+        mod.CudaPagedExecutor(copy.deepcopy(small_llama).float(), None, pkg.KV8Pool.from_model(small_llama, 4))
+
+
 def test_pool_block_moves(pkg):
     pool = pkg.KV8Pool(3, 12, 16, 2, 64, DEV)
     g = torch.Generator(device=DEV).manual_seed(2)
