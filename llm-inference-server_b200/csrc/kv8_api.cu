@@ -14,9 +14,9 @@ static int32_t kv8_cuda_fail(cudaError_t e, const char* what) {
   return fail(PA_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
-// A payload pool [NB, BS, Hkv, D] as the 3-D tensor (D, Hkv, NB * BS), box (D, 1, 16), dense
-// or swizzled over the row's width.
-static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, int dim, bool swizzle, CUtensorMap* out) {
+// A payload pool [NB, BS, Hkv, D] as the 3-D tensor (D, Hkv, NB * BS), box (D, 1, 16),
+// swizzled over the row's width.
+static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, int dim, CUtensorMap* out) {
   auto fn = tensor_map_encoder();
   if (!fn) return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the CUDA driver");
   cuuint64_t gdim[3] = {cuuint64_t(dim), cuuint64_t(hkv), cuuint64_t(blocks) * cuuint64_t(bs)};
@@ -25,8 +25,7 @@ static int32_t payload_map(const void* pool, int64_t blocks, int bs, int hkv, in
   cuuint32_t estride[3] = {1u, 1u, 1u};
   CUresult r = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn)(
       out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(pool), gdim, gstride, box, estride,
-      CU_TENSOR_MAP_INTERLEAVE_NONE,
-      !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE : (dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B),
+      CU_TENSOR_MAP_INTERLEAVE_NONE, dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail(PA_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit pool) failed (CUresult %d)", int(r));
   return PA_OK;
@@ -323,8 +322,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   }
   CUtensorMap tk, tv;
   const int row_dim = f.pair ? 2 * head_dim : head_dim;
-  st = payload_map(k_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, true, &tk);
-  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, true, &tv);
+  st = payload_map(k_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, &tk);
+  if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, f.num_kv_heads, row_dim, &tv);
   if (st != PA_OK) return st;
   Kv8AttnParams p{};
   p.q = query;
@@ -367,9 +366,11 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     q.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
     q.part_o = reinterpret_cast<float*>(ws + s.tile_o);
     q.twin_o = reinterpret_cast<float*>(ws + s.twin_o);
-    st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tk);
-    if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, false, &tv);
-    if (st != PA_OK) return st;
+    if (f.pair) {  // the rows kernel's maps were of pairs
+      st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, &tk);
+      if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, &tv);
+      if (st != PA_OK) return st;
+    }
     e = launch_kv8_tiles(dtype, head_dim, tk, tv, q, err, stream);
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
     launched |= PA_LAUNCH_KV8_TILES;

@@ -126,14 +126,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
   return r;
 }
 
-// Byte offset of 16-byte chunk c of row r in a TMA tile whose rows are D bytes, with the
-// swizzle as wide as the row (128 or 64 bytes).
-template <int D>
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  if constexpr (D == 128) return uint32_t(r * 128 + ((c ^ (r & 7)) << 4));
-  return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
-}
-
 template <typename T, int D, int RG, bool PAIR>
 __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
     kv8_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,

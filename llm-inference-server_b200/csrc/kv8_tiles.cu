@@ -25,8 +25,10 @@
 //   warps 16, 17    S = Q K^T issue of either half (16 also allocates TMEM)
 //   warps 18, 19    O += P V issue of either half
 //   warps 20, 21    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
-//                   staging rings of 4 tiles (K's with V's scale bytes beside, for the rows
-//                   that stand for NaN: the softmax learns of them with the scores)
+//                   staging rings of 4 tiles, swizzled (a dense box of 16 rows of 128 bytes
+//                   lands at a quarter of the rate: 9 bytes a clock per SM; K's with V's scale
+//                   bytes beside, for the rows that stand for NaN: the softmax learns of them
+//                   with the scores)
 //   warp 22         finds the slice's pieces (a 2-slot ring)
 // TMEM columns of a half: two score buffers of 64, O [128, 128 + D).  A row's weights go over
 // the first 32 columns of the scores they came from (each thread has read its own by then),
@@ -87,8 +89,8 @@ struct TilePiece {
 // holds it back: a half passes the K and V stages of the other's tiles on itself.
 struct TileBars {
   uint64_t st_full[2][kTileRing], st_empty[2][kTileRing];  // staging of K, V: landed / read
-  uint64_t k_full[kTileKStages], k_free[2][kTileKStages];  // fp16 tiles, by g; freed by each half
-  uint64_t v_full[kTileVStages], v_free[2][kTileVStages];
+  uint64_t k_full[kTileKStages], k_free[kTileKStages];     // fp16 tiles, by g; freed by both halves
+  uint64_t v_full[kTileVStages], v_free[kTileVStages];
   uint64_t s_full[2][2], s_free[2][2], p_full[2][2];       // score buffers of a half, by n
   uint64_t q_full[2];
   uint64_t x_full, x_free;                                 // the twin's result
@@ -146,8 +148,9 @@ struct WidenPart {
     scale = lane < min(16, live) ? scales[lane] : 0u;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      x[i] = *reinterpret_cast<const uint4*>(staged + 16 * (32 * i + lane));
-      if (i * RPI + lane / LPR >= live) x[i] = make_uint4(0, 0, 0, 0);
+      const int r = i * RPI + lane / LPR;
+      x[i] = *reinterpret_cast<const uint4*>(staged + tile_at<D>(r, lane % LPR));
+      if (r >= live) x[i] = make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -211,12 +214,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       }
     for (int s = 0; s < kTileKStages; ++s) {
       mbar_init(&bars->k_full[s], 4);
-      for (int h = 0; h < 2; ++h) mbar_init(&bars->k_free[h][s], 1);
+      mbar_init(&bars->k_free[s], 2);
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars->v_full[s], 4);
+      mbar_init(&bars->v_free[s], 2);
       for (int h = 0; h < 2; ++h) {
-        mbar_init(&bars->v_free[h][s], 1);
         mbar_init(&bars->s_full[h][s], 1);
         mbar_init(&bars->s_free[h][s], 1);
         mbar_init(&bars->p_full[h][s], 128);
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               break;
             }
             if (!works(twin, h, d, j)) {
-              mbar_arrive(&bars->k_free[h][s]);
+              mbar_arrive(&bars->k_free[s]);
               continue;
             }
             if (n >= 2 && !mbar_wait(&bars->s_free[h][n & 1], ((n >> 1) - 1) & 1)) {
@@ -389,7 +392,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               umma_f16(tS + (n & 1) * kTileKeys, ad, bd, idS, kk > 0 ? 1u : 0u);
             }
             umma_commit(&bars->s_full[h][n & 1]);
-            umma_commit(&bars->k_free[h][s]);
+            umma_commit(&bars->k_free[s]);
             ++n;
           }
         }
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               break;
             }
             if (!works(twin, h, d, j)) {
-              mbar_arrive(&bars->v_free[h][s]);
+              mbar_arrive(&bars->v_free[s]);
               continue;
             }
             if (!mbar_wait(&bars->p_full[h][b], (n >> 1) & 1)) {
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
               umma_f16_ts(tO, tS + b * kTileKeys + 8 * kk, bd, idO, (!first || kk > 0) ? 1u : 0u);
             }
             umma_commit(&bars->s_free[h][b]);
-            umma_commit(&bars->v_free[h][s]);
+            umma_commit(&bars->v_free[s]);
             first = false;
             ++n;
           }
@@ -442,6 +445,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int v = warp >= 12 ? 1 : 0, row0 = 16 * (warp & 3);
     const int stages = v ? kTileVStages : kTileKStages;
     uint64_t* full = v ? bars->v_full : bars->k_full;
+    uint64_t* freed = v ? bars->v_free : bars->k_free;
     const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES + row0 * D;
     const uint8_t* scale_ring = smem + C::OFF_SCALE + (v ? 2 * kTileRing * kTileKeys : 0) + row0;
     const int scale_step = v ? kTileKeys : 2 * kTileKeys;
@@ -455,15 +459,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       for (int j = d.j0; j < d.j1; ++j, ++n) {
         const int st = n % kTileRing;
         ok = mbar_wait(&bars->st_full[v][st], (n / kTileRing) & 1);
-        // Both halves are done with the tile that was in this stage.
-        if (ok && round > 0)
-          for (int h = 0; h < 2 && ok; ++h)
-            ok = mbar_wait(v ? &bars->v_free[h][s] : &bars->k_free[h][s], (round - 1) & 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         const int live = d.ctx - j * kTileKeys - row0;
         const uint8_t* sc = scale_ring + st * scale_step;
         part.read(ring + st * C::ST_BYTES, sc, lane, live);
+        if (round > 0) ok = ok && mbar_wait(&freed[s], (round - 1) & 1);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
         if (!v) {
           const uint32_t nans = __ballot_sync(0xffffffffu, lane < min(16, live) && sc[kTileKeys + lane] == 255);
           if (lane == 0) nan_rows[4 * (n % kTileNanRing) + (warp & 3)] = uint16_t(nans);

@@ -1,4 +1,5 @@
-// e4m3 -> fp16 and queries -> fp16, shared by the KV8 attention kernels.
+// Payload tiles in shared memory, e4m3 -> fp16 and queries -> fp16: shared by the KV8 attention
+// kernels.
 #pragma once
 
 #include <stdint.h>
@@ -17,6 +18,14 @@ __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
   uint32_t r;
   asm("{\n .reg .b16 l, h;\n mov.b32 {l, h}, %1;\n cvt.rn.f16x2.e4m3x2 %0, h;\n}\n" : "=r"(r) : "r"(w));
   return r;
+}
+
+// Byte offset of 16-byte chunk c of row r in a TMA tile whose rows are D bytes, with the
+// swizzle as wide as the row (128 or 64 bytes).
+template <int D>
+__device__ __forceinline__ uint32_t tile_at(int r, int c) {
+  if constexpr (D == 128) return uint32_t(r * 128 + ((c ^ (r & 7)) << 4));
+  return uint32_t(r * 64 + ((c ^ ((r >> 1) & 3)) << 4));
 }
 
 // The power of two that brings a bf16 row with largest magnitude `big` to [2^14, 2^15), where
