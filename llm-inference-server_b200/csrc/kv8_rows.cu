@@ -14,9 +14,13 @@
 // HBM-bound: each K/V byte is read once per tile of rows.  The sequences' keys laid end to
 // end are cut into equal slices (kv8_line.cuh), a CTA per slice and KV head with the KV head
 // fastest, so that the CTAs of one slice read a pool block's heads side by side.  A CTA has
-// four consumer warps, which take stages of 32 keys in turn, and a producer warp, which
-// walks the slice's pieces, reads the block table and keeps each consumer's ring full: the
-// rings run across pieces, so a new sequence costs no drain.  Per 16 keys: K and V tile by
+// consumer warps, which take stages of 32 keys in turn, and a producer warp, which walks the
+// slice's pieces, reads the block table and keeps each consumer's ring full: the rings run
+// across pieces, so a new sequence costs no drain.  With one group of 8 rows there are three
+// CTAs of four consumers on an SM (128 registers a thread), and HBM bounds them; with more
+// rows the steps' dependent instructions do, a thread needs 168 registers, and one CTA of
+// eleven consumers is what fits (two CTAs of four: 77 and 99 us for 24 chunks of 4 and 5
+// tokens over 6,000 keys, where the data can be there in 63).  Per 16 keys: K and V tile by
 // TMA (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round
 // of 32 blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the
 // tiles: 177 against 152 us for 64 sequences of about 4,096 keys, 8 heads of 128).
@@ -44,14 +48,14 @@
 
 namespace pa {
 
-constexpr int kRowsWarps = 4;                       // consumers
-constexpr int kRowsThreads = 32 * (kRowsWarps + 1);
 constexpr int kRowsStage = 32;                      // keys a stage: two 16-key blocks
 constexpr int kRowsKeys = 16;                       // keys a block; cuts fall on these
 constexpr int kRowsDescs = 2;
-// Fewest keys a slice gets: below this a CTA's set-up and its partial cost more than the
-// keys it takes over.
-constexpr int kRowsMinKeys = 128;
+__host__ __device__ constexpr int rows_warps(int row_groups) { return row_groups == 1 ? 4 : 11; }  // consumers
+__host__ __device__ constexpr int rows_ctas(int row_groups) { return row_groups == 1 ? 3 : 1; }    // on an SM
+// Fewest keys a slice gets, a stage for each consumer: below this a CTA's set-up and its
+// partial cost more than the keys it takes over.
+__host__ __device__ constexpr int rows_min_keys(int row_groups) { return kRowsStage * rows_warps(row_groups); }
 constexpr float kWeightShift = 256.f;               // 2^8, see above
 
 // D: dims of the payload rows (two heads' with PAIR), RG: groups of 8 query rows.
@@ -60,10 +64,7 @@ struct RowsCfg {
   static_assert(!PAIR || D == 128, "pairs of heads of 64");
   static constexpr int DO = PAIR ? 64 : D;          // dims of a query and an output row
   static constexpr int SUBS = PAIR ? 2 : 1;         // KV heads of a payload row
-  // Blocks a softmax step takes.  With three groups of rows both blocks' scores do not quite
-  // fit the registers, but a block at a time is slower all the same (24 chunks of 5 tokens over
-  // 6,000 keys: 176 against 118 us): the steps are chains of dependent instructions.
-  static constexpr int NB = 2;
+  static constexpr int W = rows_warps(RG), CTAS = rows_ctas(RG), THREADS = 32 * (W + 1);
   static constexpr int SCALES = 2 * SUBS * kRowsStage;  // bytes a stage: K then V
   static constexpr int STAGES = D == 128 ? 2 : 4;   // 16 KB in flight per warp
   static constexpr int TILE = kRowsKeys * D;        // K or V of a block
@@ -71,19 +72,19 @@ struct RowsCfg {
   static constexpr int STAGE = 2 * BLOCK;
   static constexpr int CH = D / 16;                 // 16-byte chunks of a row = k steps of S
   static constexpr int NO = CH * RG * 4;            // accumulator registers
-  static constexpr int OFF_SCALE = kRowsWarps * STAGES * STAGE;
-  static constexpr int OFF_Q = OFF_SCALE + kRowsWarps * STAGES * SCALES;
+  static constexpr int MERGES = RG == 1 ? 2 : 3;    // accumulators on their way between warps
+  static constexpr int OFF_SCALE = W * STAGES * STAGE;
+  static constexpr int OFF_Q = OFF_SCALE + W * STAGES * SCALES;
   static constexpr int OFF_MERGE = OFF_Q;           // the queries are no longer read by then
-  static constexpr int OFF_ML = OFF_MERGE + 2 * NO * 32 * 4;
-  static_assert(2 * NO * 32 * 4 >= CH * RG * 32 * 8, "merge area holds the queries");
-  static constexpr int OFF_FACTOR = OFF_ML + kRowsWarps * RG * 8 * 8;
+  static constexpr int OFF_ML = OFF_MERGE + MERGES * NO * 32 * 4;
+  static_assert(MERGES * NO * 32 * 4 >= CH * RG * 32 * 8, "merge area holds the queries");
+  static constexpr int OFF_FACTOR = OFF_ML + W * RG * 8 * 8;
   static constexpr int OFF_LIMIT = OFF_FACTOR + RG * 8 * 4;
   static constexpr int OFF_DESC = OFF_LIMIT + RG * 8 * 4;
   static constexpr int OFF_BAR = OFF_DESC + kRowsDescs * 32;
-  static constexpr int SMEM = OFF_BAR + (2 * kRowsWarps * STAGES + 2 * kRowsDescs) * 8;
+  static constexpr int SMEM = OFF_BAR + (2 * W * STAGES + 2 * kRowsDescs) * 8;
   static constexpr bool Q_IN_REGS = RG <= 2;
-  // CTAs on an SM: 228 KB of shared memory, 1 KB of it taken per CTA.
-  static constexpr int CTAS = RG == 1 ? 3 : 2;
+  // 228 KB of shared memory on an SM, 1 KB of it taken per CTA.
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "shared memory for the CTAs an SM is to hold");
 };
 
@@ -94,13 +95,26 @@ struct RowsPiece {      // part of a tile that a CTA works on
   int32_t ctx;          // of the sequence
   int32_t kb0, kb1;     // blocks of 16 keys
   int32_t part;         // -1: the whole tile, else the CTA's partial slot
-  int32_t pad;
+  int32_t pair0;        // stages the CTA had before it
 };
 
 __device__ __forceinline__ void rows_arrive(uint64_t* bar) {
   asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
-__device__ __forceinline__ void rows_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * kRowsWarps) : "memory"); }
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+template <int W>
+__device__ __forceinline__ void rows_sync() {
+  asm volatile("bar.sync 1, %0;" ::"n"(32 * W) : "memory");
+}
 
 __device__ __forceinline__ void ldm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -127,11 +141,11 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
 }
 
 template <typename T, int D, int RG, bool PAIR>
-__global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
+__global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, PAIR>::CTAS)
     kv8_rows_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                     const Kv8AttnParams p, int* err) {
   using C = RowsCfg<D, RG, PAIR>;
-  constexpr int CH = C::CH, DO = C::DO;
+  constexpr int CH = C::CH, DO = C::DO, W = C::W;
   extern __shared__ __align__(1024) uint8_t smem[];
   uint2* sq = reinterpret_cast<uint2*>(smem + C::OFF_Q);
   float* merge = reinterpret_cast<float*>(smem + C::OFF_MERGE);
@@ -140,20 +154,20 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
   int* limits = reinterpret_cast<int*>(smem + C::OFF_LIMIT);
   RowsPiece* desc = reinterpret_cast<RowsPiece*>(smem + C::OFF_DESC);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
-  uint64_t* empty = full + kRowsWarps * C::STAGES;
-  uint64_t* d_full = empty + kRowsWarps * C::STAGES;
+  uint64_t* empty = full + W * C::STAGES;
+  uint64_t* d_full = empty + W * C::STAGES;
   uint64_t* d_empty = d_full + kRowsDescs;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kRowsWarps * C::STAGES; ++i) {
+    for (int i = 0; i < W * C::STAGES; ++i) {
       mbar_init(&full[i], 4);  // per block: its tiles are on their way, its scales are there
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < kRowsDescs; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], kRowsWarps);
+      mbar_init(&d_empty[i], W);
     }
     fence_mbar_init();
     prefetch_tmap(&tk);
@@ -164,16 +178,14 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
   pdl_release();
   LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
   const int64_t total = p.work[p.num_seqs];
-  const int slices = line_slices(total, p.slices, kRowsMinKeys);
+  const int slices = line_slices(total, p.slices, rows_min_keys(RG));
   if (total == 0 || slice >= slices) return;
 
-  if (warp == kRowsWarps) {
+  if (warp == W) {
     // ------------------------------------------------------------ producer
     const int64_t x1 = line_cut(total, slices, slice + 1);
     int64_t x = line_cut(total, slices, slice);
-    int issued[kRowsWarps];
-#pragma unroll
-    for (int w = 0; w < kRowsWarps; ++w) issued[w] = 0;
+    int pairs = 0;  // stages issued so far; the i-th is consumer (i % W)'s
     int pieces = 0;
     bool ok = true;
     struct BlockRef {
@@ -213,7 +225,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
       if (lane == 0) {
         RowsPiece d;
         d.row0 = -1;
-        d.pad = 0;
+        d.pair0 = pairs;
         if (more) {
           const int t0 = t.index * p.tile_tokens;
           d.row0 = t.first + t0;
@@ -237,37 +249,39 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
       for (int kb = kb0; kb < kb1 && ok; kb += 32) {
         if (kb + 32 < kb1) nxt = look_up(row, kb + 32 + lane, kb1);
         const int n = min(32, kb1 - kb);
-        for (int j = 0; j < n && ok; j += 2 * kRowsWarps) {
+        // As many stages at a time as have places of their own in the rings, each lane issuing
+        // its block as soon as its place is free: one stage after the other took about 770
+        // clocks each and held the whole kernel up.
+        constexpr int ROUND = W * C::STAGES < 16 ? W * C::STAGES : 16;
+        for (int b0 = 0; b0 < n && ok; b0 += 2 * ROUND) {
+          const int i = pairs + (lane - b0) / 2, turn = i / W, st = (i % W) * C::STAGES + turn % C::STAGES;
+          bool waiting = lane >= b0 && lane < b0 + 2 * ROUND && lane < ((n + 1) & ~1);
+          for (uint32_t tries = 0; tries < kWaitLimit; ++tries) {
+            if (waiting && (turn < C::STAGES || mbar_test(&empty[st], ((turn / C::STAGES) - 1) & 1))) {
+              waiting = false;
+              uint64_t* bar = &full[st];
+              const int half = lane & 1;
+              if (lane < n) {
+                uint8_t* stage = smem + st * C::STAGE + half * C::BLOCK;
+                mbar_arrive_expect_tx(bar, C::BLOCK);
+                tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
+                tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
+                uint8_t* sc = smem + C::OFF_SCALE + st * C::SCALES + 16 * half;
 #pragma unroll
-          for (int w = 0; w < kRowsWarps; ++w) {
-            const int b = j + 2 * w;
-            if (b < n) {
-              const int st = issued[w] % C::STAGES;
-              if (issued[w] >= C::STAGES)
-                ok = mbar_wait(&empty[w * C::STAGES + st], ((issued[w] / C::STAGES) - 1) & 1) && ok;
-              const int half = lane - b;
-              if (ok && (half == 0 || half == 1)) {
-                uint64_t* bar = &full[w * C::STAGES + st];
-                if (lane < n) {
-                  uint8_t* stage = smem + (w * C::STAGES + st) * C::STAGE + half * C::BLOCK;
-                  mbar_arrive_expect_tx(bar, C::BLOCK);
-                  tma_load_3d(stage, &tk, 0, kvh, cur.slot, bar);
-                  tma_load_3d(stage + C::TILE, &tv, 0, kvh, cur.slot, bar);
-                  uint8_t* sc = smem + C::OFF_SCALE + (w * C::STAGES + st) * C::SCALES + 16 * half;
-#pragma unroll
-                  for (int u = 0; u < C::SUBS; ++u) {
-                    *reinterpret_cast<uint4*>(sc + u * kRowsStage) = cur.ks[u];
-                    *reinterpret_cast<uint4*>(sc + (C::SUBS + u) * kRowsStage) = cur.vs[u];
-                  }
-                  rows_arrive(bar);
-                } else {
-                  rows_arrive(bar);  // the piece's last stage holds one block
-                  rows_arrive(bar);
+                for (int u = 0; u < C::SUBS; ++u) {
+                  *reinterpret_cast<uint4*>(sc + u * kRowsStage) = cur.ks[u];
+                  *reinterpret_cast<uint4*>(sc + (C::SUBS + u) * kRowsStage) = cur.vs[u];
                 }
+                rows_arrive(bar);
+              } else {
+                rows_arrive(bar);  // the piece's last stage holds one block
+                rows_arrive(bar);
               }
-              if (ok) ++issued[w];
             }
+            if (!__any_sync(0xffffffffu, waiting)) break;
           }
+          ok = !__any_sync(0xffffffffu, waiting);
+          pairs += min(ROUND, (n - b0 + 1) / 2);
         }
         ok = __all_sync(0xffffffffu, ok);
         cur = nxt;
@@ -276,10 +290,8 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
     if (!ok) {
       if (lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
       // Leave with no copy into this CTA's shared memory in flight.
-#pragma unroll
-      for (int w = 0; w < kRowsWarps; ++w)
-        for (int i = max(0, issued[w] - C::STAGES); i < issued[w]; ++i)
-          mbar_wait(&full[w * C::STAGES + i % C::STAGES], (i / C::STAGES) & 1);
+      for (int i = max(0, pairs - W * C::STAGES); i < pairs; ++i)
+        mbar_wait(&full[(i % W) * C::STAGES + i / W % C::STAGES], (i / W / C::STAGES) & 1);
     }
     return;
   }
@@ -287,7 +299,6 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
   // -------------------------------------------------------------- consumers
   const int g = lane >> 2, tig = lane & 3;
   const int mi = lane >> 3, ri = lane & 7;
-  int taken = 0;
   bool ok = true;
   for (int piece = 0;; ++piece) {
     const int slot = piece % kRowsDescs;
@@ -299,7 +310,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
       asm volatile("{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.and.pred q, 2, %2, p;\n"
                    " selp.s32 %0, 1, 0, q;\n}\n"
                    : "=r"(all)
-                   : "r"(mine), "n"(32 * kRowsWarps)
+                   : "r"(mine), "n"(32 * W)
                    : "memory");
     }
     if (!all) break;
@@ -310,9 +321,8 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
 
     // Queries as B fragments in shared memory: row r = (token r / group, head r % group),
     // brought into fp16 by a power of two; a warp takes a row.
-#pragma unroll
-    for (int i = 0; i < 2 * RG; ++i) {
-      const int r = warp + kRowsWarps * i, tok = r / p.group, head = r - tok * p.group;
+    for (int r = warp; r < 8 * RG; r += W) {
+      const int tok = r / p.group, head = r - tok * p.group;
       constexpr int E = DO / 32;
       float x[E];
 #pragma unroll
@@ -346,7 +356,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
         limits[r] = tok < d.tokens ? min(d.pos0 + tok, d.kb1 * kRowsKeys - 1) : -1;
       }
     }
-    rows_sync();
+    rows_sync<W>();
     uint2 qr[C::Q_IN_REGS ? CH : 1][RG];
     if constexpr (C::Q_IN_REGS) {
 #pragma unroll
@@ -382,21 +392,23 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
         l[rg][e] = 0.f;
       }
 
-    for (int kb = d.kb0 + 2 * warp; kb < d.kb1; kb += 2 * kRowsWarps, ++taken) {
-      const int st = taken % C::STAGES;
-      if (ok) ok = mbar_wait(&full[warp * C::STAGES + st], (taken / C::STAGES) & 1);
-      const uint32_t stage = smem_u32(smem + (warp * C::STAGES + st) * C::STAGE);
-      const uint8_t* sc = smem + C::OFF_SCALE + (warp * C::STAGES + st) * C::SCALES;
+    const int skip = (warp + W - d.pair0 % W) % W;  // stages of the piece before this warp's first
+    int turn = (d.pair0 + skip) / W;
+    for (int kb = d.kb0 + 2 * skip; kb < d.kb1; kb += 2 * W, ++turn) {
+      const int st = warp * C::STAGES + turn % C::STAGES;
+      if (ok) ok = mbar_wait(&full[st], (turn / C::STAGES) & 1);
+      const uint32_t stage = smem_u32(smem + st * C::STAGE);
+      const uint8_t* sc = smem + C::OFF_SCALE + st * C::SCALES;
       const int key0 = kb * kRowsKeys;
       // Spare rows of the tile compute, unmasked, and are not stored.
       const bool masked = key0 + kRowsStage - 1 > d.pos0 || kb + 2 > d.kb1;
       const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;  // keys of the stage that are there
-#pragma unroll
-      for (int b0 = 0; b0 < 2; b0 += C::NB) {
+      {
+        constexpr int b0 = 0;
         // ---- S^T over the payloads: element 2 h + e is key 16 b + 8 h + g, row 8 rg + 2 tig + e
-        float s[C::NB][RG][4];
+        float s[2][RG][4];
 #pragma unroll
-        for (int n = 0; n < C::NB; ++n) {
+        for (int n = 0; n < 2; ++n) {
 #pragma unroll
           for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
@@ -423,10 +435,10 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
         }
 
         // ---- online softmax
-        float ks[C::NB][2], vs[C::NB][2];  // scales of keys 16 b + 8 h + g
+        float ks[2][2], vs[2][2];  // scales of keys 16 b + 8 h + g
         if constexpr (!PAIR) {
 #pragma unroll
-          for (int n = 0; n < C::NB; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int key = 16 * (b0 + n) + 8 * h + g;
@@ -434,7 +446,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
               vs[n][h] = __uint_as_float(uint32_t(sc[kRowsStage + key]) << 23) * kWeightShift;
             }
         }
-        uint32_t wt[C::NB][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
+        uint32_t wt[2][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
         bool grown = false;
         float alpha[RG][2];
 #pragma unroll
@@ -444,7 +456,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
           if (masked) limit = my_limits[4 * rg];
           float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int n = 0; n < C::NB; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -468,7 +480,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
             m[rg][e] = mn;
           }
 #pragma unroll
-          for (int n = 0; n < C::NB; ++n)
+          for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const int key = 16 * (b0 + n) + 8 * h + g;
@@ -498,7 +510,7 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
 
         // ---- O^T += V^T W^T; bytes behind the context (or the stage's only block) read as zero
 #pragma unroll
-        for (int n = 0; n < C::NB; ++n) {
+        for (int n = 0; n < 2; ++n) {
           uint32_t pick[2] = {0x3120u, 0x3120u};  // (t0 d0, t1 d0, t0 d1, t1 d1) of (t0 d0, t0 d1, t1 d0, t1 d1)
           if (end < kRowsStage) {
 #pragma unroll
@@ -522,10 +534,10 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
         }
       }
       __syncwarp();
-      if (lane == 0) rows_arrive(&empty[warp * C::STAGES + st]);
+      if (lane == 0) rows_arrive(&empty[st]);
     }
 
-    // ---- join the four warps: common maximum, then a tree over the accumulators
+    // ---- join the warps: common maximum, then a tree over the accumulators
     float big[RG][2];
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
@@ -535,22 +547,19 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
         for (int x = 4; x < 32; x <<= 1) l[rg][e] += __shfl_xor_sync(0xffffffffu, l[rg][e], x);
         if (g == 0) ml[warp * 8 * RG + 8 * rg + 2 * tig + e] = make_float2(m[rg][e], l[rg][e]);
       }
-    rows_sync();
+    rows_sync<W>();
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float2 v[kRowsWarps];
+        const float2* v = ml + 8 * rg + 2 * tig + e;
         big[rg][e] = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) {
-          v[w] = ml[w * 8 * RG + 8 * rg + 2 * tig + e];
-          big[rg][e] = fmaxf(big[rg][e], v[w].x);
-        }
+        for (int w = 0; w < W; ++w) big[rg][e] = fmaxf(big[rg][e], v[w * 8 * RG].x);
         const float ref = big[rg][e] == -INFINITY ? 0.f : big[rg][e];
         float sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < kRowsWarps; ++w) sum += v[w].y * ex2(v[w].x - ref);
+        for (int w = 0; w < W; ++w) sum += v[w * 8 * RG].y * ex2(v[w * 8 * RG].x - ref);
         const float f = ex2(m[rg][e] - ref);
         l[rg][e] = sum;
 #pragma unroll
@@ -571,13 +580,16 @@ __global__ void __launch_bounds__(kRowsThreads, RowsCfg<D, RG, PAIR>::CTAS)
 #pragma unroll
         for (int e = 0; e < 4 * RG; ++e) o[c][e / 4][e % 4] += merge[(half * C::NO + c * 4 * RG + e) * 32 + lane];
     };
-    if (warp >= 2) put(warp - 2);
-    rows_sync();
-    if (warp < 2) add(warp);
-    if (warp == 1) put(1);
-    rows_sync();
+#pragma unroll
+    for (int left = W; left > 1;) {  // the last `moved` of the warps left hand theirs to the first
+      const int moved = left / 2 < C::MERGES ? left / 2 : C::MERGES;
+      if (warp >= left - moved && warp < left) put(warp - (left - moved));
+      rows_sync<W>();
+      if (warp < moved) add(warp);
+      left -= moved;
+      if (left > 1) rows_sync<W>();
+    }
     if (warp != 0) continue;
-    add(1);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
@@ -759,7 +771,7 @@ static cudaError_t rows_one(const CUtensorMap& tk, const CUtensorMap& tv, const 
     if (e != cudaSuccess) return e;
     configured[dev] = true;
   }
-  return launch_pdl(kern, dim3(p.slices * p.num_kv_heads), dim3(kRowsThreads), C::SMEM, stream, tk, tv, p, err);
+  return launch_pdl(kern, dim3(p.slices * p.num_kv_heads), dim3(C::THREADS), C::SMEM, stream, tk, tv, p, err);
 }
 
 template <typename T, int D, bool PAIR>
@@ -782,8 +794,7 @@ static cudaError_t rows_by_shape(int head_dim, bool pair, int row_groups, const 
 }
 
 int kv8_rows_slices(int row_groups, int num_kv_heads, int sms) {
-  // Resident CTAs per SM: three with one group of rows, else two (registers).
-  const int n = sms * (row_groups == 1 ? 3 : 2) / num_kv_heads;
+  const int n = sms * rows_ctas(row_groups) / num_kv_heads;
   return n < 1 ? 1 : n;
 }
 
@@ -816,7 +827,7 @@ cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, 
 
 cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
                                     cudaStream_t stream) {
-  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, kRowsMinKeys, p, stream);
+  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, rows_min_keys(row_groups), p, stream);
 }
 
 }  // namespace pa

@@ -25,10 +25,8 @@
 //   warps 16, 17    S = Q K^T issue of either half (16 also allocates TMEM)
 //   warps 18, 19    O += P V issue of either half
 //   warps 20, 21    K / V producers: block table, TMA of e4m3 boxes and the scale bytes into
-//                   staging rings of 4 tiles, swizzled (a dense box of 16 rows of 128 bytes
-//                   lands at a quarter of the rate: 9 bytes a clock per SM; K's with V's scale
-//                   bytes beside, for the rows that stand for NaN: the softmax learns of them
-//                   with the scores)
+//                   staging rings of 4 swizzled tiles (K's with V's scale bytes beside, for
+//                   the rows that stand for NaN: the softmax learns of them with the scores)
 //   warp 22         finds the slice's pieces (a 2-slot ring)
 // TMEM columns of a half: two score buffers of 64, O [128, 128 + D).  A row's weights go over
 // the first 32 columns of the scores they came from (each thread has read its own by then),
