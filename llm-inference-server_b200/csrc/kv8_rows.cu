@@ -17,10 +17,8 @@
 // consumer warps, which take stages of 32 keys in turn, and a producer warp, which walks the
 // slice's pieces, reads the block table and keeps each consumer's ring full: the rings run
 // across pieces, so a new sequence costs no drain.  With one group of 8 rows there are three
-// CTAs of four consumers on an SM (128 registers a thread), and HBM bounds them; with more
-// rows the steps' dependent instructions do, a thread needs 168 registers, and one CTA of
-// eleven consumers is what fits (two CTAs of four: 77 and 99 us for 24 chunks of 4 and 5
-// tokens over 6,000 keys, where the data can be there in 63).  Per 16 keys: K and V tile by
+// CTAs on an SM, and HBM bounds them; with more rows a thread needs 168 registers and there
+// are two (five consumers a CTA, or one CTA of eleven, are no faster).  Per 16 keys: K and V tile by
 // TMA (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round
 // of 32 blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the
 // tiles: 177 against 152 us for 64 sequences of about 4,096 keys, 8 heads of 128).
@@ -51,8 +49,8 @@ namespace pa {
 constexpr int kRowsStage = 32;                      // keys a stage: two 16-key blocks
 constexpr int kRowsKeys = 16;                       // keys a block; cuts fall on these
 constexpr int kRowsDescs = 2;
-__host__ __device__ constexpr int rows_warps(int row_groups) { return row_groups == 1 ? 4 : 11; }  // consumers
-__host__ __device__ constexpr int rows_ctas(int row_groups) { return row_groups == 1 ? 3 : 1; }    // on an SM
+__host__ __device__ constexpr int rows_warps(int) { return 4; }                    // consumers
+__host__ __device__ constexpr int rows_ctas(int row_groups) { return row_groups == 1 ? 3 : 2; }  // on an SM
 // Fewest keys a slice gets, a stage for each consumer: below this a CTA's set-up and its
 // partial cost more than the keys it takes over.
 __host__ __device__ constexpr int rows_min_keys(int row_groups) { return kRowsStage * rows_warps(row_groups); }
@@ -72,7 +70,7 @@ struct RowsCfg {
   static constexpr int STAGE = 2 * BLOCK;
   static constexpr int CH = D / 16;                 // 16-byte chunks of a row = k steps of S
   static constexpr int NO = CH * RG * 4;            // accumulator registers
-  static constexpr int MERGES = RG == 1 ? 2 : 3;    // accumulators on their way between warps
+  static constexpr int MERGES = 2;    // accumulators on their way between warps
   static constexpr int OFF_SCALE = W * STAGES * STAGE;
   static constexpr int OFF_Q = OFF_SCALE + W * STAGES * SCALES;
   static constexpr int OFF_MERGE = OFF_Q;           // the queries are no longer read by then
