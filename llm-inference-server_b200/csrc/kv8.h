@@ -40,7 +40,10 @@ struct Kv8AttnParams {
   const int32_t* tables;
   int64_t table_stride;
   const int32_t *ctx_lens, *cu_q;
-  const int64_t* work;  // this class's running sums [num_seqs + 1]
+  const int64_t* work;  // this class's running sums [num_seqs + 1]; NULL: made from the lengths below
+  const int32_t* query_lens;
+  int32_t num_tokens, max_query_len, max_context, small_max;
+  bool few;  // the class: sequences of at most small_max new tokens, or those of more
   int32_t num_seqs, num_heads, num_kv_heads, group, block_shift, tile_tokens, slices;
   int32_t pool_blocks;
   float qscale;  // softmax scale * log2(e)
@@ -68,14 +71,14 @@ int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
 cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
                             const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream);
 constexpr int kKv8RowGroups = 3;  // most groups of 8 rows
-cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p, int* err,
                                     cudaStream_t stream);
 int kv8_tiles_slices(int num_kv_heads, int sms);
 cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
                              const Kv8AttnParams& p, int* err, cudaStream_t stream);
-cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream);
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream);
 constexpr int kKv8TileRows = 256;  // (token, head) rows of its tiles
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
-                               cudaStream_t stream);
+                               int* err, cudaStream_t stream);
 
 }  // namespace pa

@@ -311,14 +311,16 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     b.max_query_len = max_query_len;
     b.pool_blocks = pool_num_blocks;
     b.tiling = t;
-    b.cu_query = reinterpret_cast<int32_t*>(ws + s.cu);
-    b.work = reinterpret_cast<int64_t*>(ws + s.work);
     st = check_step_sizes(b, table_stride);
     if (st != PA_OK) return st;
-    const cudaError_t eb = launch_kv8_step(b, err, stream);
-    if (eb != cudaSuccess) return kv8_cuda_fail(eb, "8-bit attention's step launch");
-    cu_query_lens = b.cu_query;
-    work = b.work;
+    if (num_seqs > 32) {  // up to 32 the kernels sum up for themselves
+      b.cu_query = reinterpret_cast<int32_t*>(ws + s.cu);
+      b.work = reinterpret_cast<int64_t*>(ws + s.work);
+      const cudaError_t eb = launch_kv8_step(b, err, stream);
+      if (eb != cudaSuccess) return kv8_cuda_fail(eb, "8-bit attention's step launch");
+      cu_query_lens = b.cu_query;
+      work = b.work;
+    }
   }
   CUtensorMap tk, tv;
   const int row_dim = f.pair ? 2 * head_dim : head_dim;
@@ -341,6 +343,12 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.ctx_lens = context_lens;
   p.cu_q = cu_query_lens;
   p.work = work;
+  p.query_lens = query_lens;
+  p.num_tokens = num_tokens;
+  p.max_query_len = max_query_len;
+  p.max_context = int32_t(std::min<int64_t>(int64_t(table_width) * block_size, 1 << 30));
+  p.small_max = t.small_max;
+  p.few = true;
   p.num_seqs = num_seqs;
   p.num_heads = num_heads;
   p.num_kv_heads = f.num_kv_heads;
@@ -358,7 +366,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   Kv8AttnParams q = p;  // of the tiles kernel
   const bool tiles = max_query_len > t.small_max;
   if (tiles) {
-    q.work = work + num_seqs + 1;
+    q.work = work ? work + num_seqs + 1 : nullptr;
+    q.few = false;
     q.num_kv_heads = num_kv_heads;
     q.group = group;
     q.tile_tokens = t.large_tokens;
@@ -375,8 +384,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
     launched |= PA_LAUNCH_KV8_TILES;
   }
-  e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, stream);
-  if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, stream);
+  e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, err, stream);
+  if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention join launch");
   if (p.slices > 1 || (tiles && q.slices > 1)) launched |= PA_LAUNCH_KV8_COMBINE;
   note_launches(launched);

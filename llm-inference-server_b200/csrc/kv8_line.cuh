@@ -10,6 +10,9 @@
 
 #include <stdint.h>
 
+#include "kv8.h"
+#include "pa_common.cuh"
+
 namespace pa {
 
 // Keys of tile i of a sequence with q new tokens behind `base` cached ones.
@@ -53,10 +56,14 @@ __device__ __forceinline__ int line_key(const LineTile& t, int64_t x, int step) 
 // most of what a short call costs, so lane i keeps what belongs to sequence hint + i: loaded
 // in one go, before the first place is even known, and enough for any batch of up to 32
 // sequences and for walking from a sequence to the next.
+//
+// Without a step's sums (p.work NULL, at most 32 sequences) every warp makes them from the
+// lengths by a scan over its lanes, with the step kernel's checks: cheaper than a launch.
 struct LineFinder {
   const int64_t* work;
   const int32_t *ctx_lens, *cu_q;
   int num_seqs, tt, hint;
+  int64_t total;       // keys on the line
   int64_t begin, end;  // of the lane's sequence on the line
   int first, next, ctx;
 
@@ -70,10 +77,44 @@ struct LineFinder {
     ctx = ctx_lens[i];
   }
 
-  __device__ __forceinline__ LineFinder(const int64_t* work_, int num_seqs_, const int32_t* ctx_lens_,
-                                        const int32_t* cu_q_, int tile_tokens)
-      : work(work_), ctx_lens(ctx_lens_), cu_q(cu_q_), num_seqs(num_seqs_), tt(tile_tokens) {
-    load(0);
+  __device__ __forceinline__ LineFinder(const Kv8AttnParams& p, int* err)
+      : work(p.work), ctx_lens(p.ctx_lens), cu_q(p.cu_q), num_seqs(p.num_seqs), tt(p.tile_tokens) {
+    if (work) {
+      load(0);
+      total = work[num_seqs];
+      return;
+    }
+    hint = 0;
+    const int lane = threadIdx.x & 31;
+    int q = 0;
+    ctx = 0;
+    if (lane < num_seqs) {
+      ctx = ctx_lens[lane];
+      q = p.query_lens[lane];
+    }
+    const bool bad = q < 0 || q > p.max_query_len || ctx < q || ctx > p.max_context;
+    if (bad) q = ctx = 0;
+    const bool mine = (q <= p.small_max) == p.few;
+    int64_t keys = q > 0 && mine ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
+    next = q;
+    end = keys;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, next, d);
+      const int64_t up_keys = __shfl_up_sync(0xffffffffu, end, d);
+      if (lane >= d) {
+        next += up;
+        end += up_keys;
+      }
+    }
+    first = next - q;
+    begin = end - keys;
+    total = __shfl_sync(0xffffffffu, end, 31);
+    // 32 chunks of at most 2^20 tokens: the sum fits 32 bits.
+    if (__any_sync(0xffffffffu, bad) || __shfl_sync(0xffffffffu, next, 31) > p.num_tokens) {
+      total = 0;
+      if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) set_error(err, PA_KV8_ERR_STEP);
+    }
   }
 
   // The tile that holds place x, with work[hint] <= x < total.

@@ -174,8 +174,8 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
   __syncthreads();
   pdl_wait();
   pdl_release();
-  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
-  const int64_t total = p.work[p.num_seqs];
+  LineFinder finder(p, err);
+  const int64_t total = finder.total;
   const int slices = line_slices(total, p.slices, rows_min_keys(RG));
   if (total == 0 || slice >= slices) return;
 
@@ -626,14 +626,14 @@ constexpr int kCombineWarps = 8;
 
 template <typename T, int D, int NR, bool BY_PARTS>
 __global__ void __launch_bounds__(32 * kCombineWarps)
-    kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys) {
+    kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys, int* err) {
   constexpr int E = D / 32, P = 2;
   __shared__ float s_acc[BY_PARTS ? kCombineWarps : 1][NR][D];
   __shared__ float2 s_ml[BY_PARTS ? kCombineWarps : 1][NR];
   pdl_wait();
   pdl_release();
-  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
-  const int64_t total = p.work[p.num_seqs];
+  LineFinder finder(p, err);
+  const int64_t total = finder.total;
   const int slices = line_slices(total, p.slices, min_keys);
   const int s = blockIdx.x + 1, kvh = blockIdx.y;
   if (total == 0 || s >= slices) return;
@@ -803,29 +803,30 @@ cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, 
 }
 
 template <typename T, int D>
-static cudaError_t combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, cudaStream_t stream) {
+static cudaError_t combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, int* err,
+                               cudaStream_t stream) {
   const int live = p.tile_tokens * p.group;
   const dim3 block(32 * kCombineWarps);
   if (rows <= 8 * kKv8RowGroups)
     return launch_pdl(kv8_combine_kernel<T, D, 4, true>, dim3(p.slices - 1, p.num_kv_heads, (live + 3) / 4), block, 0,
-                      stream, p, rows, key_step, min_keys);
+                      stream, p, rows, key_step, min_keys, err);
   return launch_pdl(kv8_combine_kernel<T, D, 4, false>, dim3(p.slices - 1, p.num_kv_heads, (live + 63) / 64), block, 0,
-                    stream, p, rows, key_step, min_keys);
+                    stream, p, rows, key_step, min_keys, err);
 }
 
 cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
-                               cudaStream_t stream) {
+                               int* err, cudaStream_t stream) {
   if (p.slices < 2) return cudaSuccess;
   if (dtype == PA_DTYPE_F16)
-    return head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, stream)
-                          : combine_one<__half, 128>(rows, key_step, min_keys, p, stream);
-  return head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, stream)
-                        : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, stream);
+    return head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, err, stream)
+                          : combine_one<__half, 128>(rows, key_step, min_keys, p, err, stream);
+  return head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, err, stream)
+                        : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, err, stream);
 }
 
-cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p, int* err,
                                     cudaStream_t stream) {
-  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, rows_min_keys(row_groups), p, stream);
+  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, rows_min_keys(row_groups), p, err, stream);
 }
 
 }  // namespace pa

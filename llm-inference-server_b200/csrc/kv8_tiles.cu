@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   // What this reads was complete before the kernel for few rows let it start; the wait before
   // every end makes its completion imply that kernel's.
   pdl_release();
-  LineFinder finder(p.work, p.num_seqs, p.ctx_lens, p.cu_q, p.tile_tokens);
-  const int64_t total = p.work[p.num_seqs];
+  LineFinder finder(p, err);
+  const int64_t total = finder.total;
   const int slices = line_slices(total, p.slices, kTileMinKeys);
   if (total == 0 || slice >= slices) {
     pdl_wait();
@@ -746,8 +746,8 @@ cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, con
                                : tiles_by_dim<__nv_bfloat16>(head_dim, tk, tv, p, err, stream);
 }
 
-cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream) {
-  return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, stream);
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
+  return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, err, stream);
 }
 
 }  // namespace pa
