@@ -37,6 +37,8 @@
 // head's dims are kept; the columns that this costs were zeros before.
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "kv8.h"
 #include "kv8_launch.cuh"
 #include "kv8_line.cuh"
@@ -64,13 +66,14 @@ struct RowsCfg {
   static constexpr int SUBS = PAIR ? 2 : 1;         // KV heads of a payload row
   static constexpr int W = rows_warps(RG), CTAS = rows_ctas(RG), THREADS = 32 * (W + 1);
   static constexpr int SCALES = 2 * SUBS * kRowsStage;  // bytes a stage: K then V
-  static constexpr int STAGES = D == 128 ? 2 : 4;   // 16 KB in flight per warp
+  // 16 KB in flight per consumer, or with fewer consumers 24.
+  static constexpr int STAGES = (D == 128 ? 1 : 2) * (RG == 1 ? 2 : 3);
   static constexpr int TILE = kRowsKeys * D;        // K or V of a block
   static constexpr int BLOCK = 2 * TILE;
   static constexpr int STAGE = 2 * BLOCK;
   static constexpr int CH = D / 16;                 // 16-byte chunks of a row = k steps of S
   static constexpr int NO = CH * RG * 4;            // accumulator registers
-  static constexpr int MERGES = 2;    // accumulators on their way between warps
+  static constexpr int MERGES = RG == 1 ? 2 : 1;    // accumulators on their way between warps
   static constexpr int OFF_SCALE = W * STAGES * STAGE;
   static constexpr int OFF_Q = OFF_SCALE + W * STAGES * SCALES;
   static constexpr int OFF_MERGE = OFF_Q;           // the queries are no longer read by then
@@ -392,35 +395,37 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
 
     const int skip = (warp + W - d.pair0 % W) % W;  // stages of the piece before this warp's first
     int turn = (d.pair0 + skip) / W;
-    for (int kb = d.kb0 + 2 * skip; kb < d.kb1; kb += 2 * W, ++turn) {
-      const int st = warp * C::STAGES + turn % C::STAGES;
-      if (ok) ok = mbar_wait(&full[st], (turn / C::STAGES) & 1);
-      const uint32_t stage = smem_u32(smem + st * C::STAGE);
-      const uint8_t* sc = smem + C::OFF_SCALE + st * C::SCALES;
-      const int key0 = kb * kRowsKeys;
-      // Spare rows of the tile compute, unmasked, and are not stored.
-      const bool masked = key0 + kRowsStage - 1 > d.pos0 || kb + 2 > d.kb1;
-      const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;  // keys of the stage that are there
-      {
-        constexpr int b0 = 0;
+    // The piece's stages with the first LG groups of rows: a tile of fewer tokens than the
+    // widest leaves groups empty.
+    auto stages = [&](auto groups) {
+      constexpr int LG = decltype(groups)::value;
+      for (int kb = d.kb0 + 2 * skip; kb < d.kb1; kb += 2 * W, ++turn) {
+        const int st = warp * C::STAGES + turn % C::STAGES;
+        if (ok) ok = mbar_wait(&full[st], (turn / C::STAGES) & 1);
+        const uint32_t stage = smem_u32(smem + st * C::STAGE);
+        const uint8_t* sc = smem + C::OFF_SCALE + st * C::SCALES;
+        const int key0 = kb * kRowsKeys;
+        // Spare rows of the tile compute, unmasked, and are not stored.
+        const bool masked = key0 + kRowsStage - 1 > d.pos0 || kb + 2 > d.kb1;
+        const int end = min(d.ctx, d.kb1 * kRowsKeys) - key0;  // keys of the stage that are there
         // ---- S^T over the payloads: element 2 h + e is key 16 b + 8 h + g, row 8 rg + 2 tig + e
-        float s[2][RG][4];
+        float s[2][LG][4];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
 #pragma unroll
-          for (int rg = 0; rg < RG; ++rg)
+          for (int rg = 0; rg < LG; ++rg)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[n][rg][e] = 0.f;
 #pragma unroll
           for (int c = 0; c < CH; c += 2) {
             uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
-            ldm4(stage + (b0 + n) * C::BLOCK + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+            ldm4(stage + n * C::BLOCK + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t a0 = widen_lo(w[2 * i]), a1 = widen_lo(w[2 * i + 1]), a2 = widen_hi(w[2 * i]),
                              a3 = widen_hi(w[2 * i + 1]);
 #pragma unroll
-              for (int rg = 0; rg < RG; ++rg) {
+              for (int rg = 0; rg < LG; ++rg) {
                 uint2 q;
                 if constexpr (C::Q_IN_REGS)
                   q = qr[c + i][rg];
@@ -439,16 +444,16 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int key = 16 * (b0 + n) + 8 * h + g;
+              const int key = 16 * n + 8 * h + g;
               ks[n][h] = __uint_as_float(uint32_t(sc[key]) << 23);
               vs[n][h] = __uint_as_float(uint32_t(sc[kRowsStage + key]) << 23) * kWeightShift;
             }
         }
-        uint32_t wt[2][RG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
+        uint32_t wt[2][LG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
         bool grown = false;
-        float alpha[RG][2];
+        float alpha[LG][2];
 #pragma unroll
-        for (int rg = 0; rg < RG; ++rg) {
+        for (int rg = 0; rg < LG; ++rg) {
           const float2 factor = my_factors[4 * rg];
           int2 limit = make_int2(0, 0);
           if (masked) limit = my_limits[4 * rg];
@@ -459,7 +464,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
             for (int h = 0; h < 2; ++h)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int key = 16 * (b0 + n) + 8 * h + g;
+                const int key = 16 * n + 8 * h + g;
                 float& v = s[n][rg][2 * h + e];
                 const float k = PAIR ? __uint_as_float(uint32_t(sc[own[rg][e] + key]) << 23) : ks[n][h];
                 v *= k * (e ? factor.y : factor.x);
@@ -481,7 +486,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int key = 16 * (b0 + n) + 8 * h + g;
+              const int key = 16 * n + 8 * h + g;
               float w[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
@@ -501,7 +506,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
 #pragma unroll
           for (int c = 0; c < CH; ++c)
 #pragma unroll
-            for (int rg = 0; rg < RG; ++rg)
+            for (int rg = 0; rg < LG; ++rg)
 #pragma unroll
               for (int e = 0; e < 4; ++e) o[c][rg][e] *= alpha[rg][e & 1];
         }
@@ -513,27 +518,34 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
           if (end < kRowsStage) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int t0 = 16 * (b0 + n) + 8 * h + 2 * tig;
+              const int t0 = 16 * n + 8 * h + 2 * tig;
               pick[h] = t0 + 1 < end ? 0x3120u : (t0 < end ? 0x4140u : 0x4444u);
             }
           }
 #pragma unroll
           for (int c = 0; c < CH; c += 2) {
             uint32_t w[4];  // (keys 0-7, chunk c), (keys 8-15, c), (0-7, c + 1), (8-15, c + 1)
-            ldm4t(stage + (b0 + n) * C::BLOCK + C::TILE + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
+            ldm4t(stage + n * C::BLOCK + C::TILE + tile_at<D>(8 * (mi & 1) + ri, c + (mi >> 1)), w);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t x = __byte_perm(w[2 * i], 0, pick[0]), y = __byte_perm(w[2 * i + 1], 0, pick[1]);
               const uint32_t a0 = widen_lo(x), a1 = widen_hi(x), a2 = widen_lo(y), a3 = widen_hi(y);
 #pragma unroll
-              for (int rg = 0; rg < RG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[n][rg][0], wt[n][rg][1]);
+              for (int rg = 0; rg < LG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[n][rg][0], wt[n][rg][1]);
             }
           }
         }
+        __syncwarp();
+        if (lane == 0) rows_arrive(&empty[st]);
       }
-      __syncwarp();
-      if (lane == 0) rows_arrive(&empty[st]);
-    }
+    };
+    const int live = (d.tokens * p.group + 7) / 8;
+    if (RG == 1 || live <= 1)
+      stages(std::integral_constant<int, 1>{});
+    else if (RG == 2 || live == 2)
+      stages(std::integral_constant<int, RG < 2 ? RG : 2>{});
+    else
+      stages(std::integral_constant<int, RG>{});
 
     // ---- join the warps: common maximum, then a tree over the accumulators
     float big[RG][2];
