@@ -16,15 +16,15 @@
 namespace pa {
 
 // Keys of tile i of a sequence with q new tokens behind `base` cached ones.
-__host__ __device__ __forceinline__ int64_t line_tile_keys(int64_t base, int64_t q, int64_t tt, int64_t i) {
-  const int64_t last = (i + 1) * tt;
-  return base + (last < q ? last : q);
+__host__ __device__ __forceinline__ int line_tile_keys(int base, int q, int tt, int i) {
+  const int64_t last = int64_t(i + 1) * tt;
+  return base + (last < q ? int(last) : q);
 }
 
 // Keys of the first n tiles: full tiles visit base + tt, base + 2 tt, ...
-__host__ __device__ __forceinline__ int64_t line_keys_before(int64_t base, int64_t q, int64_t tt, int64_t n) {
-  const int64_t full = n < q / tt ? n : q / tt;
-  return full * base + tt * (full * (full + 1) / 2) + (n > full ? base + q : 0);
+__host__ __device__ __forceinline__ int64_t line_keys_before(int base, int q, int tt, int n) {
+  const int whole = q / tt, full = n < whole ? n : whole;
+  return int64_t(full) * base + int64_t(tt) * (int64_t(full) * (full + 1) / 2) + (n > full ? int64_t(base) + q : 0);
 }
 
 struct LineTile {
@@ -35,21 +35,35 @@ struct LineTile {
   int first, q, ctx;  // of the sequence: packed index of its first token, new tokens, context
 };
 
-// End of slice s - 1 / start of slice s out of n over a line of `total` keys.
-__device__ __forceinline__ int64_t line_cut(int64_t total, int n, int s) { return total * s / n; }
+// The line's cuts: at least `min_keys` keys a slice (a power of two times 32 or so), at most
+// `most` slices; slice s is [at(s), at(s + 1)).  Divisions of 64 bits are worth avoiding: they
+// stand before a CTA's first load.
+struct LineCuts {
+  int64_t each;
+  uint32_t rest;
+  int n;
 
-// Slices that a line of `total` keys is worth: at least `min_keys` each.
-__device__ __forceinline__ int line_slices(int64_t total, int most, int min_keys) {
-  const int64_t n = (total + min_keys - 1) / min_keys;
-  return n < 1 ? 1 : (n < most ? int(n) : most);
-}
+  __device__ __forceinline__ LineCuts(int64_t total, int most, int min_keys) {
+    if (total >> 32) {
+      n = most;  // 2^32 keys are worth any number of slices
+      each = total / n;
+      rest = uint32_t(total % n);
+    } else {
+      const uint32_t t = uint32_t(total), worth = t / uint32_t(min_keys) + (t % uint32_t(min_keys) ? 1 : 0);
+      n = worth < 1 ? 1 : (worth < uint32_t(most) ? int(worth) : most);
+      each = t / uint32_t(n);
+      rest = t % uint32_t(n);
+    }
+  }
+  __device__ __forceinline__ int64_t at(int s) const { return each * s + rest * uint32_t(s) / uint32_t(n); }
+};
 
-// A place x of the line as a key of the tile, moved up to a multiple of `step`.
+// A place x of the line as a key of the tile, moved up to a multiple of `step`, a power of two.
 __device__ __forceinline__ int line_key(const LineTile& t, int64_t x, int step) {
   const int64_t d = x - t.start;
   if (d <= 0) return 0;
-  const int64_t k = (d + step - 1) / step * step;
-  return k < t.keys ? int(k) : t.keys;
+  if (d >= t.keys) return t.keys;
+  return min((int(d) + step - 1) & ~(step - 1), t.keys);
 }
 
 // Looks tiles up by place; a whole warp's.  Finding one is a chain of dependent loads, which is
@@ -95,7 +109,7 @@ struct LineFinder {
     const bool bad = q < 0 || q > p.max_query_len || ctx < q || ctx > p.max_context;
     if (bad) q = ctx = 0;
     const bool mine = (q <= p.small_max) == p.few;
-    int64_t keys = q > 0 && mine ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
+    const int64_t keys = q > 0 && mine ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
     next = q;
     end = keys;
 #pragma unroll
@@ -140,7 +154,8 @@ struct LineFinder {
     t.first = __shfl_sync(0xffffffffu, first, f);
     t.q = __shfl_sync(0xffffffffu, next, f) - t.first;
     t.ctx = __shfl_sync(0xffffffffu, ctx, f);
-    const int64_t at = __shfl_sync(0xffffffffu, begin, f), base = t.ctx - t.q, rest = x - at;
+    const int base = t.ctx - t.q;
+    const int64_t at = __shfl_sync(0xffffffffu, begin, f), rest = x - at;
     int a = 0, b = (t.q + tt - 1) / tt;  // keys_before(a) <= rest < keys_before(b)
     while (b - a > 1) {
       const int m = (a + b) / 2;
@@ -151,7 +166,7 @@ struct LineFinder {
     }
     t.index = a;
     t.start = at + line_keys_before(base, t.q, tt, a);
-    t.keys = int(line_tile_keys(base, t.q, tt, a));
+    t.keys = line_tile_keys(base, t.q, tt, a);
     return t;
   }
 };

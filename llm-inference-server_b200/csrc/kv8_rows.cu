@@ -179,13 +179,13 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
   pdl_release();
   LineFinder finder(p, err);
   const int64_t total = finder.total;
-  const int slices = line_slices(total, p.slices, rows_min_keys(RG));
-  if (total == 0 || slice >= slices) return;
+  const LineCuts cuts(total, p.slices, rows_min_keys(RG));
+  if (total == 0 || slice >= cuts.n) return;
 
   if (warp == W) {
     // ------------------------------------------------------------ producer
-    const int64_t x1 = line_cut(total, slices, slice + 1);
-    int64_t x = line_cut(total, slices, slice);
+    const int64_t x1 = cuts.at(slice + 1);
+    int64_t x = cuts.at(slice);
     int pairs = 0;  // stages issued so far; the i-th is consumer (i % W)'s
     int pieces = 0;
     bool ok = true;
@@ -193,11 +193,13 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
       int slot;  // first slot of the 16 keys
       uint4 ks[C::SUBS], vs[C::SUBS];
     };
-    auto look_up = [&](const int32_t* row, int kb, int end) {
+    // A block's id, and with it its place and scales: in two steps, so that neither a round's
+    // ids nor its scales are waited for before the round before it is on its way.
+    auto read_id = [&](const int32_t* row, int kb, int end) { return kb < end ? __ldg(row + (kb >> p.block_shift)) : 0; };
+    auto look_up = [&](int id, int kb, int end) {
       BlockRef r;
       r.slot = 0;
       if (kb < end) {
-        int id = row[kb >> p.block_shift];
         if (id < 0 || id >= p.pool_blocks) {
           set_error(err, PA_KV8_ERR_BLOCK);
           id = 0;
@@ -206,8 +208,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
         r.slot = (id << (p.block_shift + 4)) + sub;
 #pragma unroll
         for (int u = 0; u < C::SUBS; ++u) {
-          const int64_t at =
-              (((int64_t(id) * p.num_kv_heads + kvh) * C::SUBS + u) << (p.block_shift + 4)) + sub;
+          const int64_t at = (((int64_t(id) * p.num_kv_heads + kvh) * C::SUBS + u) << (p.block_shift + 4)) + sub;
           r.ks[u] = __ldg(reinterpret_cast<const uint4*>(p.k_scale + at));
           r.vs[u] = __ldg(reinterpret_cast<const uint4*>(p.v_scale + at));
         }
@@ -243,12 +244,13 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
       ++pieces;
       if (!more) break;
       const int32_t* row = p.tables + int64_t(t.seq) * p.table_stride;
-      // Each lane looks up one of the next 32 blocks and reads its scales, one round ahead of
-      // the round whose tiles are being issued; lanes then issue their own blocks, two (a
-      // stage) at a time.
-      BlockRef cur = look_up(row, kb0 + lane, kb1), nxt = cur;
+      // Each lane looks after one of the next 32 blocks: its id is read two rounds ahead of the
+      // round whose tiles are being issued, its scales one round; lanes then issue their own
+      // blocks, two (a stage) at a time.
+      const int id = read_id(row, kb0 + lane, kb1);
+      int id_next = read_id(row, kb0 + 32 + lane, kb1);
+      BlockRef cur = look_up(id, kb0 + lane, kb1), nxt = cur;
       for (int kb = kb0; kb < kb1 && ok; kb += 32) {
-        if (kb + 32 < kb1) nxt = look_up(row, kb + 32 + lane, kb1);
         const int n = min(32, kb1 - kb);
         // As many stages at a time as have places of their own in the rings, each lane issuing
         // its block as soon as its place is free: one stage after the other took about 770
@@ -283,8 +285,11 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
           }
           ok = !__any_sync(0xffffffffu, waiting);
           pairs += min(ROUND, (n - b0 + 1) / 2);
+          if (b0 == 0 && kb + 32 < kb1) {
+            nxt = look_up(id_next, kb + 32 + lane, kb1);
+            id_next = read_id(row, kb + 64 + lane, kb1);
+          }
         }
-        ok = __all_sync(0xffffffffu, ok);
         cur = nxt;
       }
     }
@@ -646,18 +651,20 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
   pdl_release();
   LineFinder finder(p, err);
   const int64_t total = finder.total;
-  const int slices = line_slices(total, p.slices, min_keys);
+  const LineCuts cuts(total, p.slices, min_keys);
   const int s = blockIdx.x + 1, kvh = blockIdx.y;
-  if (total == 0 || s >= slices) return;
-  const int64_t x = line_cut(total, slices, s);
+  if (total == 0 || s >= cuts.n) return;
+  const int64_t x = cuts.at(s);
   const LineTile t = finder.find(x);
-  if (x <= t.start || line_cut(total, slices, s - 1) > t.start) return;
+  if (x <= t.start || cuts.at(s - 1) > t.start) return;
   if (line_key(t, x, key_step) >= t.keys) return;  // the first slice did the whole tile
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t end = t.start + t.keys;
-  // The last slice with a part of the tile: the largest i with cut(i) < end.
-  int last = int((end * slices - 1) / total);
-  last = min(last, slices - 1);
+  // The last slice with a part of the tile: the largest i with at(i) < end; slices differ by
+  // one key at most, so a guess by their length is next to it.
+  int last = min(s + int((end - x) / max(cuts.each, int64_t(1))), cuts.n - 1);
+  while (last + 1 < cuts.n && cuts.at(last + 1) < end) ++last;
+  while (last > s && cuts.at(last) >= end) --last;
   const int t0 = t.index * p.tile_tokens;
   const int live = min(p.tile_tokens, t.q - t0) * p.group;  // rows of the tile
   constexpr int ROWS = BY_PARTS ? NR : kCombineWarps * NR;  // of the CTA at a time
@@ -676,8 +683,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
     }
     for (int i0 = s - 1 + first_part; i0 <= last; i0 += 32 * part_step) {
       const int i = i0 + lane * part_step;
-      const bool mine = i <= last && line_key(t, line_cut(total, slices, i + 1), key_step) >
-                                         line_key(t, line_cut(total, slices, i), key_step);
+      const bool mine = i <= last && line_key(t, cuts.at(i + 1), key_step) > line_key(t, cuts.at(i), key_step);
       const int64_t at = mine ? ((int64_t(i) * p.num_kv_heads + kvh) * 2 + (i == s - 1 ? 1 : 0)) * rows + r0 : -1;
       float2 v[NR];
 #pragma unroll

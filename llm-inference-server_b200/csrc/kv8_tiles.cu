@@ -194,8 +194,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   pdl_release();
   LineFinder finder(p, err);
   const int64_t total = finder.total;
-  const int slices = line_slices(total, p.slices, kTileMinKeys);
-  if (total == 0 || slice >= slices) {
+  const LineCuts cuts(total, p.slices, kTileMinKeys);
+  if (total == 0 || slice >= cuts.n) {
     pdl_wait();
     return;
   }
@@ -255,8 +255,8 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
     if (warp == 22) {
       // ---------------------------------------------------------- pieces
-      const int64_t x1 = line_cut(total, slices, slice + 1);
-      int64_t x = line_cut(total, slices, slice);
+      const int64_t x1 = cuts.at(slice + 1);
+      int64_t x = cuts.at(slice);
       for (int k = 0;; ++k) {
         LinePiece at;
         const bool more = line_next_piece(finder, x, x1, kTileKeys, at);
