@@ -126,6 +126,7 @@ class DeviceStep:
         self._views: tuple[torch.Tensor, ...] | None = None
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
         self._row_ids: torch.Tensor | None = None
+        self._counted = False
 
     @property
     def _arrays(self) -> tuple[torch.Tensor, ...]:
@@ -297,7 +298,7 @@ class DeviceBlockTables:
                               own_tables=True)
         elif step._tables is not None:
             raise ValueError("out was made by device_step")
-        step._row_ids = ids
+        step._row_ids, step._counted = ids, False
         p = step._ptr
         _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
                 self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
@@ -311,6 +312,8 @@ class DeviceBlockTables:
         cached now and its blocks are held.  An emptied step changes nothing."""
         if step._row_ids is None:
             raise ValueError("commit needs a step made by reserve")
+        if step._counted:
+            raise ValueError("this step was committed before")
         acc = None
         if accepted is not None:
             if tuple(accepted.shape) != (step.num_seqs,):
@@ -320,6 +323,7 @@ class DeviceBlockTables:
         _launch(self.device, _lib.lib().pa_kv8_commit, step._row_ids.data_ptr(), p[_QL],
                 acc.data_ptr() if acc is not None else None, p[_HELD], p[_FREE], step.num_seqs, self.max_requests,
                 self.lens.data_ptr(), self.held.data_ptr(), self.num_free.data_ptr())
+        step._counted = True
 
     def release(self, request_ids: torch.Tensor) -> None:
         """Return the blocks of these request slots (-1 is passed over; a slot at most once) to

@@ -648,6 +648,138 @@ def test_a_decode_loop_on_the_gpu(pkg):
     assert torch.equal(outs, third)
 
 
+def test_a_captured_call_follows_the_lengths(pkg):
+    """One captured call over both kernels, replayed with other lengths (other splits, other
+    classes of chunks, an empty sequence), on either way of making the sums."""
+    lengths = [[(40, 3), (700, 60), (5, 5)], [(2000, 2), (65, 65), (1, 1)], [(0, 0), (4000, 68), (0, 0)],
+               [(300, 20), (300, 20), (300, 28)]]
+    for extra in (0, 40):                                  # 43 sequences: the sums take a launch
+        hq, hkv, d = 8, 2, 128
+        pad = [(0, 0)] * extra
+        query, pools, tables, _, _ = _batch([(4200, 68)] * 3 + pad, hq, hkv, d, 16, torch.bfloat16, seed=31)
+        query = query[:68].contiguous()
+        k, v = (ref.dequantise(pools[i].view(torch.uint8), pools[i + 2]) for i in (0, 1))
+        ctx, ql = _i32([40, 700, 5] + [0] * extra), _i32([3, 60, 5] + [0] * extra)
+        out = torch.zeros_like(query)
+        call = lambda: pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.1, max_query_len=68, out=out)  # noqa: E731
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+            call()
+        torch.cuda.current_stream().wait_stream(side)
+        for pairs in lengths:
+            ctx.copy_(_i32([c for c, _ in pairs] + [0] * extra))
+            ql.copy_(_i32([q for _, q in pairs] + [0] * extra))
+            out.fill_(9.0)
+            graph.replay()
+            n = sum(q for _, q in pairs)
+            want, mean, slip = ref.attention(query[:n], k, v, tables, ctx.tolist(), ql.tolist(), 0.1)
+            tol = ref.tolerance(want, mean, slip, torch.bfloat16, d, 4200)
+            assert ((out[:n].double() - want).abs() <= tol).all()
+            assert (out[n:] == 9.0).all()
+            eager = torch.full_like(out, 9.0)
+            pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.1, max_query_len=68, out=eager)
+            assert torch.equal(out, eager)
+
+
+def test_calls_on_two_streams_at_once(pkg):
+    a = _batch([(900, 2), (4000, 1)], 8, 2, 128, 16, torch.bfloat16, seed=41)
+    b = _batch([(700, 90), (33, 33)], 8, 2, 128, 16, torch.float16, seed=42)
+    run = lambda x, most: pkg.paged_attention_kv8(x[0], *x[1], *x[2:], 0.1, max_query_len=most)  # noqa: E731
+    want = run(a, 2), run(b, 90)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, most) in enumerate(((a, 2), (b, 90))):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(run(x, most))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(want[i], g) for g in got[i])
+
+
+def test_pools_past_four_gigabytes(pkg):
+    """Blocks whose bytes lie past 2^32 in the pool: append and both attention kernels."""
+    hkv, d, bs, nb = 8, 128, 16, 290_000
+    zeros = lambda *shape: torch.zeros(shape, dtype=torch.uint8, device=DEV)  # noqa: E731
+    payload = [zeros(nb, bs, hkv, d) for _ in range(2)]
+    scale = [zeros(nb, hkv, bs) for _ in range(2)]
+    pools = [payload[0].view(ref.E4M3), payload[1].view(ref.E4M3), *scale]
+    tables = _i32([[nb - 1, nb - 7, 3, nb - 2], [nb - 5, nb - 4, nb - 3, 0]])
+    ctx, ql = _i32([60, 40]), _i32([3, 30])
+    step = pkg.device_step(tables, ctx, ctx, num_tokens=100, max_query_len=60, num_blocks=nb, block_size=bs, group=2)
+    kv = torch.randn(100, 2 * hkv, d, device=DEV).bfloat16()
+    pkg.reshape_and_cache_kv8(kv[:, :hkv], kv[:, hkv:], *pools, step.slot_mapping)
+    used = tables.flatten().long()
+    local = _i32([[0, 1, 2, 3], [4, 5, 6, 7]])
+    k, v = (ref.dequantise(payload[i][used], scale[i][used]) for i in (0, 1))
+    codes, byte = ref.quantise(kv[:, :hkv].double().cpu().numpy())
+    assert np.array_equal(k.view(2, 64, hkv, d)[0, :60].cpu().numpy(),
+                          ref.e4m3_table()[codes[:60]] * 2.0 ** (byte[:60].astype(int) - 127)[..., None])
+    query = torch.randn(33, 2 * hkv, d, device=DEV).bfloat16()
+    got = pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.09, max_query_len=30)
+    want, mean, slip = ref.attention(query, k, v, local, [60, 40], [3, 30], 0.09)
+    assert ((got.double() - want).abs() <= ref.tolerance(want, mean, slip, torch.bfloat16, d, 60)).all()
+    assert {"kv8_rows", "kv8_tiles"} <= pkg._lib.last_launches()
+
+
+def test_the_most_rows_and_request_slots(pkg):
+    """4,096 rows over 131,072 slots, one token each; every eighth slot needs a block."""
+    r, b, w, bs = 131072, 4096, 2, 16
+    nb = 2 * r
+    bt = pkg.DeviceBlockTables(r, w, nb, bs, DEV)
+    ids = torch.randperm(r, generator=torch.Generator().manual_seed(0))[:b].to(DEV)
+    bt.lens[ids[::8]] = 16
+    bt.held[ids] = 1
+    step = bt.reserve(ids, torch.ones(b, dtype=torch.int32, device=DEV), num_tokens=b, max_query_len=1)
+    assert int(step.num_free) == nb - b // 8
+    assert torch.equal(step.cu_query_lens, torch.arange(b + 1, dtype=torch.int32, device=DEV))
+    assert torch.equal(step.q_pos, bt.lens[ids])
+    new = step.block_tables[::8, 1]
+    assert torch.equal(new, torch.arange(b // 8, dtype=torch.int32, device=DEV))   # from the list's end, in row order
+    assert torch.equal(step.slot_mapping[::8], new * bs)
+    with pytest.raises(NotImplementedError, match="at most 4096"):
+        more = torch.arange(b + 1, device=DEV)
+        bt.reserve(more, torch.ones_like(more), num_tokens=b + 1, max_query_len=1)
+
+
+def test_a_step_counts_once(pkg):
+    bt = pkg.DeviceBlockTables(4, 4, 20, 16, DEV)
+    step = bt.reserve(_i32([0]), _i32([3]), num_tokens=3, max_query_len=3)
+    bt.commit(step)
+    with pytest.raises(ValueError, match="committed before"):
+        bt.commit(step)
+    bt.commit(bt.reserve(_i32([0]), _i32([3]), num_tokens=3, max_query_len=3, out=step))
+    assert int(bt.lens[0]) == 6
+
+
+def test_an_attached_step_of_other_sizes_is_refused(pkg):
+    query, pools, tables, ctx, ql = _batch([(40, 3)], 8, 2, 128, 16, torch.bfloat16, seed=43)
+    step = pkg.device_step(tables, ctx, ql, num_tokens=3, max_query_len=3, num_blocks=pools[0].shape[0], block_size=16,
+                           group=2)
+    with pytest.raises(ValueError, match="attached step"):
+        pkg.paged_attention_kv8(query, *pools, pkg.kv8.attach_step(tables, step), ctx, ql, 0.1)
+
+
+def test_empty_calls(pkg):
+    query, pools, tables, ctx, ql = _batch([(40, 3)], 8, 2, 128, 16, torch.bfloat16, seed=44)
+    assert pkg.paged_attention_kv8(query[:0], *pools, tables[:0], ctx[:0], ql[:0], 0.1).shape == (0, 8, 128)
+    out = torch.full_like(query, 2.0)
+    pkg.paged_attention_kv8(query, *pools, tables[:0], ctx[:0], ql[:0], 0.1, out=out)
+    assert (out == 2.0).all()
+    step = pkg.device_step(tables[:0], ctx[:0], ql[:0], num_tokens=2, max_query_len=1, num_blocks=3, block_size=16)
+    assert step.slot_mapping.tolist() == [-1, -1] and step.cu_query_lens.tolist() == [0]
+    bt = pkg.DeviceBlockTables(4, 4, 20, 16, DEV)
+    step = bt.reserve(_i32([]), _i32([]), num_tokens=0, max_query_len=1)
+    bt.commit(step)
+    bt.release(_i32([]))
+    assert int(bt.num_free) == 20
+
+
 @pytest.fixture(scope="module")
 def small_llama():
     from transformers import LlamaConfig, LlamaForCausalLM
