@@ -59,9 +59,10 @@ typedef struct pa_kv8_tiling {
   int32_t row_groups; /* groups of 8 (token, head) rows that the kernel for few rows holds */
 } pa_kv8_tiling;
 
-/* The tiling for chunks of at most max_query_len tokens, `group` query heads per KV head.
- * No reference counterpart. */
-int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, pa_kv8_tiling* tiling);
+/* The tiling for a step of num_seqs chunks of at most max_query_len tokens, num_tokens in
+ * all, with `group` query heads per KV head.  No reference counterpart. */
+int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, int32_t num_seqs, int32_t num_tokens,
+                             pa_kv8_tiling* tiling);
 
 /*
  * Build one step's metadata on the GPU.  No reference counterpart (the host builds it in
@@ -129,8 +130,8 @@ int32_t pa_kv8_append(const void* key, int64_t k_stride_token, int64_t k_stride_
 
 /* Bytes of scratch that pa_kv8_attention needs for these sizes, whatever the lengths.
  * No reference counterpart. */
-uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                int32_t max_query_len);
+uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t max_query_len);
 
 /*
  * Causal attention of each sequence's new tokens over the 8-bit pools: token t of sequence
@@ -138,7 +139,7 @@ uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num
  * the block table (the rule of inference_server/core/attention.py:19-58).  Lengths and
  * tables stay on the device; the launches depend on the host's sizes only, so a captured
  * call can be replayed with other lengths.  cu_query_lens and work come from
- * pa_kv8_build_step with the tiling of the same group and max_query_len; with both NULL
+ * pa_kv8_build_step with the tiling of the same group, sizes and max_query_len; with both NULL
  * the call sums query_lens and the work up by itself (over 32 sequences in one more launch),
  * with pa_kv8_build_step's checks.  table_width blocks of a table row are used.  Rows past the
  * last sequence's are left as they were.  head_dim 64 or 128, block_size a power of two

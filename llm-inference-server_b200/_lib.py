@@ -132,7 +132,7 @@ _SIGNATURES = {
                                      c_void_p, c_void_p]),
     "pa_plan_decode_padded": (c_int32, [c_void_p, c_int32, c_void_p, c_int64, c_int32, c_int64, c_int32, c_int32,
                                         c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, POINTER(StepPlan)]),
-    "pa_kv8_choose_tiling": (c_int32, [c_int32, c_int32, POINTER(Kv8Tiling)]),
+    "pa_kv8_choose_tiling": (c_int32, [c_int32, c_int32, c_int32, c_int32, POINTER(Kv8Tiling)]),
     "pa_kv8_build_step": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,
                                     c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
                                     POINTER(Kv8Tiling), c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
@@ -144,7 +144,7 @@ _SIGNATURES = {
     "pa_kv8_append": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32,
                                 c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p,
                                 c_void_p]),
-    "pa_kv8_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "pa_kv8_workspace_bytes": (c_uint64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "pa_kv8_attention": (c_int32, [c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
                                    c_void_p, c_int64, c_int32, c_int32, c_int32, c_float, c_int32, c_int32, c_void_p,
                                    c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,

@@ -49,7 +49,7 @@ struct Kv8AttnParams {
   float qscale;  // softmax scale * log2(e)
   float* part_o;
   float2* part_ml;
-  float* twin_o;  // tiles kernel: 128 x head_dim floats per CTA
+  bool first;  // tiles kernel: the call's first kernel
 };
 
 int* kv8_error_word();  // device address of the current device's error word

@@ -58,7 +58,7 @@ static Kv8Rows rows_form(const pa_kv8_tiling& t, int num_kv_heads, int group, in
 }
 
 struct Kv8Scratch {
-  uint64_t work, cu, ml, o, tile_ml, tile_o, twin_o, bytes;
+  uint64_t work, cu, ml, o, tile_ml, tile_o, bytes;
 };
 static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int sms,
                                     bool tiles) {
@@ -72,8 +72,7 @@ static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t 
   s.tile_ml = (s.o + rows * head_dim * sizeof(float) + 255) / 256 * 256;
   const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * kKv8TileRows : 0;
   s.tile_o = (s.tile_ml + tile_rows * sizeof(float2) + 255) / 256 * 256;
-  s.twin_o = s.tile_o + tile_rows * head_dim * sizeof(float);
-  s.bytes = s.twin_o + tile_rows / 4 * head_dim * sizeof(float);  // 128 rows per CTA
+  s.bytes = s.tile_o + tile_rows * head_dim * sizeof(float);
   return s;
 }
 
@@ -99,18 +98,22 @@ static int32_t check_step_sizes(const Kv8StepParams& p, int64_t table_stride) {
 
 extern "C" {
 
-int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, pa_kv8_tiling* tiling) {
+int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, int32_t num_seqs, int32_t num_tokens,
+                             pa_kv8_tiling* tiling) {
   using namespace pa;
   if (!tiling) return fail(PA_ERR_INVALID_ARGUMENT, "tiling must not be NULL");
-  if (group < 1 || max_query_len < 0) return fail(PA_ERR_INVALID_ARGUMENT, "bad group or max_query_len");
+  if (group < 1 || max_query_len < 0 || num_seqs < 0 || num_tokens < 0)
+    return fail(PA_ERR_INVALID_ARGUMENT, "bad group, max_query_len or sizes");
   if (group > 16) return fail(PA_ERR_UNSUPPORTED, "%d query heads per KV head: at most 16 are supported", group);
   // A sequence of up to 24 (token, head) rows goes to the kernel for few rows, one of more to
-  // the 256-row tiles.
+  // the 256-row tiles.  Where the sizes leave no room for a short chunk beside the longest ones
+  // (one prompt, chunks of one length) the first class has none: its two launches are spared.
   const int few = std::max(1, 8 * kKv8RowGroups / group);
+  const bool none = max_query_len > few && num_tokens - int64_t(num_seqs - 1) * max_query_len > few;
   const int rows = group * std::max(1, std::min(max_query_len, few));
   tiling->row_groups = (rows + 7) / 8;
   tiling->small_tokens = std::max(1, 8 * tiling->row_groups / group);
-  tiling->small_max = std::min(max_query_len, few);
+  tiling->small_max = none ? 0 : std::min(max_query_len, few);
   tiling->large_tokens = kKv8TileRows / group;
   return PA_OK;
 }
@@ -239,12 +242,13 @@ int32_t pa_kv8_append(const void* key, int64_t k_stride_token, int64_t k_stride_
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "8-bit append launch");
 }
 
-uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
-                                int32_t max_query_len) {
+uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t num_heads, int32_t num_kv_heads,
+                                int32_t head_dim, int32_t max_query_len) {
   using namespace pa;
   pa_kv8_tiling t;
-  if (num_seqs < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 || num_heads % num_kv_heads ||
-      pa_kv8_choose_tiling(num_heads / num_kv_heads, max_query_len, &t) != PA_OK)
+  if (num_seqs < 0 || num_tokens < 0 || num_heads <= 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      num_heads % num_kv_heads ||
+      pa_kv8_choose_tiling(num_heads / num_kv_heads, max_query_len, num_seqs, num_tokens, &t) != PA_OK)
     return 0;
   const Kv8Rows f = rows_form(t, num_kv_heads, num_heads / num_kv_heads, head_dim, max_query_len);
   return attention_scratch(f, num_seqs, num_kv_heads, head_dim, kMaxSms, max_query_len > t.small_max).bytes;
@@ -276,7 +280,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     return fail(PA_ERR_UNSUPPORTED, "pool has more than 2^31 slots");
   pa_kv8_tiling t;
   const int group = num_heads / num_kv_heads;
-  int32_t st = pa_kv8_choose_tiling(group, max_query_len, &t);
+  int32_t st = pa_kv8_choose_tiling(group, max_query_len, num_seqs, num_tokens, &t);
   if (st != PA_OK) return st;
   if (num_tokens == 0 || num_seqs == 0 || pool_num_blocks == 0) return PA_OK;
   const bool build = !work && !cu_query_lens;
@@ -360,11 +364,16 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.qscale = scale * kLog2e;
   p.part_ml = reinterpret_cast<float2*>(ws + s.ml);
   p.part_o = reinterpret_cast<float*>(ws + s.o);
-  cudaError_t e = launch_kv8_rows(dtype, head_dim, f.pair, f.row_groups, tk, tv, p, err, stream);
-  if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
-  int32_t launched = PA_LAUNCH_KV8_ROWS;
+  // Small_max 0 with longer chunks: the first class is empty.
+  const bool tiles = max_query_len > t.small_max, rows = t.small_max > 0 || !tiles;
+  int32_t launched = 0;
+  cudaError_t e = cudaSuccess;
+  if (rows) {
+    e = launch_kv8_rows(dtype, head_dim, f.pair, f.row_groups, tk, tv, p, err, stream);
+    if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention launch");
+    launched |= PA_LAUNCH_KV8_ROWS;
+  }
   Kv8AttnParams q = p;  // of the tiles kernel
-  const bool tiles = max_query_len > t.small_max;
   if (tiles) {
     q.work = work ? work + num_seqs + 1 : nullptr;
     q.few = false;
@@ -374,7 +383,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     q.slices = kv8_tiles_slices(num_kv_heads, sms);
     q.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
     q.part_o = reinterpret_cast<float*>(ws + s.tile_o);
-    q.twin_o = reinterpret_cast<float*>(ws + s.twin_o);
+    q.first = !rows;
     if (f.pair) {  // the rows kernel's maps were of pairs
       st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, &tk);
       if (st == PA_OK) st = payload_map(v_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, &tv);
@@ -384,10 +393,10 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
     launched |= PA_LAUNCH_KV8_TILES;
   }
-  e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, err, stream);
+  if (rows) e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, err, stream);
   if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, err, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention join launch");
-  if (p.slices > 1 || (tiles && q.slices > 1)) launched |= PA_LAUNCH_KV8_COMBINE;
+  if ((rows && p.slices > 1) || (tiles && q.slices > 1)) launched |= PA_LAUNCH_KV8_COMBINE;
   note_launches(launched);
   return PA_OK;
 }

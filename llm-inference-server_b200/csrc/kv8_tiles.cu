@@ -16,9 +16,11 @@
 // leaves float32 partials that kv8_combine joins.
 //
 // Roles (768 threads, registers dealt out by setmaxnreg):
-//   warps 0-3, 4-7  softmax of rows 0-127 / 128-255, one thread per row (TMEM lane): loads its
-//                   query row into shared memory, reads scores, keeps maximum and sum, writes
-//                   P to TMEM, the epilogue
+//   warps 0-3, 4-7  softmax of rows 0-127 / 128-255, one thread per row (TMEM lane): brings the
+//                   warp's query rows into shared memory, reads scores, keeps maximum and sum,
+//                   writes P to TMEM, the epilogue.  Rows are read and written in global memory
+//                   by D / 8 lanes each, through the query tile: with a thread per row a piece
+//                   cost 4 us more (333 tokens 43 us against 34, 1,000 over 16,384 298 : 294)
 //   warps 8-11      K: staged e4m3 -> fp16 in the swizzled layout (3 stages), 16 keys a warp;
 //                   12-15: V (2 stages).  Two warps each took 1 us per tile of 64 keys, more
 //                   than anything else
@@ -34,10 +36,10 @@
 // score buffer and P beside it a tile of keys took 1.6 us, of which the softmax is 0.7.
 //
 // A piece of at most 128 rows runs as twins: both halves hold the same rows and take every
-// other key tile, each with its own maximum, sum and accumulator, and the second half's are
-// joined to the first's through scratch memory at the end.  What bounds a half is the chain
-// scores -> softmax -> P V -> buffer free of one tile (about 2 us over two buffers), not
-// arithmetic, so two chains do almost twice the keys.
+// other key tile, each with its own maximum, sum and accumulator; at the end the first half's
+// threads read the second's accumulator (the same TMEM lanes, other columns) and join them.
+// What bounds a half is the chain scores -> softmax -> P V -> buffer free of one tile (about
+// 2 us over two buffers), not arithmetic, so two chains do almost twice the keys.
 //
 // The staging rings are what the widening needs: with a tile's loads in registers, one tile
 // ahead, 128-row tiles and two CTAs per SM the loads' latency (over 1 us per tile) was
@@ -67,8 +69,10 @@ constexpr int kTileThreads = 768;
 constexpr int kTileQBox = kHalfRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kTileBox = kTileKeys * 128;   // 64 keys x 64 elements
 constexpr int kTileConsumers = 22;          // warps that read a piece: 8 softmax, 8 widening, 4 issuers, 2 producers
-// Fewest keys a slice gets: below this its partial costs more than the keys it takes over.
-constexpr int kTileMinKeys = 512;
+// Fewest keys a slice gets: below this its partial costs more than the keys it takes over.  A
+// prompt of 333 tokens takes 43 us with 128, 63 with 512; one of 60 beside another 26 with 128
+// and 36 with 256; calls that fill the GPU do not care.
+constexpr int kTileMinKeys = 128;
 // The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 and the
 // output accumulator is rarely rescaled.
 constexpr float kTileLazy = 8.f;
@@ -91,7 +95,7 @@ struct TileBars {
   uint64_t v_full[kTileVStages], v_free[kTileVStages];
   uint64_t s_full[2][2], s_free[2][2], p_full[2][2];       // score buffers of a half, by n
   uint64_t q_full[2];
-  uint64_t x_full, x_free;                                 // the twin's result
+  uint64_t x_full, x_free;                                 // the second half's result: there / read
   uint64_t d_full[2], d_empty[2];
   uint32_t tmem_base;
 };
@@ -189,8 +193,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int slice = blockIdx.x / p.num_kv_heads, kvh = blockIdx.x % p.num_kv_heads;
-  // What this reads was complete before the kernel for few rows let it start; the wait before
-  // every end makes its completion imply that kernel's.
+  // Behind the kernel for few rows: what this reads was complete before that let it start; the
+  // wait before every end makes this kernel's completion imply that one's.
+  if (p.first) pdl_wait();
   pdl_release();
   LineFinder finder(p, err);
   const int64_t total = finder.total;
@@ -489,7 +494,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const uint32_t tS = tbase, tO = tbase + C::COL_O;
     uint8_t* sQ = smem + h * (C::Q_BYTES / 2);
     const int lane_row = tid & (kHalfRows - 1);
-    float* twin_o = p.twin_o + int64_t(blockIdx.x) * kHalfRows * D + lane_row;  // [D][rows]
+    // Rows in global memory are read and written by kRowLanes lanes each, kRowsAtOnce at a time.
+    constexpr int kRowLanes = D / 8, kRowsAtOnce = 32 / kRowLanes, kRowBatch = 4;
+    const int warp_row = lane_row & ~31, row_of = lane / kRowLanes, row_chunk = lane % kRowLanes;
     int g0 = 0, n = 0, twins = 0;  // tiles of the CTA before this piece, tiles of this half, twin pieces
     for (int k = 0; ok; ++k) {
       TilePiece d;
@@ -500,44 +507,55 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       const int t_eff = min(t_row, d.tokens - 1);  // spare rows repeat the last token and are not stored
       const int qpos = d.pos0 + t_eff;
 
-      // The query row as fp16 into the swizzled tile.  The previous piece's last S has retired
-      // (its scores were read), so the tile is free.
+      // The query rows as fp16 into the swizzled tile.  The previous piece's last S has retired
+      // (its scores were read), so the tile is free.  A warp brings its own 32 rows, kRowLanes
+      // lanes on each: a lane that read its own row alone would touch a line a load.
       float qs = 0.f;
       if (!is_idle(twin, h, d)) {
         const T* src = static_cast<const T*>(p.q) + int64_t(d.row0 + t_eff) * p.q_st + int64_t(head) * p.q_sh;
-        float big = 0.f;
-        if (DType<T>::code == PA_DTYPE_BF16) {
-#pragma unroll 4
-          for (int c = 0; c < D / 8; ++c) {
-            const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * c);
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+        float up_own = query_power<T>(0.f);
+#pragma unroll 1
+        for (int i0 = 0; i0 < kRowLanes; i0 += kRowBatch) {
+          uint4 w[kRowBatch];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 f = unpack2(u[i], (T*)nullptr);
-              big = fmaxf(big, fmaxf(fabsf(f.x), fabsf(f.y)));
+          for (int i = 0; i < kRowBatch; ++i) {
+            const T* from = reinterpret_cast<const T*>(
+                __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(src), (i0 + i) * kRowsAtOnce + row_of));
+            w[i] = *reinterpret_cast<const uint4*>(from + 8 * row_chunk);
+          }
+#pragma unroll
+          for (int i = 0; i < kRowBatch; ++i) {
+            const int row = (i0 + i) * kRowsAtOnce + row_of;
+            const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+            float2 f[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) f[e] = unpack2(u[e], (T*)nullptr);
+            float up = up_own;
+            if (DType<T>::code == PA_DTYPE_BF16) {
+              float big = 0.f;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) big = fmaxf(big, fmaxf(fabsf(f[e].x), fabsf(f[e].y)));
+#pragma unroll
+              for (int m = 1; m < kRowLanes; m <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, m));
+              up = query_power<T>(big);
+              const float mine = __shfl_sync(0xffffffffu, up, (lane % kRowsAtOnce) * kRowLanes);
+              if (lane / kRowsAtOnce == i0 + i) up_own = mine;
             }
+            // The scores' maximum is taken before the scale, so the scale's sign goes into the row.
+            const float mul = p.qscale < 0.f ? -up : up;
+            *reinterpret_cast<uint4*>(sQ + (row_chunk >> 3) * kTileQBox + sw_off(warp_row + row, row_chunk & 7)) =
+                make_uint4(pack2<__half>(f[0].x * mul, f[0].y * mul), pack2<__half>(f[1].x * mul, f[1].y * mul),
+                           pack2<__half>(f[2].x * mul, f[2].y * mul), pack2<__half>(f[3].x * mul, f[3].y * mul));
           }
         }
-        // The scores' maximum is taken before the scale, so the scale's sign goes into the row.
-        const float up = query_power<T>(big);
-        qs = fmaxf(fabsf(p.qscale) / up, 1e-37f);
-        const float mul = p.qscale < 0.f ? -up : up;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-          const uint4 w = *reinterpret_cast<const uint4*>(src + 8 * c);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          uint32_t o[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 f = unpack2(u[i], (T*)nullptr);
-            o[i] = pack2<__half>(f.x * mul, f.y * mul);
-          }
-          *reinterpret_cast<uint4*>(sQ + (c >> 3) * kTileQBox + sw_off(lane_row, c & 7)) = make_uint4(o[0], o[1], o[2], o[3]);
-        }
+        qs = fmaxf(fabsf(p.qscale) / up_own, 1e-37f);
         fence_proxy_async_smem();
         mbar_arrive(&bars->q_full[h]);
       }
 
+      // The second half's accumulator is the first's to read until it says so.
+      if (h == 1 && twins > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_free, (twins - 1) & 1));
+      if (!ok) break;
       float m_run = -INFINITY, l_run = 0.f;
       bool first = true;
       for (int j = d.j0 + (twin ? h : 0); j < d.j1; j += twin ? 2 : 1, ++n) {
@@ -620,26 +638,16 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       float mine = 1.f, other = 0.f;  // weights of the two halves' accumulators
       if (twin) {
         if (h == 1) {
-          if (twins > 0) ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_free, (twins - 1) & 1));
-          if (!ok) break;
           ++twins;
           twin_ml[lane_row] = make_float2(m_run, l_run);
-          if (!first) {
-#pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              tmem_ld32(tO + 32 * c, o);
-              tmem_wait_ld();
-#pragma unroll
-              for (int e = 0; e < 32; ++e) twin_o[(32 * c + e) * kHalfRows] = __uint_as_float(o[e]);
-            }
-          }
+          tc_fence_before();
           mbar_arrive(&bars->x_full);
           continue;
         }
         ok = __all_sync(0xffffffffu, mbar_wait(&bars->x_full, twins & 1));
         if (!ok) break;
         ++twins;
+        tc_fence_after();
         const float2 v = twin_ml[lane_row];
         const float m = fmaxf(m_run, v.x), ref = m == -INFINITY ? 0.f : m;
         mine = ex2(m_run - ref);
@@ -647,18 +655,29 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         l_run = l_run * mine + v.y * other;
         m_run = m;
       }
-      // A twin without a tile left nothing in its scratch.
-      const bool joined = twin && d.j1 - d.j0 > 1;
+      const bool joined = twin && d.j1 - d.j0 > 1;  // else the second half has no accumulator
       auto result = [&](int c, uint32_t (&o)[32]) {
         tmem_ld32(tO + 32 * c, o);
-        tmem_wait_ld();
         if (joined) {
+          uint32_t v[32];
+          tmem_ld32(tO + C::COL_HALF + 32 * c, v);
+          tmem_wait_ld();
 #pragma unroll
           for (int e = 0; e < 32; ++e)
-            o[e] = __float_as_uint(__uint_as_float(o[e]) * mine + twin_o[(32 * c + e) * kHalfRows] * other);
+            o[e] = __float_as_uint(__uint_as_float(o[e]) * mine + __uint_as_float(v[e]) * other);
+        } else {
+          tmem_wait_ld();
         }
       };
-      const bool stored = t_row < d.tokens;
+      // The rows go out through the half's query tile, free by now, each warp's own 32.
+      uint8_t* const sO = sQ;
+      auto put = [&](int chunk, const uint4& w) {
+        *reinterpret_cast<uint4*>(sO + (chunk >> 3) * kTileQBox + sw_off(lane_row, chunk & 7)) = w;
+      };
+      auto get = [&](int row) {
+        return *reinterpret_cast<const uint4*>(sO + (row_chunk >> 3) * kTileQBox + sw_off(warp_row + row, row_chunk & 7));
+      };
+      const int stored = d.tokens * p.group - (r - lane);  // rows of the warp that exist
       if (d.part < 0) {
         const float inv = 1.f / l_run;
         T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + t_eff) * p.o_st + int64_t(head) * p.o_sh;
@@ -666,33 +685,51 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
           result(c, o);
-          if (stored) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint4 w;
-              w.x = pack2<T>(__uint_as_float(o[e + 0]) * inv, __uint_as_float(o[e + 1]) * inv);
-              w.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-              w.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-              w.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-              *reinterpret_cast<uint4*>(dst + 32 * c + e) = w;
-            }
+          for (int e = 0; e < 32; e += 8) {
+            uint4 w;
+            w.x = pack2<T>(__uint_as_float(o[e + 0]) * inv, __uint_as_float(o[e + 1]) * inv);
+            w.y = pack2<T>(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            w.z = pack2<T>(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            w.w = pack2<T>(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            put(4 * c + e / 8, w);
           }
         }
+        __syncwarp();
+#pragma unroll 4
+        for (int i = 0; i < kRowLanes; ++i) {
+          const int row = i * kRowsAtOnce + row_of;
+          T* to = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), row));
+          if (row < stored) *reinterpret_cast<uint4*>(to + 8 * row_chunk) = get(row);
+        }
+        __syncwarp();
       } else {
+        // 32-bit values: half a row at a time.
         const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * kTileRows + r;
+        float* to = p.part_o + (at - lane) * D + 4 * row_chunk;
 #pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          result(c, o);
-          if (stored) {
+        for (int half = 0; half < 2; ++half) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<uint4*>(p.part_o + at * D + 32 * c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          for (int c = 0; c < D / 64; ++c) {
+            uint32_t o[32];
+            result(half * (D / 64) + c, o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) put(8 * c + e / 4, make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
           }
+          __syncwarp();
+#pragma unroll 4
+          for (int i = 0; i < kRowLanes; ++i) {
+            const int row = i * kRowsAtOnce + row_of;
+            if (row < stored) *reinterpret_cast<uint4*>(to + row * D + half * (D / 2)) = get(row);
+          }
+          __syncwarp();
         }
-        if (stored) p.part_ml[at] = make_float2(m_run, l_run);
+        if (lane < stored) p.part_ml[at] = make_float2(m_run, l_run);
       }
-      if (twin) mbar_arrive(&bars->x_free);
+      if (twin) {
+        tc_fence_before();
+        mbar_arrive(&bars->x_free);
+      }
       // The next piece's first P.V overwrites O only after p_full, which these threads arrive
       // on after the loads above completed (tcgen05.wait::ld).
     }

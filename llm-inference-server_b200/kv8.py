@@ -74,17 +74,18 @@ def read_kv8_error(device=None, clear: bool = True) -> int:
 
 
 # ---------------------------------------------------------------------------- steps
-_TILINGS: dict[tuple[int, int], _lib.Kv8Tiling] = {}
+_TILINGS: dict[tuple[int, int, int, int], _lib.Kv8Tiling] = {}
 
 
-def _tiling(group: int, max_query_len: int) -> _lib.Kv8Tiling:
-    t = _TILINGS.get((group, max_query_len))
+def _tiling(group: int, max_query_len: int, num_seqs: int, num_tokens: int) -> _lib.Kv8Tiling:
+    key = (group, max_query_len, num_seqs, num_tokens)
+    t = _TILINGS.get(key)
     if t is None:
         t = _lib.Kv8Tiling()
-        _lib.check(_lib.lib().pa_kv8_choose_tiling(int(group), int(max_query_len), ctypes.byref(t)))
+        _lib.check(_lib.lib().pa_kv8_choose_tiling(*key, ctypes.byref(t)))
         if len(_TILINGS) > 1024:
             _TILINGS.clear()
-        _TILINGS[(group, max_query_len)] = t
+        _TILINGS[key] = t
     return t
 
 
@@ -200,7 +201,7 @@ def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_le
         raise ValueError("context_lens and query_lens must be [batch] to match block_tables")
     tables = _table_rows(block_tables, dev)
     ctx, ql = _int32("context_lens", context_lens, dev), _int32("query_lens", query_lens, dev)
-    tiling = _tiling(group, max_query_len)
+    tiling = _tiling(group, max_query_len, b, num_tokens)
     step = _reusable(out, (b, num_tokens, w, max_query_len, block_size, num_blocks, group), dev)
     if step is None:
         step = DeviceStep(b, num_tokens, w, max_query_len, block_size, num_blocks, group, dev, own_tables=False)
@@ -291,7 +292,7 @@ class DeviceBlockTables:
             raise ValueError("request_ids and query_lens must both be [rows]")
         ids, ql = _int32("request_ids", request_ids, dev), _int32("query_lens", query_lens, dev)
         b = ids.shape[0]
-        tiling = _tiling(group, max_query_len)
+        tiling = _tiling(group, max_query_len, b, num_tokens)
         step = _reusable(out, (b, num_tokens, self.width, max_query_len, self.block_size, self.num_blocks, group), dev)
         if step is None:
             step = DeviceStep(b, num_tokens, self.width, max_query_len, self.block_size, self.num_blocks, group, dev,
@@ -460,14 +461,14 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         most = tokens if max_query_len is None else min(int(max_query_len), tokens)
         _check_step_sizes(tokens, most, bs, nb)
         ctx, lens, cu, work = context_lens.data_ptr(), query_lens.data_ptr(), None, None
-    _tiling(group, most)                              # refuses what has no kernel, also for empty calls
+    _tiling(group, most, b, tokens)                   # refuses what has no kernel, also for empty calls
     if tokens == 0:
         return out
     qs = query.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
         query = query.contiguous()
         qs = query.stride()
-    scratch = _scratch(dev, b, heads, hkv, dim, most)
+    scratch = _scratch(dev, b, tokens, heads, hkv, dim, most)
     _launch(dev, _lib.lib().pa_kv8_attention, query.data_ptr(), qs[0], qs[1], tokens, heads, dim, k_pool.data_ptr(),
             v_pool.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nb, bs, hkv, _DTYPE_CODE[query.dtype], scale, b,
             most, tables.data_ptr(), max(tables.stride(0), w), w, ctx, lens, cu, work, out.data_ptr(), heads * dim, dim,

@@ -80,7 +80,7 @@ def test_step_work_sums_are_the_keys_of_the_tiles(pkg):
         b = 65
         ql = rng.integers(0, most + 1, size=b)
         ctx = ql + rng.integers(0, 500, size=b)
-        t = pkg.kv8._tiling(group, most)
+        t = pkg.kv8._tiling(group, most, b, int(ql.sum()))
         step = pkg.device_step(torch.zeros(b, 64, dtype=torch.int32, device=DEV), _i32(ctx), _i32(ql),
                                num_tokens=int(ql.sum()), max_query_len=most, num_blocks=1, block_size=16, group=group)
         want = np.zeros((2, b + 1), np.int64)

@@ -40,7 +40,7 @@ def test_header_is_plain_c(pkg, tmp_path):
 @pytest.mark.parametrize("group", [1, 2, 3, 4, 7, 8, 12, 16])
 def test_tiling_fits_its_kernels(pkg, group):
     for most in (0, 1, 2, 3, 4, 5, 8, 9, 16, 31, 33, 100, 4096):
-        t = pkg.kv8._tiling(group, most)
+        t = pkg.kv8._tiling(group, most, 10, 2 * most)
         assert t.row_groups in (1, 2, 3)
         assert t.small_tokens >= 1
         assert t.small_tokens * group <= 8 * t.row_groups
@@ -48,11 +48,18 @@ def test_tiling_fits_its_kernels(pkg, group):
         assert t.small_max >= 0
 
 
+def test_tiling_leaves_the_first_class_out_where_no_chunk_can_be_short(pkg):
+    assert pkg.kv8._tiling(4, 500, 1, 500).small_max == 0
+    assert pkg.kv8._tiling(4, 500, 3, 1007).small_max == 0     # 500 + 500 + 7
+    assert pkg.kv8._tiling(4, 500, 3, 1006).small_max == 6
+    assert pkg.kv8._tiling(4, 6, 1, 6).small_max == 6          # few rows: their kernel
+
+
 def test_tiling_refusals(pkg):
     with pytest.raises(NotImplementedError, match="at most 16"):
-        pkg.kv8._tiling(17, 1)
+        pkg.kv8._tiling(17, 1, 1, 1)
     with pytest.raises(ValueError):
-        pkg.kv8._tiling(0, 1)
+        pkg.kv8._tiling(0, 1, 1, 1)
 
 
 def test_the_reference_quantiser_is_torchs_rounding():
