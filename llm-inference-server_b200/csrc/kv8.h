@@ -31,6 +31,15 @@ struct Kv8AppendParams {
   bool vec16;  // every row starts on a 16-byte boundary
 };
 
+// A tile that slices share: what joins its partials has to know.
+struct Kv8Join {
+  int64_t start, each;  // the tile's place on the work line; the line's cuts
+  uint32_t rest;
+  int32_t n, keys;
+  int32_t row0, tokens;  // tokens 0: no such tile starts in the slice
+  int32_t last;          // the last slice with a part of it
+};
+
 struct Kv8AttnParams {
   const void* q;
   int64_t q_st, q_sh;
@@ -49,6 +58,7 @@ struct Kv8AttnParams {
   float qscale;  // softmax scale * log2(e)
   float* part_o;
   float2* part_ml;
+  Kv8Join* joins;  // [slices], by the slice that a shared tile starts in
   bool first;  // tiles kernel: the call's first kernel
 };
 
@@ -71,14 +81,14 @@ int kv8_rows_slices(int row_groups, int num_kv_heads, int sms);
 cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, const CUtensorMap& tk,
                             const CUtensorMap& tv, const Kv8AttnParams& p, int* err, cudaStream_t stream);
 constexpr int kKv8RowGroups = 3;  // most groups of 8 rows
-cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p, int* err,
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
                                     cudaStream_t stream);
 int kv8_tiles_slices(int num_kv_heads, int sms);
 cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, const CUtensorMap& tv,
                              const Kv8AttnParams& p, int* err, cudaStream_t stream);
-cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream);
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream);
 constexpr int kKv8TileRows = 256;  // (token, head) rows of its tiles
-cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
-                               int* err, cudaStream_t stream);
+cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, const Kv8AttnParams& p,
+                               cudaStream_t stream);
 
 }  // namespace pa

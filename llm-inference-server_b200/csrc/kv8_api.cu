@@ -58,19 +58,22 @@ static Kv8Rows rows_form(const pa_kv8_tiling& t, int num_kv_heads, int group, in
 }
 
 struct Kv8Scratch {
-  uint64_t work, cu, ml, o, tile_ml, tile_o, bytes;
+  uint64_t work, cu, joins, tile_joins, ml, o, tile_ml, tile_o, bytes;
 };
 static Kv8Scratch attention_scratch(const Kv8Rows& f, int32_t num_seqs, int32_t num_kv_heads, int32_t head_dim, int sms,
                                     bool tiles) {
-  const uint64_t rows =
-      uint64_t(kv8_rows_slices(f.row_groups, f.num_kv_heads, sms)) * f.num_kv_heads * 2 * (8 * f.row_groups);
+  const uint64_t slices = kv8_rows_slices(f.row_groups, f.num_kv_heads, sms);
+  const uint64_t tile_slices = tiles ? kv8_tiles_slices(num_kv_heads, sms) : 0;
+  const uint64_t rows = slices * f.num_kv_heads * 2 * (8 * f.row_groups);
+  const uint64_t tile_rows = tile_slices * num_kv_heads * 2 * kKv8TileRows;
   Kv8Scratch s;
   s.work = 0;
   s.cu = (uint64_t(num_seqs) + 1) * 2 * sizeof(int64_t);
-  s.ml = (s.cu + (uint64_t(num_seqs) + 1) * sizeof(int32_t) + 255) / 256 * 256;
+  s.joins = (s.cu + (uint64_t(num_seqs) + 1) * sizeof(int32_t) + 255) / 256 * 256;
+  s.tile_joins = s.joins + slices * sizeof(Kv8Join);
+  s.ml = (s.tile_joins + tile_slices * sizeof(Kv8Join) + 255) / 256 * 256;
   s.o = (s.ml + rows * sizeof(float2) + 255) / 256 * 256;
   s.tile_ml = (s.o + rows * head_dim * sizeof(float) + 255) / 256 * 256;
-  const uint64_t tile_rows = tiles ? uint64_t(kv8_tiles_slices(num_kv_heads, sms)) * num_kv_heads * 2 * kKv8TileRows : 0;
   s.tile_o = (s.tile_ml + tile_rows * sizeof(float2) + 255) / 256 * 256;
   s.bytes = s.tile_o + tile_rows * head_dim * sizeof(float);
   return s;
@@ -364,6 +367,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   p.qscale = scale * kLog2e;
   p.part_ml = reinterpret_cast<float2*>(ws + s.ml);
   p.part_o = reinterpret_cast<float*>(ws + s.o);
+  p.joins = reinterpret_cast<Kv8Join*>(ws + s.joins);
   // Small_max 0 with longer chunks: the first class is empty.
   const bool tiles = max_query_len > t.small_max, rows = t.small_max > 0 || !tiles;
   int32_t launched = 0;
@@ -383,6 +387,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     q.slices = kv8_tiles_slices(num_kv_heads, sms);
     q.part_ml = reinterpret_cast<float2*>(ws + s.tile_ml);
     q.part_o = reinterpret_cast<float*>(ws + s.tile_o);
+    q.joins = reinterpret_cast<Kv8Join*>(ws + s.tile_joins);
     q.first = !rows;
     if (f.pair) {  // the rows kernel's maps were of pairs
       st = payload_map(k_pool, pool_num_blocks, block_size, num_kv_heads, head_dim, &tk);
@@ -393,8 +398,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention tiles launch");
     launched |= PA_LAUNCH_KV8_TILES;
   }
-  if (rows) e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, err, stream);
-  if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, err, stream);
+  if (rows) e = launch_kv8_rows_combine(dtype, head_dim, f.row_groups, p, stream);
+  if (e == cudaSuccess && tiles) e = launch_kv8_tiles_combine(dtype, head_dim, q, stream);
   if (e != cudaSuccess) return kv8_cuda_fail(e, "8-bit attention join launch");
   if ((rows && p.slices > 1) || (tiles && q.slices > 1)) launched |= PA_LAUNCH_KV8_COMBINE;
   note_launches(launched);

@@ -55,6 +55,7 @@ struct LineCuts {
       rest = t % uint32_t(n);
     }
   }
+  __device__ __forceinline__ explicit LineCuts(const Kv8Join& j) : each(j.each), rest(j.rest), n(j.n) {}
   __device__ __forceinline__ int64_t at(int s) const { return each * s + rest * uint32_t(s) / uint32_t(n); }
 };
 
@@ -185,6 +186,19 @@ __device__ __forceinline__ bool line_next_piece(LineFinder& f, int64_t& x, int64
     if (d.k1 > d.k0) return true;
   }
   return false;
+}
+
+// Tile t, which starts in slice s and does not end there: at most one a slice, so whoever works
+// on it leaves word and nobody has to look for shared tiles.
+__device__ __forceinline__ Kv8Join line_join(const LineTile& t, const LineCuts& cuts, int s, int tile_tokens) {
+  const int64_t end = t.start + t.keys;
+  // The last slice with a part: the largest i with at(i) < end; slices differ by one key at
+  // most, so a guess by their length is next to it.
+  int last = min(s + 1 + int((end - cuts.at(s + 1)) / max(cuts.each, int64_t(1))), cuts.n - 1);
+  while (last + 1 < cuts.n && cuts.at(last + 1) < end) ++last;
+  while (last > s + 1 && cuts.at(last) >= end) --last;
+  const int t0 = t.index * tile_tokens;
+  return {t.start, cuts.each, cuts.rest, cuts.n, t.keys, t.first + t0, min(tile_tokens, t.q - t0), last};
 }
 
 }  // namespace pa

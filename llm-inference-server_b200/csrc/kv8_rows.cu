@@ -180,6 +180,8 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
   LineFinder finder(p, err);
   const int64_t total = finder.total;
   const LineCuts cuts(total, p.slices, rows_min_keys(RG));
+  const bool tells = warp == W && lane == 0 && kvh == 0;  // of the tile that its slice shares with the next ones
+  if (tells) p.joins[slice].tokens = 0;
   if (total == 0 || slice >= cuts.n) return;
 
   if (warp == W) {
@@ -243,6 +245,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
       }
       ++pieces;
       if (!more) break;
+      if (tells && at.k0 == 0 && at.k1 < t.keys) p.joins[slice] = line_join(t, cuts, slice, p.tile_tokens);
       const int32_t* row = p.tables + int64_t(t.seq) * p.table_stride;
       // Each lane looks after one of the next 32 blocks: its id is read two rounds ahead of the
       // round whose tiles are being issued, its scales one round; lanes then issue their own
@@ -633,40 +636,34 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
 }
 
-// Joins the partials of tiles that a cut fell into.  CTA (s, kvh, z): the tile that the end of
-// slice s falls into, if this is the first cut inside it, and some of its rows; a lane takes
-// D / 32 elements of a row.  What bounds it is latency (places, then (m, l), then
-// accumulators), so loads are kept in flight side by side: in small tiles, which a long
-// context leaves in many parts, the CTA's warps share out the parts of NR rows (BY_PARTS); in
-// 256-row tiles, of two or three parts, every warp has rows of its own, NR at a time.
-constexpr int kCombineWarps = 8;
+// Joins the partials of tiles that a cut fell into.  CTA (s, kvh, z): the shared tile that
+// starts in slice s, if there is one (the attention kernel left word), and some of its rows; a
+// lane takes D / 32 elements of a row.  What bounds it is latency (the tile, then (m, l), then
+// accumulators) and that most CTAs have nothing to do, so they learn that from one load; when
+// each looked its place up on the work line, one token over 517 keys took 11.5 us instead of
+// 9.4 and 64 x 4,096 keys 119 instead of 114.  In small tiles, which a long context leaves in
+// many parts, the CTA's warps share out the parts of kCombineRows rows (BY_PARTS); in 256-row
+// tiles every warp has rows of its own, as many at a time.  Four rows took 3 us more for 100
+// tokens over 4,000 keys and for 24 chunks of five over 6,000, one row 3 us more for 48 x 700.
+constexpr int kCombineWarps = 8, kCombineRows = 2;
 
-template <typename T, int D, int NR, bool BY_PARTS>
+template <typename T, int D, bool BY_PARTS>
 __global__ void __launch_bounds__(32 * kCombineWarps)
-    kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step, int min_keys, int* err) {
-  constexpr int E = D / 32, P = 2;
+    kv8_combine_kernel(const Kv8AttnParams p, int rows, int key_step) {
+  constexpr int E = D / 32, P = 2, NR = kCombineRows;
   __shared__ float s_acc[BY_PARTS ? kCombineWarps : 1][NR][D];
   __shared__ float2 s_ml[BY_PARTS ? kCombineWarps : 1][NR];
   pdl_wait();
   pdl_release();
-  LineFinder finder(p, err);
-  const int64_t total = finder.total;
-  const LineCuts cuts(total, p.slices, min_keys);
-  const int s = blockIdx.x + 1, kvh = blockIdx.y;
-  if (total == 0 || s >= cuts.n) return;
-  const int64_t x = cuts.at(s);
-  const LineTile t = finder.find(x);
-  if (x <= t.start || cuts.at(s - 1) > t.start) return;
-  if (line_key(t, x, key_step) >= t.keys) return;  // the first slice did the whole tile
+  const Kv8Join join = p.joins[blockIdx.x];
+  const int live = join.tokens * p.group;  // rows of the tile
+  if (live == 0) return;
+  const LineCuts cuts(join);
+  LineTile t{};
+  t.start = join.start;
+  t.keys = join.keys;
+  const int s = blockIdx.x + 1, kvh = blockIdx.y, last = join.last;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t end = t.start + t.keys;
-  // The last slice with a part of the tile: the largest i with at(i) < end; slices differ by
-  // one key at most, so a guess by their length is next to it.
-  int last = min(s + int((end - x) / max(cuts.each, int64_t(1))), cuts.n - 1);
-  while (last + 1 < cuts.n && cuts.at(last + 1) < end) ++last;
-  while (last > s && cuts.at(last) >= end) --last;
-  const int t0 = t.index * p.tile_tokens;
-  const int live = min(p.tile_tokens, t.q - t0) * p.group;  // rows of the tile
   constexpr int ROWS = BY_PARTS ? NR : kCombineWarps * NR;  // of the CTA at a time
   const int first_part = BY_PARTS ? warp : 0, part_step = BY_PARTS ? kCombineWarps : 1;
   for (int z0 = blockIdx.z * ROWS; z0 < live; z0 += ROWS * gridDim.z) {
@@ -761,7 +758,7 @@ __global__ void __launch_bounds__(32 * kCombineWarps)
     for (int n = 0; n < (BY_PARTS ? 1 : NR); ++n) {
       const int r = BY_PARTS ? r0 + warp : r0 + n, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
       if (r >= live || (BY_PARTS && warp >= NR)) break;
-      T* dst = static_cast<T*>(p.out) + int64_t(t.first + t0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
+      T* dst = static_cast<T*>(p.out) + int64_t(join.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + E * lane;
       const float inv = 1.f / sum[n];
 #pragma unroll
       for (int e = 0; e < E; e += 2)
@@ -821,30 +818,31 @@ cudaError_t launch_kv8_rows(int dtype, int head_dim, bool pair, int row_groups, 
 }
 
 template <typename T, int D>
-static cudaError_t combine_one(int rows, int key_step, int min_keys, const Kv8AttnParams& p, int* err,
-                               cudaStream_t stream) {
+static cudaError_t combine_one(int rows, int key_step, const Kv8AttnParams& p, cudaStream_t stream) {
   const int live = p.tile_tokens * p.group;
   const dim3 block(32 * kCombineWarps);
+  constexpr int kPerCta = kCombineWarps * kCombineRows;
   if (rows <= 8 * kKv8RowGroups)
-    return launch_pdl(kv8_combine_kernel<T, D, 4, true>, dim3(p.slices - 1, p.num_kv_heads, (live + 3) / 4), block, 0,
-                      stream, p, rows, key_step, min_keys, err);
-  return launch_pdl(kv8_combine_kernel<T, D, 4, false>, dim3(p.slices - 1, p.num_kv_heads, (live + 63) / 64), block, 0,
-                    stream, p, rows, key_step, min_keys, err);
+    return launch_pdl(kv8_combine_kernel<T, D, true>,
+                      dim3(p.slices - 1, p.num_kv_heads, (live + kCombineRows - 1) / kCombineRows), block, 0, stream, p,
+                      rows, key_step);
+  return launch_pdl(kv8_combine_kernel<T, D, false>,
+                    dim3(p.slices - 1, p.num_kv_heads, (live + kPerCta - 1) / kPerCta), block, 0, stream, p, rows, key_step);
 }
 
-cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, int min_keys, const Kv8AttnParams& p,
-                               int* err, cudaStream_t stream) {
+cudaError_t launch_kv8_combine(int dtype, int head_dim, int rows, int key_step, const Kv8AttnParams& p,
+                               cudaStream_t stream) {
   if (p.slices < 2) return cudaSuccess;
   if (dtype == PA_DTYPE_F16)
-    return head_dim == 64 ? combine_one<__half, 64>(rows, key_step, min_keys, p, err, stream)
-                          : combine_one<__half, 128>(rows, key_step, min_keys, p, err, stream);
-  return head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, min_keys, p, err, stream)
-                        : combine_one<__nv_bfloat16, 128>(rows, key_step, min_keys, p, err, stream);
+    return head_dim == 64 ? combine_one<__half, 64>(rows, key_step, p, stream)
+                          : combine_one<__half, 128>(rows, key_step, p, stream);
+  return head_dim == 64 ? combine_one<__nv_bfloat16, 64>(rows, key_step, p, stream)
+                        : combine_one<__nv_bfloat16, 128>(rows, key_step, p, stream);
 }
 
-cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p, int* err,
+cudaError_t launch_kv8_rows_combine(int dtype, int head_dim, int row_groups, const Kv8AttnParams& p,
                                     cudaStream_t stream) {
-  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, rows_min_keys(row_groups), p, err, stream);
+  return launch_kv8_combine(dtype, head_dim, 8 * row_groups, kRowsKeys, p, stream);
 }
 
 }  // namespace pa

@@ -200,7 +200,9 @@ __global__ void __launch_bounds__(kTileThreads, 1)
   LineFinder finder(p, err);
   const int64_t total = finder.total;
   const LineCuts cuts(total, p.slices, kTileMinKeys);
+  const bool tells = kvh == 0;  // of the tile that its slice shares with the next ones
   if (total == 0 || slice >= cuts.n) {
+    if (tid == 0 && tells) p.joins[slice].tokens = 0;
     pdl_wait();
     return;
   }
@@ -262,6 +264,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
       // ---------------------------------------------------------- pieces
       const int64_t x1 = cuts.at(slice + 1);
       int64_t x = cuts.at(slice);
+      if (lane == 0 && tells) p.joins[slice].tokens = 0;
       for (int k = 0;; ++k) {
         LinePiece at;
         const bool more = line_next_piece(finder, x, x1, kTileKeys, at);
@@ -284,6 +287,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           }
           desc[k & 1] = d;
           mbar_arrive(&bars->d_full[k & 1]);
+          if (d.part == 1 && tells) p.joins[slice] = line_join(at.t, cuts, slice, p.tile_tokens);
         }
         if (!more) break;
       }
@@ -783,8 +787,8 @@ cudaError_t launch_kv8_tiles(int dtype, int head_dim, const CUtensorMap& tk, con
                                : tiles_by_dim<__nv_bfloat16>(head_dim, tk, tv, p, err, stream);
 }
 
-cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, int* err, cudaStream_t stream) {
-  return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, kTileMinKeys, p, err, stream);
+cudaError_t launch_kv8_tiles_combine(int dtype, int head_dim, const Kv8AttnParams& p, cudaStream_t stream) {
+  return launch_kv8_combine(dtype, head_dim, kTileRows, kTileKeys, p, stream);
 }
 
 }  // namespace pa
