@@ -129,6 +129,15 @@ __device__ __forceinline__ uint32_t scale_h2(uint32_t b) {
   return h | (h << 16);
 }
 
+// A value that is the same in the whole warp, known to the compiler as such.
+__device__ __forceinline__ int warp_uniform(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(r));
+  return r != 0;
+}
+
 __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -152,7 +161,11 @@ struct WidenPart {
     for (int i = 0; i < N; ++i) {
       const int r = i * RPI + lane / LPR;
       x[i] = *reinterpret_cast<const uint4*>(staged + tile_at<D>(r, lane % LPR));
-      if (r >= live) x[i] = make_uint4(0, 0, 0, 0);
+    }
+    if (live < 16) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i * RPI + lane / LPR >= live) x[i] = make_uint4(0, 0, 0, 0);
     }
   }
 
@@ -252,8 +265,6 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     return ok;
   };
   auto is_twin = [&](const TilePiece& d) { return d.tokens * p.group <= kHalfRows; };
-  // Whether half h works on key tile j of a piece.
-  auto works = [](bool twin, int h, const TilePiece& d, int j) { return !twin || ((j - d.j0) & 1) == h; };
   // The second twin of a piece with one key tile: its query rows are not loaded and not waited for.
   auto is_idle = [](bool twin, int h, const TilePiece& d) { return twin && h == 1 && d.j1 - d.j0 < 2; };
 
@@ -361,89 +372,88 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
-    const int h = warp & 1;
-    const uint32_t tbase = bars->tmem_base + h * C::COL_HALF;
+    // These loops are written for uniform registers: what an MMA needs (its descriptors above
+    // all) is the same in the whole warp and known to be, and one elected thread issues.  With
+    // a loop of lane 0's alone an S of 8 MMAs was 150 instructions, each waiting for the last.
+    const int h = warp_uniform(warp) & 1;
+    const bool leader = elect_one();
+    const uint32_t tbase = warp_uniform(bars->tmem_base) + h * C::COL_HALF;
     const uint32_t tS = tbase, tO = tbase + C::COL_O;
     if (warp < 18) {
       // ---------------------------------------------------------- S issue of half h
-      int g = 0, n = 0, queries = 0;
+      constexpr uint32_t idS = idesc_f16<__half>(kHalfRows, kTileKeys, false);
+      const uint64_t q0 = smem_desc_sw128(smem_u32(smem + h * (C::Q_BYTES / 2)), 16, 1024);
+      const uint64_t k0 = smem_desc_sw128(smem_u32(sK), 16, 1024);
+      int s = 0, turn = 0, n = 0, queries = 0;  // K stage and its phase
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
-        if (!ok || d.row0 < 0) break;
-        const bool twin = is_twin(d);
-        if (lane == 0) {
-          constexpr uint32_t idS = idesc_f16<__half>(kHalfRows, kTileKeys, false);
-          const uint32_t q0 = smem_u32(smem + h * (C::Q_BYTES / 2));
-          if (!is_idle(twin, h, d) && !mbar_wait(&bars->q_full[h], queries++ & 1)) ok = false;
-          for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
-            const int s = g % kTileKStages;
-            if (!mbar_wait(&bars->k_full[s], (g / kTileKStages) & 1)) {
-              ok = false;
-              break;
-            }
-            if (!works(twin, h, d, j)) {
-              mbar_arrive(&bars->k_free[s]);
-              continue;
-            }
-            if (n >= 2 && !mbar_wait(&bars->s_free[h][n & 1], ((n >> 1) - 1) & 1)) {
-              ok = false;
-              break;
-            }
+        if (!ok || warp_uniform(d.row0) < 0) break;
+        const int tiles = warp_uniform(d.j1 - d.j0);
+        const bool twin = warp_uniform(d.tokens) * p.group <= kHalfRows;
+        if (!(twin && h == 1 && tiles < 2)) ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full[h], queries++ & 1));
+        for (int i = 0; i < tiles && ok; ++i) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->k_full[s], turn));
+          if (!ok) break;
+          if (twin && (i & 1) != h) {
+            if (leader) mbar_arrive(&bars->k_free[s]);
+          } else {
+            if (n >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_free[h][n & 1], ((n >> 1) - 1) & 1));
+            if (!ok) break;
             tc_fence_after();
-            const uint32_t k0 = smem_u32(sK + s * C::KV_BYTES);
+            const uint32_t to = tS + (n & 1) * kTileKeys;
+            const uint64_t kd = k0 + uint32_t(s * (C::KV_BYTES >> 4));
+            if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < D / 16; ++kk) {
-              const uint64_t ad = smem_desc_sw128(q0 + (kk >> 2) * kTileQBox + (kk & 3) * 32, 16, 1024);
-              const uint64_t bd = smem_desc_sw128(k0 + (kk >> 2) * kTileBox + (kk & 3) * 32, 16, 1024);
-              umma_f16(tS + (n & 1) * kTileKeys, ad, bd, idS, kk > 0 ? 1u : 0u);
+              for (int kk = 0; kk < D / 16; ++kk)
+                umma_f16(to, q0 + ((kk >> 2) * (kTileQBox >> 4) + (kk & 3) * 2),
+                         kd + ((kk >> 2) * (kTileBox >> 4) + (kk & 3) * 2), idS, kk > 0 ? 1u : 0u);
+              umma_commit(&bars->s_full[h][n & 1]);
+              umma_commit(&bars->k_free[s]);
             }
-            umma_commit(&bars->s_full[h][n & 1]);
-            umma_commit(&bars->k_free[s]);
             ++n;
           }
+          if (++s == kTileKStages) {
+            s = 0;
+            turn ^= 1;
+          }
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
     } else {
       // ---------------------------------------------------------- P.V issue of half h
+      constexpr uint32_t idO = idesc_f16<__half>(kHalfRows, D, true);
+      const uint64_t v0 = smem_desc_sw128(smem_u32(sV), kTileBox, 1024);
       int g = 0, n = 0;
       for (int k = 0; ok; ++k) {
         TilePiece d;
         ok = next_piece(k, d);
-        if (!ok || d.row0 < 0) break;
-        const bool twin = is_twin(d);
-        if (lane == 0) {
-          constexpr uint32_t idO = idesc_f16<__half>(kHalfRows, D, true);
-          bool first = true;
-          for (int j = d.j0; j < d.j1 && ok; ++j, ++g) {
-            const int s = g & 1, b = n & 1;
-            if (!mbar_wait(&bars->v_full[s], (g >> 1) & 1)) {
-              ok = false;
-              break;
-            }
-            if (!works(twin, h, d, j)) {
-              mbar_arrive(&bars->v_free[s]);
-              continue;
-            }
-            if (!mbar_wait(&bars->p_full[h][b], (n >> 1) & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint32_t v0 = smem_u32(sV + s * C::KV_BYTES);
+        if (!ok || warp_uniform(d.row0) < 0) break;
+        const int tiles = warp_uniform(d.j1 - d.j0);
+        const bool twin = warp_uniform(d.tokens) * p.group <= kHalfRows;
+        uint32_t accumulate = 0;
+        for (int i = 0; i < tiles && ok; ++i, ++g) {
+          const int s = g & 1, b = n & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->v_full[s], (g >> 1) & 1));
+          if (!ok) break;
+          if (twin && (i & 1) != h) {
+            if (leader) mbar_arrive(&bars->v_free[s]);
+            continue;
+          }
+          ok = __all_sync(0xffffffffu, mbar_wait(&bars->p_full[h][b], (n >> 1) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          const uint32_t from = tS + b * kTileKeys;
+          const uint64_t vd = v0 + uint32_t(s * (C::KV_BYTES >> 4));
+          if (leader) {
 #pragma unroll
-            for (int kk = 0; kk < kTileKeys / 16; ++kk) {
-              const uint64_t bd = smem_desc_sw128(v0 + kk * 2048, kTileBox, 1024);
-              umma_f16_ts(tO, tS + b * kTileKeys + 8 * kk, bd, idO, (!first || kk > 0) ? 1u : 0u);
-            }
+            for (int kk = 0; kk < kTileKeys / 16; ++kk)
+              umma_f16_ts(tO, from + 8 * kk, vd + kk * (2048 >> 4), idO, kk > 0 ? 1u : accumulate);
             umma_commit(&bars->s_free[h][b]);
             umma_commit(&bars->v_free[s]);
-            first = false;
-            ++n;
           }
+          accumulate = 1;
+          ++n;
         }
-        ok = __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
       }
     }
   } else if (warp >= 8) {
