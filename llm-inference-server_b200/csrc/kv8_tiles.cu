@@ -145,48 +145,63 @@ __device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
 }
 
 // A widening warp's 16 keys of a staged 64-key tile: read into registers, then widened into the
-// swizzled tile.  Lanes take 16-byte chunks, D / 16 lanes a row.
+// swizzled tile.  A lane takes a 16-byte chunk of N rows, D / 16 lanes a row.  With 128 dims the
+// eight lanes that one access serves at a time hold half of two rows that differ in bits 0 and
+// 2: their chunks then lie in different banks both where they are read and where they are
+// written, though a row's two 64-column boxes map to the same banks.  (Whole rows in order with
+// half of the lanes storing their second chunk first cost eight selects a row: 5 % of all
+// instructions.)
 template <int D>
 struct WidenPart {
-  static constexpr int LPR = D / 16;      // lanes a row
-  static constexpr int RPI = 32 / LPR;    // rows an instruction
-  static constexpr int N = 16 / RPI;      // instructions
+  static constexpr int N = D / 32;        // rows of a lane: 16 rows x D / 16 chunks over 32 lanes
   uint4 x[N];
   uint32_t scale;                         // of key `lane`, lanes 0-15
+  uint32_t from[2], to[2];                // of the lane's first two rows: chunk read, first chunk written
+  int row;                                // the first; the i-th is row_at(i)
+
+  __device__ __forceinline__ int row_at(int i) const {
+    return D == 128 ? (row ^ (4 * (i & 1))) + 8 * (i >> 1) : row + 8 * i;
+  }
+  __device__ __forceinline__ explicit WidenPart(int lane, int row0) {
+    const int l2 = (lane >> 2) & 1, l3 = (lane >> 3) & 1, l4 = lane >> 4;
+    row = D == 128 ? 5 * l2 + 2 * l4 : lane / 4;
+    const int chunk = D == 128 ? (lane & 3) + 4 * l3 : lane & 3;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      from[i] = tile_at<D>(row0 + row_at(i), chunk);
+      to[i] = (chunk >> 2) * kTileBox + sw_off(row0 + row_at(i), 2 * (chunk & 3));
+    }
+  }
+  // Rows i and i + 2 differ in bit 3, which no swizzle looks at.
+  __device__ __forceinline__ static uint32_t later(int i, int row_bytes) { return uint32_t(8 * row_bytes * (i >> 1)); }
 
   // Rows at and past `live` (behind the context) read as zeros.
   __device__ __forceinline__ void read(const uint8_t* staged, const uint8_t* scales, int lane, int live) {
-    scale = lane < min(16, live) ? scales[lane] : 0u;
+    scale = scales[lane & 15];
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int r = i * RPI + lane / LPR;
-      x[i] = *reinterpret_cast<const uint4*>(staged + tile_at<D>(r, lane % LPR));
-    }
+    for (int i = 0; i < N; ++i) x[i] = *reinterpret_cast<const uint4*>(staged + from[i & 1] + later(i, D));
     if (live < 16) {
+      if (lane >= live) scale = 0u;
 #pragma unroll
       for (int i = 0; i < N; ++i)
-        if (i * RPI + lane / LPR >= live) x[i] = make_uint4(0, 0, 0, 0);
+        if (row_at(i) >= live) x[i] = make_uint4(0, 0, 0, 0);
     }
   }
 
   // V's rows that stand for NaN are widened to zeros (the softmax puts the NaN in the weight).
-  __device__ __forceinline__ void store(uint8_t* tile, int row0, int lane, bool is_v) {
+  __device__ __forceinline__ void store(uint8_t* tile, bool is_v) const {
     const uint32_t s2 = is_v && scale == 255u ? 0u : scale_h2(scale);
-    const int q = lane % LPR, box = D == 128 ? q >> 2 : 0, c0 = 2 * (q & 3);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const int r = i * RPI + lane / LPR, row = row0 + r;
-      const uint32_t sc = __shfl_sync(0xffffffffu, s2, r);
+      const uint32_t sc = __shfl_sync(0xffffffffu, s2, row_at(i));
       const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-      uint4 o[2];
-      o[0] = make_uint4(mul_h2(widen_lo(w[0]), sc), mul_h2(widen_hi(w[0]), sc), mul_h2(widen_lo(w[1]), sc),
-                        mul_h2(widen_hi(w[1]), sc));
-      o[1] = make_uint4(mul_h2(widen_lo(w[2]), sc), mul_h2(widen_hi(w[2]), sc), mul_h2(widen_lo(w[3]), sc),
-                        mul_h2(widen_hi(w[3]), sc));
-      // The two 64-column boxes of a row map to the same banks: the second goes odd chunk first.
-      uint8_t* dst = tile + box * kTileBox;
-      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + box)) = box ? o[1] : o[0];
-      *reinterpret_cast<uint4*>(dst + sw_off(row, c0 + 1 - box)) = box ? o[0] : o[1];
+      uint8_t* dst = tile + later(i, 128);
+      *reinterpret_cast<uint4*>(dst + to[i & 1]) =
+          make_uint4(mul_h2(widen_lo(w[0]), sc), mul_h2(widen_hi(w[0]), sc), mul_h2(widen_lo(w[1]), sc),
+                     mul_h2(widen_hi(w[1]), sc));
+      *reinterpret_cast<uint4*>(dst + (to[i & 1] ^ 16)) =
+          make_uint4(mul_h2(widen_lo(w[2]), sc), mul_h2(widen_hi(w[2]), sc), mul_h2(widen_lo(w[3]), sc),
+                     mul_h2(widen_hi(w[3]), sc));
     }
   }
 };
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   bool ok = true;
   if (warp >= 20) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 22) {
       // ---------------------------------------------------------- pieces
       const int64_t x1 = cuts.at(slice + 1);
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = max(0, n - kTileRing); i < n; ++i) mbar_wait(&bars->st_full[v][i % kTileRing], (i / kTileRing) & 1);
     }
   } else if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
     // These loops are written for uniform registers: what an MMA needs (its descriptors above
     // all) is the same in the whole warp and known to be, and one elected thread issues.  With
     // a loop of lane 0's alone an S of 8 MMAs was 150 instructions, each waiting for the last.
@@ -463,12 +478,12 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     const int stages = v ? kTileVStages : kTileKStages;
     uint64_t* full = v ? bars->v_full : bars->k_full;
     uint64_t* freed = v ? bars->v_free : bars->k_free;
-    const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES + row0 * D;
+    const uint8_t* ring = smem + C::OFF_ST + v * kTileRing * C::ST_BYTES;
     const uint8_t* scale_ring = smem + C::OFF_SCALE + (v ? 2 * kTileRing * kTileKeys : 0) + row0;
     const int scale_step = v ? kTileKeys : 2 * kTileKeys;
     uint8_t* out = v ? sV : sK;
     int n = 0, s = 0, round = 0;
-    WidenPart<D> part;
+    WidenPart<D> part(lane, row0);
     for (int k = 0; ok; ++k) {
       TilePiece d;
       ok = next_piece(k, d);
@@ -486,7 +501,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
           const uint32_t nans = __ballot_sync(0xffffffffu, lane < min(16, live) && sc[kTileKeys + lane] == 255);
           if (lane == 0) nan_rows[4 * (n % kTileNanRing) + (warp & 3)] = uint16_t(nans);
         }
-        part.store(out + s * C::KV_BYTES, row0, lane, v != 0);
+        part.store(out + s * C::KV_BYTES, v != 0);
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
@@ -501,7 +516,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax (one row per thread)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 128;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
     const int h = warp >> 2;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
