@@ -132,7 +132,7 @@ class DeviceStep:
     @property
     def _arrays(self) -> tuple[torch.Tensor, ...]:
         if self._views is None:
-            self._views = torch.split_with_sizes(self.buffer, self._sizes)
+            self._views = torch.unsafe_split_with_sizes(self.buffer, self._sizes)  # int32: autograd has no say
         return self._views
 
     work = property(lambda self: self._arrays[0].view(torch.int64).view(2, self.num_seqs + 1))
@@ -437,7 +437,8 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if query.dtype not in (torch.float16, torch.bfloat16):
         raise NotImplementedError(f"ATTENTION=cuda: the 8-bit cache takes float16 and bfloat16 queries, not {query.dtype}")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=query.dtype, device=dev)
+        out = (torch.empty_like(query) if query.is_contiguous() else
+               torch.empty((tokens, heads, dim), dtype=query.dtype, device=dev))
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError("out must be contiguous with the query's shape, dtype and device")
     group = heads // hkv
