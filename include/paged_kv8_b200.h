@@ -40,7 +40,7 @@ extern "C" {
 /* Further bits of pa_last_launches(). */
 #define PA_LAUNCH_KV8_ROWS 128    /* KV8 attention, few rows per sequence (mma.sync) */
 #define PA_LAUNCH_KV8_COMBINE 256 /* join of tiles that several CTAs worked on */
-#define PA_LAUNCH_KV8_TILES 512   /* KV8 attention, 128-row tiles (tcgen05) */
+#define PA_LAUNCH_KV8_TILES 512   /* KV8 attention, 256-row tiles (tcgen05) */
 
 /* Most rows (sequences) of a step and most request slots of a table set. */
 #define PA_KV8_MAX_ROWS 4096
@@ -49,7 +49,7 @@ extern "C" {
 /*
  * How attention cuts a step into work: sequences of at most `small_max` new tokens are cut
  * into tiles of `small_tokens` tokens (the kernel for few rows), longer ones into tiles of
- * `large_tokens` (the tensor-memory kernel).  A step's `work` array holds, for each class,
+ * `large_tokens` (the tensor-memory kernel); small_max 0: all of them.  A step's `work` array holds, for each class,
  * the running sum over sequences of the keys that their tiles visit.
  */
 typedef struct pa_kv8_tiling {

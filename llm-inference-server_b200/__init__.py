@@ -23,8 +23,8 @@ The directory name is not a Python identifier; the package is imported under the
 from __future__ import annotations
 
 from .attention import paged_attention, paged_attention_cuda, read_device_error
-from .kv8 import (DeviceBlockTables, DeviceStep, KV8Pool, device_step, paged_attention_kv8, read_kv8_error,
-                  reshape_and_cache_kv8)
+from .kv8 import (DeviceBlockTables, DeviceStep, KV8Pool, attach_step, device_step, paged_attention_kv8,
+                  read_kv8_error, reshape_and_cache_kv8)
 from .kv_cache import HostBlocks, KVPool, allocate_pool, copy_blocks, reshape_and_cache
 from .metadata import StepMetadata, attach, attached, prefill_tile_tokens
 
@@ -47,5 +47,6 @@ __all__ = [
     "DeviceBlockTables",
     "DeviceStep",
     "device_step",
+    "attach_step",
     "read_kv8_error",
 ]

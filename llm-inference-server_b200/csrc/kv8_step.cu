@@ -10,7 +10,9 @@
 // most) and a grid-wide wait or a second launch costs more than the sums, so every CTA
 // computes them for itself in shared memory and then fills its share of the tables and of
 // the per-token arrays; no CTA reads what another writes (a new block's id comes from the
-// free list by arithmetic, not from the table that it is also written to).
+// free list by arithmetic, not from the table that it is also written to).  What bounds it is
+// latency, of the lengths' loads and of the scan: 8 rows 6.2 us, 500 rows with 2.6 MB of tables
+// 10.3.
 #include "kv8.h"
 #include "kv8_launch.cuh"
 #include "kv8_line.cuh"

@@ -38,13 +38,21 @@
 // A piece of at most 128 rows runs as twins: both halves hold the same rows and take every
 // other key tile, each with its own maximum, sum and accumulator; at the end the first half's
 // threads read the second's accumulator (the same TMEM lanes, other columns) and join them.
-// What bounds a half is the chain scores -> softmax -> P V -> buffer free of one tile (about
-// 2 us over two buffers), not arithmetic, so two chains do almost twice the keys.
+// What bounds a half is the chain of one row's softmax (1 us a tile: 64 exponentials among 240
+// instructions that wait for one another), not a unit's rate, so two chains do almost twice the
+// keys.
 //
 // The staging rings are what the widening needs: with a tile's loads in registers, one tile
 // ahead, 128-row tiles and two CTAs per SM the loads' latency (over 1 us per tile) was
 // exposed and 1,000 tokens over 16,384 keys took 546 us; without any loads the same kernel
 // took 291, without widening 254.
+//
+// Measured with the join (32 query heads, 8 KV heads of 128): 1,000 tokens over 16,384 keys 264 us
+// (987 TFLOP/s, 59 % of the measured bf16 GEMM rate; floor 157), 13 x 2,047 tokens 612, 30 tokens
+// over 100,000 keys 82, a prompt of 333 tokens 26.  A tile of 64 keys takes 1.1 us, the softmax's
+// chain; the tensor pipe is busy 53 % of the time, the exponential unit 50 %, issue slots 58 %.
+// What did not help: two threads per row (a meeting of two warps a tile, 1.2 times the
+// instructions: 297 us), turns at the exponential unit (277), 16 widening warps (281).
 //
 // Every mbarrier wait is bounded; the TMEM allocation is released on every path.
 #include <cuda_fp16.h>
@@ -66,6 +74,10 @@ constexpr int kTileKStages = 3;
 constexpr int kTileVStages = 2;  // equal to the P buffer count: one "P.V retired" barrier frees both
 constexpr int kTileRing = 4;     // staged e4m3 tiles, K and V each
 constexpr int kTileThreads = 768;
+// Registers a thread: at launch and by role.  What the softmax takes, the others have given back.
+constexpr int kTileRegs = 80, kSoftmaxRegs = 136, kWidenRegs = 64, kIssueRegs = 32, kLoadRegs = 48;
+static_assert(256 * (kSoftmaxRegs + kWidenRegs) + 128 * (kIssueRegs + kLoadRegs) <= kTileThreads * kTileRegs,
+              "a share above the launch's would be waited for");
 constexpr int kTileQBox = kHalfRows * 128;  // 128 rows x 64 elements, 128-byte swizzle
 constexpr int kTileBox = kTileKeys * 128;   // 64 keys x 64 elements
 constexpr int kTileConsumers = 22;          // warps that read a piece: 8 softmax, 8 widening, 4 issuers, 2 producers
@@ -285,7 +297,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
 
   bool ok = true;
   if (warp >= 20) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kLoadRegs));
     if (warp == 22) {
       // ---------------------------------------------------------- pieces
       const int64_t x1 = cuts.at(slice + 1);
@@ -386,7 +398,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         for (int i = max(0, n - kTileRing); i < n; ++i) mbar_wait(&bars->st_full[v][i % kTileRing], (i / kTileRing) & 1);
     }
   } else if (warp >= 16) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 32;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
     // These loops are written for uniform registers: what an MMA needs (its descriptors above
     // all) is the same in the whole warp and known to be, and one elected thread issues.  With
     // a loop of lane 0's alone an S of 8 MMAs was 150 instructions, each waiting for the last.
@@ -473,7 +485,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else if (warp >= 8) {
     // ------------------------------------------------------------ widening: warps 8-11 K, 12-15 V
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWidenRegs));
     const int v = warp >= 12 ? 1 : 0, row0 = 16 * (warp & 3);
     const int stages = v ? kTileVStages : kTileKStages;
     uint64_t* full = v ? bars->v_full : bars->k_full;
@@ -516,7 +528,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax (one row per thread)
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 136;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int h = warp >> 2;
     const uint32_t lane_base = uint32_t((warp & 3) * 32) << 16;
     const uint32_t tbase = bars->tmem_base + h * C::COL_HALF + lane_base;
@@ -790,6 +802,10 @@ static cudaError_t tiles_one(const CUtensorMap& tk, const CUtensorMap& tv, const
     if (e != cudaSuccess) return e;
     e = cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     if (e != cudaSuccess) return e;
+    cudaFuncAttributes built;
+    e = cudaFuncGetAttributes(&built, kern);
+    if (e != cudaSuccess) return e;
+    if (built.numRegs < kTileRegs) return cudaErrorInvalidConfiguration;  // see kTileRegs
     configured[dev] = true;
   }
   return launch_pdl(kern, dim3(p.slices * p.num_kv_heads), dim3(kTileThreads), C::SMEM, stream, tk, tv, p, err);
