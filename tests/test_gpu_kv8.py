@@ -685,6 +685,48 @@ def test_a_captured_call_follows_the_lengths(pkg):
             assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("n,most,hq,hkv,d", [(1, 300, 8, 2, 128), (3, 70, 4, 4, 64), (40, 33, 6, 2, 128)])
+@pytest.mark.parametrize("attached", [False, True])
+def test_a_captured_call_without_room_for_short_chunks_gets_some(pkg, n, most, hq, hkv, d, attached):
+    """Sizes that leave the kernel for few rows out, then lengths below them: single tokens,
+    empty sequences, contexts that several CTAs share, twins of one key tile."""
+    assert pkg.kv8._tiling(hq // hkv, most, n, n * most).small_max == 0
+    query, pools, tables, _, _ = _batch([(3000, most)] * n, hq, hkv, d, 16, torch.float16, seed=51)
+    k, v = (ref.dequantise(pools[i].view(torch.uint8), pools[i + 2]) for i in (0, 1))
+    ctx, ql = _i32([3000] * n), _i32([most] * n)
+    out = torch.zeros_like(query)
+    step = pkg.device_step(tables, ctx, ql, num_tokens=n * most, max_query_len=most, num_blocks=pools[0].shape[0],
+                           block_size=16, group=hq // hkv)
+
+    def call():
+        if attached:
+            pkg.device_step(tables, ctx, ql, num_tokens=n * most, max_query_len=most, num_blocks=pools[0].shape[0],
+                            block_size=16, group=hq // hkv, out=step)
+        return pkg.paged_attention_kv8(query, *pools, pkg.attach_step(tables.view_as(tables), step) if attached else tables,
+                                       ctx, ql, 0.1, max_query_len=most, out=out)
+
+    call()
+    torch.cuda.synchronize()
+    assert "kv8_rows" not in pkg._lib.last_launches()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    cycle = [[(3000, most)], [(1, 1), (2999, 1), (0, 0)], [(most + 40, most), (64, 2), (130, 17), (0, 0)], [(1500, most), (65, 1)]]
+    for pairs in cycle:
+        pairs = (pairs * n)[:n]
+        ctx.copy_(_i32([c for c, _ in pairs]))
+        ql.copy_(_i32([q for _, q in pairs]))
+        out.fill_(9.0)
+        graph.replay()
+        t = sum(q for _, q in pairs)
+        want, mean, slip = ref.attention(query[:t], k, v, tables, ctx.tolist(), ql.tolist(), 0.1)
+        tol = ref.tolerance(want, mean, slip, torch.float16, d, 3000)
+        assert ((out[:t].double() - want).abs() <= tol).all()
+        assert (out[t:] == 9.0).all()
+
+
 def test_calls_on_two_streams_at_once(pkg):
     a = _batch([(900, 2), (4000, 1)], 8, 2, 128, 16, torch.bfloat16, seed=41)
     b = _batch([(700, 90), (33, 33)], 8, 2, 128, 16, torch.float16, seed=42)
