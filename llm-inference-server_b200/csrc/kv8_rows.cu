@@ -38,8 +38,8 @@
 //
 // Measured with the join (8 heads of 128 and 32 query heads; floors at 6,535 GB/s): 64 x ~4,096
 // keys 114 us (floor 98), 131,071 keys 55 (41): a slice of 2,400 keys, of which the first loads
-// and the join are 12 us; 517 keys 9.3, all of it launches, first loads and the join; 24 chunks
-// of five over ~6,000 keys 108 (50), bound by the latency of the consumers' arithmetic (20 rows,
+// and the join are 12 us; 517 keys 9.1, all of it launches, first loads and the join; 24 chunks
+// of five over ~6,000 keys 103 (50), bound by the latency of the consumers' arithmetic (20 rows,
 // two CTAs an SM); 48 x ~700 keys of 12 heads of 64, one query head each, 27 (9).
 #include <cuda_fp16.h>
 
@@ -335,17 +335,23 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
     if (d.row0 < 0) break;
 
     // Queries as B fragments in shared memory: row r = (token r / group, head r % group),
-    // brought into fp16 by a power of two; a warp takes a row.
-    for (int r = warp; r < 8 * RG; r += W) {
-      const int tok = r / p.group, head = r - tok * p.group;
-      constexpr int E = DO / 32;
-      float x[E];
+    // brought into fp16 by a power of two; a warp takes a row at a time, all of its rows' loads
+    // (spare rows repeat the last token) before the first is used: one after the other cost
+    // 1,000 clocks a row, with three groups 3 us a piece (100 chunks of five over ~300 keys 70 : 65 us).
+    constexpr int E = DO / 32, PER = 8 * RG / W;
+    static_assert(PER * W == 8 * RG, "rows a warp");
+    float xs[PER][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[e] = 0.f;
-      if (tok < d.tokens)
-        VecLoad<T, E>::run(static_cast<const T*>(p.q) + int64_t(d.row0 + tok) * p.q_st +
-                               int64_t(kvh * p.group + head) * p.q_sh + E * lane,
-                           x);
+    for (int i = 0; i < PER; ++i) {
+      const int r = warp + W * i, tok = r / p.group, head = r - tok * p.group;
+      VecLoad<T, E>::run(static_cast<const T*>(p.q) + int64_t(d.row0 + min(tok, d.tokens - 1)) * p.q_st +
+                             int64_t(kvh * p.group + head) * p.q_sh + E * lane,
+                         xs[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = warp + W * i, tok = r / p.group, head = r - tok * p.group;
+      const float(&x)[E] = xs[i];
       float big = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) big = fmaxf(big, fabsf(x[e]));
@@ -592,28 +598,41 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
           o[c][rg][2 + e] *= f;
         }
       }
-    auto put = [&](int half) {
+    // Halves of the dims go to the neighbour, then quarters to the other pair, so that all four
+    // warps add and store: with a tree that ends in one warp, 100 chunks of five tokens over
+    // about 300 keys took 78 us instead of 70.
+    static_assert(W == 4, "two exchanges");
+    constexpr int H = CH / 2, Q4 = CH / 4, N4 = 4 * RG;
+    constexpr int STEP = W * H * N4 <= C::MERGES * C::NO ? H : Q4;  // chunks an exchange has room for
+    const bool odd = warp & 1, upper = warp & 2;
+    float two[H][N4], all4[Q4][N4];  // sums of two warps, of all
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+    for (int c0 = 0; c0 < H; c0 += STEP) {
 #pragma unroll
-        for (int e = 0; e < 4 * RG; ++e) merge[(half * C::NO + c * 4 * RG + e) * 32 + lane] = o[c][e / 4][e % 4];
-    };
-    auto add = [&](int half) {
+      for (int c = 0; c < STEP; ++c)
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
-#pragma unroll
-        for (int e = 0; e < 4 * RG; ++e) o[c][e / 4][e % 4] += merge[(half * C::NO + c * 4 * RG + e) * 32 + lane];
-    };
-#pragma unroll
-    for (int left = W; left > 1;) {  // the last `moved` of the warps left hand theirs to the first
-      const int moved = left / 2 < C::MERGES ? left / 2 : C::MERGES;
-      if (warp >= left - moved && warp < left) put(warp - (left - moved));
+        for (int e = 0; e < N4; ++e)
+          merge[((warp * STEP + c) * N4 + e) * 32 + lane] = odd ? o[c0 + c][e / 4][e % 4] : o[H + c0 + c][e / 4][e % 4];
       rows_sync<W>();
-      if (warp < moved) add(warp);
-      left -= moved;
-      if (left > 1) rows_sync<W>();
+#pragma unroll
+      for (int c = 0; c < STEP; ++c)
+#pragma unroll
+        for (int e = 0; e < N4; ++e)
+          two[c0 + c][e] = (odd ? o[H + c0 + c][e / 4][e % 4] : o[c0 + c][e / 4][e % 4]) +
+                           merge[(((warp ^ 1) * STEP + c) * N4 + e) * 32 + lane];
+      rows_sync<W>();
     }
-    if (warp != 0) continue;
+#pragma unroll
+    for (int c = 0; c < Q4; ++c)
+#pragma unroll
+      for (int e = 0; e < N4; ++e) merge[((warp * Q4 + c) * N4 + e) * 32 + lane] = upper ? two[c][e] : two[Q4 + c][e];
+    rows_sync<W>();
+#pragma unroll
+    for (int c = 0; c < Q4; ++c)
+#pragma unroll
+      for (int e = 0; e < N4; ++e)
+        all4[c][e] = (upper ? two[Q4 + c][e] : two[c][e]) + merge[(((warp ^ 2) * Q4 + c) * N4 + e) * 32 + lane];
+    const int chunk0 = (odd ? H : 0) + (upper ? Q4 : 0);
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
@@ -621,22 +640,21 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
         const int r = 8 * rg + 2 * tig + e, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
         if (tok >= d.tokens) continue;
         const float f = (d.part < 0 ? 1.f / l[rg][e] : 1.f) * (1.f / kWeightShift);
-        const bool second = PAIR && own[rg][e] != 0;  // its head's dims are the second 64
         const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
         T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 2 * g;
+        // With PAIR a row's dims are its own head's, the first 64 or the second.
+        if (!PAIR || (own[rg][e] != 0) == odd) {
 #pragma unroll
-        for (int c = 0; c < DO / 16; ++c) {
-          float x = o[c][rg][e], y = o[c][rg][2 + e];
-          if (PAIR && second) {
-            x = o[(c + 4) % CH][rg][e];
-            y = o[(c + 4) % CH][rg][2 + e];
+          for (int c = 0; c < Q4; ++c) {
+            const int chunk = PAIR ? (chunk0 + c) % H : chunk0 + c;
+            const float x = all4[c][4 * rg + e] * f, y = all4[c][4 * rg + 2 + e] * f;
+            if (d.part < 0)
+              *reinterpret_cast<uint32_t*>(dst + 16 * chunk) = pack2<T>(x, y);
+            else
+              *reinterpret_cast<float2*>(p.part_o + at * DO + 16 * chunk + 2 * g) = make_float2(x, y);
           }
-          if (d.part < 0)
-            *reinterpret_cast<uint32_t*>(dst + 16 * c) = pack2<T>(x * f, y * f);
-          else
-            *reinterpret_cast<float2*>(p.part_o + at * DO + 16 * c + 2 * g) = make_float2(x * f, y * f);
         }
-        if (d.part >= 0 && g == 0) p.part_ml[at] = make_float2(big[rg][e], l[rg][e]);
+        if (warp == 0 && d.part >= 0 && g == 0) p.part_ml[at] = make_float2(big[rg][e], l[rg][e]);
       }
   }
   if (!ok && lane == 0) set_error(err, PA_KV8_ERR_TIMEOUT);
