@@ -140,7 +140,7 @@ uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t nu
  * tables stay on the device; the launches depend on the host's sizes only, so a captured
  * call can be replayed with other lengths.  cu_query_lens and work come from
  * pa_kv8_build_step with the tiling of the same group, sizes and max_query_len; with both NULL
- * the call sums query_lens and the work up by itself (over 32 sequences in one more launch),
+ * the call sums query_lens and the work up by itself (over 64 sequences in one more launch),
  * with pa_kv8_build_step's checks.  table_width blocks of a table row are used.  Rows past the
  * last sequence's are left as they were.  head_dim 64 or 128, block_size a power of two
  * times 16, query fp16 or bf16 (strides in elements, multiples of 8; rows 16-byte aligned).

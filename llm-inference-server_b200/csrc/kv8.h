@@ -31,6 +31,8 @@ struct Kv8AppendParams {
   bool vec16;  // every row starts on a 16-byte boundary
 };
 
+constexpr int kKv8Direct = 64;  // sequences up to which attention sums a step up for itself
+
 // A tile that slices share: what joins its partials has to know.
 struct Kv8Join {
   int64_t start, each;  // the tile's place on the work line; the line's cuts

@@ -320,7 +320,7 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
     b.tiling = t;
     st = check_step_sizes(b, table_stride);
     if (st != PA_OK) return st;
-    if (num_seqs > 32) {  // up to 32 the kernels sum up for themselves
+    if (num_seqs > kKv8Direct) {  // fewer the kernels sum up for themselves
       b.cu_query = reinterpret_cast<int32_t*>(ws + s.cu);
       b.work = reinterpret_cast<int64_t*>(ws + s.work);
       const cudaError_t eb = launch_kv8_step(b, err, stream);

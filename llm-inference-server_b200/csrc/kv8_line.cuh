@@ -72,8 +72,11 @@ __device__ __forceinline__ int line_key(const LineTile& t, int64_t x, int step) 
 // in one go, before the first place is even known, and enough for any batch of up to 32
 // sequences and for walking from a sequence to the next.
 //
-// Without a step's sums (p.work NULL, at most 32 sequences) every warp makes them from the
-// lengths by a scan over its lanes, with the step kernel's checks: cheaper than a launch.
+// Without a step's sums (p.work NULL, at most kKv8Direct sequences) every warp makes them from
+// the lengths by scans over its lanes, with the step kernel's checks: with a launch for them
+// 48 x ~700 keys took 26.7 us instead of 23.7, 50 chunks of 50 over ~700 95 instead of 90.  A
+// lane then has two sequences, i and i + 32; places only grow, so the second 32 take the
+// first's registers when a place lies behind those.
 struct LineFinder {
   const int64_t* work;
   const int32_t *ctx_lens, *cu_q;
@@ -81,6 +84,8 @@ struct LineFinder {
   int64_t total;       // keys on the line
   int64_t begin, end;  // of the lane's sequence on the line
   int first, next, ctx;
+  int64_t begin2, end2;  // without a step's sums: of sequence 32 + lane
+  int first2, next2, ctx2;
 
   __device__ __forceinline__ void load(int from) {
     hint = from;
@@ -101,14 +106,41 @@ struct LineFinder {
     }
     hint = 0;
     const int lane = threadIdx.x & 31;
-    int q = 0;
-    ctx = 0;
+    int q = 0, q2 = 0;
+    ctx = ctx2 = 0;
     if (lane < num_seqs) {
       ctx = ctx_lens[lane];
       q = p.query_lens[lane];
     }
-    const bool bad = q < 0 || q > p.max_query_len || ctx < q || ctx > p.max_context;
-    if (bad) q = ctx = 0;
+    if (lane + 32 < num_seqs) {
+      ctx2 = ctx_lens[lane + 32];
+      q2 = p.query_lens[lane + 32];
+    }
+    bool bad = false;
+    const int n1 = sum_up(p, q, 0, 0, begin, end, first, next, ctx, bad);
+    total = __shfl_sync(0xffffffffu, end, 31);
+    int n2 = n1;
+    if (num_seqs > 32) {
+      n2 = sum_up(p, q2, total, n1, begin2, end2, first2, next2, ctx2, bad);
+      total = __shfl_sync(0xffffffffu, end2, 31);
+    }
+    // 64 chunks of at most 2^20 tokens: the sum fits 32 bits.
+    if (__any_sync(0xffffffffu, bad) || n2 > p.num_tokens) {
+      total = 0;
+      if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) set_error(err, PA_KV8_ERR_STEP);
+    }
+  }
+
+  // The sums of 32 sequences, the lane's with q new tokens and ctx keys, behind `keys0` keys and
+  // `tokens0` tokens; gives the tokens of all so far.
+  __device__ __forceinline__ static int sum_up(const Kv8AttnParams& p, int q, int64_t keys0, int tokens0,
+                                               int64_t& begin, int64_t& end, int& first, int& next, int& ctx,
+                                               bool& bad) {
+    const int lane = threadIdx.x & 31, tt = p.tile_tokens;
+    if (q < 0 || q > p.max_query_len || ctx < q || ctx > p.max_context) {
+      bad = true;
+      q = ctx = 0;
+    }
     const bool mine = (q <= p.small_max) == p.few;
     const int64_t keys = q > 0 && mine ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
     next = q;
@@ -122,21 +154,26 @@ struct LineFinder {
         end += up_keys;
       }
     }
+    next += tokens0;
+    end += keys0;
     first = next - q;
     begin = end - keys;
-    total = __shfl_sync(0xffffffffu, end, 31);
-    // 32 chunks of at most 2^20 tokens: the sum fits 32 bits.
-    if (__any_sync(0xffffffffu, bad) || __shfl_sync(0xffffffffu, next, 31) > p.num_tokens) {
-      total = 0;
-      if (blockIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0) set_error(err, PA_KV8_ERR_STEP);
-    }
+    return __shfl_sync(0xffffffffu, next, 31);
   }
 
   // The tile that holds place x, with work[hint] <= x < total.
   __device__ __forceinline__ LineTile find(int64_t x) {
     const int lane = threadIdx.x & 31;
     unsigned above = __ballot_sync(0xffffffffu, end > x);
-    if (!above) {
+    if (!above && !work) {
+      hint = 32;
+      begin = begin2;
+      end = end2;
+      first = first2;
+      next = next2;
+      ctx = ctx2;
+      above = __ballot_sync(0xffffffffu, end > x);
+    } else if (!above) {
       // Largest i with work[i] <= x: a 32-way search, then the sequences from there.
       int lo = min(hint + 32, num_seqs - 1), hi = num_seqs;  // work[lo] <= x < work[hi]
       while (hi - lo > 1) {

@@ -37,10 +37,10 @@
 // head's dims are kept; the columns that this costs were zeros before.
 //
 // Measured with the join (8 heads of 128 and 32 query heads; floors at 6,535 GB/s): 64 x ~4,096
-// keys 114 us (floor 98), 131,071 keys 55 (41): a slice of 2,400 keys, of which the first loads
+// keys 112 us (floor 98), 131,071 keys 55 (41): a slice of 2,400 keys, of which the first loads
 // and the join are 12 us; 517 keys 9.1, all of it launches, first loads and the join; 24 chunks
 // of five over ~6,000 keys 103 (50), bound by the latency of the consumers' arithmetic (20 rows,
-// two CTAs an SM); 48 x ~700 keys of 12 heads of 64, one query head each, 27 (9).
+// two CTAs an SM); 48 x ~700 keys of 12 heads of 64, one query head each, 24 (9).
 #include <cuda_fp16.h>
 
 #include <type_traits>

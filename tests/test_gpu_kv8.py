@@ -653,7 +653,7 @@ def test_a_captured_call_follows_the_lengths(pkg):
     classes of chunks, an empty sequence), on either way of making the sums."""
     lengths = [[(40, 3), (700, 60), (5, 5)], [(2000, 2), (65, 65), (1, 1)], [(0, 0), (4000, 68), (0, 0)],
                [(300, 20), (300, 20), (300, 28)]]
-    for extra in (0, 40):                                  # 43 sequences: the sums take a launch
+    for extra in (0, 40, 80):                              # 83 sequences: the sums take a launch
         hq, hkv, d = 8, 2, 128
         pad = [(0, 0)] * extra
         query, pools, tables, _, _ = _batch([(4200, 68)] * 3 + pad, hq, hkv, d, 16, torch.bfloat16, seed=31)
