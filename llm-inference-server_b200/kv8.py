@@ -418,8 +418,9 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                         out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal paged attention over the 8-bit pools: :func:`paged_attention_cuda`'s arguments
     and rule with the pools' scales.  Lengths and tables are device tensors that the host never
-    reads; ``max_query_len`` bounds the chunks (default: the token count).  Builds the step
-    (one launch) unless ``block_tables`` carries one (:func:`attach_step`).
+    reads; ``max_query_len`` bounds the chunks (default: the token count).  Sums the step up by
+    itself (past 64 sequences in a launch of its own) unless ``block_tables`` carries one
+    (:func:`attach_step`).
 
     query ``[T, Hq, D]``, float16 or bfloat16, D 64 or 128, at most 16 query heads per KV
     head; pools' block size a power of two times 16.  Rows past the last sequence's are left

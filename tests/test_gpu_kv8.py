@@ -685,6 +685,28 @@ def test_a_captured_call_follows_the_lengths(pkg):
             assert torch.equal(out, eager)
 
 
+@pytest.mark.parametrize("n", [31, 32, 33, 63, 64, 65])
+def test_attention_at_the_counts_where_the_sums_change_hands(pkg, n):
+    """One scan, two, a launch: single tokens, chunks for both kernels and empty sequences."""
+    lengths = [[(300, 1), (0, 0), (70, 40), (33, 2), (1, 1), (0, 0), (129, 7)][i % 7] for i in range(n)]
+    query, pools, tables, ctx, ql = _batch(lengths, 8, 2, 128, 16, torch.bfloat16, seed=60 + n)
+    got = _check_attention(pkg, query, pools, tables, ctx, ql, 0.1, most=40)
+    step = pkg.device_step(tables, ctx, ql, num_tokens=query.shape[0], max_query_len=40, num_blocks=pools[0].shape[0],
+                           block_size=16, group=4)
+    own = pkg.paged_attention_kv8(query, *pools, pkg.attach_step(tables.view_as(tables), step), ctx, ql, 0.1)
+    assert torch.equal(got, own)
+
+
+@pytest.mark.parametrize("n,at", [(40, 5), (40, 38), (64, 63)])
+def test_a_bad_sequence_anywhere_empties_the_call_and_reports(pkg, n, at):
+    query, pools, tables, ctx, ql = _batch([(50, 1)] * n, 8, 2, 128, 16, torch.bfloat16, seed=71)
+    out = torch.full_like(query, 9.0)
+    ctx[at] = 0                                            # a token of a sequence without context
+    pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.1, max_query_len=1, out=out)
+    assert (out == 9.0).all()
+    assert pkg.read_kv8_error() == pkg._lib.PA_KV8_ERR_STEP
+
+
 @pytest.mark.parametrize("n,most,hq,hkv,d", [(1, 300, 8, 2, 128), (3, 70, 4, 4, 64), (40, 33, 6, 2, 128)])
 @pytest.mark.parametrize("attached", [False, True])
 def test_a_captured_call_without_room_for_short_chunks_gets_some(pkg, n, most, hq, hkv, d, attached):
