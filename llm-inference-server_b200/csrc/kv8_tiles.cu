@@ -48,11 +48,12 @@
 // took 291, without widening 254.
 //
 // Measured with the join (32 query heads, 8 KV heads of 128): 1,000 tokens over 16,384 keys 264 us
-// (987 TFLOP/s, 59 % of the measured bf16 GEMM rate; floor 157), 13 x 2,047 tokens 612, 30 tokens
+// (985 TFLOP/s, 59 % of the measured bf16 GEMM rate; floor 157), 13 x 2,047 tokens 619, 30 tokens
 // over 100,000 keys 82, a prompt of 333 tokens 26.  A tile of 64 keys takes 1.1 us, the softmax's
 // chain; the tensor pipe is busy 53 % of the time, the exponential unit 50 %, issue slots 58 %.
 // What did not help: two threads per row (a meeting of two warps a tile, 1.2 times the
-// instructions: 297 us), turns at the exponential unit (277), 16 widening warps (281).
+// instructions: 297 us), turns at the exponential unit (277), 16 widening warps (281), the tile's
+// maximum taken only where the weights with the old one sum past 2^14 (278).
 //
 // Every mbarrier wait is bounded; the TMEM allocation is released on every path.
 #include <cuda_fp16.h>
