@@ -118,16 +118,12 @@ def _power(byte):
 
 def _quantise(x):
     """Rows [..., D] -> (e4m3 payload, scale bytes [...]).  The scale is the least power of
-    two (exponent in [E_MIN, E_MAX]) that brings the row's largest magnitude to 448; a row
-    with a NaN is stored as zeros with the scale 255, which stands for NaN."""
+    two (exponent in [E_MIN, E_MAX]) that brings the row's largest magnitude to 448."""
     x = x.float()
-    broken = x.isnan().any(-1)
-    x = torch.where(broken[..., None], 0.0, x)
-    big = x.abs().amax(-1)
+    big = torch.where(x.isnan(), 0.0, x.abs()).amax(-1)
     m, e = torch.frexp(big.clamp(2.0 ** -30, 2.0 ** 30))         # big = m * 2^e, m in [0.5, 1)
     byte = (e - 9 + (m > 0.875).int()).clamp(E_MIN, E_MAX) + 127  # 448 = 0.875 * 2^9
-    payload = (x / _power(byte)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn)
-    return payload, torch.where(broken, 255, byte).to(torch.uint8)
+    return (x / _power(byte)[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn), byte.to(torch.uint8)
 
 
 def _pool(g, blocks, kv_heads, dim, device):
