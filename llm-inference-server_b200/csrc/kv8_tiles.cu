@@ -86,9 +86,13 @@ constexpr int kTileConsumers = 22;          // warps that read a piece: 8 softma
 // prompt of 333 tokens takes 43 us with 128, 63 with 512; one of 60 beside another 26 with 128
 // and 36 with 256; calls that fill the GPU do not care.
 constexpr int kTileMinKeys = 128;
-// The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 and the
-// output accumulator is rarely rescaled.
+// The subtracted maximum is raised only past this headroom (log2): P stays below 2^8 times the
+// shift and the output accumulator is rarely rescaled.
 constexpr float kTileLazy = 8.f;
+// Weights and their sum stand times 2^7, which cancels: at most 2^15, and fp16 keeps 11 bits down
+// to 2^-21 of the maximum and loses at most 2^-32 of it below (unshifted 2^-25: with 100,000 keys
+// that far below a few, 0.3 % of the values).
+constexpr float kTileWeightLog2 = 7.f;
 
 struct TilePiece {
   int32_t row0;    // packed index of the tile's first token; -1: no more pieces
@@ -624,7 +628,7 @@ __global__ void __launch_bounds__(kTileThreads, 1)
         const float m_new = grow ? mx_s : m_run;
         const float alpha = grow ? ex2(m_run - m_new) : 1.f;
         // A piece may start past a row's last key: nothing seen, all weights 0.
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
+        const float ref = (m_new == -INFINITY ? 0.f : m_new) - kTileWeightLog2;
         const uint64_t sc2 = f2pack(qs, qs), mn2 = f2pack(-ref, -ref);
         uint64_t rs2[2] = {0ull, 0ull};
         uint32_t pk[kTileKeys / 2];

@@ -127,3 +127,28 @@ def step_tables(request_ids, query_lens, tables, lens, held, free, num_free, wid
         out["cu_query_lens"][i + 1] = at
     out["num_free"] = np.array([left], np.int32)
     return out
+
+
+def lost_weight(tables, ctx, ql, v, hq, floor):
+    """What a row may lose to weights below fp16's normal range: each of its keys is off by at
+    most ``floor`` of the largest weight, times the largest |v| that the row's head sees."""
+    bs, hkv = v.shape[1], v.shape[2]
+    rows = []
+    for i, (c, n) in enumerate(zip(ctx, ql)):
+        if n == 0:
+            continue
+        vv = torch.nan_to_num(v[tables[i, :-(-c // bs)].long()].reshape(-1, hkv, v.shape[3])[:c], nan=0.0)
+        rows.append((c * floor * vv.abs().amax((0, 2))).repeat_interleave(hq // hkv).expand(n, hq))
+    return torch.cat(rows)[..., None]
+
+
+def tight_tolerance(want, mean, slip, lost, dtype, d):
+    """``tolerance`` with what small weights lose counted per row and relative to its values:
+    output's rounding, 2^-11 and 2^-12 of sum p |v| for the weights' rounding and the float32
+    arithmetic, the scores' error, and ``lost``.  The rounding is half a step: eps / 2 of the
+    value, and below the type's least normal number, where steps no longer shrink, eps / 2 of
+    that one (fp16: 2^-25)."""
+    score = (d + 8) * 2.0 ** -24 * slip[..., None]
+    n = lost.shape[0]
+    info = torch.finfo(dtype)
+    return info.eps / 2 * want[:n].abs().clamp_min(info.tiny) + (2.0 ** -11 + 2.0 ** -12 + 2 * score[:n]) * mean[:n] + lost
