@@ -5,11 +5,12 @@
 //   s_j = scale * q_r . K_j,  out_r = sum_j softmax_j(s) V_j,  j <= position of t
 // with K_j = k_j 2^a_j and V_j = v_j 2^b_j, where k, v are e4m3 and a, b the rows' exponents.
 // e4m3 widens to fp16 exactly, so S runs over the payloads and column j is scaled by 2^a_j;
-// the weight that multiplies v_j is exp2(s_j - m) 2^(b_j + 8), rounded to fp16 (11 bits; the
-// shift keeps weights of rows with the smallest exponent, -14, out of fp16's subnormals down
-// to 2^-8 of the maximum, the largest is 2^15).  bf16 queries are brought into fp16 by a
-// power of two per row, which is exact but for elements 2^-28 below the row's largest.
-// Maximum, sum and accumulators are float32.
+// v_j takes its 2^b_j as it is widened, exactly (b_j in [-14, 7]).  The weight that multiplies
+// V_j is exp2(s_j - m + 15) rounded to fp16: 11 bits down to 2^-29 of the maximum, and at most
+// 2^-40 of it lost below.  The sum takes the same shift, so it cancels.  (With 2^b_j in the
+// weight, rows of small values lost whole keys: a weight of 2^-19 of the maximum was 0 for
+// b_j = -14.)  bf16 queries are brought into fp16 by a power of two per row, which is exact but
+// for elements 2^-28 below the row's largest.  Maximum, sum and accumulators are float32.
 //
 // HBM-bound: each K/V byte is read once per tile of rows.  The sequences' keys laid end to
 // end are cut into equal slices (kv8_line.cuh), a CTA per slice and KV head with the KV head
@@ -39,8 +40,8 @@
 // Measured with the join (8 heads of 128 and 32 query heads; floors at 6,535 GB/s): 64 x ~4,096
 // keys 112 us (floor 98), 131,071 keys 55 (41): a slice of 2,400 keys, of which the first loads
 // and the join are 12 us; 517 keys 9.1, all of it launches, first loads and the join; 24 chunks
-// of five over ~6,000 keys 103 (50), bound by the latency of the consumers' arithmetic (20 rows,
-// two CTAs an SM); 48 x ~700 keys of 12 heads of 64, one query head each, 24 (9).
+// of five over ~6,000 keys 98 (50), bound by the latency of the consumers' arithmetic (20 rows,
+// two CTAs an SM); 48 x ~700 keys of 12 heads of 64, one query head each, 25 (9).
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -62,7 +63,7 @@ __host__ __device__ constexpr int rows_ctas(int row_groups) { return row_groups 
 // Fewest keys a slice gets, a stage for each consumer: below this a CTA's set-up and its
 // partial cost more than the keys it takes over.
 __host__ __device__ constexpr int rows_min_keys(int row_groups) { return kRowsStage * rows_warps(row_groups); }
-constexpr float kWeightShift = 256.f;               // 2^8, see above
+constexpr float kWeightLog2 = 15.f;                 // weights stand times 2^15, see above
 
 // D: dims of the payload rows (two heads' with PAIR), RG: groups of 8 query rows.
 template <int D, int RG, bool PAIR>
@@ -385,16 +386,16 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
 #pragma unroll
         for (int c = 0; c < CH; ++c) qr[c][rg] = sq[(c * RG + rg) * 32 + lane];
     }
-    // Rows 8 rg + 2 tig + {0, 1} of this lane; with PAIR, where their head's scales lie.
+    // Rows 8 rg + 2 tig + {0, 1} of this lane.
     const float2* my_factors = reinterpret_cast<const float2*>(factors) + tig;
     const int2* my_limits = reinterpret_cast<const int2*>(limits) + tig;
-    int own[RG][2];
+    bool second[RG][2];  // with PAIR: of the pair's second head
 #pragma unroll
     for (int rg = 0; rg < RG; ++rg)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * rg + 2 * tig + e;
-        own[rg][e] = PAIR && 2 * (r % p.group) >= p.group ? kRowsStage : 0;
+        second[rg][e] = PAIR && 2 * (r % p.group) >= p.group;
       }
 
     float o[CH][RG][4];  // dims 16 c + 2 g (+1: elements 2, 3), rows 8 rg + 2 tig + {0, 1}
@@ -458,17 +459,20 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
         }
 
         // ---- online softmax
-        float ks[2][2], vs[2][2];  // scales of keys 16 b + 8 h + g
-        if constexpr (!PAIR) {
+        // K scales of keys 16 n + 8 h + g, or NaN where the key's K or V row stands for it: a score
+        // of NaN makes the whole output row NaN, and only of tokens that see the key.  (A branch of
+        // its own for V's cost 20 us of 24 chunks of five over 6,000 keys.)
+        float ks[2][2][C::SUBS];
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const int key = 16 * n + 8 * h + g;
-              ks[n][h] = __uint_as_float(uint32_t(sc[key]) << 23);
-              vs[n][h] = __uint_as_float(uint32_t(sc[kRowsStage + key]) << 23) * kWeightShift;
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int u = 0; u < C::SUBS; ++u) {
+              const int at = u * kRowsStage + 16 * n + 8 * h + g;
+              const uint32_t kb = sc[at], vb = sc[C::SUBS * kRowsStage + at];
+              ks[n][h][u] = __uint_as_float(max(kb, vb) == 255u ? 0x7fffffffu : kb << 23);
             }
-        }
         uint32_t wt[2][LG][2];  // weights as B fragments: keys 8 h + 2 tig (+1), row 8 rg + g
         bool grown = false;
         float alpha[LG][2];
@@ -486,8 +490,7 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
               for (int e = 0; e < 2; ++e) {
                 const int key = 16 * n + 8 * h + g;
                 float& v = s[n][rg][2 * h + e];
-                const float k = PAIR ? __uint_as_float(uint32_t(sc[own[rg][e] + key]) << 23) : ks[n][h];
-                v *= k * (e ? factor.y : factor.x);
+                v *= ks[n][h][PAIR && second[rg][e] ? C::SUBS - 1 : 0] * (e ? factor.y : factor.x);
                 if (masked && key0 + key > (e ? limit.y : limit.x)) v = -INFINITY;
                 mx[e] = fmaxf(mx[e], v);
               }
@@ -501,21 +504,17 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
             alpha[rg][e] = ex2(m[rg][e] - ref[e]);
             grown |= alpha[rg][e] != 1.f;
             m[rg][e] = mn;
+            ref[e] -= kWeightLog2;
           }
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const int key = 16 * n + 8 * h + g;
               float w[2];
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float pr = ex2(s[n][rg][2 * h + e] - ref[e]);
-                sum[e] += pr;
-                w[e] = pr * (PAIR ? __uint_as_float(uint32_t(sc[2 * kRowsStage + own[rg][e] + key]) << 23) * kWeightShift
-                                  : vs[n][h]);
-                // A hidden key's row may stand for NaN.
-                if (masked && key0 + key > (e ? limit.y : limit.x)) w[e] = 0.f;
+                w[e] = ex2(s[n][rg][2 * h + e] - ref[e]);
+                sum[e] += w[e];
               }
               wt[n][rg][h] = transpose8(pack2<__half>(w[0], w[1]));
             }
@@ -534,6 +533,13 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
         // ---- O^T += V^T W^T; bytes behind the context (or the stage's only block) read as zero
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
+          uint32_t vs[C::SUBS][2];  // V scales of keys 16 n + 8 h + 2 tig (+1)
+#pragma unroll
+          for (int u = 0; u < C::SUBS; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              vs[u][h] = scale_pair(*reinterpret_cast<const uint16_t*>(sc + (C::SUBS + u) * kRowsStage + 16 * n + 8 * h +
+                                                                       2 * tig));
           uint32_t pick[2] = {0x3120u, 0x3120u};  // (t0 d0, t1 d0, t0 d1, t1 d1) of (t0 d0, t0 d1, t1 d0, t1 d1)
           if (end < kRowsStage) {
 #pragma unroll
@@ -549,7 +555,9 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const uint32_t x = __byte_perm(w[2 * i], 0, pick[0]), y = __byte_perm(w[2 * i + 1], 0, pick[1]);
-              const uint32_t a0 = widen_lo(x), a1 = widen_hi(x), a2 = widen_lo(y), a3 = widen_hi(y);
+              const uint32_t(&v2)[2] = vs[PAIR && c + i >= CH / 2 ? 1 : 0];
+              const uint32_t a0 = mul_h2(widen_lo(x), v2[0]), a1 = mul_h2(widen_hi(x), v2[0]),
+                             a2 = mul_h2(widen_lo(y), v2[1]), a3 = mul_h2(widen_hi(y), v2[1]);
 #pragma unroll
               for (int rg = 0; rg < LG; ++rg) mma16(o[c + i][rg], a0, a1, a2, a3, wt[n][rg][0], wt[n][rg][1]);
             }
@@ -639,11 +647,11 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
       for (int e = 0; e < 2; ++e) {
         const int r = 8 * rg + 2 * tig + e, tok = r / p.group, head = kvh * p.group + (r - tok * p.group);
         if (tok >= d.tokens) continue;
-        const float f = (d.part < 0 ? 1.f / l[rg][e] : 1.f) * (1.f / kWeightShift);
+        const float f = d.part < 0 ? 1.f / l[rg][e] : 1.f;
         const int64_t at = ((int64_t(slice) * p.num_kv_heads + kvh) * 2 + d.part) * (8 * RG) + r;
         T* dst = static_cast<T*>(p.out) + int64_t(d.row0 + tok) * p.o_st + int64_t(head) * p.o_sh + 2 * g;
         // With PAIR a row's dims are its own head's, the first 64 or the second.
-        if (!PAIR || (own[rg][e] != 0) == odd) {
+        if (!PAIR || second[rg][e] == odd) {
 #pragma unroll
           for (int c = 0; c < Q4; ++c) {
             const int chunk = PAIR ? (chunk0 + c) % H : chunk0 + c;

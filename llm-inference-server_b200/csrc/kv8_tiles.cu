@@ -155,12 +155,6 @@ __device__ __forceinline__ bool elect_one() {
   return r != 0;
 }
 
-__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-
 // A widening warp's 16 keys of a staged 64-key tile: read into registers, then widened into the
 // swizzled tile.  A lane takes a 16-byte chunk of N rows, D / 16 lanes a row.  With 128 dims the
 // eight lanes that one access serves at a time hold half of two rows that differ in bits 0 and

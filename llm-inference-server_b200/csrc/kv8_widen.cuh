@@ -20,6 +20,20 @@ __device__ __forceinline__ uint32_t widen_hi(uint32_t w) {
   return r;
 }
 
+// Two fp16 products; no value of the cache loses a bit in one by its row's scale.
+__device__ __forceinline__ uint32_t mul_h2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Two scale bytes as fp16, 2^(b - 127); bytes outside the format's [113, 134] (NaN's 255, those
+// behind a context) give its ends, so that a product with a finite payload is finite.
+__device__ __forceinline__ uint32_t scale_pair(uint32_t two) {
+  const uint32_t b = __vmaxu2(__vminu2(__byte_perm(two, 0u, 0x4140u), 0x00860086u), 0x00710071u);
+  return (b - 0x00700070u) << 10;  // the exponent of fp16 is b - 112
+}
+
 // Byte offset of 16-byte chunk c of row r in a TMA tile whose rows are D bytes, with the
 // swizzle as wide as the row (128 or 64 bytes).
 template <int D>

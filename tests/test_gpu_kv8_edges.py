@@ -36,7 +36,7 @@ def _peaked(lengths, hq, hkv, d, dtype, every, drop, v_bytes, seed=0):
     return query, pools, tables, ctx, ql
 
 
-TILES = 2.0 ** -32     # of the largest weight: half of fp16's least step under the kernel's shift
+ROWS, TILES = 2.0 ** -40, 2.0 ** -32     # of the largest weight: half of fp16's least step under the kernels' shifts
 
 
 def _check_tight(pkg, query, pools, tables, ctx, ql, scale, most, floor):
@@ -53,6 +53,21 @@ def _check_tight(pkg, query, pools, tables, ctx, ql, scale, most, floor):
 
 # ------------------------------------------------------------------ weights far below the maximum
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64), (8, 1, 64), (6, 3, 128)])
+@pytest.mark.parametrize("drop,v_bytes", [(9.0, (113,)), (13.0, (113,)), (13.0, (113, 114, 120)), (18.0, (119,)),
+                                          (18.0, (134,)), (13.0, (113, 134))])
+def test_few_rows_keep_small_weights_of_any_value_scale(pkg, dtype, hq, hkv, d, drop, v_bytes):
+    """Weights carry 11 bits down to 2^-29 of the maximum, whatever the V rows' scales are; one
+    token, and chunks that take two and three groups of rows (with eight heads a chunk of four
+    has 32 rows, which the tiles take)."""
+    for lengths, most in (([(2000, 1), (300, 1)], 1), ([(1500, 3), (700, 2), (64, 4)], 4)):
+        batch = _peaked(lengths, hq, hkv, d, dtype, 32, drop, v_bytes, seed=d + hq)
+        tiles = most * hq // hkv > 24
+        _check_tight(pkg, *batch, 1.0, most, TILES if tiles else ROWS)
+        assert ("kv8_tiles" in pkg._lib.last_launches()) == tiles
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("hq,hkv,d", [(8, 2, 128), (4, 4, 64)])
 @pytest.mark.parametrize("lengths", [[(700, 300)], [(2000, 60), (130, 30)]])
 def test_long_chunks_keep_small_weights(pkg, dtype, hq, hkv, d, lengths):
@@ -60,3 +75,26 @@ def test_long_chunks_keep_small_weights(pkg, dtype, hq, hkv, d, lengths):
     batch = _peaked(lengths, hq, hkv, d, dtype, 64, 15.0, (113, 120), seed=d)
     _check_tight(pkg, *batch, 1.0, max(q for _, q in lengths), TILES)
     assert "kv8_tiles" in pkg._lib.last_launches()
+
+
+def test_few_rows_of_one_cta_over_a_long_context(pkg):
+    """As many KV heads as there are CTAs, so that each walks a whole context."""
+    hq = hkv = 446
+    batch = _peaked([(6000, 1)], hq, hkv, 64, torch.bfloat16, 2048, 13.0, (113,), seed=3)
+    _check_tight(pkg, *batch, 1.0, 1, ROWS)
+
+
+def test_few_rows_nan_value_rows_among_small_weights(pkg):
+    """A V row that stands for NaN reaches every token that sees it, even where its weight has
+    vanished, and no other token or head."""
+    for hq, hkv, d in ((8, 2, 128), (4, 4, 64)):
+        query, pools, tables, ctx, ql = _peaked([(90, 4), (40, 2)], hq, hkv, d, torch.bfloat16, 32, 120.0, (113,), seed=6)
+        clean = pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 1.0, max_query_len=4)
+        slot = int(tables[0, 88 // 16]) * 16 + 88 % 16         # seen by the tokens at 88 and 89
+        pools[1].view(torch.uint8).view(-1, hkv, d)[slot, 1] = 0
+        pools[3][slot // 16, 1, slot % 16] = 255
+        got = pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 1.0, max_query_len=4)
+        g = hq // hkv
+        assert got[2:4, g:2 * g].isnan().all()
+        got[2:4, g:2 * g] = clean[2:4, g:2 * g]
+        assert torch.equal(got, clean)
