@@ -48,8 +48,9 @@ PA_KV8_ERR_STEP = 8
 PA_KV8_ERR_NO_BLOCKS = 16
 PA_KV8_MAX_ROWS = 4096
 PA_KV8_MAX_REQUESTS = 131072
+PA_KV8_STEP_WORDS = 24
 
-ABI_VERSION = 7
+ABI_VERSION = 8
 
 
 class StepPlan(ctypes.Structure):

@@ -9,6 +9,18 @@
 
 namespace pa {
 
+// What a reserved step leaves in device memory, for the commit to see whether it still fits:
+// num_free comes first, as the step's num_free_out.
+struct Kv8StepRecord {
+  int32_t num_free;  // the free list's length once the step counts; -1: the step was emptied
+  int32_t rows, width, block_size, free_capacity, spare;
+  const int32_t *lens, *held, *num_free_at, *free_blocks;  // what it was built from
+  int32_t* tables;
+  int64_t table_stride;
+  const int32_t *out_tables, *context_lens, *held_out;  // the step's arrays
+};
+static_assert(sizeof(Kv8StepRecord) == 4 * PA_KV8_STEP_WORDS, "the header's size of num_free_out");
+
 struct Kv8StepParams {
   const int32_t *row_ids, *lens, *query_lens;
   int32_t* tables;
@@ -68,8 +80,8 @@ int* kv8_error_word();  // device address of the current device's error word
 
 cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t stream);
 cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
-                              const int32_t* held_out, const int32_t* num_free_out, int32_t rows, int32_t slots,
-                              int32_t* lens, int32_t* held, int32_t* num_free, cudaStream_t stream);
+                              const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
+                              int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream);
 cudaError_t launch_kv8_release(const int32_t* ids, int32_t count, const int32_t* tables, int64_t table_stride,
                                int32_t width, int32_t slots, int32_t* lens, int32_t* held, int32_t* free_blocks,
                                int32_t free_capacity, int32_t* num_free, int* err, cudaStream_t stream);

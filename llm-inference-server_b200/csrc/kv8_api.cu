@@ -166,6 +166,8 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
       (num_rows > 0 && width > 0 && !tables) ||
       (held && (!num_free || (free_capacity > 0 && !free_blocks) || (num_rows > 0 && width > 0 && !out_tables))))
     return fail(PA_ERR_INVALID_ARGUMENT, "build_step: NULL device pointer");
+  if (reinterpret_cast<uintptr_t>(num_free_out) % 8)
+    return fail(PA_ERR_INVALID_ARGUMENT, "build_step: num_free_out must be 8-byte aligned");
   int* err = kv8_error_word();
   if (!err) return fail(PA_ERR_CUDA, "build_step: no CUDA device");
   cudaError_t e = launch_kv8_step(p, err, static_cast<cudaStream_t>(stream_ptr));
@@ -177,10 +179,17 @@ int32_t pa_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const i
                       int32_t* lens, int32_t* held, int32_t* num_free, void* stream_ptr) {
   using namespace pa;
   if (num_rows < 0 || num_slots < 0) return fail(PA_ERR_INVALID_ARGUMENT, "commit: bad sizes");
+  if (num_rows > PA_KV8_MAX_ROWS)
+    return fail(PA_ERR_UNSUPPORTED, "commit: %d rows, at most %d are supported", num_rows, PA_KV8_MAX_ROWS);
   if (!num_free_out || !num_free || (num_rows > 0 && (!query_lens || !held_out || !lens || !held)))
     return fail(PA_ERR_INVALID_ARGUMENT, "commit: NULL device pointer");
-  cudaError_t e = launch_kv8_commit(row_ids, query_lens, accepted, held_out, num_free_out, num_rows, num_slots, lens,
-                                    held, num_free, static_cast<cudaStream_t>(stream_ptr));
+  if (reinterpret_cast<uintptr_t>(num_free_out) % 8)
+    return fail(PA_ERR_INVALID_ARGUMENT, "commit: num_free_out must be 8-byte aligned");
+  int* err = kv8_error_word();
+  if (!err) return fail(PA_ERR_CUDA, "commit: no CUDA device");
+  cudaError_t e = launch_kv8_commit(row_ids, query_lens, accepted, held_out,
+                                    reinterpret_cast<const Kv8StepRecord*>(num_free_out), num_rows, num_slots, lens,
+                                    held, num_free, err, static_cast<cudaStream_t>(stream_ptr));
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "commit launch");
 }
 

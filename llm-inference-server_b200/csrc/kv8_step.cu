@@ -152,7 +152,13 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
         p.work[rows] = small;
         p.work[2 * rows + 1] = large;
       }
-      if (p.num_free_out) *p.num_free_out = reject ? -1 : avail - int32_t(blocks);
+      const int left = reject ? -1 : avail - int32_t(blocks);
+      if (p.held)
+        *reinterpret_cast<Kv8StepRecord*>(p.num_free_out) = {
+            left,     rows,          p.width,  p.block_size,   p.free_capacity, 0,            p.lens,    p.held,
+            p.num_free, p.free_blocks, p.tables, p.table_stride, p.out_tables,    p.context_lens, p.held_out};
+      else if (p.num_free_out)
+        *p.num_free_out = left;
     }
   }
 
@@ -206,20 +212,90 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
   }
 }
 
-__global__ void __launch_bounds__(256) kv8_commit_kernel(const int32_t* row_ids, const int32_t* query_lens,
-                                                         const int32_t* accepted, const int32_t* held_out,
-                                                         const int32_t* num_free_out, int rows, int slots,
-                                                         int32_t* lens, int32_t* held, int32_t* num_free) {
-  const int left = *num_free_out;
-  if (left < 0) return;  // the step was emptied
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) {
+// Row of item b in running sums at[0 .. rows] (at[row] <= b < at[row + 1]).
+__device__ __forceinline__ int row_of(const int32_t* at, int rows, int b) {
+  int lo = 0, hi = rows;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) / 2;
+    if (at[m] <= b)
+      lo = m;
+    else
+      hi = m;
+  }
+  return lo;
+}
+
+// One CTA.  A step is planned from the slots and the free list as they are then, and other steps
+// may count or blocks come back before it does, so the plan is compared first: each slot's
+// length, the blocks that its new tokens went into, and that the step's new blocks are still the
+// free list's last ones.  Then all of it is written, or nothing.
+__global__ void __launch_bounds__(kStepThreads)
+    kv8_commit_kernel(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+                      const int32_t* held_out, const Kv8StepRecord* record, int rows, int slots, int32_t* lens,
+                      int32_t* held, int32_t* num_free, int* err) {
+  extern __shared__ int32_t s_at[];  // [rows + 1] new blocks before the row
+  __shared__ int64_t scan[kStepThreads / 32][1];
+  const int tid = threadIdx.x;
+  const Kv8StepRecord r = *record;
+  if (r.num_free < 0) return;  // the step was emptied
+  if (r.lens != lens || r.held != held || r.num_free_at != num_free || r.held_out != held_out || r.rows != rows) {
+    if (tid == 0) set_error(err, PA_KV8_ERR_STEP);  // of other tables
+    return;
+  }
+  const int have = *num_free;
+  auto slot_of = [&](int i) {
     const int row = row_ids ? row_ids[i] : i;
-    if (row < 0 || row >= slots) continue;
+    return row < slots ? row : -1;
+  };
+  int bad = 0;
+  int64_t blocks = 0;
+  for (int first = 0; first < rows; first += blockDim.x) {
+    const int i = first + tid, row = i < rows ? slot_of(i) : -1;
+    int need = 0;
+    if (row >= 0) {
+      const int q = query_lens[i], ctx = r.context_lens[i], mine = held[row], base = lens[row];
+      need = held_out[i] - mine;
+      if (mine < 0 || need < 0 || held_out[i] > r.width || base < 0 || base + q != ctx) {
+        bad = 1;
+        need = 0;
+      } else if (q > 0) {
+        const int32_t *now = r.tables + int64_t(row) * r.table_stride, *then = r.out_tables + int64_t(i) * r.width;
+        for (int j = base / r.block_size; j < mine && j * r.block_size < ctx; ++j) bad |= now[j] != then[j];
+      }
+    }
+    int64_t at[1] = {need}, sum[1];
+    block_scan(at, sum, scan);
+    if (i < rows) s_at[i] = int32_t(blocks + at[0]);
+    blocks += sum[0];
+  }
+  if (tid == 0) s_at[rows] = int32_t(blocks);
+  if (have > r.free_capacity || blocks > have) bad = 1;
+  bool stale = __syncthreads_or(bad) != 0;
+  if (!stale) {
+    for (int b = tid; b < int(blocks); b += blockDim.x) {
+      const int i = row_of(s_at, rows, b), j = held[slot_of(i)] + b - s_at[i];
+      bad |= r.free_blocks[have - 1 - b] != r.out_tables[int64_t(i) * r.width + j];
+    }
+    stale = __syncthreads_or(bad) != 0;
+  }
+  if (stale) {
+    if (tid == 0) set_error(err, PA_KV8_ERR_STEP);
+    return;
+  }
+  // The slots' tables too: a step that was dropped may have been written over this one's blocks.
+  for (int b = tid; b < int(blocks); b += blockDim.x) {
+    const int i = row_of(s_at, rows, b), row = slot_of(i), j = held[row] + b - s_at[i];
+    r.tables[int64_t(row) * r.table_stride + j] = r.free_blocks[have - 1 - b];
+  }
+  __syncthreads();
+  for (int i = tid; i < rows; i += blockDim.x) {
+    const int row = slot_of(i);
+    if (row < 0) continue;
     const int q = query_lens[i];
     lens[row] += accepted ? max(0, min(accepted[i], q)) : q;
     held[row] = held_out[i];
   }
-  if (threadIdx.x == 0) *num_free = left;
+  if (tid == 0) *num_free = have - int(blocks);
 }
 
 // One CTA: a release is rare and short, and its places on the free list depend on one
@@ -266,15 +342,8 @@ __global__ void __launch_bounds__(kStepThreads) kv8_release_kernel(const int32_t
     return;
   }
   for (int b = tid; b < int(blocks); b += blockDim.x) {
-    int lo = 0, hi = count;
-    while (hi - lo > 1) {
-      const int m = (lo + hi) / 2;
-      if (s_at[m] <= b)
-        lo = m;
-      else
-        hi = m;
-    }
-    free_blocks[have + b] = tables[int64_t(ids[lo]) * table_stride + (s_at[lo + 1] - 1 - b)];
+    const int i = row_of(s_at, count, b);
+    free_blocks[have + b] = tables[int64_t(ids[i]) * table_stride + (s_at[i + 1] - 1 - b)];
   }
   for (int i = tid; i < count; i += blockDim.x)
     if (ids[i] >= 0) lens[ids[i]] = held[ids[i]] = 0;
@@ -316,10 +385,11 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
 }
 
 cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
-                              const int32_t* held_out, const int32_t* num_free_out, int32_t rows, int32_t slots,
-                              int32_t* lens, int32_t* held, int32_t* num_free, cudaStream_t stream) {
-  kv8_commit_kernel<<<1, 256, 0, stream>>>(row_ids, query_lens, accepted, held_out, num_free_out, rows, slots, lens,
-                                           held, num_free);
+                              const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
+                              int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream) {
+  const int threads = rows <= 128 ? 128 : kStepThreads;
+  kv8_commit_kernel<<<1, threads, sizeof(int32_t) * (size_t(rows) + 1), stream>>>(
+      row_ids, query_lens, accepted, held_out, record, rows, slots, lens, held, num_free, err);
   return cudaGetLastError();
 }
 

@@ -89,9 +89,10 @@ def _tiling(group: int, max_query_len: int, num_seqs: int, num_tokens: int) -> _
     return t
 
 
-# The step's arrays in one int32 buffer: work (int64, so first), context_lens, query_lens,
-# held, cu_query_lens, seq_idx, q_pos, slot_mapping, num_free, block_tables.
-_CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _FREE, _TABLES = range(1, 10)
+# The step's arrays in one int32 buffer: work (int64, so first), num_free and the rest of what a
+# commit has to know (8-byte words among it), context_lens, query_lens, held, cu_query_lens,
+# seq_idx, q_pos, slot_mapping, block_tables.
+_FREE, _RECORD, _CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _TABLES = range(1, 11)
 
 
 _LAYOUTS: dict[tuple[int, int, int], tuple[tuple[int, ...], tuple[int, ...], int]] = {}
@@ -101,7 +102,7 @@ def _layout(b: int, t: int, cells: int) -> tuple[tuple[int, ...], tuple[int, ...
     """(words of each array, their byte offsets, words in all)."""
     got = _LAYOUTS.get((b, t, cells))
     if got is None:
-        sizes = (4 * (b + 1), b, b, b, b + 1, t, t, t, 1, cells)
+        sizes = (4 * (b + 1), 1, _lib.PA_KV8_STEP_WORDS - 1, b, b, b, b + 1, t, t, t, cells)
         got = (sizes, tuple(4 * sum(sizes[:i]) for i in range(len(sizes))), sum(sizes))
         if len(_LAYOUTS) > 1024:
             _LAYOUTS.clear()
@@ -128,6 +129,7 @@ class DeviceStep:
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
         self._row_ids: torch.Tensor | None = None
         self._counted = False
+        self._home = 0                                # the address of the num_free it was reserved against
 
     @property
     def _arrays(self) -> tuple[torch.Tensor, ...]:
@@ -232,7 +234,9 @@ class DeviceBlockTables:
 
     A step is ``reserve`` (blocks for the new tokens, the step's metadata), then the layers,
     then ``commit`` — with the accepted counts, where a chunk of speculated tokens was only
-    partly accepted.  Until ``commit``, a step can be reserved again or dropped.  ``release``
+    partly accepted.  Until ``commit``, a step can be reserved again or dropped; one that no
+    longer fits when it is committed (its slots moved on, its blocks went to another step, blocks
+    were released after it took its own) changes nothing and leaves an error bit.  ``release``
     returns a finished request's blocks.  Nothing here reads the GPU from the host, so the
     whole loop can be captured in a CUDA graph.  Prefix sharing stays with the host allocator:
     a block is held by one slot."""
@@ -299,20 +303,24 @@ class DeviceBlockTables:
                               own_tables=True)
         elif step._tables is not None:
             raise ValueError("out was made by device_step")
-        step._row_ids, step._counted = ids, False
+        home = self.num_free.data_ptr()
+        step._row_ids, step._counted, step._home = ids, False, home
         p = step._ptr
         _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
                 self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
-                self.num_free.data_ptr(), self.free.shape[0], b, self.max_requests, self.width, self.block_size,
+                home, self.free.shape[0], b, self.max_requests, self.width, self.block_size,
                 self.num_blocks, num_tokens, max_query_len, ctypes.byref(tiling), p[_TABLES], p[_CTX], p[_QL], p[_HELD],
                 p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[0])
         return step
 
     def commit(self, step: DeviceStep, accepted: torch.Tensor | None = None) -> None:
         """Make a reserved step count: its tokens (or the ``accepted[i]`` first of row i) are
-        cached now and its blocks are held.  An emptied step changes nothing."""
+        cached now and its blocks are held.  An emptied step changes nothing; nor does one that
+        no longer fits the slots and the free list, which :func:`read_kv8_error` reports."""
         if step._row_ids is None:
             raise ValueError("commit needs a step made by reserve")
+        if step._home != self.num_free.data_ptr():
+            raise ValueError("this step was reserved in other tables")
         if step._counted:
             raise ValueError("this step was committed before")
         acc = None

@@ -4,11 +4,12 @@ stale, ids that the GPU has to refuse, views at odd offsets (tests/_kv8_ref.py h
 
 from __future__ import annotations
 
+import numpy as np
 import pytest
 import torch
 
 import _kv8_ref as ref
-from test_gpu_kv8 import DEV, _batch, _no_device_error  # noqa: F401  (the fixture reads the error word)
+from test_gpu_kv8 import DEV, _batch, _i32, _no_device_error  # noqa: F401  (the fixture reads the error word)
 
 pytestmark = pytest.mark.gpu
 
@@ -98,3 +99,150 @@ def test_few_rows_nan_value_rows_among_small_weights(pkg):
         assert got[2:4, g:2 * g].isnan().all()
         got[2:4, g:2 * g] = clean[2:4, g:2 * g]
         assert torch.equal(got, clean)
+
+
+# ------------------------------------------------------------------ steps that went stale
+def _tables(pkg, lens=(20, 5, 40, 0), nb=24, width=6, bs=16):
+    """Four slots with some tokens in them, 24 blocks."""
+    bt = pkg.DeviceBlockTables(len(lens), width, nb, bs, DEV)
+    step = bt.reserve(_i32(range(len(lens))), _i32(lens), num_tokens=sum(lens), max_query_len=max(lens))
+    bt.commit(step)
+    return bt
+
+
+def _owned(bt):
+    """Every block of the pool by its holder: the slots' blocks, then the free list's."""
+    held, tables = bt.held.tolist(), bt.tables.tolist()
+    return [b for row, n in zip(tables, held) for b in row[:n]] + bt.free[:int(bt.num_free)].tolist()
+
+
+def _state_of(bt):
+    n = int(bt.num_free)
+    return [bt.lens.tolist(), bt.held.tolist(), [r[:h] for r, h in zip(bt.tables.tolist(), bt.held.tolist())],
+            bt.free[:n].tolist()]
+
+
+def _reserve(bt, ids, ql):
+    return bt.reserve(_i32(ids), _i32(ql), num_tokens=sum(ql), max_query_len=max(ql))
+
+
+def test_a_step_under_released_blocks_is_not_committed_and_reports(pkg):
+    """Blocks that came back after the step took its own lie over them on the list: committing
+    it set the list's length back and lost them."""
+    bt = _tables(pkg)
+    step = _reserve(bt, [0, 1], [13, 1])                       # slot 0 needs a block
+    bt.release(_i32([2]))
+    before = _state_of(bt)
+    bt.commit(step)
+    assert _state_of(bt) == before and sorted(_owned(bt)) == list(range(24))
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+    bt.commit(_reserve(bt, [0, 1], [13, 1]))                   # made again, it counts
+    assert bt.lens.tolist() == [33, 6, 0, 0] and sorted(_owned(bt)) == list(range(24))
+
+
+def test_a_step_without_new_blocks_survives_a_release(pkg):
+    bt = _tables(pkg)
+    step = _reserve(bt, [0, 1], [2, 1])
+    bt.release(_i32([2]))
+    free = int(bt.num_free)
+    bt.commit(step)
+    assert int(bt.num_free) == free and bt.lens.tolist() == [22, 6, 0, 0]
+    assert sorted(_owned(bt)) == list(range(24))
+
+
+def test_two_steps_with_the_same_free_blocks_do_not_both_count_and_reports(pkg):
+    bt = _tables(pkg)
+    a, b = _reserve(bt, [0], [13]), _reserve(bt, [3], [1])     # both plan with the list's last block
+    assert int(a.block_tables[0, 2]) == int(b.block_tables[0, 0])
+    bt.commit(a)
+    before = _state_of(bt)
+    bt.commit(b)
+    assert _state_of(bt) == before and sorted(_owned(bt)) == list(range(24))
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
+def test_two_steps_of_which_one_needs_no_block_both_count(pkg):
+    bt = _tables(pkg)
+    a, b = _reserve(bt, [0], [13]), _reserve(bt, [1], [1])
+    bt.commit(a)
+    bt.commit(b)
+    assert bt.lens.tolist() == [33, 6, 40, 0] and sorted(_owned(bt)) == list(range(24))
+
+
+@pytest.mark.parametrize("ids,ql", [([2], [1]), ([2], [9]), ([0, 2], [13, 3])])
+def test_a_step_of_a_released_slot_is_not_committed_and_reports(pkg, ids, ql):
+    bt = _tables(pkg)
+    step = _reserve(bt, ids, ql)
+    bt.release(_i32([2]))
+    before = _state_of(bt)
+    bt.commit(step)
+    assert _state_of(bt) == before and sorted(_owned(bt)) == list(range(24))
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
+def test_a_slot_that_was_filled_again_elsewhere_is_not_committed_and_reports(pkg):
+    """The same slot with the same length, in other blocks: the step's K and V went into the old ones."""
+    bt = _tables(pkg)
+    step = _reserve(bt, [2], [1])
+    bt.release(_i32([2]))
+    bt.commit(_reserve(bt, [3, 2], [3, 40]))
+    before = _state_of(bt)
+    bt.commit(step)
+    assert _state_of(bt) == before and sorted(_owned(bt)) == list(range(24))
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
+def test_a_dropped_step_leaves_no_trace_in_one_that_counts(pkg):
+    """The dropped one planned the same free blocks for other rows and wrote them into the tables."""
+    bt = _tables(pkg)
+    a = _reserve(bt, [0, 3], [30, 20])
+    want = a.block_tables.tolist()
+    _reserve(bt, [3, 0], [20, 30])
+    bt.commit(a)
+    assert [bt.tables[0].tolist()[:4], bt.tables[3].tolist()[:2]] == [want[0][:4], want[1][:2]]
+    assert sorted(_owned(bt)) == list(range(24))
+
+
+def test_a_step_of_other_tables_is_refused(pkg):
+    bt, other = _tables(pkg), _tables(pkg)
+    with pytest.raises(ValueError, match="other tables"):
+        other.commit(_reserve(bt, [0], [1]))
+
+
+def test_a_step_of_many_rows_counts(pkg):
+    """More rows than a CTA has threads, some of them padding, several new blocks a row."""
+    rows, bs, width = 1300, 16, 9
+    rng = np.random.default_rng(2)
+    bt = pkg.DeviceBlockTables(rows, width, rows * width, bs, DEV)
+    ids = rng.permutation(rows).astype(np.int32)
+    ids[::7] = -1
+    lens = np.zeros(rows, int)
+    for most in (50, 3, 70):
+        ql = rng.integers(0, most + 1, size=rows)
+        step = bt.reserve(_i32(ids), _i32(ql), num_tokens=int(ql.sum()), max_query_len=most)
+        want = step.block_tables.tolist()
+        bt.commit(step)
+        live = ids >= 0
+        lens[ids[live]] += ql[live]
+        np.testing.assert_array_equal(bt.lens.cpu().numpy(), lens)
+        np.testing.assert_array_equal(bt.held.cpu().numpy()[ids[live]], -(-lens[ids[live]] // bs))
+        tables, held = bt.tables.tolist(), bt.held.tolist()
+        assert all(tables[r][:held[r]] == want[i][:held[r]] for i, r in enumerate(ids) if r >= 0)
+        assert sorted(_owned(bt)) == list(range(rows * width))
+
+
+def test_a_captured_commit_counts_its_step_once_and_reports(pkg):
+    """Replayed without the reserve before it, a commit meets lengths that have moved on."""
+    bt = _tables(pkg)
+    step = _reserve(bt, [0, 1], [2, 1])
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        bt.commit(step)
+    torch.cuda.current_stream().wait_stream(side)
+    graph.replay()
+    assert bt.lens.tolist() == [22, 6, 40, 0]
+    graph.replay()
+    assert bt.lens.tolist() == [22, 6, 40, 0]
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
