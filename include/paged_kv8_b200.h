@@ -45,7 +45,7 @@ extern "C" {
 /* Most rows (sequences) of a step and most request slots of a table set. */
 #define PA_KV8_MAX_ROWS 4096
 #define PA_KV8_MAX_REQUESTS 131072
-/* int32 words of a step's num_free_out. */
+/* int32 words of a step's num_free_out before its rows'. */
 #define PA_KV8_STEP_WORDS 24
 
 /*
@@ -85,8 +85,8 @@ int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, int32_t num_s
  * Outputs (device): out_tables [num_rows, width], 0-padded (NULL without `held`),
  * context_lens / query_lens_out / held_out [num_rows], cu_query_lens [num_rows + 1],
  * seq_idx / q_pos / slot_mapping [num_tokens], work int64 [2, num_rows + 1], num_free_out
- * [PA_KV8_STEP_WORDS], 8-byte aligned: the free list's length once the step counts, then what
- * pa_kv8_commit has to know of it.
+ * [PA_KV8_STEP_WORDS + num_rows], 8-byte aligned: the free list's length once the step counts,
+ * then what pa_kv8_commit has to know of it (without `held` the first word only).
  * Nothing but `tables` is updated in place, so a step can be built again; pa_kv8_commit
  * makes it count.  A step whose lengths or ids are inconsistent (a slot named twice, more
  * tokens than num_tokens, a chunk over max_query_len, a context over width * block_size, a
@@ -104,7 +104,8 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
 /*
  * Make a step count that was built with `held`: lens += accepted (NULL: the step's query_lens;
  * clamped to them), held = held_out, its new blocks leave the free list and stand in the tables.
- * query_lens, held_out and num_free_out are the step's.  A step that was emptied changes
+ * query_lens, held_out and num_free_out are the step's; its rows' slots are those that the step
+ * was built with, whatever row_ids holds by now.  A step that was emptied changes
  * nothing, nor does one that no longer fits, which sets PA_KV8_ERR_STEP: one of other lens, held
  * or num_free, one whose slots have other lengths by now, or whose new blocks are not the free
  * list's last ones any more (another step took them, or blocks were released over them).

@@ -10,7 +10,7 @@
 namespace pa {
 
 // What a reserved step leaves in device memory, for the commit to see whether it still fits:
-// num_free comes first, as the step's num_free_out.
+// num_free comes first, as the step's num_free_out; the rows' request slots follow.
 struct Kv8StepRecord {
   int32_t num_free;  // the free list's length once the step counts; -1: the step was emptied
   int32_t rows, width, block_size, free_capacity, spare;
@@ -79,7 +79,7 @@ struct Kv8AttnParams {
 int* kv8_error_word();  // device address of the current device's error word
 
 cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t stream);
-cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+cudaError_t launch_kv8_commit(const int32_t* query_lens, const int32_t* accepted,
                               const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
                               int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream);
 cudaError_t launch_kv8_release(const int32_t* ids, int32_t count, const int32_t* tables, int64_t table_stride,

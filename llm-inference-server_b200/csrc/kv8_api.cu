@@ -174,7 +174,7 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "build_step launch");
 }
 
-int32_t pa_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+int32_t pa_kv8_commit(const int32_t*, const int32_t* query_lens, const int32_t* accepted,
                       const int32_t* held_out, const int32_t* num_free_out, int32_t num_rows, int32_t num_slots,
                       int32_t* lens, int32_t* held, int32_t* num_free, void* stream_ptr) {
   using namespace pa;
@@ -187,7 +187,7 @@ int32_t pa_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const i
     return fail(PA_ERR_INVALID_ARGUMENT, "commit: num_free_out must be 8-byte aligned");
   int* err = kv8_error_word();
   if (!err) return fail(PA_ERR_CUDA, "commit: no CUDA device");
-  cudaError_t e = launch_kv8_commit(row_ids, query_lens, accepted, held_out,
+  cudaError_t e = launch_kv8_commit(query_lens, accepted, held_out,
                                     reinterpret_cast<const Kv8StepRecord*>(num_free_out), num_rows, num_slots, lens,
                                     held, num_free, err, static_cast<cudaStream_t>(stream_ptr));
   return e == cudaSuccess ? PA_OK : kv8_cuda_fail(e, "commit launch");

@@ -140,6 +140,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
       if (reject) p.work[i] = p.work[rows + 1 + i] = 0;
       if (i < rows) {
         const int need = (i + 1 < rows ? s_new[i + 1] : int32_t(blocks)) - s_new[i];
+        if (p.held) p.num_free_out[PA_KV8_STEP_WORDS + i] = s_row[i];
         if (p.context_lens) {
           p.context_lens[i] = reject ? 0 : s_ctx[i];
           p.query_out[i] = reject ? 0 : s_cu[i + 1] - s_cu[i];
@@ -230,13 +231,14 @@ __device__ __forceinline__ int row_of(const int32_t* at, int rows, int b) {
 // length, the blocks that its new tokens went into, and that the step's new blocks are still the
 // free list's last ones.  Then all of it is written, or nothing.
 __global__ void __launch_bounds__(kStepThreads)
-    kv8_commit_kernel(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+    kv8_commit_kernel(const int32_t* query_lens, const int32_t* accepted,
                       const int32_t* held_out, const Kv8StepRecord* record, int rows, int slots, int32_t* lens,
                       int32_t* held, int32_t* num_free, int* err) {
   extern __shared__ int32_t s_at[];  // [rows + 1] new blocks before the row
   __shared__ int64_t scan[kStepThreads / 32][1];
   const int tid = threadIdx.x;
   const Kv8StepRecord r = *record;
+  const int32_t* rows_of_step = reinterpret_cast<const int32_t*>(record + 1);
   if (r.num_free < 0) return;  // the step was emptied
   if (r.lens != lens || r.held != held || r.num_free_at != num_free || r.held_out != held_out || r.rows != rows) {
     if (tid == 0) set_error(err, PA_KV8_ERR_STEP);  // of other tables
@@ -244,7 +246,7 @@ __global__ void __launch_bounds__(kStepThreads)
   }
   const int have = *num_free;
   auto slot_of = [&](int i) {
-    const int row = row_ids ? row_ids[i] : i;
+    const int row = rows_of_step[i];
     return row < slots ? row : -1;
   };
   int bad = 0;
@@ -384,12 +386,12 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
   return cudaGetLastError();
 }
 
-cudaError_t launch_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,
+cudaError_t launch_kv8_commit(const int32_t* query_lens, const int32_t* accepted,
                               const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
                               int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream) {
   const int threads = rows <= 128 ? 128 : kStepThreads;
   kv8_commit_kernel<<<1, threads, sizeof(int32_t) * (size_t(rows) + 1), stream>>>(
-      row_ids, query_lens, accepted, held_out, record, rows, slots, lens, held, num_free, err);
+      query_lens, accepted, held_out, record, rows, slots, lens, held, num_free, err);
   return cudaGetLastError();
 }
 

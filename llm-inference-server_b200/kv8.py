@@ -90,7 +90,7 @@ def _tiling(group: int, max_query_len: int, num_seqs: int, num_tokens: int) -> _
 
 
 # The step's arrays in one int32 buffer: work (int64, so first), num_free and the rest of what a
-# commit has to know (8-byte words among it), context_lens, query_lens, held, cu_query_lens,
+# commit has to know (8-byte words and the rows' slots among it), context_lens, query_lens, held, cu_query_lens,
 # seq_idx, q_pos, slot_mapping, block_tables.
 _FREE, _RECORD, _CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _TABLES = range(1, 11)
 
@@ -102,7 +102,7 @@ def _layout(b: int, t: int, cells: int) -> tuple[tuple[int, ...], tuple[int, ...
     """(words of each array, their byte offsets, words in all)."""
     got = _LAYOUTS.get((b, t, cells))
     if got is None:
-        sizes = (4 * (b + 1), 1, _lib.PA_KV8_STEP_WORDS - 1, b, b, b, b + 1, t, t, t, cells)
+        sizes = (4 * (b + 1), 1, _lib.PA_KV8_STEP_WORDS - 1 + b, b, b, b, b + 1, t, t, t, cells)
         got = (sizes, tuple(4 * sum(sizes[:i]) for i in range(len(sizes))), sum(sizes))
         if len(_LAYOUTS) > 1024:
             _LAYOUTS.clear()
@@ -127,9 +127,8 @@ class DeviceStep:
         self._ptr = [at + o for o in offsets]
         self._views: tuple[torch.Tensor, ...] | None = None
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
-        self._row_ids: torch.Tensor | None = None
         self._counted = False
-        self._home = 0                                # the address of the num_free it was reserved against
+        self._home = 0                                # the address of the num_free it was reserved against, if any
 
     @property
     def _arrays(self) -> tuple[torch.Tensor, ...]:
@@ -209,7 +208,7 @@ def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_le
         step = DeviceStep(b, num_tokens, w, max_query_len, block_size, num_blocks, group, dev, own_tables=False)
     elif step._sizes[_TABLES]:
         raise ValueError("out was made by DeviceBlockTables.reserve")
-    step._tables, step._row_ids = tables, None
+    step._tables = tables
     p = step._ptr
     _launch(dev, _lib.lib().pa_kv8_build_step, None, ctx.data_ptr(), ql.data_ptr(), tables.data_ptr(),
             max(tables.stride(0), w), None, None, None, 0, b, b, w, block_size, num_blocks, num_tokens, max_query_len,
@@ -304,7 +303,7 @@ class DeviceBlockTables:
         elif step._tables is not None:
             raise ValueError("out was made by device_step")
         home = self.num_free.data_ptr()
-        step._row_ids, step._counted, step._home = ids, False, home
+        step._counted, step._home = False, home
         p = step._ptr
         _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
                 self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
@@ -317,7 +316,7 @@ class DeviceBlockTables:
         """Make a reserved step count: its tokens (or the ``accepted[i]`` first of row i) are
         cached now and its blocks are held.  An emptied step changes nothing; nor does one that
         no longer fits the slots and the free list, which :func:`read_kv8_error` reports."""
-        if step._row_ids is None:
+        if not step._home:
             raise ValueError("commit needs a step made by reserve")
         if step._home != self.num_free.data_ptr():
             raise ValueError("this step was reserved in other tables")
@@ -329,7 +328,7 @@ class DeviceBlockTables:
                 raise ValueError(f"accepted must be [{step.num_seqs}], got {tuple(accepted.shape)}")
             acc = _int32("accepted", accepted, self.device)
         p = step._ptr
-        _launch(self.device, _lib.lib().pa_kv8_commit, step._row_ids.data_ptr(), p[_QL],
+        _launch(self.device, _lib.lib().pa_kv8_commit, None, p[_QL],
                 acc.data_ptr() if acc is not None else None, p[_HELD], p[_FREE], step.num_seqs, self.max_requests,
                 self.lens.data_ptr(), self.held.data_ptr(), self.num_free.data_ptr())
         step._counted = True

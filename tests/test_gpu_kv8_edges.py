@@ -246,3 +246,14 @@ def test_a_captured_commit_counts_its_step_once_and_reports(pkg):
     graph.replay()
     assert bt.lens.tolist() == [22, 6, 40, 0]
     assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
+def test_request_ids_may_be_filled_anew_before_the_commit(pkg):
+    """The step keeps its rows' slots: the caller's tensor is the next step's by then."""
+    bt = _tables(pkg)
+    ids = _i32([0, 1])
+    step = bt.reserve(ids, _i32([13, 1]), num_tokens=14, max_query_len=13)
+    ids.copy_(_i32([1, 2]))
+    bt.commit(step)
+    assert bt.lens.tolist() == [33, 6, 40, 0] and bt.held.tolist() == [3, 1, 3, 0]
+    assert sorted(_owned(bt)) == list(range(24))
