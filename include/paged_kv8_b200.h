@@ -32,7 +32,7 @@ extern "C" {
 #endif
 
 /* Bits of the KV8 error word. */
-#define PA_KV8_ERR_BLOCK 1    /* a block id outside the pool */
+#define PA_KV8_ERR_BLOCK 1    /* a block id outside the pool; a reserved step that would use it was emptied */
 #define PA_KV8_ERR_TIMEOUT 4  /* a bounded wait inside a kernel ran out */
 #define PA_KV8_ERR_STEP 8     /* inconsistent lengths or ids; the step was emptied */
 #define PA_KV8_ERR_NO_BLOCKS 16 /* the free list is too short; the step was emptied */
@@ -90,7 +90,8 @@ int32_t pa_kv8_choose_tiling(int32_t group, int32_t max_query_len, int32_t num_s
  * Nothing but `tables` is updated in place, so a step can be built again; pa_kv8_commit
  * makes it count.  A step whose lengths or ids are inconsistent (a slot named twice, more
  * tokens than num_tokens, a chunk over max_query_len, a context over width * block_size, a
- * free list too short) is emptied: all lengths 0, tables untouched, num_free_out -1.
+ * free list too short, with `held` a block id outside the pool where a new token goes) is
+ * emptied: all lengths 0, tables untouched, num_free_out -1.
  */
 int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int32_t* query_lens, int32_t* tables,
                           int64_t table_stride, const int32_t* held, const int32_t* free_blocks,

@@ -99,7 +99,14 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
           q = held = 0;
         } else {
           ctx = int(c);
-          if (p.held) need = max(0, (ctx + p.block_size - 1) / p.block_size - held);
+          if (p.held) {
+            need = max(0, (ctx + p.block_size - 1) / p.block_size - held);
+            // Blocks held before that take new tokens: a token without a place must not count.
+            for (int j = int(len) / p.block_size; q > 0 && j < held && j * p.block_size < ctx; ++j) {
+              const int id = p.tables[int64_t(row) * p.table_stride + j];
+              if (id < 0 || id >= p.pool_blocks) bad |= PA_KV8_ERR_BLOCK;
+            }
+          }
         }
       }
       s_ctx[i] = ctx;
@@ -130,6 +137,13 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
       bad |= PA_KV8_ERR_STEP;
     else if (blocks > avail)
       bad |= PA_KV8_ERR_NO_BLOCKS;
+    else {
+#pragma unroll 4
+      for (int b = tid; b < int(blocks); b += blockDim.x) {  // the new blocks: the list's last ones
+        const int id = p.free_blocks[avail - 1 - b];
+        if (id < 0 || id >= p.pool_blocks) bad |= PA_KV8_ERR_BLOCK;
+      }
+    }
   }
   if (tid == 0) s_cu[rows] = int32_t(tokens);
   const bool reject = __syncthreads_or(bad) != 0;
@@ -377,8 +391,8 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
                       (p.row_ids ? sizeof(uint32_t) * ((size_t(p.num_slots) + 31) / 32) : 0);
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_step_kernel), smem);
   if (e != cudaSuccess) return e;
-  // As many threads as rows, within limits: a sum over fewer warps is quicker.
-  const int threads = p.num_rows <= 128 ? 128 : kStepThreads;
+  // As many threads as rows or new blocks, within limits: a sum over fewer warps is quicker.
+  const int threads = p.num_rows <= 128 && p.num_tokens <= 128 * p.block_size ? 128 : kStepThreads;
   const int64_t cells = (p.held ? int64_t(p.num_rows) * p.width : 0) + (p.seq_idx ? p.num_tokens : 0);
   const int64_t want = (cells + threads - 1) / threads;
   const int grid = int(want < 1 ? 1 : (want < 148 ? want : 148));

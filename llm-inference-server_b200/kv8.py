@@ -286,9 +286,9 @@ class DeviceBlockTables:
                 group: int = 1, out: DeviceStep | None = None) -> DeviceStep:
         """The step that appends ``query_lens[i]`` tokens to request slot ``request_ids[i]``
         (-1: a padding row; a slot at most once), in one launch.  A slot that needs more blocks
-        than it holds takes them from the free list, rows in order.  When the list is too short
-        or the arguments do not fit together, the step is emptied (``num_free`` -1, an error
-        bit) and no table changes."""
+        than it holds takes them from the free list, rows in order.  When the list is too short,
+        a new token's block is outside the pool or the arguments do not fit together, the step
+        is emptied (``num_free`` -1, an error bit) and no table changes."""
         dev = self.device
         _check_step_sizes(num_tokens, max_query_len, self.block_size, self.num_blocks)
         if request_ids.dim() != 1 or query_lens.shape != request_ids.shape:

@@ -257,3 +257,27 @@ def test_request_ids_may_be_filled_anew_before_the_commit(pkg):
     bt.commit(step)
     assert bt.lens.tolist() == [33, 6, 40, 0] and bt.held.tolist() == [3, 1, 3, 0]
     assert sorted(_owned(bt)) == list(range(24))
+
+
+@pytest.mark.parametrize("bad", [24, -1, 1 << 30])
+@pytest.mark.parametrize("where", ["list", "held", "row of many"])
+def test_a_step_whose_new_tokens_have_a_bad_block_is_emptied_and_reports(pkg, where, bad):
+    """A block id outside the pool, new or held before: no token of the step counts and the id
+    does not reach the slots' tables."""
+    bt = _tables(pkg)
+    ids, ql = [0, 1, 3], [13, 1, 2]                            # slots 0 and 3 need a block, slot 1 has room
+    if where == "list":
+        bt.free[int(bt.num_free) - 2] = bad                    # slot 3's
+    elif where == "held":
+        bt.tables[1, 0] = bad
+    else:                                                      # a chunk over blocks that were held for it
+        bt.held[2] = 5
+        bt.tables[2, 3:5] = _i32([7, bad])
+        ids, ql = [1, 2], [1, 33]
+    before = _state_of(bt)
+    step = _reserve(bt, ids, ql)
+    assert int(step.num_free) == -1 and not step.context_lens.any() and not step.block_tables.any()
+    assert (step.slot_mapping == -1).all()
+    bt.commit(step)
+    assert _state_of(bt) == before
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_BLOCK
