@@ -281,3 +281,16 @@ def test_a_step_whose_new_tokens_have_a_bad_block_is_emptied_and_reports(pkg, wh
     bt.commit(step)
     assert _state_of(bt) == before
     assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_BLOCK
+
+
+@pytest.mark.parametrize("rows", [2380, 2400, 2430, 2440, 2460, 4070, 4085, 4095])
+def test_reserve_and_commit_of_any_row_count(pkg, rows):
+    """Among them the counts whose sums fill the shared memory that a launch has without asking."""
+    bt = pkg.DeviceBlockTables(rows, 2, 2 * rows, 16, DEV)
+    ids = torch.arange(rows, dtype=torch.int32, device=DEV)
+    step = bt.reserve(ids, torch.ones_like(ids), num_tokens=rows, max_query_len=1)
+    assert torch.equal(step.slot_mapping, 16 * ids)
+    bt.commit(step)
+    assert bool((bt.lens == 1).all()) and int(bt.num_free) == rows
+    bt.release(ids)
+    assert int(bt.num_free) == 2 * rows
