@@ -43,10 +43,10 @@ __device__ __forceinline__ void block_scan(int64_t (&v)[N], int64_t (&total)[N],
   __syncthreads();
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    // One warp's worth of partial sums (at most 16 warps), added up by every warp.
+    // One warp's worth of partial sums, added up by every warp.
     int64_t w = lane < warps ? scratch[lane][n] : 0;
 #pragma unroll
-    for (int d = 1; d < 16; d <<= 1) {
+    for (int d = 1; d < 32; d <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, w, d);
       if (lane >= d) w += up;
     }
@@ -243,41 +243,51 @@ __device__ __forceinline__ int row_of(const int32_t* at, int rows, int b) {
 // One CTA.  A step is planned from the slots and the free list as they are then, and other steps
 // may count or blocks come back before it does, so the plan is compared first: each slot's
 // length, the blocks that its new tokens went into, and that the step's new blocks are still the
-// free list's last ones.  Then all of it is written, or nothing.
-__global__ void __launch_bounds__(kStepThreads)
-    kv8_commit_kernel(const int32_t* query_lens, const int32_t* accepted,
-                      const int32_t* held_out, const Kv8StepRecord* record, int rows, int slots, int32_t* lens,
-                      int32_t* held, int32_t* num_free, int* err) {
-  extern __shared__ int32_t s_at[];  // [rows + 1] new blocks before the row
-  __shared__ int64_t scan[kStepThreads / 32][1];
+// free list's last ones.  Then all of it is written, or nothing.  What bounds it is latency: the
+// rows, their slots, the new blocks are three dependent loads, so a block's thread has nothing
+// else to look up in global memory (with its slot and place read there: 12 us for 8 prompts of
+// 4,096 tokens, 2,048 blocks, instead of 4.5).
+constexpr int kCommitThreads = 1024;
+__global__ void __launch_bounds__(kCommitThreads)
+    kv8_commit_kernel(const int32_t* query_lens, const int32_t* accepted, const int32_t* held_out,
+                      const Kv8StepRecord* record, int rows, int slots, int32_t* lens, int32_t* held,
+                      int32_t* num_free, int* err) {
+  extern __shared__ int32_t sm[];
+  int32_t* s_at = sm;              // [rows + 1] new blocks before the row
+  int32_t* s_row = s_at + rows + 1;  // [rows] request slot or -1
+  int32_t* s_held = s_row + rows;  // [rows]
+  __shared__ int64_t scan[kCommitThreads / 32][1];
   const int tid = threadIdx.x;
   const Kv8StepRecord r = *record;
   const int32_t* rows_of_step = reinterpret_cast<const int32_t*>(record + 1);
+  const int have = *num_free;
   if (r.num_free < 0) return;  // the step was emptied
   if (r.lens != lens || r.held != held || r.num_free_at != num_free || r.held_out != held_out || r.rows != rows) {
     if (tid == 0) set_error(err, PA_KV8_ERR_STEP);  // of other tables
     return;
   }
-  const int have = *num_free;
-  auto slot_of = [&](int i) {
-    const int row = rows_of_step[i];
-    return row < slots ? row : -1;
-  };
   int bad = 0;
   int64_t blocks = 0;
   for (int first = 0; first < rows; first += blockDim.x) {
-    const int i = first + tid, row = i < rows ? slot_of(i) : -1;
+    const int i = first + tid;
     int need = 0;
-    if (row >= 0) {
-      const int q = query_lens[i], ctx = r.context_lens[i], mine = held[row], base = lens[row];
-      need = held_out[i] - mine;
-      if (mine < 0 || need < 0 || held_out[i] > r.width || base < 0 || base + q != ctx) {
-        bad = 1;
-        need = 0;
-      } else if (q > 0) {
-        const int32_t *now = r.tables + int64_t(row) * r.table_stride, *then = r.out_tables + int64_t(i) * r.width;
-        for (int j = base / r.block_size; j < mine && j * r.block_size < ctx; ++j) bad |= now[j] != then[j];
+    if (i < rows) {
+      int row = rows_of_step[i], mine = 0;
+      if (row >= slots) row = -1;
+      if (row >= 0) {
+        const int q = query_lens[i], ctx = r.context_lens[i], base = lens[row];
+        mine = held[row];
+        need = held_out[i] - mine;
+        if (mine < 0 || need < 0 || held_out[i] > r.width || base < 0 || base + q != ctx) {
+          bad = 1;
+          need = 0;
+        } else if (q > 0) {
+          const int32_t *now = r.tables + int64_t(row) * r.table_stride, *then = r.out_tables + int64_t(i) * r.width;
+          for (int j = base / r.block_size; j < mine && j * r.block_size < ctx; ++j) bad |= now[j] != then[j];
+        }
       }
+      s_row[i] = row;
+      s_held[i] = mine;
     }
     int64_t at[1] = {need}, sum[1];
     block_scan(at, sum, scan);
@@ -286,11 +296,15 @@ __global__ void __launch_bounds__(kStepThreads)
   }
   if (tid == 0) s_at[rows] = int32_t(blocks);
   if (have > r.free_capacity || blocks > have) bad = 1;
-  bool stale = __syncthreads_or(bad) != 0;
-  if (!stale) {
+  bool stale = __syncthreads_or(bad) != 0, other = false;
+  // A new block's place in its slot's table, of which `other` learns that another plan, one that
+  // was dropped, has been written there.
+  auto place = [&](int i, int b) { return r.tables + int64_t(s_row[i]) * r.table_stride + s_held[i] + b - s_at[i]; };
+  if (!stale && blocks > 0) {
     for (int b = tid; b < int(blocks); b += blockDim.x) {
-      const int i = row_of(s_at, rows, b), j = held[slot_of(i)] + b - s_at[i];
-      bad |= r.free_blocks[have - 1 - b] != r.out_tables[int64_t(i) * r.width + j];
+      const int i = row_of(s_at, rows, b), id = r.out_tables[int64_t(i) * r.width + s_held[i] + b - s_at[i]];
+      bad |= r.free_blocks[have - 1 - b] != id;
+      other |= *place(i, b) != id;
     }
     stale = __syncthreads_or(bad) != 0;
   }
@@ -298,14 +312,10 @@ __global__ void __launch_bounds__(kStepThreads)
     if (tid == 0) set_error(err, PA_KV8_ERR_STEP);
     return;
   }
-  // The slots' tables too: a step that was dropped may have been written over this one's blocks.
-  for (int b = tid; b < int(blocks); b += blockDim.x) {
-    const int i = row_of(s_at, rows, b), row = slot_of(i), j = held[row] + b - s_at[i];
-    r.tables[int64_t(row) * r.table_stride + j] = r.free_blocks[have - 1 - b];
-  }
-  __syncthreads();
+  if (other)
+    for (int b = tid; b < int(blocks); b += blockDim.x) *place(row_of(s_at, rows, b), b) = r.free_blocks[have - 1 - b];
   for (int i = tid; i < rows; i += blockDim.x) {
-    const int row = slot_of(i);
+    const int row = s_row[i];
     if (row < 0) continue;
     const int q = query_lens[i];
     lens[row] += accepted ? max(0, min(accepted[i], q)) : q;
@@ -404,9 +414,11 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
 cudaError_t launch_kv8_commit(const int32_t* query_lens, const int32_t* accepted,
                               const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
                               int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream) {
-  const int threads = rows <= 128 ? 128 : kStepThreads;
-  kv8_commit_kernel<<<1, threads, sizeof(int32_t) * (size_t(rows) + 1), stream>>>(
-      query_lens, accepted, held_out, record, rows, slots, lens, held, num_free, err);
+  const size_t smem = sizeof(int32_t) * (3 * size_t(rows) + 1);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_commit_kernel), smem);
+  if (e != cudaSuccess) return e;
+  kv8_commit_kernel<<<1, kCommitThreads, smem, stream>>>(query_lens, accepted, held_out, record, rows, slots, lens, held,
+                                                         num_free, err);
   return cudaGetLastError();
 }
 
