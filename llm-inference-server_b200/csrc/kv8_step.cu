@@ -391,16 +391,27 @@ int* kv8_error_word() {
   return known[dev];
 }
 
-// The limit without asking is 48 KB with the kernel's own static shared memory (under 1 KB).
-static cudaError_t allow_smem(const void* kern, size_t bytes) {
-  return bytes <= 47 * 1024 ? cudaSuccess
-                            : cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+// Asked for once per device and for the largest call: a request per call, of its own size, took
+// back what another host thread had just asked for.
+static cudaError_t allow_smem(const void* kern, size_t most, bool (&asked)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 0 || dev >= 64) return cudaErrorInvalidDevice;
+  if (asked[dev]) return cudaSuccess;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(most));
+  if (e == cudaSuccess) asked[dev] = true;
+  return e;
 }
+static constexpr size_t step_smem(size_t rows, size_t slots) { return 4 * (5 * rows + 1) + 4 * ((slots + 31) / 32); }
+static constexpr size_t commit_smem(size_t rows) { return 4 * (3 * rows + 1); }
+static constexpr size_t release_smem(size_t count, size_t slots) { return 4 * (count + 1) + 4 * ((slots + 31) / 32); }
 
 cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t stream) {
-  const size_t smem = sizeof(int32_t) * (5 * size_t(p.num_rows) + 1) +
-                      (p.row_ids ? sizeof(uint32_t) * ((size_t(p.num_slots) + 31) / 32) : 0);
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_step_kernel), smem);
+  const size_t smem = step_smem(size_t(p.num_rows), p.row_ids ? size_t(p.num_slots) : 0);
+  static bool asked[64];
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_step_kernel),
+                             step_smem(PA_KV8_MAX_ROWS, PA_KV8_MAX_REQUESTS), asked);
   if (e != cudaSuccess) return e;
   // As many threads as rows or new blocks, within limits: a sum over fewer warps is quicker.
   const int threads = p.num_rows <= 128 && p.num_tokens <= 128 * p.block_size ? 128 : kStepThreads;
@@ -414,8 +425,9 @@ cudaError_t launch_kv8_step(const Kv8StepParams& p, int* err, cudaStream_t strea
 cudaError_t launch_kv8_commit(const int32_t* query_lens, const int32_t* accepted,
                               const int32_t* held_out, const Kv8StepRecord* record, int32_t rows, int32_t slots,
                               int32_t* lens, int32_t* held, int32_t* num_free, int* err, cudaStream_t stream) {
-  const size_t smem = sizeof(int32_t) * (3 * size_t(rows) + 1);
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_commit_kernel), smem);
+  const size_t smem = commit_smem(size_t(rows));
+  static bool asked[64];
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_commit_kernel), commit_smem(PA_KV8_MAX_ROWS), asked);
   if (e != cudaSuccess) return e;
   kv8_commit_kernel<<<1, kCommitThreads, smem, stream>>>(query_lens, accepted, held_out, record, rows, slots, lens, held,
                                                          num_free, err);
@@ -425,8 +437,10 @@ cudaError_t launch_kv8_commit(const int32_t* query_lens, const int32_t* accepted
 cudaError_t launch_kv8_release(const int32_t* ids, int32_t count, const int32_t* tables, int64_t table_stride,
                                int32_t width, int32_t slots, int32_t* lens, int32_t* held, int32_t* free_blocks,
                                int32_t free_capacity, int32_t* num_free, int* err, cudaStream_t stream) {
-  const size_t smem = sizeof(int32_t) * (size_t(count) + 1) + sizeof(uint32_t) * ((size_t(slots) + 31) / 32);
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_release_kernel), smem);
+  const size_t smem = release_smem(size_t(count), size_t(slots));
+  static bool asked[64];
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(kv8_release_kernel),
+                             release_smem(PA_KV8_MAX_ROWS, PA_KV8_MAX_REQUESTS), asked);
   if (e != cudaSuccess) return e;
   kv8_release_kernel<<<1, kStepThreads, smem, stream>>>(ids, count, tables, table_stride, width, slots, lens, held,
                                                         free_blocks, free_capacity, num_free, err);

@@ -294,3 +294,30 @@ def test_reserve_and_commit_of_any_row_count(pkg, rows):
     assert bool((bt.lens == 1).all()) and int(bt.num_free) == rows
     bt.release(ids)
     assert int(bt.num_free) == 2 * rows
+
+
+def test_reserve_on_two_host_threads(pkg):
+    """Steps of different sizes, whose shared memory has to be asked for, side by side."""
+    import threading
+
+    failed = []
+
+    def work(rows):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                bt = pkg.DeviceBlockTables(rows, 2, rows, 16, DEV)
+                ids = torch.arange(rows, dtype=torch.int32, device=DEV)
+                one = torch.ones_like(ids)
+                step = None
+                for _ in range(2000):
+                    step = bt.reserve(ids, one, num_tokens=rows, max_query_len=1, out=step)
+                assert torch.equal(step.slot_mapping, 16 * ids)
+        except BaseException as e:  # noqa: BLE001  (to the test's own thread)
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(n,)) for n in (4096, 2700, 3300)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed, failed
