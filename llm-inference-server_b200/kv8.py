@@ -429,9 +429,10 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     itself (past 64 sequences in a launch of its own) unless ``block_tables`` carries one
     (:func:`attach_step`).
 
-    query ``[T, Hq, D]``, float16 or bfloat16, D 64 or 128, at most 16 query heads per KV
-    head; pools' block size a power of two times 16.  Rows past the last sequence's are left
-    as they were in ``out`` (undefined without ``out``)."""
+    query ``[T, Hq, D]``, float16 or bfloat16, any strides and offset (rows that are not 16-byte
+    aligned are copied first), D 64 or 128, at most 16 query heads per KV head; ``out``
+    contiguous and 16-byte aligned; pools' block size a power of two times 16.  Rows past the
+    last sequence's are left as they were in ``out`` (undefined without ``out``)."""
     if query.dim() != 3:
         raise ValueError(f"query must be [num_tokens, heads, dim], got {tuple(query.shape)}")
     dev = query.device
@@ -475,7 +476,7 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         return out
     qs = query.stride()
     if qs[2] != 1 or qs[0] % 8 or qs[1] % 8 or query.data_ptr() % 16:
-        query = query.contiguous()
+        query = query.clone(memory_format=torch.contiguous_format)   # rows of 16 bytes, contiguous before or not
         qs = query.stride()
     scratch = _scratch(dev, b, tokens, heads, hkv, dim, most)
     _launch(dev, _lib.lib().pa_kv8_attention, query.data_ptr(), qs[0], qs[1], tokens, heads, dim, k_pool.data_ptr(),

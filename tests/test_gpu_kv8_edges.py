@@ -321,3 +321,21 @@ def test_reserve_on_two_host_threads(pkg):
     for t in threads:
         t.join()
     assert not failed, failed
+
+
+# ------------------------------------------------------------------ views, ids and sizes of any kind
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_queries_at_odd_offsets(pkg, tokens):
+    """Contiguous queries that do not start on 16 bytes, and one token whose token stride (which no
+    address depends on) is odd."""
+    query, pools, tables, ctx, ql = _batch([(90, tokens)], 8, 2, 128, 16, torch.bfloat16, seed=9)
+    want = pkg.paged_attention_kv8(query, *pools, tables, ctx, ql, 0.1, max_query_len=tokens)
+    for off in (1, 4):
+        flat = torch.zeros(query.numel() + off, dtype=query.dtype, device=DEV)
+        view = flat[off:].view_as(query)
+        view.copy_(query)
+        assert view.is_contiguous() and view.data_ptr() % 16
+        assert torch.equal(want, pkg.paged_attention_kv8(view, *pools, tables, ctx, ql, 0.1, max_query_len=tokens))
+    view = torch.zeros(tokens * 1027, dtype=query.dtype, device=DEV).as_strided((tokens, 8, 128), (1027, 128, 1))
+    view.copy_(query)
+    assert torch.equal(want, pkg.paged_attention_kv8(view, *pools, tables, ctx, ql, 0.1, max_query_len=tokens))
