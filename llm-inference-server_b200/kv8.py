@@ -56,8 +56,8 @@ def _int32(name: str, t: torch.Tensor, device: torch.device) -> torch.Tensor:
         raise ValueError(f"{name} must be int32 or int64, got {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, expected {device}")
-    if t.dtype != torch.int32:
-        t = t.to(torch.int32)
+    if t.dtype != torch.int32:   # what 32 bits do not hold stays out of range, not its low half
+        t = t.clamp(-2 ** 31, 2 ** 31 - 1).to(torch.int32)
     return t if t.is_contiguous() else t.contiguous()
 
 

@@ -339,3 +339,22 @@ def test_queries_at_odd_offsets(pkg, tokens):
     view = torch.zeros(tokens * 1027, dtype=query.dtype, device=DEV).as_strided((tokens, 8, 128), (1027, 128, 1))
     view.copy_(query)
     assert torch.equal(want, pkg.paged_attention_kv8(view, *pools, tables, ctx, ql, 0.1, max_query_len=tokens))
+
+
+def test_wide_ids_are_not_wrapped_and_reports(pkg):
+    """64-bit slots, ids and lengths past 32 bits are out of range, not their low halves."""
+    nb, hkv, d = 4, 2, 64
+    pools = [torch.zeros(nb, 16, hkv, d, dtype=torch.uint8, device=DEV).view(ref.E4M3) for _ in range(2)]
+    pools += [torch.zeros(nb, hkv, 16, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    rows = torch.ones(3, hkv, d, device=DEV)
+    pkg.reshape_and_cache_kv8(rows, rows, *pools, torch.tensor([(1 << 32) + 5, 7, -(1 << 32) + 9], device=DEV))
+    assert pools[2][0, 0].nonzero().flatten().tolist() == [7]
+    bt = _tables(pkg)
+    step = bt.reserve(torch.tensor([1 << 32], device=DEV), _i32([1]), num_tokens=1, max_query_len=1)
+    assert int(step.num_free) == -1 and pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+    step = pkg.device_step(_i32([[0, 1]]), torch.tensor([(1 << 32) + 3], device=DEV), _i32([1]), num_tokens=1,
+                           max_query_len=1, num_blocks=4, block_size=16)
+    assert step.slot_mapping.tolist() == [-1] and pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+    step = pkg.device_step(torch.tensor([[1 << 32, 1]], device=DEV), _i32([3]), _i32([1]), num_tokens=1,
+                           max_query_len=1, num_blocks=4, block_size=16)
+    assert step.slot_mapping.tolist() == [-1] and pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_BLOCK
