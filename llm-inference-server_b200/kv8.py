@@ -128,6 +128,7 @@ class DeviceStep:
         self._views: tuple[torch.Tensor, ...] | None = None
         self._tables: torch.Tensor | None = None      # the caller's, when the step has none of its own
         self._counted = False
+        self._captured = False                        # a graph's replays make it again, unseen here
         self._home = 0                                # the address of the num_free it was reserved against, if any
 
     @property
@@ -304,6 +305,7 @@ class DeviceBlockTables:
             raise ValueError("out was made by device_step")
         home = self.num_free.data_ptr()
         step._counted, step._home = False, home
+        step._captured |= torch.cuda.is_current_stream_capturing()
         p = step._ptr
         _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
                 self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
@@ -315,12 +317,13 @@ class DeviceBlockTables:
     def commit(self, step: DeviceStep, accepted: torch.Tensor | None = None) -> None:
         """Make a reserved step count: its tokens (or the ``accepted[i]`` first of row i) are
         cached now and its blocks are held.  An emptied step changes nothing; nor does one that
-        no longer fits the slots and the free list, which :func:`read_kv8_error` reports."""
+        no longer fits the slots and the free list, which :func:`read_kv8_error` reports.  A
+        step counts once (one whose ``reserve`` was captured, once a replay)."""
         if not step._home:
             raise ValueError("commit needs a step made by reserve")
         if step._home != self.num_free.data_ptr():
             raise ValueError("this step was reserved in other tables")
-        if step._counted:
+        if step._counted and not step._captured:
             raise ValueError("this step was committed before")
         acc = None
         if accepted is not None:

@@ -358,3 +358,25 @@ def test_wide_ids_are_not_wrapped_and_reports(pkg):
     step = pkg.device_step(torch.tensor([[1 << 32, 1]], device=DEV), _i32([3]), _i32([1]), num_tokens=1,
                            max_query_len=1, num_blocks=4, block_size=16)
     assert step.slot_mapping.tolist() == [-1] and pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_BLOCK
+
+
+def test_a_replayed_reserve_may_be_committed_outside_the_graph_and_reports(pkg):
+    """A captured step with the commit outside: the accepted counts come from somewhere else."""
+    bt = _tables(pkg)
+    ids, ql = _i32([0, 1]), _i32([4, 4])
+    step = bt.reserve(ids, ql, num_tokens=8, max_query_len=4)
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        bt.reserve(ids, ql, num_tokens=8, max_query_len=4, out=step)
+    torch.cuda.current_stream().wait_stream(side)
+    want = [20, 5]
+    for accepted in ([1, 4], [0, 3], [4, 2]):
+        graph.replay()
+        bt.commit(step, _i32(accepted))
+        want = [a + b for a, b in zip(want, accepted)]
+        assert bt.lens.tolist()[:2] == want
+    bt.commit(step)                                            # without a replay: the lengths have moved on
+    assert bt.lens.tolist()[:2] == want
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
