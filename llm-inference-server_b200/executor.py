@@ -37,7 +37,7 @@ import torch
 from transformers import AttentionInterface, Cache
 
 from .attention import paged_attention_cuda
-from .kv8 import KV8Pool, attach_step, paged_attention_kv8, reshape_and_cache_kv8, step_of_metadata
+from .kv8 import KV8Pool, attach_step, check_group, paged_attention_kv8, reshape_and_cache_kv8, step_of_metadata
 from .kv_cache import copy_blocks, reshape_and_cache
 from .metadata import StepMetadata, attach, prefill_tile_tokens
 
@@ -130,6 +130,8 @@ class CudaPagedExecutor:
         self.group = heads // self.num_kv_heads
         if isinstance(pool, KV8Pool) and next(model.parameters()).dtype == torch.float32:
             raise NotImplementedError("ATTENTION=cuda: the 8-bit cache takes float16 and bfloat16 models, not float32")
+        if isinstance(pool, KV8Pool):
+            check_group(self.group)
         self.tile_tokens = prefill_tile_tokens(heads, self.num_kv_heads, head_dim)
 
     @torch.inference_mode()

@@ -89,6 +89,11 @@ def _tiling(group: int, max_query_len: int, num_seqs: int, num_tokens: int) -> _
     return t
 
 
+def check_group(group: int) -> None:
+    """Refuses what the attention kernels do not take of query heads per KV head."""
+    _tiling(group, 1, 1, 1)
+
+
 # The step's arrays in one int32 buffer: work (int64, so first), num_free and the rest of what a
 # commit has to know (8-byte words and the rows' slots among it), context_lens, query_lens, held, cu_query_lens,
 # seq_idx, q_pos, slot_mapping, block_tables.

@@ -380,3 +380,14 @@ def test_a_replayed_reserve_may_be_committed_outside_the_graph_and_reports(pkg):
     bt.commit(step)                                            # without a replay: the lengths have moved on
     assert bt.lens.tolist()[:2] == want
     assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
+def test_the_executor_refuses_too_many_query_heads_at_once(pkg):
+    import importlib
+    from types import SimpleNamespace
+
+    mod = importlib.import_module(f"{pkg.__name__}.executor")
+    model = SimpleNamespace(config=SimpleNamespace(num_attention_heads=34),
+                            parameters=lambda: iter([torch.zeros(1, dtype=torch.bfloat16)]))
+    with pytest.raises(NotImplementedError, match="17 query heads per KV head: at most 16"):
+        mod.CudaPagedExecutor(model, None, pkg.KV8Pool(1, 4, 16, 2, 64, DEV))
