@@ -44,6 +44,9 @@ class DecodeStepGraph:
         ref = self.k_pools[0]
         if ref.device.type != "cuda":
             raise NotImplementedError(f"ATTENTION=cuda: decode graphs need CUDA pools, got {ref.device}")
+        if ref.dtype not in _DTYPE_CODE:
+            raise NotImplementedError(f"ATTENTION=cuda: decode graphs need float32, float16 or bfloat16 pools, got "
+                                      f"{ref.dtype}; over 8-bit pools CudaPagedExecutor's decode graphs run")
         self.device = torch.device(device) if device is not None else ref.device
         self.L = len(self.k_pools)
         self.NB, self.BS, self.Hkv, self.D = (int(x) for x in ref.shape)

@@ -391,3 +391,12 @@ def test_the_executor_refuses_too_many_query_heads_at_once(pkg):
                             parameters=lambda: iter([torch.zeros(1, dtype=torch.bfloat16)]))
     with pytest.raises(NotImplementedError, match="17 query heads per KV head: at most 16"):
         mod.CudaPagedExecutor(model, None, pkg.KV8Pool(1, 4, 16, 2, 64, DEV))
+
+
+def test_decode_step_graphs_refuse_8_bit_pools(pkg):
+    import importlib
+
+    mod = importlib.import_module(f"{pkg.__name__}.graphs")
+    pool = pkg.KV8Pool(1, 4, 16, 2, 64, DEV)
+    with pytest.raises(NotImplementedError, match="float32, float16 or bfloat16"):
+        mod.DecodeStepGraph(pool.k, pool.v, num_heads=4, scale=0.1, batch=1, width=2)
