@@ -72,7 +72,7 @@ constexpr int kTileRows = kKv8TileRows;
 constexpr int kHalfRows = 128;
 constexpr int kTileKeys = 64;
 constexpr int kTileKStages = 3;
-constexpr int kTileVStages = 2;  // equal to the P buffer count: one "P.V retired" barrier frees both
+constexpr int kTileVStages = 2;
 constexpr int kTileRing = 4;     // staged e4m3 tiles, K and V each
 constexpr int kTileThreads = 768;
 // Registers a thread: at launch and by role.  What the softmax takes, the others have given back.

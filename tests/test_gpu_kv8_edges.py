@@ -400,3 +400,34 @@ def test_decode_step_graphs_refuse_8_bit_pools(pkg):
     pool = pkg.KV8Pool(1, 4, 16, 2, 64, DEV)
     with pytest.raises(NotImplementedError, match="float32, float16 or bfloat16"):
         mod.DecodeStepGraph(pool.k, pool.v, num_heads=4, scale=0.1, batch=1, width=2)
+
+
+# ------------------------------------------------------------------ neighbours
+@pytest.mark.parametrize("own", [(700, 2), (1500, 3), (517, 1), (600, 70), (130, 130), (2000, 300)])
+def test_a_sequence_among_neighbours(pkg, own):
+    """A sequence alone and first, between and last among others, whose keys move the cuts that fall
+    into its own: each time as near to 64 bits as alone."""
+    hq, hkv, d = 8, 2, 128
+    around = [(90, 1), (4000, 2), (33, 33), (0, 0), (900, 64), (5, 5)]
+    query, pools, tables, ctx, ql = _batch([own] + around, hq, hkv, d, 16, torch.bfloat16, seed=own[0])
+    k, v = (ref.dequantise(pools[i].view(torch.uint8), pools[i + 2]) for i in (0, 1))
+    starts = torch.cat([ql.new_zeros(1), ql.cumsum(0)]).tolist()
+    for order in ([0], [0, 1, 2], [2, 0, 4], [1, 4, 0], [3, 2, 1, 0, 5, 4], [5, 4, 3, 2, 1, 0]):
+        q = torch.cat([query[starts[i]:starts[i + 1]] for i in order])
+        c, n, t = ctx[order], ql[order], tables[order]
+        got = pkg.paged_attention_kv8(q, *pools, t, c, n, 0.09, max_query_len=int(n.max()))
+        want, mean, slip = ref.attention(q, k, v, t, c.tolist(), n.tolist(), 0.09)
+        lost = ref.lost_weight(t, c.tolist(), n.tolist(), v, hq, TILES)
+        assert ((got.double() - want).abs() <= ref.tight_tolerance(want, mean, slip, lost, torch.bfloat16, d)).all(), order
+
+
+def test_few_rows_keep_small_weights_over_a_long_context(pkg):
+    """131,071 keys of which all but every 32nd have a weight of 2^-18.8 of the maximum and V rows
+    of the smallest scale, cut over many CTAs and joined."""
+    batch = _peaked([(131071, 1), (40, 1)], 8, 2, 128, torch.bfloat16, 32, 13.0, (113,), seed=5)
+    _check_tight(pkg, *batch, 1.0, 1, ROWS)
+
+
+def test_long_chunks_keep_small_weights_over_a_long_context(pkg):
+    batch = _peaked([(60001, 40)], 8, 2, 128, torch.float16, 64, 13.0, (113, 116), seed=7)
+    _check_tight(pkg, *batch, 1.0, 40, TILES)
