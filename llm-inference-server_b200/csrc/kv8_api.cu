@@ -294,7 +294,8 @@ int32_t pa_kv8_attention(const void* query, int64_t q_stride_token, int64_t q_st
   const int group = num_heads / num_kv_heads;
   int32_t st = pa_kv8_choose_tiling(group, max_query_len, num_seqs, num_tokens, &t);
   if (st != PA_OK) return st;
-  if (num_tokens == 0 || num_seqs == 0 || pool_num_blocks == 0) return PA_OK;
+  if (num_tokens == 0 || num_seqs == 0) return PA_OK;
+  if (pool_num_blocks == 0) return fail(PA_ERR_INVALID_ARGUMENT, "the pool has no blocks");
   const bool build = !work && !cu_query_lens;
   if (!query || !k_pool || !v_pool || !k_scale || !v_scale || !block_tables || !context_lens || !out || !workspace ||
       (build ? !query_lens : (!cu_query_lens || !work)))

@@ -210,3 +210,11 @@ def test_commit_and_release_refusals(pkg):
     with pytest.raises(NotImplementedError, match="at most"):
         check(lib.pa_kv8_release(16, 5000, 16, 4, 4, 1, 16, 16, 16, 4, 16, None))
     check(lib.pa_kv8_release(None, 0, None, 4, 4, 1, None, None, None, 4, None, None))  # nothing to do
+
+
+def test_attention_over_a_pool_without_blocks_is_refused(pkg):
+    """It returned at once, the output unwritten and nothing reported."""
+    with pytest.raises(ValueError, match="no blocks"):
+        pkg._lib.check(pkg._lib.lib().pa_kv8_attention(*(_ATTN | dict(blocks=0)).values()))
+    for nothing in (dict(tokens=0), dict(seqs=0)):
+        pkg._lib.check(pkg._lib.lib().pa_kv8_attention(*(_ATTN | dict(blocks=0) | nothing).values()))
