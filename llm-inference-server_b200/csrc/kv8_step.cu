@@ -80,7 +80,8 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
   int64_t tokens = 0, blocks = 0, small = 0, large = 0;  // totals so far
   for (int first = 0; first < rows; first += blockDim.x) {
     const int i = first + tid;
-    int q = 0, ctx = 0, held = 0, need = 0, row = -1;
+    int q = 0, ctx = 0, held = 0, need = 0, row = -1, into = 0;
+    bool touches = false;
     if (i < rows) {
       row = p.row_ids ? p.row_ids[i] : i;
       if (row >= p.num_slots || row < -1) {
@@ -101,11 +102,14 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
           ctx = int(c);
           if (p.held) {
             need = max(0, (ctx + p.block_size - 1) / p.block_size - held);
-            // Blocks held before that take new tokens: a token without a place must not count.
-            for (int j = int(len) / p.block_size; q > 0 && j < held && j * p.block_size < ctx; ++j) {
-              const int id = p.tables[int64_t(row) * p.table_stride + j];
-              if (id < 0 || id >= p.pool_blocks) bad |= PA_KV8_ERR_BLOCK;
-            }
+            // Blocks held before that take new tokens: a token without a place must not count.  The
+            // first, mostly the only one, is looked at behind the sums, which hide its load.
+            const int32_t* mine = p.tables + int64_t(row) * p.table_stride;
+            const int last = q > 0 ? min(held, (ctx + p.block_size - 1) / p.block_size) : 0;
+            int j = int(len) / p.block_size;
+            touches = j < last;
+            if (touches) into = mine[j];
+            while (++j < last) bad |= mine[j] < 0 || mine[j] >= p.pool_blocks ? PA_KV8_ERR_BLOCK : 0;
           }
         }
       }
@@ -118,6 +122,7 @@ __global__ void __launch_bounds__(kStepThreads) kv8_step_kernel(const Kv8StepPar
     const int64_t keys = q > 0 ? line_keys_before(ctx - q, q, tt, (q + tt - 1) / tt) : 0;
     int64_t v[4] = {q, need, few ? keys : 0, few ? 0 : keys}, total[4];
     block_scan(v, total, scan);
+    if (touches && (into < 0 || into >= p.pool_blocks)) bad |= PA_KV8_ERR_BLOCK;
     if (i < rows) {
       s_cu[i] = int32_t(tokens + v[0]);
       s_new[i] = int32_t(blocks + v[1]);
