@@ -490,7 +490,8 @@ __global__ void __launch_bounds__(RowsCfg<D, RG, PAIR>::THREADS, RowsCfg<D, RG, 
               for (int e = 0; e < 2; ++e) {
                 const int key = 16 * n + 8 * h + g;
                 float& v = s[n][rg][2 * h + e];
-                v *= ks[n][h][PAIR && second[rg][e] ? C::SUBS - 1 : 0] * (e ? factor.y : factor.x);
+                const float k = PAIR && second[rg][e] ? ks[n][h][C::SUBS - 1] : ks[n][h][0];
+                v *= k * (e ? factor.y : factor.x);
                 if (masked && key0 + key > (e ? limit.y : limit.x)) v = -INFINITY;
                 mx[e] = fmaxf(mx[e], v);
               }
