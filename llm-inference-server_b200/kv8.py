@@ -94,21 +94,25 @@ def check_group(group: int) -> None:
     _tiling(group, 1, 1, 1)
 
 
-# The step's arrays in one int32 buffer: work (int64, so first), num_free and the rest of what a
-# commit has to know (8-byte words and the rows' slots among it), context_lens, query_lens, held, cu_query_lens,
+# The step's arrays in one int32 buffer: num_free with the rest of what a commit has to know (8-byte
+# words and the rows' slots among it), work (int64), context_lens, query_lens, held, cu_query_lens,
 # seq_idx, q_pos, slot_mapping, block_tables.
-_FREE, _RECORD, _CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _TABLES = range(1, 11)
+_FREE, _WORK, _CTX, _QL, _HELD, _CU, _SEQ, _POS, _SLOT, _TABLES = range(10)
 
 
 _LAYOUTS: dict[tuple[int, int, int], tuple[tuple[int, ...], tuple[int, ...], int]] = {}
 
 
 def _layout(b: int, t: int, cells: int) -> tuple[tuple[int, ...], tuple[int, ...], int]:
-    """(words of each array, their byte offsets, words in all)."""
+    """(words of each array, their byte offsets, words in all); work's words have the rest of the
+    commit's record before them."""
     got = _LAYOUTS.get((b, t, cells))
     if got is None:
-        sizes = (4 * (b + 1), 1, _lib.PA_KV8_STEP_WORDS - 1 + b, b, b, b, b + 1, t, t, t, cells)
-        got = (sizes, tuple(4 * sum(sizes[:i]) for i in range(len(sizes))), sum(sizes))
+        record = (_lib.PA_KV8_STEP_WORDS + b + 1) // 2 * 2
+        sizes = (1, record - 1 + 4 * (b + 1), b, b, b, b + 1, t, t, t, cells)
+        offsets = [4 * sum(sizes[:i]) for i in range(len(sizes))]
+        offsets[_WORK] = 4 * record
+        got = (sizes, tuple(offsets), sum(sizes))
         if len(_LAYOUTS) > 1024:
             _LAYOUTS.clear()
         _LAYOUTS[(b, t, cells)] = got
@@ -142,7 +146,8 @@ class DeviceStep:
             self._views = torch.unsafe_split_with_sizes(self.buffer, self._sizes)  # int32: autograd has no say
         return self._views
 
-    work = property(lambda self: self._arrays[0].view(torch.int64).view(2, self.num_seqs + 1))
+    work = property(lambda self: self._arrays[_WORK][-4 * (self.num_seqs + 1):].view(torch.int64)
+                    .view(2, self.num_seqs + 1))
     context_lens = property(lambda self: self._arrays[_CTX])
     query_lens = property(lambda self: self._arrays[_QL])
     held = property(lambda self: self._arrays[_HELD])
@@ -218,7 +223,7 @@ def device_step(block_tables: torch.Tensor, context_lens: torch.Tensor, query_le
     p = step._ptr
     _launch(dev, _lib.lib().pa_kv8_build_step, None, ctx.data_ptr(), ql.data_ptr(), tables.data_ptr(),
             max(tables.stride(0), w), None, None, None, 0, b, b, w, block_size, num_blocks, num_tokens, max_query_len,
-            ctypes.byref(tiling), None, p[_CTX], p[_QL], p[_HELD], p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[0])
+            ctypes.byref(tiling), None, p[_CTX], p[_QL], p[_HELD], p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[_WORK])
     return step
 
 
@@ -310,13 +315,13 @@ class DeviceBlockTables:
             raise ValueError("out was made by device_step")
         home = self.num_free.data_ptr()
         step._counted, step._home = False, home
-        step._captured |= torch.cuda.is_current_stream_capturing()
+        step._captured |= torch._C._cuda_isCurrentStreamCapturing()
         p = step._ptr
         _launch(dev, _lib.lib().pa_kv8_build_step, ids.data_ptr(), self.lens.data_ptr(), ql.data_ptr(),
                 self.tables.data_ptr(), self.width, self.held.data_ptr(), self.free.data_ptr(),
                 home, self.free.shape[0], b, self.max_requests, self.width, self.block_size,
                 self.num_blocks, num_tokens, max_query_len, ctypes.byref(tiling), p[_TABLES], p[_CTX], p[_QL], p[_HELD],
-                p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[0])
+                p[_CU], p[_SEQ], p[_POS], p[_SLOT], p[_FREE], p[_WORK])
         return step
 
     def commit(self, step: DeviceStep, accepted: torch.Tensor | None = None) -> None:
@@ -467,7 +472,7 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                              f"{group}, {nb} of {bs} on {dev}")
         tables, p = step.block_tables, step._ptr
         b, w, most = step.num_seqs, step.width, step.max_query_len
-        ctx, lens, cu, work = p[_CTX], None, p[_CU], p[0]
+        ctx, lens, cu, work = p[_CTX], None, p[_CU], p[_WORK]
     else:
         if block_tables.dim() != 2:
             raise ValueError("block_tables must be [batch, max_blocks]")
