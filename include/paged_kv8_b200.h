@@ -13,8 +13,8 @@
  * payload and one scale byte b that stands for 2^(b - 127), b in [113, 134]:
  *   b       = 127 + the least e in [-14, 7] with max|x| <= 448 * 2^e
  *   payload = e4m3(x * 2^-e), round to nearest even, saturating
- * so every cached value is exactly an fp16 number; magnitudes past 57,344 saturate.  A row
- * that holds a NaN is stored as zeros with b = 255, which stands for NaN.
+ * so every cached value is exactly an fp16 number; magnitudes past 57,344 saturate, and rows
+ * below 448 * 2^-15 keep e = -14, a step of 2^-23.  A row that holds a NaN is stored as zeros with b = 255, which stands for NaN.
  *   payload pool [num_blocks, block_size, num_kv_heads, head_dim]   1 byte each
  *   scale pool   [num_blocks, num_kv_heads, block_size]             1 byte each
  *
@@ -34,7 +34,7 @@ extern "C" {
 /* Bits of the KV8 error word. */
 #define PA_KV8_ERR_BLOCK 1    /* a block id outside the pool; a reserved step that would use it was emptied */
 #define PA_KV8_ERR_TIMEOUT 4  /* a bounded wait inside a kernel ran out */
-#define PA_KV8_ERR_STEP 8     /* inconsistent lengths or ids; the step was emptied */
+#define PA_KV8_ERR_STEP 8     /* inconsistent lengths or ids: the step was emptied; or it was stale: not committed */
 #define PA_KV8_ERR_NO_BLOCKS 16 /* the free list is too short; the step was emptied */
 
 /* Further bits of pa_last_launches(). */
@@ -148,7 +148,8 @@ uint64_t pa_kv8_workspace_bytes(int32_t num_seqs, int32_t num_tokens, int32_t nu
  * i stands at p = context_lens[i] - query_lens[i] + t and attends to keys 0 .. p through
  * the block table (the rule of inference_server/core/attention.py:19-58).  Lengths and
  * tables stay on the device; the launches depend on the host's sizes only, so a captured
- * call can be replayed with other lengths.  cu_query_lens and work come from
+ * call can be replayed with other lengths.  Sums are float32; softmax weights are rounded to fp16
+ * for the product with V: 11 bits, and at most 2^-32 of a row's largest weight lost a key.  cu_query_lens and work come from
  * pa_kv8_build_step with the tiling of the same group, sizes and max_query_len; with both NULL
  * the call sums query_lens and the work up by itself (over 64 sequences in one more launch),
  * with pa_kv8_build_step's checks.  table_width blocks of a table row are used.  Rows past the

@@ -18,8 +18,9 @@
 // consumer warps, which take stages of 32 keys in turn, and a producer warp, which walks the
 // slice's pieces, reads the block table and keeps each consumer's ring full: the rings run
 // across pieces, so a new sequence costs no drain.  With one group of 8 rows there are three
-// CTAs on an SM, and HBM bounds them; with more rows a thread needs 168 registers and there
-// are two (five consumers a CTA, or one CTA of eleven, are no faster).  Per 16 keys: K and V tile by
+// CTAs on an SM, and HBM bounds them; with more rows a thread needs 168 registers, three groups
+// of 128 dims spill 120 bytes of them (pairs of heads 188), and there are two (five consumers a
+// CTA, or one CTA of eleven, are no faster).  Per 16 keys: K and V tile by
 // TMA (a 16-row box); the 16 + 16 scale bytes through a producer lane's registers, a round
 // of 32 blocks ahead (as bulk copies of 16 bytes they cost the copy engine as much as the
 // tiles: 177 against 152 us for 64 sequences of about 4,096 keys, 8 heads of 128).

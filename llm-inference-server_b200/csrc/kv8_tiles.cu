@@ -48,8 +48,10 @@
 // took 291, without widening 254.
 //
 // Measured with the join (32 query heads, 8 KV heads of 128): 1,000 tokens over 16,384 keys 264 us
-// (985 TFLOP/s, 59 % of the measured bf16 GEMM rate; floor 157), 13 x 2,047 tokens 619, 30 tokens
-// over 100,000 keys 82, a prompt of 333 tokens 26.  A tile of 64 keys takes 1.1 us, the softmax's
+// in short bursts (985 TFLOP/s, 59 % of the measured bf16 GEMM rate; floor 157) and 284 to 291 call
+// after call under the power cap, 13 x 2,047 tokens 612 (the 16-bit path's prefill 501), 30 tokens
+// over 100,000 keys 81, a prompt of 333 tokens 26.  40 bytes of a thread's registers are spilled
+// (64 dims: 56).  A tile of 64 keys takes 1.1 us, the softmax's
 // chain; the tensor pipe is busy 53 % of the time, the exponential unit 50 %, issue slots 58 %.
 // What did not help: two threads per row (a meeting of two warps a tile, 1.2 times the
 // instructions: 297 us), turns at the exponential unit (277), 16 widening warps (281), the tile's

@@ -13,7 +13,8 @@ bounds it and twice the tokens a pool holds.  Three operators that work together
 Format: a row (one token of one KV head) is e4m3 payload ``[NB, BS, Hkv, D]`` and a scale
 byte ``[NB, Hkv, BS]`` that stands for ``2^(byte - 127)`` (``torch.float8_e8m0fnu``): the least
 exponent in [-14, 7] that brings the row's largest magnitude to 448.  Every cached value is
-exactly an fp16 number; magnitudes past 57,344 saturate; a row with a NaN reads as NaN.
+exactly an fp16 number; magnitudes past 57,344 saturate; rows below 448 * 2^-15 are kept in steps
+of 2^-23; a row with a NaN reads as NaN.
 
 Lengths and ids that only the GPU sees are checked there: a bad step is emptied and leaves
 a bit in the device's error word, which :func:`read_kv8_error` returns.
@@ -440,7 +441,8 @@ def paged_attention_kv8(query: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     and rule with the pools' scales.  Lengths and tables are device tensors that the host never
     reads; ``max_query_len`` bounds the chunks (default: the token count).  Sums the step up by
     itself (past 64 sequences in a launch of its own) unless ``block_tables`` carries one
-    (:func:`attach_step`).
+    (:func:`attach_step`).  Sums are float32; softmax weights are rounded to fp16 for the product
+    with V (11 bits; of a key far below the maximum at most 2^-32 of the largest weight is lost).
 
     query ``[T, Hq, D]``, float16 or bfloat16, any strides and offset (rows that are not 16-byte
     aligned are copied first), D 64 or 128, at most 16 query heads per KV head; ``out``
