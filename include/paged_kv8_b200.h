@@ -109,7 +109,9 @@ int32_t pa_kv8_build_step(const int32_t* row_ids, const int32_t* lens, const int
  * was built with, whatever row_ids holds by now.  A step that was emptied changes
  * nothing, nor does one that no longer fits, which sets PA_KV8_ERR_STEP: one of other lens, held
  * or num_free, one whose slots have other lengths by now, or whose new blocks are not the free
- * list's last ones any more (another step took them, or blocks were released over them).
+ * list's last ones any more (another step took them, or blocks were released over them).  A slot
+ * that was released and filled again, to the same length in the same blocks, looks the same:
+ * drop the steps of slots that are released.
  * No reference counterpart.
  */
 int32_t pa_kv8_commit(const int32_t* row_ids, const int32_t* query_lens, const int32_t* accepted,

@@ -248,8 +248,9 @@ __device__ __forceinline__ int row_of(const int32_t* at, int rows, int b) {
 
 // One CTA.  A step is planned from the slots and the free list as they are then, and other steps
 // may count or blocks come back before it does, so the plan is compared first: each slot's
-// length, the blocks that its new tokens went into, and that the step's new blocks are still the
-// free list's last ones.  Then all of it is written, or nothing.  What bounds it is latency: the
+// length, the blocks of its last token and of those that the step brings, and that the step's new
+// blocks are still the free list's last ones.  Then all of it is written, or nothing.  (A slot that
+// was released and filled again to the same length with the same blocks looks the same.)  What bounds it is latency: the
 // rows, their slots, the new blocks are three dependent loads, so a block's thread has nothing
 // else to look up in global memory (with its slot and place read there: 12 us for 8 prompts of
 // 4,096 tokens, 2,048 blocks, instead of 4.5).
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(kCommitThreads)
           need = 0;
         } else if (q > 0) {
           const int32_t *now = r.tables + int64_t(row) * r.table_stride, *then = r.out_tables + int64_t(i) * r.width;
-          for (int j = base / r.block_size; j < mine && j * r.block_size < ctx; ++j) bad |= now[j] != then[j];
+          for (int j = max(base - 1, 0) / r.block_size; j < mine && j * r.block_size < ctx; ++j) bad |= now[j] != then[j];
         }
       }
       s_row[i] = row;

@@ -192,6 +192,21 @@ def test_a_slot_that_was_filled_again_elsewhere_is_not_committed_and_reports(pkg
     assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
 
 
+def test_a_slot_that_was_filled_again_up_to_a_block_is_not_committed_and_reports(pkg):
+    """The step's token starts a block of its own, so only the block before it tells."""
+    bt = _tables(pkg, lens=(20, 5, 32, 0))
+    step = _reserve(bt, [0, 2], [1, 1])
+    want = int(step.block_tables[1, 2])
+    bt.release(_i32([2]))
+    bt.commit(_reserve(bt, [3], [1]))
+    bt.commit(_reserve(bt, [2], [32]))
+    bt.free[int(bt.num_free) - 1] = want                       # as if it had come back on top of the list
+    before = _state_of(bt)
+    bt.commit(step)
+    assert _state_of(bt) == before
+    assert pkg.read_kv8_error(DEV) == pkg._lib.PA_KV8_ERR_STEP
+
+
 def test_a_dropped_step_leaves_no_trace_in_one_that_counts(pkg):
     """The dropped one planned the same free blocks for other rows and wrote them into the tables."""
     bt = _tables(pkg)
